@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define NT_ABI_VERSION 8
+#define NT_ABI_VERSION 9
 #define NT_MAX_GROUPS 32      /* coefficient groups per nt_adamw_mt call */
 #define NT_MAX_FOUND_INF 16   /* optimizers combined by one nt_scaler_update call */
 
@@ -412,6 +412,102 @@ typedef struct nt_fused_args {
 /* One fused elementwise operation, the kernel bodies of namitorch/backends/cuda/fused.py:
    8-69 (float32 there; float16 / bfloat16 here too, computed in float32 and rounded once). */
 int nt_fused_elementwise(const nt_fused_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* Sliding-window attention with sinks                                                   */
+/* ------------------------------------------------------------------------------------ */
+
+#define NT_ATTENTION_MAX_HEAD_DIM 128
+
+/* q: [batch, query_heads, queries, head_dim]; k, v: [batch, kv_heads, keys, head_dim], each with
+   any element strides of its first three dimensions and unit stride of the last. Query head h
+   reads key / value head h / (query_heads / kv_heads). Query i stands at position
+   p = query_offset + i; key j of sequence b is visible to it when
+     j < lengths[b]  and  j <= p  and  (window == 0 or p - j < window or j < sinks).
+   A query that sees no key has the output 0 and the statistic -inf. What lies at or past
+   lengths[b] is never used, whatever it holds. */
+typedef struct nt_attention_args {
+  int32_t dtype;             /* NT_F32 / NT_F16 / NT_BF16 of every tensor but lse */
+  int32_t head_dim;          /* 1..NT_ATTENTION_MAX_HEAD_DIM */
+  int64_t batch;
+  int64_t query_heads;       /* a multiple of kv_heads */
+  int64_t kv_heads;
+  int64_t queries;
+  int64_t keys;
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t query_strides[3];  /* batch, head, token; in elements */
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  const int32_t* lengths;    /* device [batch], clamped to [0, keys], or NULL: every key is there */
+  int64_t window;            /* 0: no window */
+  int64_t sinks;
+  int64_t query_offset;
+  float scale;               /* of q k^T before the softmax: positive, finite */
+  int32_t reserved;
+  void* output;              /* forward: written; backward: read */
+  int64_t output_strides[3];
+  float* lse;                /* [batch, query_heads, queries] log-sum-exp of a row's scaled scores:
+                                written by the forward (NULL: not saved), read by the backward */
+  const void* gradient;      /* backward: of the output */
+  void* grad_query;
+  void* grad_key;
+  void* grad_value;
+  int64_t gradient_strides[3];
+  int64_t grad_query_strides[3];
+  int64_t grad_key_strides[3];
+  int64_t grad_value_strides[3];
+  void* workspace;           /* backward: nt_attention_workspace_size bytes, contents ignored */
+  size_t workspace_bytes;
+  int32_t* error;            /* device word or NULL, sticky: |= 1 when a bounded wait inside a kernel
+                                ran out (the outputs are then incomplete) */
+} nt_attention_args;
+
+/* Bytes of scratch that nt_attention_backward needs for these sizes (pointers and strides are
+   not looked at). */
+size_t nt_attention_workspace_size(const nt_attention_args* args);
+
+/* softmax(scale q k^T restricted to the visible keys) v in one pass over the keys. */
+int nt_attention_forward(const nt_attention_args* args, void* stream);
+
+/* Gradients of q, k and v from the forward's output and lse. A fixed order of every sum: two
+   calls on the same inputs give the same bits. */
+int nt_attention_backward(const nt_attention_args* args, void* stream);
+
+/* One new token per sequence over a cache: queries == 1, the query of sequence b stands at
+   lengths[b] - 1 (lengths is required, query_offset is ignored). */
+int nt_attention_step(const nt_attention_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* Dropout from a counter-based generator, with the bias before it and the residual after */
+/* ------------------------------------------------------------------------------------ */
+
+/* Element e of the contiguous [rows, width] input is dropped when word e % 4 of
+   Philox4x32-7 (Salmon, Moraes, Dror, Shaw 2011) with the counter (low and high half of e / 4,
+   low and high half of offset) under the key (low and high half of seed) is below
+   floor(p 2^32). The mask is a function of (seed, offset, e) alone and is never stored. */
+typedef struct nt_dropout_args {
+  int32_t dtype;           /* NT_F32 / NT_F16 / NT_BF16 of every tensor */
+  int32_t reserved;
+  int64_t rows;
+  int64_t width;
+  double p;                /* in [0, 1) */
+  uint64_t seed;
+  uint64_t offset;
+  const void* input;       /* forward: [rows, width]; backward: the upstream gradient */
+  const void* bias;        /* forward: [width] or NULL */
+  const void* residual;    /* forward: [rows, width] or NULL */
+  void* output;            /* forward: residual + keep (input + bias) / (1 - p);
+                              backward: keep input / (1 - p), the input's gradient, or NULL */
+  void* grad_bias;         /* backward: [width] column sums of the input's gradient, or NULL */
+  void* workspace;         /* backward with grad_bias: nt_dropout_workspace_size bytes, contents ignored */
+  size_t workspace_bytes;
+} nt_dropout_args;
+
+size_t nt_dropout_workspace_size(int64_t rows, int64_t width);
+int nt_dropout_forward(const nt_dropout_args* args, void* stream);
+int nt_dropout_backward(const nt_dropout_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------ */
 /* ZeRO-1 over peer memory (NVLink / NVSwitch)                                           */

@@ -22,7 +22,7 @@ NT_DECAY_NONE, NT_DECAY_DECOUPLED, NT_DECAY_COUPLED = 0, 1, 2
 NT_MAX_GROUPS = 32
 NT_MAX_FOUND_INF = 16
 NT_MAX_RANKS = 8
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 
 class Segment(C.Structure):
@@ -126,6 +126,30 @@ class NormArgs(C.Structure):
                 ("width", C.c_int64), ("eps", C.c_float)]
 
 
+NT_ATTENTION_MAX_HEAD_DIM = 128
+_Strides = C.c_int64 * 3
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("batch", C.c_int64), ("query_heads", C.c_int64),
+                ("kv_heads", C.c_int64), ("queries", C.c_int64), ("keys", C.c_int64), ("query", C.c_void_p),
+                ("key", C.c_void_p), ("value", C.c_void_p), ("query_strides", _Strides), ("key_strides", _Strides),
+                ("value_strides", _Strides), ("lengths", C.c_void_p), ("window", C.c_int64), ("sinks", C.c_int64),
+                ("query_offset", C.c_int64), ("scale", C.c_float), ("reserved", C.c_int32), ("output", C.c_void_p),
+                ("output_strides", _Strides), ("lse", C.c_void_p), ("gradient", C.c_void_p),
+                ("grad_query", C.c_void_p), ("grad_key", C.c_void_p), ("grad_value", C.c_void_p),
+                ("gradient_strides", _Strides), ("grad_query_strides", _Strides), ("grad_key_strides", _Strides),
+                ("grad_value_strides", _Strides), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("error", C.c_void_p)]
+
+
+class DropoutArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32), ("rows", C.c_int64), ("width", C.c_int64),
+                ("p", C.c_double), ("seed", C.c_uint64), ("offset", C.c_uint64), ("input", C.c_void_p),
+                ("bias", C.c_void_p), ("residual", C.c_void_p), ("output", C.c_void_p), ("grad_bias", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class ZeroReduceArgs(C.Structure):
     _fields_ = [("sources", C.c_void_p * NT_MAX_RANKS), ("num_ranks", C.c_int32), ("dtype", C.c_int32),
                 ("count", C.c_int64), ("average", C.c_int32), ("dest", C.c_void_p), ("scale", C.c_void_p),
@@ -194,6 +218,13 @@ SIGNATURES: dict[str, tuple] = {
     "nt_norm_forward": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
     "nt_norm_backward": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
     "nt_fused_elementwise": (C.c_int, [C.POINTER(FusedArgs), C.c_void_p]),
+    "nt_attention_workspace_size": (C.c_size_t, [C.POINTER(AttentionArgs)]),
+    "nt_attention_forward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "nt_attention_backward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "nt_attention_step": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "nt_dropout_workspace_size": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "nt_dropout_forward": (C.c_int, [C.POINTER(DropoutArgs), C.c_void_p]),
+    "nt_dropout_backward": (C.c_int, [C.POINTER(DropoutArgs), C.c_void_p]),
     "nt_xent_workspace_size": (C.c_size_t, []),
     "nt_softmax_xent": (C.c_int, [C.POINTER(XentArgs), C.c_void_p]),
     "nt_xent_backward_scale": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int32,
@@ -254,6 +285,7 @@ LAUNCHES_PER_CALL = {"nt_adamw_f32": 1, "nt_adamw_mt": 1, "nt_adamw_mt_push": 1,
                      "nt_zero_flag_exchange": 1, "nt_zero_stats_exchange": 1,
                      "nt_grad_stats": 1, "nt_grad_stats_finalize": 1, "nt_schedule_step": 1, "nt_row_softmax": 1, "nt_norm_forward": 1,
                      "nt_grad_transform": 1, "nt_grad_clip_value": 1, "nt_scaler_update": 1,
+                     "nt_attention_forward": 1, "nt_attention_step": 1, "nt_dropout_forward": 1,
                      "nt_softmax_xent": 2, "nt_xent_backward_scale": 1, "nt_cast": 1, "nt_fused_elementwise": 1}
 launch_count = 0
 

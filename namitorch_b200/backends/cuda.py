@@ -58,18 +58,23 @@ class AdamWCUDAKernel:
 
 class CUDABackend:
     """One per device (namitorch/backends/cuda/__init__.py:23-45); ``adamw``, ``fused``,
-    ``softmax`` and ``normalization`` are the plugin seams."""
+    ``softmax`` and ``normalization`` are the plugin seams; ``attention`` and ``dropout`` hold
+    the operators that the reference's backend has no seam for."""
 
     def __init__(self, device: torch.device):
         N.load()
         self.device = device
         self.adamw = AdamWCUDAKernel(self)
+        from .attention import AttentionCUDAKernels
+        from .dropout import DropoutCUDAKernels
         from .fused import FusedCUDAKernels
         from .normalization import NormalizationCUDAKernels
         from .softmax import SoftmaxCUDAKernels
         self.fused = FusedCUDAKernels(self)
         self.softmax = SoftmaxCUDAKernels(self)
         self.normalization = NormalizationCUDAKernels(self)
+        self.attention = AttentionCUDAKernels(self)
+        self.dropout = DropoutCUDAKernels(self)
 
     @staticmethod
     def supports_float16() -> bool:

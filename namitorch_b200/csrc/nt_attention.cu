@@ -1,0 +1,814 @@
+// Sliding-window attention with sinks: the C entry points, the kernels for float32 (and for
+// 16-bit rows that are no whole 16-byte vectors) and the one-token step.
+//
+//   S = scale q k^T over the visible keys,  m = max S,  l = sum exp(S - m),
+//   o = sum exp(S - m) v / l,  lse = m + ln l
+//   P = exp(S - lse),  dv = P^T g,  dP = g v^T,  delta = sum(g o),  dS = P (dP - delta),
+//   dq = scale dS k,  dk = scale dS^T q, dk and dv summed over the query heads of a group
+//
+// Nothing of size queries x keys is stored: the forward keeps the running maximum and sum, the
+// backward computes S again from lse. All sums are float32. The gradients of queries and of
+// keys are two passes over the pairs (each computes S and dP), so that every sum has one owner
+// and a fixed order: no atomics.
+#include <cmath>
+#include <climits>
+
+#include "nt_attention.cuh"
+
+namespace nt {
+
+// ---- float32 kernels: 64 x 64 blocks on the FP32 pipe ---------------------------------
+// 256 threads as 16 x 16; a thread holds rows 4 ty .. 4 ty + 3 and columns tx + 16 j. Rows in
+// shared memory are DP + 4 floats apart, so the eight threads of a 16-byte wavefront that read
+// eight consecutive rows touch different banks. A product step reads 8 vectors of 16 bytes for
+// 64 fused multiply-adds, which keeps the FP32 pipe and not shared memory the limit.
+constexpr int kRows = 64;
+constexpr int kSimtThreads = 256;
+constexpr int kWeightStride = kRows + 4;
+
+// rows [first, first + 64) of one head into shared memory as float32; zero past `end` and past
+// the head's width.
+template <int DT, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const void* base, int64_t row_stride, int64_t first, int64_t end,
+                                          int dim, int vec) {
+  using T = typename Elem<DT>::T;
+  constexpr int EPV = 16 / (int)sizeof(T);
+  const T* src = static_cast<const T*>(base);
+  if (vec) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kRows * (DP / EPV); i += kSimtThreads) {
+      const int r = i / (DP / EPV), c = i % (DP / EPV) * EPV;
+      float v[EPV];
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) v[e] = 0.0f;
+      if (first + r < end && c < dim)
+        unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(src + (first + r) * row_stride + c)), v);
+#pragma unroll
+      for (int e = 0; e < EPV; e += 4)
+        *reinterpret_cast<float4*>(dst + r * (DP + 4) + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    }
+  } else {
+    for (int i = threadIdx.x; i < kRows * DP; i += kSimtThreads) {
+      const int r = i / DP, c = i % DP;
+      dst[r * (DP + 4) + c] = first + r < end && c < dim ? Elem<DT>::to_f32(src[(first + r) * row_stride + c]) : 0.0f;
+    }
+  }
+}
+
+// s[i][j] = sum over the width of a[4 ty + i] . b[tx + 16 j]
+template <int DP>
+__device__ __forceinline__ void tile_product(const float* a, const float* b, int tx, int ty, float (&s)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * (DP + 4) + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (DP + 4) + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        s[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, s[i][j]))));
+  }
+}
+
+// acc[i][u] += sum over the 64 columns c of w[4 ty + i][c] * b[c][4 tx + 64 u ..]
+template <int DP>
+__device__ __forceinline__ void tile_accumulate(const float* w, const float* b, int tx, int ty, float4 (&acc)[4][DP / 64]) {
+#pragma unroll 2
+  for (int c = 0; c < kRows; c += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(w + (4 * ty + i) * kWeightStride + c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int u = 0; u < DP / 64; ++u) {
+        const float4 y = *reinterpret_cast<const float4*>(b + (c + k) * (DP + 4) + 4 * tx + 64 * u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w;
+          acc[i][u].x = fmaf(f, y.x, acc[i][u].x);
+          acc[i][u].y = fmaf(f, y.y, acc[i][u].y);
+          acc[i][u].z = fmaf(f, y.z, acc[i][u].z);
+          acc[i][u].w = fmaf(f, y.w, acc[i][u].w);
+        }
+      }
+  }
+}
+
+template <int DT, int DP>
+__device__ __forceinline__ void store_row4(void* base, int64_t at, int tx, int dim, const float4 (&acc)[DP / 64], float f) {
+#pragma unroll
+  for (int u = 0; u < DP / 64; ++u) {
+    const float v[4] = {acc[u].x, acc[u].y, acc[u].z, acc[u].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = 4 * tx + 64 * u + e;
+      if (c < dim) store1<DT>(base, at + c, v[e] * f);
+    }
+  }
+}
+
+__device__ __forceinline__ float lanes16_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float lanes16_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The maximum is kept of the scores before the scale: a difference of scores is formed before it
+// is scaled, so that scores near the ends of float32 do not overflow on the way.
+template <int DT, int DP>
+__global__ void __launch_bounds__(kSimtThreads) attention_forward_kernel(const __grid_constant__ AttnParams P) {
+  extern __shared__ __align__(16) float smem[];
+  float* q = smem;
+  float* kv = q + kRows * (DP + 4);
+  float* w = kv + kRows * (DP + 4);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int b = blockIdx.z, h = blockIdx.y, hk = h / P.group;
+  const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows, i1 = min(P.queries, i0 + kRows);
+  const int length = attn_length(P, b);
+  const AttnKeys range(P, length, i0, i1);
+  const int es = sizeof(typename Elem<DT>::T);
+  load_tile<DT, DP>(q, static_cast<const char*>(P.q) + P.qs.at(b, h, 0) * es, P.qs.t, i0, i1, P.dim, P.vec);
+  float m[4], l[4];
+  float4 acc[4][DP / 64];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < DP / 64; ++u) acc[i][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  const int blocks = range.blocks(kRows);
+  for (int t = 0; t < blocks; ++t) {
+    int begin, end;
+    range.block(t, kRows, begin, end);
+    __syncthreads();
+    load_tile<DT, DP>(kv, static_cast<const char*>(P.k) + P.ks.at(b, hk, 0) * es, P.ks.t, begin, end, P.dim, P.vec);
+    __syncthreads();
+    float s[4][4];
+    tile_product<DP>(q, kv, tx, ty, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = P.offset + i0 + 4 * ty + i;
+      float top = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = begin + tx + 16 * j;
+        s[i][j] = key < end && attn_visible(P, length, p, key) ? s[i][j] : -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+      top = lanes16_max(top);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      const float old = exp2f((m[i] - shift) * P.scale_log2);
+      m[i] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f((s[i][j] - shift) * P.scale_log2);
+        sum += e;
+        w[(4 * ty + i) * kWeightStride + tx + 16 * j] = e;
+      }
+      l[i] = l[i] * old + lanes16_sum(sum);
+#pragma unroll
+      for (int u = 0; u < DP / 64; ++u) {
+        acc[i][u].x *= old; acc[i][u].y *= old; acc[i][u].z *= old; acc[i][u].w *= old;
+      }
+    }
+    __syncthreads();
+    load_tile<DT, DP>(kv, static_cast<const char*>(P.v) + P.vs.at(b, hk, 0) * es, P.vs.t, begin, end, P.dim, P.vec);
+    __syncthreads();
+    tile_accumulate<DP>(w, kv, tx, ty, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i0 + 4 * ty + i;
+    if (row >= i1) continue;
+    store_row4<DT, DP>(P.o, P.os.at(b, h, row), tx, P.dim, acc[i], l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]));
+    if (P.lse != nullptr && tx == 0)
+      P.lse[((int64_t)b * P.heads + h) * P.queries + row] = l[i] == 0.0f ? -INFINITY : fmaf(m[i], P.scale, log2f(l[i]) * kLn2F);
+  }
+}
+
+// One pass of the backward. DKV = false: a block owns 64 queries and walks the keys (x1 = q,
+// x2 = g; y1 = k, y2 = v), giving dq and writing delta. DKV = true: a block owns 64 keys and
+// walks the queries of its group's heads (x1 = k, x2 = v; y1 = q, y2 = g), giving dk and dv.
+// In both, s = x1 y1^T and dp = x2 y2^T, out1 = dS y1, and with DKV out2 = P y2.
+template <int DT, int DP, bool DKV>
+__global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const __grid_constant__ AttnParams P) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int TILE = kRows * (DP + 4);
+  float *x1 = smem, *x2 = x1 + TILE, *y1 = x2 + TILE, *y2 = y1 + TILE;
+  float *wds = y2 + TILE, *wp = wds + kRows * kWeightStride;
+  __shared__ float row_lse[kRows], row_delta[kRows];
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int es = sizeof(typename Elem<DT>::T);
+  const int b = blockIdx.z;
+  const int length = attn_length(P, b);
+  const char *qb = static_cast<const char*>(P.q), *kb = static_cast<const char*>(P.k), *vb = static_cast<const char*>(P.v),
+             *gb = static_cast<const char*>(P.g);
+  float4 out1[4][DP / 64], out2[4][DP / 64];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int u = 0; u < DP / 64; ++u) out1[i][u] = out2[i][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+
+  if constexpr (!DKV) {
+    const int h = blockIdx.y, hk = h / P.group;
+    const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows, i1 = min(P.queries, i0 + kRows);
+    const AttnKeys range(P, length, i0, i1);
+    load_tile<DT, DP>(x1, qb + P.qs.at(b, h, 0) * es, P.qs.t, i0, i1, P.dim, P.vec);
+    load_tile<DT, DP>(x2, gb + P.gs.at(b, h, 0) * es, P.gs.t, i0, i1, P.dim, P.vec);
+    load_tile<DT, DP>(y1, static_cast<const char*>(P.o) + P.os.at(b, h, 0) * es, P.os.t, i0, i1, P.dim, P.vec);
+    __syncthreads();
+    const int64_t stat = ((int64_t)b * P.heads + h) * P.queries;
+    float lse[4], delta[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * ty + i;
+      float d = 0.0f;
+      for (int c = tx; c < P.dim; c += 16) d = fmaf(x2[r * (DP + 4) + c], y1[r * (DP + 4) + c], d);
+      delta[i] = lanes16_sum(d);
+      lse[i] = i0 + r < i1 ? P.lse[stat + i0 + r] * kLog2eF : 0.0f;
+      if (tx == 0 && i0 + r < i1) P.delta[stat + i0 + r] = delta[i];
+    }
+    const int blocks = range.blocks(kRows);
+    for (int t = 0; t < blocks; ++t) {
+      int begin, end;
+      range.block(t, kRows, begin, end);
+      __syncthreads();
+      load_tile<DT, DP>(y1, kb + P.ks.at(b, hk, 0) * es, P.ks.t, begin, end, P.dim, P.vec);
+      load_tile<DT, DP>(y2, vb + P.vs.at(b, hk, 0) * es, P.vs.t, begin, end, P.dim, P.vec);
+      __syncthreads();
+      float s[4][4], dp[4][4];
+      tile_product<DP>(x1, y1, tx, ty, s);
+      tile_product<DP>(x2, y2, tx, ty, dp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = begin + tx + 16 * j;
+          const bool seen = key < end && attn_visible(P, length, P.offset + i0 + 4 * ty + i, key);
+          const float pr = exp2f(fmaf(s[i][j], P.scale_log2, -lse[i]));
+          wds[(4 * ty + i) * kWeightStride + tx + 16 * j] = seen ? pr * (dp[i][j] - delta[i]) : 0.0f;
+        }
+      __syncthreads();
+      tile_accumulate<DP>(wds, y1, tx, ty, out1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + 4 * ty + i < i1) store_row4<DT, DP>(P.dq, P.dqs.at(b, h, i0 + 4 * ty + i), tx, P.dim, out1[i], P.scale);
+  } else {
+    const int hk = blockIdx.y;
+    const int split = P.sink_tiles * P.parts;
+    const int tile = (int)blockIdx.x < split ? (int)blockIdx.x / P.parts : (int)blockIdx.x - split + P.sink_tiles;
+    const int part = (int)blockIdx.x < split ? (int)blockIdx.x % P.parts : 0;
+    const int parts = (int)blockIdx.x < split ? P.parts : 1;
+    const int k0 = tile * kRows, k1 = min(P.keys, k0 + kRows);
+    const AttnQueries range(P, length, k0, k1);
+    load_tile<DT, DP>(x1, kb + P.ks.at(b, hk, 0) * es, P.ks.t, k0, k1, P.dim, P.vec);
+    load_tile<DT, DP>(x2, vb + P.vs.at(b, hk, 0) * es, P.vs.t, k0, k1, P.dim, P.vec);
+    const int steps = (range.hi - range.lo + kRows - 1) / kRows;
+    const int64_t total = (int64_t)steps * P.group;
+    const int64_t from = total * part / parts, to = total * (part + 1) / parts;
+    for (int64_t t = from; t < to; ++t) {
+      const int h = hk * P.group + (int)(t / steps);
+      const int begin = range.lo + (int)(t % steps) * kRows, end = min(range.hi, begin + kRows);
+      __syncthreads();
+      load_tile<DT, DP>(y1, qb + P.qs.at(b, h, 0) * es, P.qs.t, begin, end, P.dim, P.vec);
+      load_tile<DT, DP>(y2, gb + P.gs.at(b, h, 0) * es, P.gs.t, begin, end, P.dim, P.vec);
+      const int64_t stat = ((int64_t)b * P.heads + h) * P.queries;
+      if (threadIdx.x < kRows) {
+        const bool in = begin + (int)threadIdx.x < end;
+        row_lse[threadIdx.x] = in ? P.lse[stat + begin + threadIdx.x] * kLog2eF : 0.0f;
+        row_delta[threadIdx.x] = in ? P.delta[stat + begin + threadIdx.x] : 0.0f;
+      }
+      __syncthreads();
+      float s[4][4], dp[4][4];
+      tile_product<DP>(x1, y1, tx, ty, s);
+      tile_product<DP>(x2, y2, tx, ty, dp);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = tx + 16 * j, key = k0 + 4 * ty + i;
+          const bool seen = begin + c < end && attn_visible(P, length, P.offset + begin + c, key);
+          const float pr = seen ? exp2f(fmaf(s[i][j], P.scale_log2, -row_lse[c])) : 0.0f;
+          wp[(4 * ty + i) * kWeightStride + c] = pr;
+          wds[(4 * ty + i) * kWeightStride + c] = seen ? pr * (dp[i][j] - row_delta[c]) : 0.0f;
+        }
+      __syncthreads();
+      tile_accumulate<DP>(wds, y1, tx, ty, out1);
+      tile_accumulate<DP>(wp, y2, tx, ty, out2);
+    }
+    if (parts == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = k0 + 4 * ty + i;
+        if (row >= k1) continue;
+        store_row4<DT, DP>(P.dk, P.dks.at(b, hk, row), tx, P.dim, out1[i], P.scale);
+        store_row4<DT, DP>(P.dv, P.dvs.at(b, hk, row), tx, P.dim, out2[i], 1.0f);
+      }
+    } else {
+      // [batch, kv head, sink block, part, 2, 64, dim]
+      const int64_t at = ((((int64_t)b * P.kv_heads + hk) * P.sink_tiles + tile) * parts + part) * 2 * kRows * P.dim;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t r = 4 * ty + i;
+        store_row4<NT_F32, DP>(P.partial, at + r * P.dim, tx, P.dim, out1[i], P.scale);
+        store_row4<NT_F32, DP>(P.partial, at + (kRows + r) * P.dim, tx, P.dim, out2[i], 1.0f);
+      }
+    }
+  }
+}
+
+// dk and dv of the sink blocks: the parts added in order. One thread per element; `tile_rows`
+// keys a block.
+template <int DT>
+__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnParams P, int tile_rows) {
+  const int64_t per_tile = (int64_t)2 * tile_rows * P.dim;
+  const int64_t total = (int64_t)P.batch * P.kv_heads * P.sink_tiles * per_tile;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t block = e / per_tile, in = e % per_tile;
+    const int which = (int)(in / ((int64_t)tile_rows * P.dim));
+    const int row = (int)(in / P.dim % tile_rows), c = (int)(in % P.dim);
+    const int key = (int)(block % P.sink_tiles) * tile_rows + row;
+    if (key >= P.keys) continue;
+    const int64_t bh = block / P.sink_tiles;
+    const float* src = P.partial + block * P.parts * per_tile + in;
+    float s = 0.0f;
+    for (int k = 0; k < P.parts; ++k) s += src[k * per_tile];
+    const int b = (int)(bh / P.kv_heads), hk = (int)(bh % P.kv_heads);
+    if (which == 0) store1<DT>(P.dk, P.dks.at(b, hk, key) + c, s);
+    else store1<DT>(P.dv, P.dvs.at(b, hk, key) + c, s);
+  }
+}
+
+// ---- one token over a cache ----------------------------------------------------------
+// Bound: HBM, one read of the visible keys and values. A cluster of blocks shares one
+// (sequence, key head, HG query heads): each block takes a contiguous piece of the visible keys,
+// each warp rows of it, LPR lanes of 16 bytes to a row. Every lane group keeps its own running
+// maximum, sum and output; they are joined over the warp by shuffles, over the block in shared
+// memory and over the cluster in distributed shared memory, always in the same order.
+constexpr int kStepThreads = 256;
+constexpr int kStepWarps = kStepThreads / 32;
+constexpr int kStepRows = 4;   // rows in flight per lane group
+constexpr int kStepMaxCluster = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
+  uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p)), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+  return v;
+}
+
+template <int DT, int LPR, int HG>
+__global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __grid_constant__ AttnParams P) {
+  using T = typename Elem<DT>::T;
+  constexpr int EPV = 16 / (int)sizeof(T);
+  constexpr int DP = LPR * EPV;
+  constexpr int RPL = 32 / LPR;
+  __shared__ float part_ml[kStepWarps][HG][2];
+  __shared__ float part_acc[kStepWarps][HG][DP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / LPR, col = lane % LPR * EPV;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int passes = P.group / HG;
+  const int hk = blockIdx.y / passes, h0 = hk * P.group + blockIdx.y % passes * HG;
+  const int b = blockIdx.z;
+  const int length = attn_length(P, b);
+  int lo = P.window == 0 ? 0 : max(0, length - P.window);
+  const int sink_end = min(P.sinks, lo);
+  const int visible = sink_end + length - lo;
+  const int chunk = (visible + splits - 1) / splits;
+  const int from = min(visible, rank * chunk), to = min(visible, from + chunk);
+  const int skip = lo - sink_end;    // visible key n >= sink_end is row n + skip
+
+  float q[HG][EPV], acc[HG][EPV], m[HG], l[HG];
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      acc[g][e] = 0.0f;
+      q[g][e] = col + e < P.dim ? load1<DT>(P.q, P.qs.at(b, h0 + g, 0) + col + e) : 0.0f;
+    }
+  }
+  const T* kb = static_cast<const T*>(P.k) + P.ks.at(b, hk, 0) + col;
+  const T* vb = static_cast<const T*>(P.v) + P.vs.at(b, hk, 0) + col;
+  auto load = [&](const T* base, int64_t stride, int n, uint4& raw) {
+    raw = make_uint4(0, 0, 0, 0);
+    if (n < to && col < P.dim) {
+      const int64_t row = n < sink_end ? n : n + skip;
+      const T* src = base + row * stride;
+      if (P.vec) {
+        raw = __ldcs(reinterpret_cast<const uint4*>(src));
+      } else {
+        T* out = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e)
+          if (col + e < P.dim) out[e] = src[e];
+      }
+    }
+  };
+  constexpr int STRIDE = kStepWarps * RPL;
+  for (int n0 = from + warp * RPL + sub; n0 - sub < to; n0 += STRIDE * kStepRows) {
+    uint4 kr[kStepRows], vr[kStepRows];
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) load(kb, P.ks.t, n0 + r * STRIDE, kr[r]);
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) load(vb, P.vs.t, n0 + r * STRIDE, vr[r]);
+    float s[kStepRows][HG];
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) {
+      float kf[EPV];
+      unpack16<DT>(kr[r], kf);
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        float d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) d = fmaf(q[g][e], kf[e], d);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        s[r][g] = n0 + r * STRIDE < to ? d : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < HG; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int r = 0; r < kStepRows; ++r) top = fmaxf(top, s[r][g]);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      const float old = exp2f((m[g] - shift) * P.scale_log2);
+      m[g] = top;
+      l[g] *= old;
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) acc[g][e] *= old;
+#pragma unroll
+      for (int r = 0; r < kStepRows; ++r) {
+        s[r][g] = exp2f((s[r][g] - shift) * P.scale_log2);
+        l[g] += s[r][g];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) {
+      float vf[EPV];
+      unpack16<DT>(vr[r], vf);
+#pragma unroll
+      for (int g = 0; g < HG; ++g)
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) acc[g][e] = fmaf(s[r][g], vf[e], acc[g][e]);
+    }
+  }
+  // Join the lane groups of a warp, then the warps.
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    float top = m[g];
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = top == -INFINITY ? 0.0f : exp2f((m[g] - top) * P.scale_log2);
+    l[g] *= f;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) acc[g][e] *= f;
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) part_acc[warp][g][col + e] = acc[g][e];
+      if (lane == 0) {
+        part_ml[warp][g][0] = top;
+        part_ml[warp][g][1] = l[g];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < HG * DP; i += kStepThreads) {
+    const int g = i / DP, c = i % DP;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_ml[w][g][0]);
+    float sum = 0.0f, a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float f = top == -INFINITY ? 0.0f : exp2f((part_ml[w][g][0] - top) * P.scale_log2);
+      sum = fmaf(part_ml[w][g][1], f, sum);
+      a = fmaf(part_acc[w][g][c], f, a);
+    }
+    part_acc[0][g][c] = a;   // only this thread reads column c
+    if (splits == 1) {
+      if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
+    } else {
+      part_acc[1][g][c] = c == 0 ? top : sum;   // statistics of the block: columns 0 and 1
+    }
+  }
+  if (splits == 1) return;
+  __syncthreads();
+  cluster_sync_all();
+  for (int i = rank * kStepThreads + threadIdx.x; i < HG * DP; i += splits * kStepThreads) {
+    const int g = i / DP, c = i % DP;
+    float top = -INFINITY;
+    for (int r = 0; r < splits; ++r) top = fmaxf(top, load_cluster(&part_acc[1][g][0], r));
+    float sum = 0.0f, a = 0.0f;
+    for (int r = 0; r < splits; ++r) {
+      const float t = load_cluster(&part_acc[1][g][0], r);
+      const float f = top == -INFINITY ? 0.0f : exp2f((t - top) * P.scale_log2);
+      sum = fmaf(load_cluster(&part_acc[1][g][1], r), f, sum);
+      a = fmaf(load_cluster(&part_acc[0][g][c], r), f, a);
+    }
+    if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
+  }
+  cluster_sync_all();   // a block's shared memory stays until every block has read it
+}
+
+// ---- launches ------------------------------------------------------------------------
+
+static int smem_limit(const void* kernel, size_t bytes, const char* what) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == cudaSuccess ? NT_OK : cuda_fail(e, what);
+}
+
+template <int DT, int DP>
+static int launch_forward(const AttnParams& P, cudaStream_t s) {
+  const size_t bytes = (size_t)(2 * kRows * (DP + 4) + kRows * kWeightStride) * 4;
+  auto kernel = attention_forward_kernel<DT, DP>;
+  int rc = smem_limit((const void*)kernel, bytes, "nt_attention_forward");
+  if (rc) return rc;
+  const dim3 grid((P.queries + kRows - 1) / kRows, P.heads, P.batch);
+  kernel<<<grid, kSimtThreads, bytes, s>>>(P);
+  return launch_status("nt_attention_forward launch");
+}
+
+template <int DT, int DP>
+static int launch_backward(const AttnParams& P, cudaStream_t s) {
+  const size_t bytes = (size_t)(4 * kRows * (DP + 4) + 2 * kRows * kWeightStride) * 4;
+  auto dq = attention_backward_kernel<DT, DP, false>;
+  auto dkv = attention_backward_kernel<DT, DP, true>;
+  int rc = smem_limit((const void*)dq, bytes, "nt_attention_backward");
+  if (!rc) rc = smem_limit((const void*)dkv, bytes, "nt_attention_backward");
+  if (rc) return rc;
+  if (P.queries > 0) {
+    dq<<<dim3((P.queries + kRows - 1) / kRows, P.heads, P.batch), kSimtThreads, bytes, s>>>(P);
+    rc = launch_status("nt_attention_backward launch");
+    if (rc) return rc;
+  }
+  const int tiles = (P.keys + kRows - 1) / kRows;
+  if (tiles == 0) return NT_OK;
+  dkv<<<dim3(tiles + P.sink_tiles * (P.parts - 1), P.kv_heads, P.batch), kSimtThreads, bytes, s>>>(P);
+  return launch_status("nt_attention_backward launch");
+}
+
+template <int DT, int LPR, int HG>
+static int launch_step(const AttnParams& P, cudaStream_t s) {
+  const int passes = P.group / HG;
+  // Visible keys at most; blocks of one cluster share them, at least 64 keys to a block.
+  const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
+  const int64_t units = (int64_t)P.batch * P.kv_heads * passes;
+  int splits = 1;
+  while (splits < kStepMaxCluster && units * splits < 2 * current_sm_count() && most > 64 * splits) splits *= 2;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(splits, P.kv_heads * passes, P.batch);
+  config.blockDim = dim3(kStepThreads);
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = splits > 1 ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&config, attention_step_kernel<DT, LPR, HG>, P);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_step launch"); }
+  return launch_status("nt_attention_step launch");
+}
+
+template <int DT, int LPR>
+static int dispatch_step_heads(const AttnParams& P, cudaStream_t s) {
+  if (P.group % 8 == 0) return launch_step<DT, LPR, 8>(P, s);
+  if (P.group % 4 == 0) return launch_step<DT, LPR, 4>(P, s);
+  if (P.group % 2 == 0) return launch_step<DT, LPR, 2>(P, s);
+  return launch_step<DT, LPR, 1>(P, s);
+}
+
+template <int DT>
+static int dispatch_step(const AttnParams& P, cudaStream_t s) {
+  constexpr int EPV = DT == NT_F32 ? 4 : 8;
+  if (P.dim <= 64) return dispatch_step_heads<DT, 64 / EPV>(P, s);
+  return dispatch_step_heads<DT, 128 / EPV>(P, s);
+}
+
+template <int DT>
+static int dispatch_forward(const AttnParams& P, cudaStream_t s) {
+  return P.dim <= 64 ? launch_forward<DT, 64>(P, s) : launch_forward<DT, 128>(P, s);
+}
+template <int DT>
+static int dispatch_backward(const AttnParams& P, cudaStream_t s) {
+  int rc = P.dim <= 64 ? launch_backward<DT, 64>(P, s) : launch_backward<DT, 128>(P, s);
+  if (rc || P.parts == 1 || P.sink_tiles == 0) return rc;
+  attention_join_kernel<DT><<<(unsigned)(current_sm_count() * 4), 256, 0, s>>>(P, kRows);
+  return launch_status("nt_attention_backward (join) launch");
+}
+
+// Pieces of the queries of a sink key block: an ordinary key block sees the queries of its own
+// width and one window, a sink block all later ones. A piece is no longer than an ordinary
+// block's work, nor shorter than 16 steps.
+static int sink_parts(int64_t queries, int64_t window, int64_t group, int64_t tile_rows, int64_t step_rows) {
+  const int64_t most = (queries + step_rows - 1) / step_rows * group;
+  int64_t piece = ((tile_rows + window - 1 + step_rows - 1) / step_rows + 1) * group;
+  if (piece < 16) piece = 16;
+  const int64_t parts = (most + piece - 1) / piece;
+  return (int)(parts < 1 ? 1 : parts);
+}
+
+static size_t delta_bytes(const nt_attention_args& a) {
+  return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
+}
+
+static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows) {
+  if (a.window <= 0 || a.sinks <= 0 || a.keys == 0) return 0;
+  const int64_t sinks = a.sinks < a.keys ? a.sinks : a.keys;
+  const int64_t tiles = (sinks + tile_rows - 1) / tile_rows;
+  const int64_t parts = sink_parts(a.queries, a.window < a.keys ? a.window : a.keys, a.query_heads / a.kv_heads, tile_rows, step_rows);
+  if (parts == 1) return 0;
+  return (size_t)a.batch * a.kv_heads * tiles * parts * 2 * tile_rows * a.head_dim * 4;
+}
+
+static int check_attention(const nt_attention_args& a, const char* who) {
+  if (dtype_size(a.dtype) == 0) { set_error("%s: unsupported dtype %d", who, a.dtype); return NT_EUNSUPPORTED; }
+  if (a.head_dim < 1 || a.head_dim > NT_ATTENTION_MAX_HEAD_DIM) {
+    set_error("%s: head_dim must be in [1, %d]", who, NT_ATTENTION_MAX_HEAD_DIM);
+    return NT_EINVAL;
+  }
+  if (a.batch < 0 || a.queries < 0 || a.keys < 0 || a.kv_heads < 1 || a.query_heads < 1 || a.query_heads % a.kv_heads) {
+    set_error("%s: sizes must be nonnegative and query_heads a positive multiple of kv_heads", who);
+    return NT_EINVAL;
+  }
+  if (a.batch > 65535 || a.query_heads > 65535 || a.keys >= INT_MAX / 2 || a.queries >= INT_MAX / 2) {
+    set_error("%s: batch and heads must be below 65536, queries and keys below 2^30", who);
+    return NT_EINVAL;
+  }
+  if (a.window < 0 || a.sinks < 0 || a.query_offset < 0 || a.query_offset >= INT_MAX / 2) {
+    set_error("%s: window, sinks and query_offset must be nonnegative, query_offset below 2^30", who);
+    return NT_EINVAL;
+  }
+  if (!(a.scale > 0.0f) || !std::isfinite(a.scale)) { set_error("%s: scale must be positive and finite", who); return NT_EINVAL; }
+  return NT_OK;
+}
+
+static AttnStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
+
+// Rows are whole 16-byte vectors at 16-byte aligned addresses (the stride of a dimension of
+// one element does not matter).
+static bool vector_rows(const nt_attention_args& a, const void* p, const int64_t* s, int64_t heads, int64_t tokens) {
+  const int es = dtype_size(a.dtype);
+  const int64_t sizes[3] = {a.batch, heads, tokens};
+  if (!p) return true;
+  if (!aligned16(p) || a.head_dim * es % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (sizes[i] > 1 && s[i] * es % 16) return false;
+  return true;
+}
+static bool vector_query(const nt_attention_args& a, const void* p, const int64_t* s) {
+  return vector_rows(a, p, s, a.query_heads, a.queries);
+}
+static bool vector_key(const nt_attention_args& a, const void* p, const int64_t* s) {
+  return vector_rows(a, p, s, a.kv_heads, a.keys);
+}
+
+static AttnParams attention_params(const nt_attention_args& a) {
+  AttnParams P{};
+  P.q = a.query; P.k = a.key; P.v = a.value; P.g = a.gradient; P.o = a.output;
+  P.dq = a.grad_query; P.dk = a.grad_key; P.dv = a.grad_value;
+  P.qs = strides(a.query_strides); P.ks = strides(a.key_strides); P.vs = strides(a.value_strides);
+  P.gs = strides(a.gradient_strides); P.os = strides(a.output_strides); P.dqs = strides(a.grad_query_strides);
+  P.dks = strides(a.grad_key_strides); P.dvs = strides(a.grad_value_strides);
+  P.lse = a.lse; P.lengths = a.lengths; P.error = a.error;
+  P.batch = (int)a.batch; P.heads = (int)a.query_heads; P.kv_heads = (int)a.kv_heads;
+  P.group = (int)(a.query_heads / a.kv_heads); P.queries = (int)a.queries; P.keys = (int)a.keys; P.dim = a.head_dim;
+  // Positions stay below 2^31 - 1, so a window or a sink count past that hides or shows the same keys.
+  P.window = (int)(a.window < INT_MAX ? a.window : INT_MAX);
+  P.sinks = a.window == 0 ? 0 : (int)(a.sinks < a.keys ? a.sinks : a.keys);
+  P.offset = (int)a.query_offset;
+  P.scale = a.scale;
+  P.scale_log2 = a.scale * kLog2eF;
+  P.parts = 1;
+  return P;
+}
+
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+size_t nt_attention_workspace_size(const nt_attention_args* args) {
+  if (!args || check_attention(*args, "nt_attention_workspace_size")) return 0;
+  const size_t a = partial_bytes(*args, kRows, kRows), b = partial_bytes(*args, kTcKeyRows, kTcQueryStep);
+  return delta_bytes(*args) + (a > b ? a : b);
+}
+
+int nt_attention_forward(const nt_attention_args* args, void* stream) {
+  nt::TraceRange trace("nt_attention_forward");
+  if (!args) { set_error("nt_attention_forward: args is NULL"); return NT_EINVAL; }
+  const nt_attention_args& a = *args;
+  int rc = check_attention(a, "nt_attention_forward");
+  if (rc) return rc;
+  if (a.batch == 0 || a.queries == 0) return NT_OK;
+  if (!a.query || !a.output || (a.keys > 0 && (!a.key || !a.value))) {
+    set_error("nt_attention_forward: NULL query/key/value/output");
+    return NT_EINVAL;
+  }
+  AttnParams P = attention_params(a);
+  P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
+          vector_key(a, a.value, a.value_strides);
+  cudaStream_t s = as_stream(stream);
+  switch (a.dtype) {
+    case NT_F32: return dispatch_forward<NT_F32>(P, s);
+    case NT_F16: return dispatch_forward<NT_F16>(P, s);
+    default: return dispatch_forward<NT_BF16>(P, s);
+  }
+}
+
+int nt_attention_backward(const nt_attention_args* args, void* stream) {
+  nt::TraceRange trace("nt_attention_backward");
+  if (!args) { set_error("nt_attention_backward: args is NULL"); return NT_EINVAL; }
+  const nt_attention_args& a = *args;
+  int rc = check_attention(a, "nt_attention_backward");
+  if (rc) return rc;
+  if (a.batch == 0 || (a.queries == 0 && a.keys == 0)) return NT_OK;
+  if (a.queries > 0 && (!a.query || !a.output || !a.gradient || !a.grad_query || !a.lse)) {
+    set_error("nt_attention_backward: NULL query/output/gradient/grad_query/lse");
+    return NT_EINVAL;
+  }
+  if (a.keys > 0 && (!a.key || !a.value || !a.grad_key || !a.grad_value)) {
+    set_error("nt_attention_backward: NULL key/value/grad_key/grad_value");
+    return NT_EINVAL;
+  }
+  const size_t need = nt_attention_workspace_size(&a);
+  if (need > 0 && (!a.workspace || a.workspace_bytes < need || !aligned16(a.workspace))) {
+    set_error("nt_attention_backward: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, a.workspace_bytes);
+    return NT_EINVAL;
+  }
+  AttnParams P = attention_params(a);
+  P.delta = static_cast<float*>(a.workspace);
+  P.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + delta_bytes(a));
+  P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
+          vector_key(a, a.value, a.value_strides) && vector_query(a, a.gradient, a.gradient_strides) &&
+          vector_query(a, a.output, a.output_strides);
+  const int64_t window = a.window < a.keys ? a.window : a.keys;
+  P.sink_tiles = (P.sinks + kRows - 1) / kRows;
+  P.parts = P.sink_tiles ? sink_parts(a.queries, window, P.group, kRows, kRows) : 1;
+  cudaStream_t s = as_stream(stream);
+  switch (a.dtype) {
+    case NT_F32: return dispatch_backward<NT_F32>(P, s);
+    case NT_F16: return dispatch_backward<NT_F16>(P, s);
+    default: return dispatch_backward<NT_BF16>(P, s);
+  }
+}
+
+int nt_attention_step(const nt_attention_args* args, void* stream) {
+  nt::TraceRange trace("nt_attention_step");
+  if (!args) { set_error("nt_attention_step: args is NULL"); return NT_EINVAL; }
+  const nt_attention_args& a = *args;
+  int rc = check_attention(a, "nt_attention_step");
+  if (rc) return rc;
+  if (a.queries != 1) { set_error("nt_attention_step: queries must be 1"); return NT_EINVAL; }
+  if (a.batch == 0) return NT_OK;
+  if (!a.query || !a.output || !a.lengths || (a.keys > 0 && (!a.key || !a.value))) {
+    set_error("nt_attention_step: NULL query/key/value/lengths/output");
+    return NT_EINVAL;
+  }
+  AttnParams P = attention_params(a);
+  P.vec = vector_key(a, a.key, a.key_strides) && vector_key(a, a.value, a.value_strides);
+  cudaStream_t s = as_stream(stream);
+  switch (a.dtype) {
+    case NT_F32: return dispatch_step<NT_F32>(P, s);
+    case NT_F16: return dispatch_step<NT_F16>(P, s);
+    default: return dispatch_step<NT_BF16>(P, s);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,84 @@
+// What the attention kernels share: the problem, which keys a query sees, and the ranges of
+// keys (of a block of queries) and of queries (of a block of keys) that hold every visible pair.
+#pragma once
+
+#include "nt_common.cuh"
+
+namespace nt {
+
+// Element strides of the first three dimensions: batch, head, token.
+struct AttnStrides {
+  int64_t b, h, t;
+  __host__ __device__ __forceinline__ int64_t at(int64_t batch, int64_t head, int64_t token) const {
+    return batch * b + head * h + token * t;
+  }
+};
+
+struct AttnParams {
+  const void *q, *k, *v, *g;
+  void *o, *dq, *dk, *dv;
+  AttnStrides qs, ks, vs, gs, os, dqs, dks, dvs;
+  float* lse;        // [batch, heads, queries]
+  float* delta;      // [batch, heads, queries]: sum over head_dim of g * o
+  float* partial;    // backward: partial gradients of the sink key blocks, or NULL
+  const int32_t* lengths;
+  int32_t* error;
+  int batch, heads, kv_heads, group, queries, keys, dim;
+  int window;        // 0: none
+  int sinks;         // 0 without a window
+  int offset;
+  int vec;           // rows are 16-byte aligned runs of whole 16-byte vectors
+  // Backward over key blocks: the first `sink_tiles` blocks hold sinks, which every later query
+  // sees, so their queries are cut into `parts` pieces.
+  int sink_tiles, parts;
+  float scale, scale_log2;
+};
+
+constexpr float kLog2eF = 1.4426950408889634f;
+constexpr float kLn2F = 0.6931471805599453f;
+
+__device__ __forceinline__ int attn_length(const AttnParams& P, int b) {
+  return P.lengths == nullptr ? P.keys : min(max(P.lengths[b], 0), P.keys);
+}
+
+__device__ __forceinline__ bool attn_visible(const AttnParams& P, int length, int p, int j) {
+  return j < length && j <= p && (P.window == 0 || p - j < P.window || j < P.sinks);
+}
+
+// Keys that queries [i0, i1) see: [0, sink_end) and [lo, hi), disjoint. The window's range
+// starts where the first query's window does, not at a multiple of the block.
+struct AttnKeys {
+  int sink_end, lo, hi;
+  __device__ __forceinline__ AttnKeys(const AttnParams& P, int length, int i0, int i1) {
+    hi = min(length, P.offset + i1);
+    lo = P.window == 0 ? 0 : min(hi, max(0, P.offset + i0 - P.window + 1));
+    sink_end = min(P.sinks, hi);
+    if (lo <= sink_end) { lo = 0; sink_end = 0; }
+  }
+  __device__ __forceinline__ int sink_blocks(int width) const { return (sink_end + width - 1) / width; }
+  __device__ __forceinline__ int blocks(int width) const { return sink_blocks(width) + (hi - lo + width - 1) / width; }
+  // First key and end (exclusive) of block j.
+  __device__ __forceinline__ void block(int j, int width, int& begin, int& end) const {
+    const int s = sink_blocks(width);
+    begin = j < s ? j * width : lo + (j - s) * width;
+    end = min(begin + width, j < s ? sink_end : hi);
+  }
+};
+
+// Queries [lo, hi) that see a key of [k0, k1).
+struct AttnQueries {
+  int lo, hi;
+  __device__ __forceinline__ AttnQueries(const AttnParams& P, int length, int k0, int k1) {
+    const int64_t last = P.window == 0 || k0 < P.sinks ? (int64_t)P.queries
+                                                        : (int64_t)k1 - 1 + P.window - P.offset;
+    lo = max(0, k0 - P.offset);
+    hi = (int)(last < P.queries ? last : P.queries);
+    if (k0 >= length || hi < lo) hi = lo;
+  }
+};
+
+// nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
+constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
+constexpr int kTcQueryStep = 64;   // queries it takes at a time
+
+}  // namespace nt

@@ -1,4 +1,5 @@
-"""Fused softmax cross-entropy (namitorch/nn/functional.py:792-863).
+"""Fused softmax cross-entropy (namitorch/nn/functional.py:792-863), sliding-window attention
+with sinks and counter-based dropout.
 
 ``cross_entropy`` keeps the reference signature and validation. One kernel launch
 (``nt_softmax_xent``) reads the logits once and produces both the loss and, when the logits
@@ -7,6 +8,11 @@ it by the incoming gradient (and skips even that when the incoming gradient is e
 float16 / bfloat16 logits are read directly and reduced in float32 — the reference promotes
 them to float32 first (``float32_function``) — and the gradient comes back in the logits'
 dtype. ``softmax_cross_entropy`` exposes the fused forward + backward without autograd.
+
+``sliding_window_attention`` (forward and backward), ``sliding_window_attention_step`` (one
+new token over a cache) and ``dropout`` (with the bias before it and the residual after it;
+its mask is a function of a seed and an offset and is never stored) run in the kernels of
+``backends.attention`` and ``backends.dropout``.
 """
 from __future__ import annotations
 
@@ -182,4 +188,173 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     return torch.nn.functional.linear(input, weight, bias)
 
 
-__all__ = ["cross_entropy", "linear", "softmax_cross_entropy"]
+def _count(name: str, value, low: int = 0) -> int:
+    if isinstance(value, (bool, np.bool_)) or not isinstance(value, Integral):
+        raise TypeError(f"{name} must be an integer.")
+    if value < low:
+        raise ValueError(f"{name} must be at least {low}, got {value}.")
+    return int(value)
+
+
+def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale):
+    for name, tensor, want in (("query", query, rank), ("key", key, 4), ("value", value, 4)):
+        if not isinstance(tensor, torch.Tensor):
+            raise TypeError(f"Attention {name} must be a NamiTorch Tensor.")
+        if tensor.dim() != want:
+            raise ValueError(f"Attention {name} must have rank {want}, got shape {tuple(tensor.shape)}.")
+    batch, heads, dim = query.shape[0], query.shape[1], query.shape[-1]
+    if key.shape != value.shape or key.shape[0] != batch or key.shape[3] != dim:
+        raise ValueError(f"Attention key and value must have shape [{batch}, kv_heads, keys, {dim}], got "
+                         f"{tuple(key.shape)} and {tuple(value.shape)}.")
+    if not 1 <= dim <= N.NT_ATTENTION_MAX_HEAD_DIM:
+        raise ValueError(f"Attention head dimension must be in [1, {N.NT_ATTENTION_MAX_HEAD_DIM}], got {dim}.")
+    if heads < 1 or key.shape[1] < 1 or heads % key.shape[1]:
+        raise ValueError(f"Attention needs a whole number of query heads per key head, got {heads} and {key.shape[1]}.")
+    if query.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"Attention supports float32, float16 and bfloat16 tensors, got {query.dtype}.")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise TypeError(f"Attention query, key and value must have one dtype, got {query.dtype}, {key.dtype} and "
+                        f"{value.dtype}.")
+    if query.device.type != "cuda" or key.device != query.device or value.device != query.device:
+        raise RuntimeError("namitorch_b200 attention runs on one CUDA device; move query, key and value there first.")
+    window = 0 if window is None else _count("window", window, 1)
+    sinks = _count("sinks", sinks)
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError("Attention lengths must be an int32 or int64 Tensor or None.")
+        if tuple(lengths.shape) != (batch,):
+            raise ValueError(f"Attention lengths must have shape {(batch,)}, got {tuple(lengths.shape)}.")
+        if lengths.device != query.device:
+            raise RuntimeError("Attention lengths must be on the device of the query.")
+        if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+            lengths = lengths.clamp(0, key.shape[2]).to(torch.int32).contiguous()
+    if scale is None:
+        scale = dim ** -0.5
+    else:
+        if isinstance(scale, (bool, np.bool_)) or not isinstance(scale, Real):
+            raise TypeError("Attention scale must be a real scalar or None.")
+        scale = float(scale)
+        if not 0 < scale <= float(np.finfo(np.float32).max):
+            raise ValueError("Attention scale must be positive and finite in float32.")
+    return window, sinks, lengths, scale
+
+
+class _SlidingWindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, value, lengths, options):
+        from ..backends import get_backend
+        output, lse = get_backend(query).attention.forward(query, key, value, lengths, save_lse=True, **options)
+        ctx.save_for_backward(query, key, value, output, lse, lengths)
+        ctx.options = options
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        from ..backends import get_backend
+        query, key, value, output, lse, lengths = ctx.saved_tensors
+        grads = get_backend(query).attention.backward(query, key, value, output, lse, grad_output, lengths,
+                                                      **ctx.options)
+        return (*grads, None, None)
+
+
+def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: int | None = None,
+                             sinks: int = 0, lengths: torch.Tensor | None = None, query_position_offset: int = 0,
+                             scale: float | None = None) -> torch.Tensor:
+    """Causal attention limited to the last ``window`` positions and the first ``sinks`` ones.
+
+    ``query`` is [batch, heads, queries, head_dim], ``key`` and ``value`` [batch, kv_heads,
+    keys, head_dim], with heads a multiple of kv_heads (query head h reads key head
+    h // (heads // kv_heads)), head_dim at most 128 and any strides. Query i stands at position
+    p = query_position_offset + i and sees key j when ``j < lengths[b]``, ``j <= p`` and
+    ``p - j < window or j < sinks`` (every earlier key without a window). The weights are
+    softmax(scale * query @ key.T) over the keys it sees, ``scale`` 1 / sqrt(head_dim) by
+    default; a query that sees none gives zeros. What ``key`` and ``value`` hold at or past
+    ``lengths[b]`` (an integer tensor [batch], clamped to the keys) has no effect; a NaN or an
+    infinity that some query sees can reach other queries of its block of 128.
+
+    Differentiable in query, key and value; sums run in float32 in a fixed order."""
+    window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
+    options = {"window": window, "sinks": sinks, "query_offset": _count("query_position_offset", query_position_offset),
+               "scale": scale}
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        return _SlidingWindowAttention.apply(query, key, value, lengths, options)
+    from ..backends import get_backend
+    return get_backend(query).attention.forward(query, key, value, lengths, save_lse=False, **options)[0]
+
+
+def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                  lengths: torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                                  scale: float | None = None) -> torch.Tensor:
+    """``sliding_window_attention`` for one new token per sequence over a cache.
+
+    ``query`` is [batch, heads, head_dim], the caches [batch, kv_heads, capacity, head_dim].
+    Sequence b holds ``lengths[b]`` keys, the new token's among them, and its query stands at
+    the last of them. Reads the keys and values it sees and nothing else of the cache."""
+    if lengths is None:
+        raise TypeError("Attention lengths must be an int32 or int64 Tensor.")
+    window, sinks, lengths, scale = _attention_arguments(query, key_cache, value_cache, 3, window, sinks, lengths, scale)
+    from ..backends import get_backend
+    return get_backend(query).attention.step(query, key_cache, value_cache, lengths, window=window, sinks=sinks,
+                                             scale=scale)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, bias, residual, p, seed, offset):
+        from ..backends import get_backend
+        ctx.call = (p, seed, offset)
+        return get_backend(input).dropout.forward(input, p, seed=seed, offset=offset, bias=bias, residual=residual)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        from ..backends import get_backend
+        p, seed, offset = ctx.call
+        need_input, need_bias, need_residual = ctx.needs_input_grad[:3]
+        grad_input, grad_bias = get_backend(grad_output).dropout.backward(
+            grad_output, p, seed=seed, offset=offset, needs=(need_input, need_bias))
+        return grad_input, grad_bias, grad_output if need_residual else None, None, None, None
+
+
+def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: torch.Tensor | None = None,
+            residual: torch.Tensor | None = None, training: bool = True) -> torch.Tensor:
+    """``residual + keep * (input + bias) / (1 - p)``, each element kept with probability 1 - p.
+
+    Element e of ``input`` in row-major order is dropped when word e % 4 of Philox4x32-7 at the
+    counter (e // 4, ``offset``) under the key ``seed`` (both in [0, 2^64)) is below p * 2^32: the
+    mask depends on (seed, offset, e) alone, is computed again by the backward and never stored.
+    Use another offset for every call that needs a mask of its own. ``bias`` has the shape
+    [width] of the last dimension, ``residual`` that of ``input``. With ``training=False``
+    nothing is dropped."""
+    if not isinstance(input, torch.Tensor):
+        raise TypeError("dropout input must be a NamiTorch Tensor.")
+    if input.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"dropout supports float32, float16 and bfloat16 tensors, got {input.dtype}.")
+    if input.dim() < 1:
+        raise ValueError("dropout input must have rank >= 1.")
+    if isinstance(p, (bool, np.bool_)) or not isinstance(p, Real):
+        raise TypeError("dropout probability must be a real scalar.")
+    if not 0 <= p < 1:
+        raise ValueError("dropout probability must be in [0, 1).")
+    for name, value in (("seed", seed), ("offset", offset)):
+        if _count(f"dropout {name}", value) >= 1 << 64:
+            raise ValueError(f"dropout {name} must be below 2^64.")
+    if type(training) is not bool:
+        raise TypeError("training must be a Python bool.")
+    for name, tensor, shape in (("bias", bias, input.shape[-1:]), ("residual", residual, input.shape)):
+        if tensor is None:
+            continue
+        if not isinstance(tensor, torch.Tensor):
+            raise TypeError(f"dropout {name} must be a NamiTorch Tensor or None.")
+        if tensor.shape != shape:
+            raise ValueError(f"dropout {name} must have shape {tuple(shape)}, got {tuple(tensor.shape)}.")
+        if tensor.dtype != input.dtype:
+            raise TypeError(f"dropout {name} must have the dtype of the input, got {tensor.dtype} and {input.dtype}.")
+        if tensor.device != input.device:
+            raise RuntimeError(f"dropout {name} must be on the device of the input.")
+    if input.device.type != "cuda":
+        raise RuntimeError("namitorch_b200 dropout runs on a CUDA device; move the input there first.")
+    return _Dropout.apply(input, bias, residual, float(p) if training else 0.0, int(seed), int(offset))
+
+
+__all__ = ["cross_entropy", "dropout", "linear", "sliding_window_attention", "sliding_window_attention_step",
+           "softmax_cross_entropy"]
