@@ -448,6 +448,9 @@ typedef struct nt_attention_args {
   int32_t reserved;
   void* output;              /* forward: written; backward: read */
   int64_t output_strides[3];
+  void* output_low;          /* 16-bit types: what the rounding of output took away, in its type and
+                                strides. Written by the forward (NULL: not saved); the backward's
+                                row sums of gradient * output use it when given */
   float* lse;                /* [batch, query_heads, queries] log-sum-exp of a row's scaled scores:
                                 written by the forward (NULL: not saved), read by the backward */
   const void* gradient;      /* backward: of the output */

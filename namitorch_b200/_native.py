@@ -136,7 +136,7 @@ class AttentionArgs(C.Structure):
                 ("key", C.c_void_p), ("value", C.c_void_p), ("query_strides", _Strides), ("key_strides", _Strides),
                 ("value_strides", _Strides), ("lengths", C.c_void_p), ("window", C.c_int64), ("sinks", C.c_int64),
                 ("query_offset", C.c_int64), ("scale", C.c_float), ("reserved", C.c_int32), ("output", C.c_void_p),
-                ("output_strides", _Strides), ("lse", C.c_void_p), ("gradient", C.c_void_p),
+                ("output_strides", _Strides), ("output_low", C.c_void_p), ("lse", C.c_void_p), ("gradient", C.c_void_p),
                 ("grad_query", C.c_void_p), ("grad_key", C.c_void_p), ("grad_value", C.c_void_p),
                 ("gradient_strides", _Strides), ("grad_query_strides", _Strides), ("grad_key_strides", _Strides),
                 ("grad_value_strides", _Strides), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),

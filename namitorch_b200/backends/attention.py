@@ -16,8 +16,19 @@ from .. import _native as N
 
 
 def _rows(tensor):
-    """The tensor itself when its last dimension is dense, else a contiguous copy."""
-    return tensor if tensor.stride(-1) == 1 or tensor.shape[-1] <= 1 else tensor.contiguous()
+    """The tensor itself when the kernels take its layout, else a contiguous copy: a dense last
+    dimension, no broadcast dimension, and 16-byte aligned rows where the width allows them (a
+    tile copy needs them)."""
+    size = tensor.element_size()
+    if tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
+        return tensor.contiguous()
+    aligned = tensor.shape[-1] * size % 16 == 0
+    if aligned and tensor.data_ptr() % 16:
+        return tensor.clone(memory_format=torch.contiguous_format)
+    for extent, stride in zip(tensor.shape[:-1], tensor.stride()[:-1]):
+        if extent > 1 and (stride == 0 or (aligned and stride * size % 16)):
+            return tensor.contiguous()
+    return tensor
 
 
 def _heads_last(batch, heads, tokens, dim, like):
@@ -40,7 +51,7 @@ class AttentionCUDAKernels:
         if self._error is not None and int(self._error.item()):
             raise RuntimeError("A wait inside an attention kernel ran out; the results of that call are incomplete.")
 
-    def _args(self, query, key, value, lengths, window, sinks, query_offset, scale, output, lse):
+    def _args(self, query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse):
         batch, heads, queries, dim = query.shape
         return N.AttentionArgs(
             dtype=N.dtype_code(query.dtype), head_dim=dim, batch=batch, query_heads=heads, kv_heads=key.shape[1],
@@ -48,20 +59,25 @@ class AttentionCUDAKernels:
             query_strides=query.stride()[:3], key_strides=key.stride()[:3], value_strides=value.stride()[:3],
             lengths=None if lengths is None else lengths.data_ptr(), window=window, sinks=sinks,
             query_offset=query_offset, scale=scale, output=output.data_ptr(), output_strides=output.stride()[:3],
-            lse=None if lse is None else lse.data_ptr(), error=self._error_word(query.device).data_ptr())
+            output_low=None if low is None else low.data_ptr(), lse=None if lse is None else lse.data_ptr(), error=self._error_word(query.device).data_ptr())
 
-    def forward(self, query, key, value, lengths=None, *, window=0, sinks=0, query_offset=0, scale, save_lse=True):
-        """(output, lse): lse is float32 [batch, heads, queries], None unless ``save_lse``."""
+    def forward(self, query, key, value, lengths=None, *, window=0, sinks=0, query_offset=0, scale, save=True):
+        """(output, low, lse). With ``save``, what the backward needs besides the output: lse, float32
+        [batch, heads, queries], and for 16-bit types ``low``, the part of the output that its
+        rounding took away (the backward subtracts the row sum of gradient * output from dP; over a
+        few keys the two nearly cancel, and the rounded output alone would cost the gradients twice
+        the error of their own rounding)."""
         query, key, value = _rows(query), _rows(key), _rows(value)
         batch, heads, queries, dim = query.shape
         output = _heads_last(batch, heads, queries, dim, query)
-        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=query.device) if save_lse else None
+        low = _heads_last(batch, heads, queries, dim, query) if save and query.dtype != torch.float32 else None
+        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=query.device) if save else None
         with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, lse)
+            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse)
             N.call("nt_attention_forward", N.C.byref(args), N.stream_handle(), launches=int(batch * queries > 0))
-        return output, lse
+        return output, low, lse
 
-    def backward(self, query, key, value, output, lse, gradient, lengths=None, *, window=0, sinks=0, query_offset=0,
+    def backward(self, query, key, value, output, low, lse, gradient, lengths=None, *, window=0, sinks=0, query_offset=0,
                  scale):
         """(grad_query, grad_key, grad_value)."""
         query, key, value, gradient = _rows(query), _rows(key), _rows(value), _rows(gradient)
@@ -71,7 +87,7 @@ class AttentionCUDAKernels:
         dk = _heads_last(batch, kv_heads, keys, dim, query)
         dv = _heads_last(batch, kv_heads, keys, dim, query)
         with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, lse)
+            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse)
             args.gradient, args.gradient_strides = gradient.data_ptr(), gradient.stride()[:3]
             args.grad_query, args.grad_query_strides = dq.data_ptr(), dq.stride()[:3]
             args.grad_key, args.grad_key_strides = dk.data_ptr(), dk.stride()[:3]
@@ -90,7 +106,7 @@ class AttentionCUDAKernels:
         batch, heads, _, dim = query.shape
         output = torch.empty((batch, heads, 1, dim), dtype=query.dtype, device=query.device)
         with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, 0, scale, output, None)
+            args = self._args(query, key, value, lengths, window, sinks, 0, scale, output, None, None)
             N.call("nt_attention_step", N.C.byref(args), N.stream_handle(), launches=int(batch > 0))
         return output.squeeze(2)
 

@@ -195,7 +195,17 @@ __global__ void __launch_bounds__(kSimtThreads) attention_forward_kernel(const _
   for (int i = 0; i < 4; ++i) {
     const int row = i0 + 4 * ty + i;
     if (row >= i1) continue;
-    store_row4<DT, DP>(P.o, P.os.at(b, h, row), tx, P.dim, acc[i], l[i] > 0.0f ? 1.0f / l[i] : (l[i] == 0.0f ? 0.0f : l[i]));
+    const float f = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    store_row4<DT, DP>(P.o, P.os.at(b, h, row), tx, P.dim, acc[i], f);
+    if (DT != NT_F32 && P.o_low != nullptr) {
+#pragma unroll
+      for (int u = 0; u < DP / 64; ++u) {
+        float* a = &acc[i][u].x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = a[e] * f - Elem<DT>::to_f32(Elem<DT>::from_f32(a[e] * f));
+      }
+      store_row4<DT, DP>(P.o_low, P.os.at(b, h, row), tx, P.dim, acc[i], 1.0f);
+    }
     if (P.lse != nullptr && tx == 0)
       P.lse[((int64_t)b * P.heads + h) * P.queries + row] = l[i] == 0.0f ? -INFINITY : fmaf(m[i], P.scale, log2f(l[i]) * kLn2F);
   }
@@ -231,6 +241,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     load_tile<DT, DP>(x1, qb + P.qs.at(b, h, 0) * es, P.qs.t, i0, i1, P.dim, P.vec);
     load_tile<DT, DP>(x2, gb + P.gs.at(b, h, 0) * es, P.gs.t, i0, i1, P.dim, P.vec);
     load_tile<DT, DP>(y1, static_cast<const char*>(P.o) + P.os.at(b, h, 0) * es, P.os.t, i0, i1, P.dim, P.vec);
+    const bool low = DT != NT_F32 && P.o_low != nullptr;
+    if (low) load_tile<DT, DP>(y2, static_cast<const char*>(P.o_low) + P.os.at(b, h, 0) * es, P.os.t, i0, i1, P.dim, P.vec);
     __syncthreads();
     const int64_t stat = ((int64_t)b * P.heads + h) * P.queries;
     float lse[4], delta[4];
@@ -238,7 +250,10 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     for (int i = 0; i < 4; ++i) {
       const int r = 4 * ty + i;
       float d = 0.0f;
-      for (int c = tx; c < P.dim; c += 16) d = fmaf(x2[r * (DP + 4) + c], y1[r * (DP + 4) + c], d);
+      for (int c = tx; c < P.dim; c += 16) {
+        const int at = r * (DP + 4) + c;
+        d = fmaf(x2[at], low ? y1[at] + y2[at] : y1[at], d);
+      }
       delta[i] = lanes16_sum(d);
       lse[i] = i0 + r < i1 ? P.lse[stat + i0 + r] * kLog2eF : 0.0f;
       if (tx == 0 && i0 + r < i1) P.delta[stat + i0 + r] = delta[i];
@@ -625,11 +640,15 @@ static int dispatch_forward(const AttnParams& P, cudaStream_t s) {
   return P.dim <= 64 ? launch_forward<DT, 64>(P, s) : launch_forward<DT, 128>(P, s);
 }
 template <int DT>
-static int dispatch_backward(const AttnParams& P, cudaStream_t s) {
-  int rc = P.dim <= 64 ? launch_backward<DT, 64>(P, s) : launch_backward<DT, 128>(P, s);
-  if (rc || P.parts == 1 || P.sink_tiles == 0) return rc;
-  attention_join_kernel<DT><<<(unsigned)(current_sm_count() * 4), 256, 0, s>>>(P, kRows);
+static int launch_join(const AttnParams& P, int tile_rows, cudaStream_t s) {
+  if (P.parts == 1 || P.sink_tiles == 0) return NT_OK;
+  attention_join_kernel<DT><<<(unsigned)(current_sm_count() * 4), 256, 0, s>>>(P, tile_rows);
   return launch_status("nt_attention_backward (join) launch");
+}
+template <int DT>
+static int dispatch_backward(const AttnParams& P, cudaStream_t s) {
+  const int rc = P.dim <= 64 ? launch_backward<DT, 64>(P, s) : launch_backward<DT, 128>(P, s);
+  return rc ? rc : launch_join<DT>(P, kRows, s);
 }
 
 // Pieces of the queries of a sink key block: an ordinary key block sees the queries of its own
@@ -670,6 +689,10 @@ static int check_attention(const nt_attention_args& a, const char* who) {
     set_error("%s: batch and heads must be below 65536, queries and keys below 2^30", who);
     return NT_EINVAL;
   }
+  if ((a.queries + kTcQueryStep - 1) / kTcQueryStep * (a.query_heads / a.kv_heads) > INT_MAX) {
+    set_error("%s: too many queries for one key head", who);
+    return NT_EINVAL;
+  }
   if (a.window < 0 || a.sinks < 0 || a.query_offset < 0 || a.query_offset >= INT_MAX / 2) {
     set_error("%s: window, sinks and query_offset must be nonnegative, query_offset below 2^30", who);
     return NT_EINVAL;
@@ -681,14 +704,14 @@ static int check_attention(const nt_attention_args& a, const char* who) {
 static AttnStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
 // Rows are whole 16-byte vectors at 16-byte aligned addresses (the stride of a dimension of
-// one element does not matter).
+// one element does not matter); strides are those a tiled copy takes.
 static bool vector_rows(const nt_attention_args& a, const void* p, const int64_t* s, int64_t heads, int64_t tokens) {
   const int es = dtype_size(a.dtype);
   const int64_t sizes[3] = {a.batch, heads, tokens};
   if (!p) return true;
   if (!aligned16(p) || a.head_dim * es % 16) return false;
   for (int i = 0; i < 3; ++i)
-    if (sizes[i] > 1 && s[i] * es % 16) return false;
+    if (sizes[i] > 1 && (s[i] * es % 16 || s[i] <= 0 || s[i] > ((int64_t)1 << 38) / es)) return false;
   return true;
 }
 static bool vector_query(const nt_attention_args& a, const void* p, const int64_t* s) {
@@ -705,7 +728,7 @@ static AttnParams attention_params(const nt_attention_args& a) {
   P.qs = strides(a.query_strides); P.ks = strides(a.key_strides); P.vs = strides(a.value_strides);
   P.gs = strides(a.gradient_strides); P.os = strides(a.output_strides); P.dqs = strides(a.grad_query_strides);
   P.dks = strides(a.grad_key_strides); P.dvs = strides(a.grad_value_strides);
-  P.lse = a.lse; P.lengths = a.lengths; P.error = a.error;
+  P.o_low = a.output_low; P.lse = a.lse; P.lengths = a.lengths; P.error = a.error;
   P.batch = (int)a.batch; P.heads = (int)a.query_heads; P.kv_heads = (int)a.kv_heads;
   P.group = (int)(a.query_heads / a.kv_heads); P.queries = (int)a.queries; P.keys = (int)a.keys; P.dim = a.head_dim;
   // Positions stay below 2^31 - 1, so a window or a sink count past that hides or shows the same keys.
@@ -745,6 +768,9 @@ int nt_attention_forward(const nt_attention_args* args, void* stream) {
   P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
           vector_key(a, a.value, a.value_strides);
   cudaStream_t s = as_stream(stream);
+  if (a.dtype != NT_F32 && a.keys > 0 && P.vec && vector_query(a, a.output, a.output_strides) &&
+      vector_query(a, a.output_low, a.output_strides))
+    return attention_tc_forward_launch(P, a.dtype, s);
   switch (a.dtype) {
     case NT_F32: return dispatch_forward<NT_F32>(P, s);
     case NT_F16: return dispatch_forward<NT_F16>(P, s);
@@ -779,9 +805,18 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
           vector_key(a, a.value, a.value_strides) && vector_query(a, a.gradient, a.gradient_strides) &&
           vector_query(a, a.output, a.output_strides);
   const int64_t window = a.window < a.keys ? a.window : a.keys;
-  P.sink_tiles = (P.sinks + kRows - 1) / kRows;
-  P.parts = P.sink_tiles ? sink_parts(a.queries, window, P.group, kRows, kRows) : 1;
+  const bool tc = a.dtype != NT_F32 && a.keys > 0 && a.queries > 0 && P.vec &&
+                  vector_query(a, a.output_low, a.output_strides) && vector_query(a, a.grad_query, a.grad_query_strides) &&
+                  vector_key(a, a.grad_key, a.grad_key_strides) && vector_key(a, a.grad_value, a.grad_value_strides);
+  const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? kTcQueryStep : kRows;
+  P.sink_tiles = (P.sinks + tile_rows - 1) / tile_rows;
+  P.parts = P.sink_tiles ? sink_parts(a.queries, window, P.group, tile_rows, step_rows) : 1;
   cudaStream_t s = as_stream(stream);
+  if (tc) {
+    rc = attention_tc_backward_launch(P, a.dtype, s);
+    if (rc) return rc;
+    return a.dtype == NT_F16 ? launch_join<NT_F16>(P, tile_rows, s) : launch_join<NT_BF16>(P, tile_rows, s);
+  }
   switch (a.dtype) {
     case NT_F32: return dispatch_backward<NT_F32>(P, s);
     case NT_F16: return dispatch_backward<NT_F16>(P, s);

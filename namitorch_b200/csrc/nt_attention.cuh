@@ -17,6 +17,7 @@ struct AttnStrides {
 struct AttnParams {
   const void *q, *k, *v, *g;
   void *o, *dq, *dk, *dv;
+  void* o_low;       // what rounding took from o, in o's type and strides, or NULL
   AttnStrides qs, ks, vs, gs, os, dqs, dks, dvs;
   float* lse;        // [batch, heads, queries]
   float* delta;      // [batch, heads, queries]: sum over head_dim of g * o
@@ -80,5 +81,7 @@ struct AttnQueries {
 // nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
 constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
 constexpr int kTcQueryStep = 64;   // queries it takes at a time
+int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s);
+int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 
 }  // namespace nt

@@ -1,0 +1,717 @@
+// Sliding-window attention on the fifth-generation tensor cores, for float16 and bfloat16 rows
+// that are whole 16-byte vectors. The mathematics and the masks are those of nt_attention.cu.
+//
+// Forward: a block owns 128 queries of one head and walks its visible keys 128 at a time. One
+// warp copies tiles, one issues the products, eight do the softmax: two threads share a query's
+// row, 64 columns each. S = q k^T accumulates in TMEM; the weights go back to TMEM over S as
+// 16-bit values and are the first operand of o += w v. Two blocks share an SM, so one's products
+// run under the other's exponentials.
+//
+// Backward: two passes of one kernel (see attention_tc_backward), each with S and dP computed
+// again. Sums that cross blocks exist only for the sink keys and are added in order afterwards.
+//
+// Roundings below 32 bits: the weights and dS are rounded to the inputs' type because the second
+// products take their operand in it; every sum, maximum and statistic is float32.
+#include <cmath>
+
+#include "nt_attention.cuh"
+#include "nt_tc.cuh"
+
+namespace nt {
+
+constexpr int kTcRows = 128;
+constexpr int kTcThreads = 320;        // 8 computing warps, 1 copying, 1 issuing products
+constexpr int kCopyWarp = 8, kMmaWarp = 9;
+constexpr uint32_t kFwdColumns = 256;  // TMEM: S (and the weights over it) 128, output up to 128
+constexpr float kRescaleLog2 = 8.0f;
+
+// A wait of a whole warp, which goes on or gives up as one.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity));
+}
+
+template <int DP> struct FwdShared {
+  static constexpr int kTile = kTcRows * DP * 2;
+  static constexpr int kBytes = 3 * kTile + 1024;
+};
+
+// Which of the columns of a tile row r sees: c < end and (c >= begin or c < sink).
+struct ColumnMask {
+  int begin, end, sink;
+  __device__ __forceinline__ bool operator()(int c) const { return c < end && (c >= begin || c < sink); }
+};
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(kTcThreads, 2)
+attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t q_full, k_full, k_free, v_full, v_free, s_full, w_full, o_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ float exchange[2][2][kTcRows];
+  constexpr int TILE = FwdShared<DP>::kTile;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  uint8_t* aligned = raw + (base - smem_u32(raw));
+  const uint32_t sq = base, sk = base + TILE, sv = base + 2 * TILE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, h = blockIdx.y, hk = h / P.group;
+  const int i0 = (gridDim.x - 1 - blockIdx.x) * kTcRows, i1 = min(P.queries, i0 + kTcRows);
+  const int length = attn_length(P, b);
+  const AttnKeys range(P, length, i0, i1);
+  const int blocks = range.blocks(kTcRows);
+
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kFwdColumns);
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1); mbar_init(&k_full, 1); mbar_init(&k_free, 1); mbar_init(&v_full, 1); mbar_init(&v_free, 1);
+    mbar_init(&s_full, 1); mbar_init(&w_full, 256); mbar_init(&o_full, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t t_s = tmem, t_o = tmem + kTcRows;
+  bool ok = true;
+
+  if (warp == kCopyWarp) {
+    if (lane == 0 && blocks > 0) {
+      auto load = [&](const CUtensorMap* map, int offset, int token, int head, uint64_t* bar) {
+        mbar_arrive_expect_tx(bar, TILE);
+#pragma unroll
+        for (int half = 0; half < DP / 64; ++half)
+          tma_load(aligned + offset + half * kTcRows * 128, map, half * 64, token, head, b, bar);
+      };
+      load(&map_q, 0, i0, h, &q_full);
+      int issued = 0;
+      for (int j = 0; j < blocks && ok; ++j) {
+        int begin, end;
+        range.block(j, kTcRows, begin, end);
+        if (j > 0) ok = wait_bar(&k_free, (j - 1) & 1);
+        if (!ok) break;
+        load(&map_k, TILE, begin, hk, &k_full);
+        if (j > 0) ok = wait_bar(&v_free, (j - 1) & 1);
+        if (!ok) { wait_bar(&k_full, j & 1); break; }
+        load(&map_v, 2 * TILE, begin, hk, &v_full);
+        issued = j + 1;
+      }
+      if (!ok) {   // the copies in flight land before the block may end
+        wait_bar(&q_full, 0);
+        if (issued > 0) { wait_bar(&k_full, (issued - 1) & 1); wait_bar(&v_full, (issued - 1) & 1); }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const int width16 = (P.dim + 15) / 16;
+    const uint32_t pv = tc_instruction<DT>(width16 * 16, true);
+    if (blocks > 0) ok = wait_warp(&q_full, 0);
+    for (int j = 0; j < blocks && ok; ++j) {
+      int begin, end;
+      range.block(j, kTcRows, begin, end);
+      const int keys16 = (end - begin + 15) / 16;
+      ok = wait_warp(&k_full, j & 1);
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t qk = tc_instruction<DT>(keys16 * 16, false);
+        for (int s = 0; s < width16; ++s) tc_mma(t_s, tc_columns(sq, kTcRows, s), tc_columns(sk, kTcRows, s), qk, s > 0);
+        tc_commit(&s_full);
+        tc_commit(&k_free);
+      }
+      __syncwarp();
+      ok = wait_warp(&v_full, j & 1);
+      if (!ok) break;
+      // Rows between the last visible key and the end of its group of 16 have weight 0 but may
+      // hold anything: 0 * NaN must not reach the sum.
+      const int tail = keys16 * 16 - (end - begin);
+      if (tail > 0) {
+        for (int i = lane; i < tail * (DP / 8); i += 32) {
+          const int row = end - begin + i / (DP / 8), c = i % (DP / 8);
+          *reinterpret_cast<uint4*>(aligned + 2 * TILE + (c / 8) * kTcRows * 128 + row * 128 + (c % 8) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
+      ok = wait_warp(&w_full, j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        for (int s = 0; s < keys16; ++s) tc_mma_tmem(t_o, t_s + s * 8, tc_rows(sv, kTcRows, s), pv, j > 0 || s > 0);
+        tc_commit(&v_free);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) tc_commit(&o_full);
+    __syncwarp();
+    if (!ok) wait_bar(&o_full, 0);   // no product is in flight when TMEM is given back
+  } else {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // lane 32 (w % 4) in the address's upper half
+    const int p = P.offset + i0 + row;
+    const int p_first = P.offset + i0, p_last = P.offset + i1 - 1;
+    const int sinks = range.sink_blocks(kTcRows);
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < blocks; ++j) {
+      int begin, end;
+      range.block(j, kTcRows, begin, end);
+      // A wait that ran out is remembered and not waited for again; the warp still takes part in
+      // every barrier, so that no other warp is left waiting for it.
+      if (ok) ok = wait_bar(&s_full, j & 1);
+      __syncwarp();
+      tc_fence_after();
+      float s[64];
+      tmem_load32(t_s + lanes + half * 64, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+      tmem_load32(t_s + lanes + half * 64 + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+      tmem_wait_load();
+      const bool full = end - begin == kTcRows && end - 1 <= p_first &&
+                        (P.window == 0 || j < sinks || p_last - begin < P.window);
+      if (!full) {
+        const ColumnMask mask{P.window == 0 ? 0 : p - P.window + 1 - begin - half * 64, min(end, p + 1) - begin - half * 64,
+                              P.sinks - begin - half * 64};
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[c] = mask(c) ? s[c] : -INFINITY;
+      }
+      float top = s[0], top1 = s[1];
+#pragma unroll
+      for (int c = 2; c < 64; c += 2) {
+        top = fmaxf(top, s[c]);
+        top1 = fmaxf(top1, s[c + 1]);
+      }
+      top = fmaxf(top, top1);
+      exchange[j & 1][half][row] = top;
+      named_barrier(1 + (warp & 3), 64);
+      top = fmaxf(top, exchange[j & 1][half ^ 1][row]);
+      // The maximum only has to keep the weights in range, so the old one stays until the new is
+      // 2^8 above it: the output is then rescaled for a few of the first tiles of a row only.
+      const bool raise = top > m && !((top - m) * P.scale_log2 <= kRescaleLog2);
+      if (__any_sync(0xffffffffu, raise)) {
+        const float f = raise ? ex2_approx((m - top) * P.scale_log2) : 1.0f;
+        if (raise) m = top;
+        l *= f;
+        if (j > 0) {
+          // Products complete in order: S of this tile is there, so o of the last one is too.
+#pragma unroll
+          for (int c = 0; c < DP / 2; c += 32) {
+            uint32_t o[32];
+            tmem_load32(t_o + lanes + half * (DP / 2) + c, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_store32(t_o + lanes + half * (DP / 2) + c, o);
+          }
+        }
+      }
+      float shift = m == -INFINITY ? 0.0f : m;
+      if (__any_sync(0xffffffffu, isinf(shift * P.scale_log2))) {
+        // Scores near the ends of float32: subtract before scaling.
+#pragma unroll
+        for (int c = 0; c < 64; ++c) s[c] -= shift;
+        shift = 0.0f;
+      }
+      const float minus = -shift * P.scale_log2;
+      float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = ex2_approx(fmaf(s[c + 2 * e], P.scale_log2, minus));
+          const float y = ex2_approx(fmaf(s[c + 2 * e + 1], P.scale_log2, minus));
+          sum0 += x;
+          sum1 += y;
+          w[e] = pack2<DT>(x, y);
+        }
+        tmem_store16(t_s + lanes + half * 32 + c / 2, w);
+      }
+      l += sum0 + sum1;
+      tmem_wait_store();
+      tc_fence_before();
+      mbar_arrive(&w_full);
+    }
+    if (ok && blocks > 0) ok = wait_bar(&o_full, 0);
+    __syncwarp();
+    tc_fence_after();
+    exchange[blocks & 1][half][row] = l;
+    named_barrier(1 + (warp & 3), 64);
+    // Halves in a fixed order, so that both threads of a row have the same sum.
+    l = exchange[blocks & 1][0][row] + exchange[blocks & 1][1][row];
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool live = i0 + row < i1;
+    uint16_t* out = static_cast<uint16_t*>(P.o) + P.os.at(b, h, i0 + row) + half * (DP / 2);
+    uint16_t* low = P.o_low == nullptr ? nullptr
+                                       : static_cast<uint16_t*>(P.o_low) + P.os.at(b, h, i0 + row) + half * (DP / 2);
+#pragma unroll
+    for (int c = 0; c < DP / 2; c += 32) {
+      uint32_t o[32];
+      if (blocks > 0) {
+        tmem_load32(t_o + lanes + half * (DP / 2) + c, o);
+        tmem_wait_load();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        if (!live || half * (DP / 2) + c + e >= P.dim) continue;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // A row without keys is 0 whatever the accumulator holds.
+          const float x = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k]) * f;
+          const float y = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k + 1]) * f;
+          hi[k] = pack2<DT>(x, y);
+          const float2 r = unpack2<DT>(hi[k]);
+          lo[k] = pack2<DT>(x - r.x, y - r.y);
+        }
+        *reinterpret_cast<uint4*>(out + c + e) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (low != nullptr) *reinterpret_cast<uint4*>(low + c + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    if (live && half == 0 && P.lse != nullptr)
+      P.lse[((int64_t)b * P.heads + h) * P.queries + i0 + row] =
+          l == 0.0f ? -INFINITY : fmaf(m, P.scale, log2f(l) * kLn2F);
+  }
+  if (!ok && P.error != nullptr) atomicOr(P.error, 1);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_free(tmem, kFwdColumns);
+}
+
+// ---- backward ------------------------------------------------------------------------
+// One block keeps 128 rows x1, x2 and walks 64 rows y1, y2 at a time:
+//   s = x1 y1^T, dp = x2 y2^T (TMEM, float32);  P = exp(scale s - lse), dS = P (dp - delta)
+//   out1 += dS y1, and with DKV out2 += P y2, with P and dS over s and dp in TMEM as the
+//   products' first operand.
+// DKV = false: rows are queries (x1 = q, x2 = g; y1 = k, y2 = v): out1 = dq; delta = sum(g o) is
+// computed on the way in and stored. DKV = true: rows are keys (x1 = k, x2 = v; y1 = q, y2 = g):
+// out1 = dk, out2 = dv, over the heads of the group.
+// s and dp have two buffers: while one group of four warps computes the weights of a step the
+// tensor cores form the next step's s and dp for the other group.
+constexpr int kStep = kTcQueryStep;
+constexpr uint32_t kBwdColumns = 512;
+
+template <int DP> struct BwdShared {
+  static constexpr int kKeep = kTcRows * DP * 2;      // x1 or x2
+  static constexpr int kStream = kStep * DP * 2;      // y1 or y2
+  static constexpr int kStages = 4;
+  static constexpr int kBytes = 2 * kKeep + kStages * 2 * kStream + 1024;
+};
+
+template <int DT, int DP, bool DKV>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_x1,
+                      const __grid_constant__ CUtensorMap map_x2, const __grid_constant__ CUtensorMap map_y1,
+                      const __grid_constant__ CUtensorMap map_y2) {
+  using Shape = BwdShared<DP>;
+  constexpr int STAGES = Shape::kStages;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t x_full, y_full[STAGES], y_free[STAGES], s_full[2], w_full[2], out_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float stats[2][2][2][kStep];   // group, parity of its step, lse / delta, column
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  uint8_t* aligned = raw + (base - smem_u32(raw));
+  constexpr int STREAM0 = 2 * Shape::kKeep;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z;
+  const int length = attn_length(P, b);
+
+  // The block's rows [r0, r1) and the steps it walks.
+  int r0, r1, part = 0, parts = 1, tile = 0, steps, per_head = 1;
+  uint32_t from = 0;
+  if constexpr (!DKV) {
+    r0 = (gridDim.x - 1 - blockIdx.x) * kTcRows;
+    r1 = min(P.queries, r0 + kTcRows);
+  } else {
+    const int split = P.sink_tiles * P.parts;
+    tile = (int)blockIdx.x < split ? (int)blockIdx.x / P.parts : (int)blockIdx.x - split + P.sink_tiles;
+    part = (int)blockIdx.x < split ? (int)blockIdx.x % P.parts : 0;
+    parts = (int)blockIdx.x < split ? P.parts : 1;
+    r0 = tile * kTcRows;
+    r1 = min(P.keys, r0 + kTcRows);
+  }
+  const AttnKeys key_range(P, length, r0, r1);
+  const AttnQueries query_range(P, length, r0, r1);
+  if constexpr (!DKV) {
+    steps = key_range.blocks(kStep);
+  } else {
+    per_head = (query_range.hi - query_range.lo + kStep - 1) / kStep;
+    const int64_t total = (int64_t)per_head * P.group;   // below 2^31, checked on the host
+    from = (uint32_t)(total * part / parts);
+    steps = (int)(total * (part + 1) / parts - from);
+  }
+  const int h0 = blockIdx.y;   // query head of dq, key head of dk and dv
+  auto step_rows = [&](int t, int& begin, int& end, int& head) {
+    if constexpr (!DKV) {
+      key_range.block(t, kStep, begin, end);
+      head = h0 / P.group;
+    } else {
+      const uint32_t n = from + t;
+      head = h0 * P.group + (int)(n / (uint32_t)per_head);
+      begin = query_range.lo + (int)(n % (uint32_t)per_head) * kStep;
+      end = min(query_range.hi, begin + kStep);
+    }
+  };
+
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kBwdColumns);
+  if (threadIdx.x == 0) {
+    mbar_init(&x_full, 1); mbar_init(&out_full, 1);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&y_full[i], 1); mbar_init(&y_free[i], 1); }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&w_full[i], 128); }
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // Columns: s 2 x 64, dp 2 x 64, out1, out2.
+  const uint32_t t_s = tmem, t_dp = tmem + 2 * kStep, t_out1 = tmem + 4 * kStep, t_out2 = t_out1 + DP;
+  bool ok = true;
+
+  if (warp == kCopyWarp) {
+    if (lane == 0 && steps > 0) {
+      mbar_arrive_expect_tx(&x_full, 2 * Shape::kKeep);
+#pragma unroll
+      for (int half = 0; half < DP / 64; ++half) {
+        tma_load(aligned + half * kTcRows * 128, &map_x1, half * 64, r0, h0, b, &x_full);
+        tma_load(aligned + Shape::kKeep + half * kTcRows * 128, &map_x2, half * 64, r0, h0, b, &x_full);
+      }
+      int t = 0;
+      for (; t < steps; ++t) {
+        const int stage = t % STAGES;
+        if (t >= STAGES) ok = wait_bar(&y_free[stage], (t / STAGES - 1) & 1);
+        if (!ok) break;
+        int begin, end, head;
+        step_rows(t, begin, end, head);
+        uint8_t* dst = aligned + STREAM0 + stage * 2 * Shape::kStream;
+        mbar_arrive_expect_tx(&y_full[stage], 2 * Shape::kStream);
+#pragma unroll
+        for (int half = 0; half < DP / 64; ++half) {
+          tma_load(dst + half * kStep * 128, &map_y1, half * 64, begin, head, b, &y_full[stage]);
+          tma_load(dst + Shape::kStream + half * kStep * 128, &map_y2, half * 64, begin, head, b, &y_full[stage]);
+        }
+      }
+      if (!ok) {   // the copies in flight land before the block may end
+        wait_bar(&x_full, 0);
+        for (int i = t > STAGES ? t - STAGES : 0; i < t; ++i) wait_bar(&y_full[i % STAGES], (i / STAGES) & 1);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const int width16 = (P.dim + 15) / 16;
+    const uint32_t accumulate = tc_instruction<DT>(width16 * 16, true);
+    if (steps > 0) ok = wait_warp(&x_full, 0);
+    for (int t = 0; t <= steps && ok; ++t) {
+      if (t < steps) {   // s and dp of step t
+        const int stage = t % STAGES;
+        int begin, end, head;
+        step_rows(t, begin, end, head);
+        const int rows16 = (end - begin + 15) / 16, tail = rows16 * 16 - (end - begin);
+        ok = wait_warp(&y_full[stage], (t / STAGES) & 1);
+        if (!ok) break;
+        const int at = STREAM0 + stage * 2 * Shape::kStream;
+        if (tail > 0) {   // weight 0, contents unknown: see the forward
+          for (int i = lane; i < tail * (DP / 8); i += 32) {
+            const int row = end - begin + i / (DP / 8), c = i % (DP / 8);
+            uint8_t* dst = aligned + at + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dst + Shape::kStream) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          const uint32_t product = tc_instruction<DT>(rows16 * 16, false);
+          const uint32_t s = t_s + (t & 1) * kStep, dp = t_dp + (t & 1) * kStep;
+          for (int k = 0; k < width16; ++k)
+            tc_mma(s, tc_columns(base, kTcRows, k), tc_columns(base + at, kStep, k), product, k > 0);
+          for (int k = 0; k < width16; ++k)
+            tc_mma(dp, tc_columns(base + Shape::kKeep, kTcRows, k), tc_columns(base + at + Shape::kStream, kStep, k), product,
+                   k > 0);
+          tc_commit(&s_full[t & 1]);
+        }
+        __syncwarp();
+      }
+      if (t > 0) {       // the sums of step t - 1
+        const int u = t - 1, stage = u % STAGES;
+        int begin, end, head;
+        step_rows(u, begin, end, head);
+        const int rows16 = (end - begin + 15) / 16;
+        ok = wait_warp(&w_full[u & 1], (u >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t at = base + STREAM0 + stage * 2 * Shape::kStream;
+          const uint32_t p = t_s + (u & 1) * kStep, ds = t_dp + (u & 1) * kStep;
+          if constexpr (DKV)
+            for (int k = 0; k < rows16; ++k)
+              tc_mma_tmem(t_out2, p + k * 8, tc_rows(at + Shape::kStream, kStep, k), accumulate, u > 0 || k > 0);
+          for (int k = 0; k < rows16; ++k)
+            tc_mma_tmem(t_out1, ds + k * 8, tc_rows(at, kStep, k), accumulate, u > 0 || k > 0);
+          tc_commit(&y_free[stage]);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) tc_commit(&out_full);
+    __syncwarp();
+    if (!ok) wait_bar(&out_full, 0);
+  } else {
+    const int group = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    float lse = 0.0f, delta = 0.0f;
+    if constexpr (!DKV) {
+      // delta of the row: each of its two threads sums half of the columns.
+      const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0 + row;
+      const bool live = r0 + row < r1;
+      float d = 0.0f;
+      if (live) {
+        const uint16_t* g = static_cast<const uint16_t*>(P.g) + P.gs.at(b, h0, r0 + row);
+        const uint16_t* o = static_cast<const uint16_t*>(P.o) + P.os.at(b, h0, r0 + row);
+        const uint16_t* low = P.o_low == nullptr ? nullptr : static_cast<const uint16_t*>(P.o_low) + P.os.at(b, h0, r0 + row);
+#pragma unroll
+        for (int c = 0; c < DP / 2; c += 8) {
+          const int at = group * (DP / 2) + c;
+          if (at >= P.dim) break;
+          float x[8], y[8], z[8];
+          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g + at)), x);
+          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(o + at)), y);
+          if (low != nullptr) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(low + at)), z);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d = fmaf(x[e], low != nullptr ? y[e] + z[e] : y[e], d);
+        }
+        lse = P.lse[stat] * kLog2eF;
+      }
+      float* halves = &stats[0][0][0][0];
+      halves[group * kTcRows + row] = d;
+      named_barrier(1, 256);
+      delta = halves[row] + halves[kTcRows + row];
+      if (live && group == 0) P.delta[stat] = delta;
+    }
+    // DKV: lse and delta belong to the columns; a thread fetches one of them ahead of its step.
+    float ahead = 0.0f;
+    auto fetch = [&](int t) {
+      if constexpr (DKV) {
+        const int tid = threadIdx.x & 127, c = tid & 63;
+        int begin, end, head;
+        step_rows(t, begin, end, head);
+        const int64_t stat = ((int64_t)b * P.heads + head) * P.queries + begin + c;
+        ahead = begin + c < end ? (tid < 64 ? P.lse[stat] * kLog2eF : P.delta[stat]) : 0.0f;
+      }
+    };
+    if (group < steps) fetch(group);
+    const int p_first = P.offset + r0, p_last = P.offset + r1 - 1;
+    for (int t = group; t < steps; t += 2) {
+      int begin, end, head;
+      step_rows(t, begin, end, head);
+      ColumnMask mask;
+      bool full;
+      if constexpr (!DKV) {
+        const int p = P.offset + r0 + row;
+        mask = {P.window == 0 ? 0 : p - P.window + 1 - begin, min(end, p + 1) - begin, P.sinks - begin};
+        full = end - begin == kStep && end - 1 <= p_first &&
+               (P.window == 0 || end <= P.sinks || p_last - begin < P.window);
+      } else {
+        stats[group][(t >> 1) & 1][(threadIdx.x & 127) >> 6][threadIdx.x & 63] = ahead;
+        named_barrier(1 + group, 128);
+        if (t + 2 < steps) fetch(t + 2);
+        const int key = r0 + row, first = P.offset + begin;
+        const bool all = P.window == 0 || key < P.sinks;
+        // (a window is at most 2^31 - 1 and positions stay below it, hence the 64-bit sum)
+        const int64_t last = all ? (int64_t)kStep : (int64_t)key + P.window - first;
+        mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
+        full = end - begin == kStep && r0 + kTcRows <= length && r0 + kTcRows - 1 <= first &&
+               (P.window == 0 || r0 + kTcRows <= P.sinks || P.offset + end - 1 - r0 < P.window);
+      }
+      if (ok) ok = wait_bar(&s_full[t & 1], (t >> 1) & 1);   // as in the forward
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < kStep; c0 += 32) {
+        float s[32], dp[32];
+        tmem_load32(t_s + lanes + group * kStep + c0, reinterpret_cast<uint32_t(&)[32]>(s));
+        tmem_load32(t_dp + lanes + group * kStep + c0, reinterpret_cast<uint32_t(&)[32]>(dp));
+        tmem_wait_load();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          float4 row_lse = make_float4(lse, lse, lse, lse), row_delta = make_float4(delta, delta, delta, delta);
+          if constexpr (DKV) {
+            row_lse = *reinterpret_cast<const float4*>(&stats[group][(t >> 1) & 1][0][c0 + c]);
+            row_delta = *reinterpret_cast<const float4*>(&stats[group][(t >> 1) & 1][1][c0 + c]);
+          }
+          const float ls[4] = {row_lse.x, row_lse.y, row_lse.z, row_lse.w};
+          const float de[4] = {row_delta.x, row_delta.y, row_delta.z, row_delta.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = ex2_approx(fmaf(s[c + e], P.scale_log2, -ls[e]));
+            s[c + e] = x;
+            dp[c + e] = x * (dp[c + e] - de[e]);
+          }
+        }
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const bool seen = mask(c0 + c);
+            s[c] = seen ? s[c] : 0.0f;
+            dp[c] = seen ? dp[c] : 0.0f;
+          }
+        }
+        uint32_t w[16];
+        if constexpr (DKV) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(s[2 * e], s[2 * e + 1]);
+          tmem_store16(t_s + lanes + group * kStep + c0 / 2, w);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(dp[2 * e], dp[2 * e + 1]);
+        tmem_store16(t_dp + lanes + group * kStep + c0 / 2, w);
+      }
+      tmem_wait_store();
+      tc_fence_before();
+      mbar_arrive(&w_full[t & 1]);
+    }
+    if (ok && steps > 0) ok = wait_bar(&out_full, 0);
+    __syncwarp();
+    tc_fence_after();
+    // DKV: the first group stores dk, the second dv; else half of dq's columns each.
+    const bool live = r0 + row < r1;
+    constexpr int WIDTH = DKV ? DP : DP / 2;
+    const int c_first = DKV ? 0 : group * WIDTH;
+    const uint32_t t_out = (DKV && group == 1 ? t_out2 : t_out1) + lanes + c_first;
+    const float f = DKV && group == 1 ? 1.0f : P.scale;
+#pragma unroll
+    for (int c = 0; c < WIDTH; c += 32) {
+      uint32_t v[32];
+      if (steps > 0) {
+        tmem_load32(t_out + c, v);
+        tmem_wait_load();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0u;
+      }
+      if (parts == 1) {
+        void* dst = DKV ? (group == 0 ? P.dk : P.dv) : P.dq;
+        const AttnStrides& st = DKV ? (group == 0 ? P.dks : P.dvs) : P.dqs;
+        uint16_t* out = static_cast<uint16_t*>(dst) + st.at(b, h0, r0 + row) + c_first + c;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (!live || c_first + c + e >= P.dim) continue;
+          uint32_t q[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            q[k] = pack2<DT>(__uint_as_float(v[e + 2 * k]) * f, __uint_as_float(v[e + 2 * k + 1]) * f);
+          *reinterpret_cast<uint4*>(out + e) = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+      } else {
+        // [batch, key head, sink block, part, 2, 128, dim]
+        float* out = P.partial + (((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + group) *
+                                     kTcRows * P.dim + (int64_t)row * P.dim + c;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          if (c + e >= P.dim) continue;
+          *reinterpret_cast<float4*>(out + e) =
+              make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f,
+                          __uint_as_float(v[e + 3]) * f);
+        }
+      }
+    }
+  }
+  if (!ok && P.error != nullptr) atomicOr(P.error, 1);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) tmem_free(tmem, kBwdColumns);
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// (column, token, head, batch) of one tensor, boxes of 64 columns x `rows` tokens, zeros outside.
+static int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st, int dim, int tokens, int heads,
+                    int batch, int rows, const char* who) {
+  EncodeTiled encode = encode_tiled();
+  if (!encode) { set_error("%s: the driver has no cuTensorMapEncodeTiled", who); return NT_ECUDA; }
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
+  // The stride of a dimension of one element is never used, but has to be a valid one.
+  const cuuint64_t row_bytes = ((cuuint64_t)dim * 2 + 15) / 16 * 16;
+  const cuuint64_t strides[3] = {tokens > 1 ? (cuuint64_t)st.t * 2 : row_bytes, heads > 1 ? (cuuint64_t)st.h * 2 : row_bytes,
+                                 batch > 1 ? (cuuint64_t)st.b * 2 : row_bytes};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult rc = encode(map, dtype == NT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                             const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) { set_error("%s: cuTensorMapEncodeTiled failed (%d)", who, (int)rc); return NT_ECUDA; }
+  return NT_OK;
+}
+
+template <typename K>
+static int large_smem(K kernel, int bytes, const char* who) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? NT_OK : cuda_fail(e, who);
+}
+
+template <int DT, int DP>
+static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
+  const char* who = "nt_attention_forward";
+  CUtensorMap q, k, v;
+  // A runtime call first: the map encoder is a driver call and needs a context on this thread.
+  int rc = large_smem(attention_tc_forward<DT, DP>, FwdShared<DP>::kBytes, who);
+  if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
+  if (rc) return rc;
+  const dim3 grid((P.queries + kTcRows - 1) / kTcRows, P.heads, P.batch);
+  attention_tc_forward<DT, DP><<<grid, kTcThreads, FwdShared<DP>::kBytes, s>>>(P, q, k, v);
+  return launch_status("nt_attention_forward launch");
+}
+
+template <int DT, int DP>
+static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
+  const char* who = "nt_attention_backward";
+  CUtensorMap keep[4], stream[4];   // q, g, k, v: 128 rows a box to keep, 64 to stream
+  const int bytes = BwdShared<DP>::kBytes;
+  int rc = large_smem(attention_tc_backward<DT, DP, false>, bytes, who);
+  if (!rc) rc = large_smem(attention_tc_backward<DT, DP, true>, bytes, who);
+  for (int i = 0; i < 2 && !rc; ++i) {
+    CUtensorMap* m = i ? stream : keep;
+    const int rows = i ? kStep : kTcRows;
+    rc = make_map(&m[0], DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, rows, who);
+    if (!rc) rc = make_map(&m[1], DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, rows, who);
+    if (!rc) rc = make_map(&m[2], DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, rows, who);
+    if (!rc) rc = make_map(&m[3], DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, rows, who);
+  }
+  if (rc) return rc;
+  attention_tc_backward<DT, DP, false><<<dim3((P.queries + kTcRows - 1) / kTcRows, P.heads, P.batch), kTcThreads, bytes, s>>>(
+      P, keep[0], keep[1], stream[2], stream[3]);
+  rc = launch_status("nt_attention_backward launch");
+  if (rc) return rc;
+  const int tiles = (P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1);
+  attention_tc_backward<DT, DP, true><<<dim3(tiles, P.kv_heads, P.batch), kTcThreads, bytes, s>>>(
+      P, keep[2], keep[3], stream[0], stream[1]);
+  return launch_status("nt_attention_backward launch");
+}
+
+int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s) {
+  if (dtype == NT_BF16) return P.dim <= 64 ? launch_tc_forward<NT_BF16, 64>(P, s) : launch_tc_forward<NT_BF16, 128>(P, s);
+  return P.dim <= 64 ? launch_tc_forward<NT_F16, 64>(P, s) : launch_tc_forward<NT_F16, 128>(P, s);
+}
+
+int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s) {
+  if (dtype == NT_BF16) return P.dim <= 64 ? launch_tc_backward<NT_BF16, 64>(P, s) : launch_tc_backward<NT_BF16, 128>(P, s);
+  return P.dim <= 64 ? launch_tc_backward<NT_F16, 64>(P, s) : launch_tc_backward<NT_F16, 128>(P, s);
+}
+
+}  // namespace nt

@@ -243,16 +243,16 @@ class _SlidingWindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, lengths, options):
         from ..backends import get_backend
-        output, lse = get_backend(query).attention.forward(query, key, value, lengths, save_lse=True, **options)
-        ctx.save_for_backward(query, key, value, output, lse, lengths)
+        output, low, lse = get_backend(query).attention.forward(query, key, value, lengths, **options)
+        ctx.save_for_backward(query, key, value, output, low, lse, lengths)
         ctx.options = options
         return output
 
     @staticmethod
     def backward(ctx, grad_output):
         from ..backends import get_backend
-        query, key, value, output, lse, lengths = ctx.saved_tensors
-        grads = get_backend(query).attention.backward(query, key, value, output, lse, grad_output, lengths,
+        query, key, value, output, low, lse, lengths = ctx.saved_tensors
+        grads = get_backend(query).attention.backward(query, key, value, output, low, lse, grad_output, lengths,
                                                       **ctx.options)
         return (*grads, None, None)
 
@@ -279,7 +279,7 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _SlidingWindowAttention.apply(query, key, value, lengths, options)
     from ..backends import get_backend
-    return get_backend(query).attention.forward(query, key, value, lengths, save_lse=False, **options)[0]
+    return get_backend(query).attention.forward(query, key, value, lengths, save=False, **options)[0]
 
 
 def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,

@@ -18,6 +18,9 @@ the products, t = u for float32):
 * dq: scale max|k| (eps_ds + n u max|dP - delta|) + t |dq| (rows of P sum to 1); dk and dv: the same
   per unit of column sum of P over the queries and the heads of the group.
 
+* float16 weights and dS below its normal range lose up to 2^-25 each: n times that, times the
+  largest factor, per output.
+
 Everything is doubled for the terms of second order.
 """
 from __future__ import annotations
@@ -112,7 +115,7 @@ def tolerances(q, k, v, dtype, g=None, *, window=0, sinks=0, lengths=None, offse
     scores = top(scale * np.abs(q64) @ np.abs(rep(k64)).swapaxes(-1, -2))
     eps_s = (dim + 4) * u * scores
     eps_p = 2 * eps_s + 16 * u
-    out_abs = (eps_p + t + n * u) * top(np.abs(v64))
+    out_abs = (eps_p + t + n * u + n * floor) * top(np.abs(v64))
     t_out = 2 * (out_abs + t * np.abs(out)) + floor
     t_lse = np.full(lse.shape, 2 * (eps_s + 16 * u + 4 * u * (scores + 16)))
     if g is None:
@@ -133,7 +136,8 @@ def tolerances(q, k, v, dtype, g=None, *, window=0, sinks=0, lengths=None, offse
             p, _ = _weights(q64[b, h], k64[b, h // group], seen, scale)
             columns[b, h // group, :, 0] += p.sum(axis=0)
     per = eps_ds + n * u * spread
-    t_dq = 2 * (scale * top(np.abs(k64)) * per + t * np.abs(dq)) + floor
-    t_dk = 2 * (scale * top(np.abs(q64)) * per * columns + t * np.abs(dk)) + floor
-    t_dv = 2 * ((eps_p + t + n * u) * columns * top(np.abs(g64)) + t * np.abs(dv)) + floor
+    lost = n * floor
+    t_dq = 2 * (scale * top(np.abs(k64)) * (per + lost) + t * np.abs(dq)) + floor
+    t_dk = 2 * (scale * top(np.abs(q64)) * (per * columns + lost) + t * np.abs(dk)) + floor
+    t_dv = 2 * (((eps_p + t + n * u) * columns + lost) * top(np.abs(g64)) + t * np.abs(dv)) + floor
     return t_out, t_lse, t_dq, t_dk, t_dv

@@ -52,7 +52,7 @@ def _check(q, k, v, g, dt, lengths=None, offset=0, scale=None, **options):
     forward_only = F.sliding_window_attention(q.detach(), k.detach(), v.detach(), lengths=n,
                                               query_position_offset=offset, scale=scale, **options)
     assert torch.equal(forward_only, out)
-    _, got_lse = get_backend(q).attention.forward(q.detach(), k.detach(), v.detach(), n, query_offset=offset,
+    _, _, got_lse = get_backend(q).attention.forward(q.detach(), k.detach(), v.detach(), n, query_offset=offset,
                                                   window=options.get("window") or 0, sinks=options.get("sinks", 0),
                                                   scale=q.shape[-1] ** -0.5 if scale is None else scale)
     _within(got_lse, lse, t_lse, "lse")
