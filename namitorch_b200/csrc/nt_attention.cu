@@ -693,6 +693,11 @@ static int check_attention(const nt_attention_args& a, const char* who) {
     set_error("%s: too many queries for one key head", who);
     return NT_EINVAL;
   }
+  if (a.batch * a.query_heads * ((a.queries + kRows - 1) / kRows + 1) > INT_MAX ||
+      a.batch * a.kv_heads * (((a.keys > a.queries ? a.keys : a.queries) + kRows - 1) / kRows + 1) > INT_MAX) {
+    set_error("%s: too many blocks of queries or keys", who);
+    return NT_EINVAL;
+  }
   if (a.window < 0 || a.sinks < 0 || a.query_offset < 0 || a.query_offset >= INT_MAX / 2) {
     set_error("%s: window, sinks and query_offset must be nonnegative, query_offset below 2^30", who);
     return NT_EINVAL;

@@ -80,7 +80,7 @@ struct AttnQueries {
 
 // nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
 constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
-constexpr int kTcQueryStep = 64;   // queries it takes at a time
+constexpr int kTcQueryStep = 128;   // queries it takes at a time
 int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 

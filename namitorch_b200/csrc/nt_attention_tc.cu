@@ -35,10 +35,16 @@ template <int DP> struct FwdShared {
   static constexpr int kBytes = 3 * kTile + 1024;
 };
 
-// Which of the columns of a tile row r sees: c < end and (c >= begin or c < sink).
+// Which columns of a tile a row sees: c < end and (c >= begin or c < sink). word(c0) has bit e set
+// for column c0 + e, so that a masked tile costs one bit test and one select per element.
 struct ColumnMask {
   int begin, end, sink;
-  __device__ __forceinline__ bool operator()(int c) const { return c < end && (c >= begin || c < sink); }
+  static __device__ __forceinline__ uint32_t below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+  }
+  __device__ __forceinline__ uint32_t word(int c0) const {
+    return below(end - c0) & (~below(begin - c0) | below(sink - c0));
+  }
 };
 
 template <int DT, int DP>
@@ -53,9 +59,11 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   uint8_t* aligned = raw + (base - smem_u32(raw));
   const uint32_t sq = base, sk = base + TILE, sv = base + 2 * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z, h = blockIdx.y, hk = h / P.group;
-  const int i0 = (gridDim.x - 1 - blockIdx.x) * kTcRows, i1 = min(P.queries, i0 + kTcRows);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // Blocks in the order of their work: the last queries of every head first.
+  const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / pairs;
+  const int b = blockIdx.x % pairs / P.heads, h = blockIdx.x % P.heads, hk = h / P.group;
+  const int i0 = (tiles - 1 - blockIdx.x / pairs) * kTcRows, i1 = min(P.queries, i0 + kTcRows);
   const int length = attn_length(P, b);
   const AttnKeys range(P, length, i0, i1);
   const int blocks = range.blocks(kTcRows);
@@ -63,7 +71,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kFwdColumns);
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1); mbar_init(&k_full, 1); mbar_init(&k_free, 1); mbar_init(&v_full, 1); mbar_init(&v_free, 1);
-    mbar_init(&s_full, 1); mbar_init(&w_full, 256); mbar_init(&o_full, 1);
+    mbar_init(&s_full, 1); mbar_init(&w_full, 8); mbar_init(&o_full, 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -102,6 +110,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   } else if (warp == kMmaWarp) {
     const int width16 = (P.dim + 15) / 16;
     const uint32_t pv = tc_instruction<DT>(width16 * 16, true);
+    const uint64_t dq = tc_columns(sq), dk = tc_columns(sk), dv = tc_rows(sv, kTcRows);
     if (blocks > 0) ok = wait_warp(&q_full, 0);
     for (int j = 0; j < blocks && ok; ++j) {
       int begin, end;
@@ -109,9 +118,11 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       const int keys16 = (end - begin + 15) / 16;
       ok = wait_warp(&k_full, j & 1);
       if (!ok) break;
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t qk = tc_instruction<DT>(keys16 * 16, false);
-        for (int s = 0; s < width16; ++s) tc_mma(t_s, tc_columns(sq, kTcRows, s), tc_columns(sk, kTcRows, s), qk, s > 0);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s)
+          if (s < width16) tc_mma(t_s, dq + tc_column_step(kTcRows, s), dk + tc_column_step(kTcRows, s), qk, s > 0);
         tc_commit(&s_full);
         tc_commit(&k_free);
       }
@@ -133,13 +144,15 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       ok = wait_warp(&w_full, j & 1);
       if (!ok) break;
       tc_fence_after();
-      if (lane == 0) {
-        for (int s = 0; s < keys16; ++s) tc_mma_tmem(t_o, t_s + s * 8, tc_rows(sv, kTcRows, s), pv, j > 0 || s > 0);
+      if (elect_one()) {
+#pragma unroll
+        for (int s = 0; s < kTcRows / 16; ++s)
+          if (s < keys16) tc_mma_tmem(t_o, t_s + s * 8, dv + tc_row_step(s), pv, j > 0 || s > 0);
         tc_commit(&v_free);
       }
       __syncwarp();
     }
-    if (lane == 0) tc_commit(&o_full);
+    if (elect_one()) tc_commit(&o_full);
     __syncwarp();
     if (!ok) wait_bar(&o_full, 0);   // no product is in flight when TMEM is given back
   } else {
@@ -157,17 +170,27 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       if (ok) ok = wait_bar(&s_full, j & 1);
       __syncwarp();
       tc_fence_after();
-      float s[64];
-      tmem_load32(t_s + lanes + half * 64, reinterpret_cast<uint32_t(&)[32]>(s[0]));
-      tmem_load32(t_s + lanes + half * 64 + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+      uint32_t r0[32], r1[32];
+      tmem_load32(t_s + lanes + half * 64, r0);
+      tmem_load32(t_s + lanes + half * 64 + 32, r1);
       tmem_wait_load();
+      float s[64];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        s[c] = __uint_as_float(r0[c]);
+        s[32 + c] = __uint_as_float(r1[c]);
+      }
       const bool full = end - begin == kTcRows && end - 1 <= p_first &&
                         (P.window == 0 || j < sinks || p_last - begin < P.window);
       if (!full) {
         const ColumnMask mask{P.window == 0 ? 0 : p - P.window + 1 - begin - half * 64, min(end, p + 1) - begin - half * 64,
                               P.sinks - begin - half * 64};
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] = mask(c) ? s[c] : -INFINITY;
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          const uint32_t seen = mask.word(c0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[c0 + c] = seen >> c & 1 ? s[c0 + c] : -INFINITY;
+        }
       }
       float top = s[0], top1 = s[1];
 #pragma unroll
@@ -224,7 +247,8 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       l += sum0 + sum1;
       tmem_wait_store();
       tc_fence_before();
-      mbar_arrive(&w_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_full);
     }
     if (ok && blocks > 0) ok = wait_bar(&o_full, 0);
     __syncwarp();
@@ -276,54 +300,56 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 }
 
 // ---- backward ------------------------------------------------------------------------
-// One block keeps 128 rows x1, x2 and walks 64 rows y1, y2 at a time:
+// One block keeps 128 rows x1, x2 and walks rows y1, y2 128 at a time:
 //   s = x1 y1^T, dp = x2 y2^T (TMEM, float32);  P = exp(scale s - lse), dS = P (dp - delta)
 //   out1 += dS y1, and with DKV out2 += P y2, with P and dS over s and dp in TMEM as the
 //   products' first operand.
 // DKV = false: rows are queries (x1 = q, x2 = g; y1 = k, y2 = v): out1 = dq; delta = sum(g o) is
 // computed on the way in and stored. DKV = true: rows are keys (x1 = k, x2 = v; y1 = q, y2 = g):
 // out1 = dk, out2 = dv, over the heads of the group.
-// s and dp have two buffers: while one group of four warps computes the weights of a step the
-// tensor cores form the next step's s and dp for the other group.
+// s, dp and the two outputs fill TMEM, so nothing has a second buffer; the order of the products
+// hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1) while
+// dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Two groups of four warps take 64 columns each.
 constexpr int kStep = kTcQueryStep;
 constexpr uint32_t kBwdColumns = 512;
 
 template <int DP> struct BwdShared {
-  static constexpr int kKeep = kTcRows * DP * 2;      // x1 or x2
-  static constexpr int kStream = kStep * DP * 2;      // y1 or y2
-  static constexpr int kStages = 4;
-  static constexpr int kBytes = 2 * kKeep + kStages * 2 * kStream + 1024;
+  static constexpr int kTile = kTcRows * DP * 2;      // x1, x2, y1 or y2
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int kBytes = (2 + 2 * kStages) * kTile + 1024;
 };
+static_assert(kStep == kTcRows, "rows kept and rows streamed have one shape");
 
 template <int DT, int DP, bool DKV>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_x1,
                       const __grid_constant__ CUtensorMap map_x2, const __grid_constant__ CUtensorMap map_y1,
                       const __grid_constant__ CUtensorMap map_y2) {
-  using Shape = BwdShared<DP>;
-  constexpr int STAGES = Shape::kStages;
+  constexpr int TILE = BwdShared<DP>::kTile, STAGES = BwdShared<DP>::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t x_full, y_full[STAGES], y_free[STAGES], s_full[2], w_full[2], out_full;
+  __shared__ uint64_t x_full, y_full[STAGES], y_free[STAGES], s_full, dp_full, p_full, ds_full, out_full;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float stats[2][2][2][kStep];   // group, parity of its step, lse / delta, column
+  __shared__ __align__(16) float stats[2][2][2][64];   // group, parity of its step, lse / delta, column
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   uint8_t* aligned = raw + (base - smem_u32(raw));
-  constexpr int STREAM0 = 2 * Shape::kKeep;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // Blocks in the order of their work: the last queries, or the first keys, of every head first.
+  const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch, tiles = gridDim.x / pairs;
+  const int b = blockIdx.x % pairs / heads, h0 = blockIdx.x % heads;   // query head of dq, key head of dk and dv
+  const int index = blockIdx.x / pairs;
   const int length = attn_length(P, b);
 
   // The block's rows [r0, r1) and the steps it walks.
   int r0, r1, part = 0, parts = 1, tile = 0, steps, per_head = 1;
   uint32_t from = 0;
   if constexpr (!DKV) {
-    r0 = (gridDim.x - 1 - blockIdx.x) * kTcRows;
+    r0 = (tiles - 1 - index) * kTcRows;
     r1 = min(P.queries, r0 + kTcRows);
   } else {
     const int split = P.sink_tiles * P.parts;
-    tile = (int)blockIdx.x < split ? (int)blockIdx.x / P.parts : (int)blockIdx.x - split + P.sink_tiles;
-    part = (int)blockIdx.x < split ? (int)blockIdx.x % P.parts : 0;
-    parts = (int)blockIdx.x < split ? P.parts : 1;
+    tile = index < split ? index / P.parts : index - split + P.sink_tiles;
+    part = index < split ? index % P.parts : 0;
+    parts = index < split ? P.parts : 1;
     r0 = tile * kTcRows;
     r1 = min(P.keys, r0 + kTcRows);
   }
@@ -337,7 +363,6 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     from = (uint32_t)(total * part / parts);
     steps = (int)(total * (part + 1) / parts - from);
   }
-  const int h0 = blockIdx.y;   // query head of dq, key head of dk and dv
   auto step_rows = [&](int t, int& begin, int& end, int& head) {
     if constexpr (!DKV) {
       key_range.block(t, kStep, begin, end);
@@ -355,25 +380,23 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     mbar_init(&x_full, 1); mbar_init(&out_full, 1);
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) { mbar_init(&y_full[i], 1); mbar_init(&y_free[i], 1); }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&w_full[i], 128); }
+    mbar_init(&s_full, 1); mbar_init(&dp_full, 1); mbar_init(&p_full, 8); mbar_init(&ds_full, 8);
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // Columns: s 2 x 64, dp 2 x 64, out1, out2.
-  const uint32_t t_s = tmem, t_dp = tmem + 2 * kStep, t_out1 = tmem + 4 * kStep, t_out2 = t_out1 + DP;
+  const uint32_t t_s = tmem, t_dp = tmem + kStep, t_out1 = tmem + 2 * kStep, t_out2 = t_out1 + DP;
   bool ok = true;
 
   if (warp == kCopyWarp) {
     if (lane == 0 && steps > 0) {
-      mbar_arrive_expect_tx(&x_full, 2 * Shape::kKeep);
+      mbar_arrive_expect_tx(&x_full, 2 * TILE);
 #pragma unroll
       for (int half = 0; half < DP / 64; ++half) {
         tma_load(aligned + half * kTcRows * 128, &map_x1, half * 64, r0, h0, b, &x_full);
-        tma_load(aligned + Shape::kKeep + half * kTcRows * 128, &map_x2, half * 64, r0, h0, b, &x_full);
+        tma_load(aligned + TILE + half * kTcRows * 128, &map_x2, half * 64, r0, h0, b, &x_full);
       }
       int t = 0;
       for (; t < steps; ++t) {
@@ -382,12 +405,12 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         if (!ok) break;
         int begin, end, head;
         step_rows(t, begin, end, head);
-        uint8_t* dst = aligned + STREAM0 + stage * 2 * Shape::kStream;
-        mbar_arrive_expect_tx(&y_full[stage], 2 * Shape::kStream);
+        uint8_t* dst = aligned + (2 + 2 * stage) * TILE;
+        mbar_arrive_expect_tx(&y_full[stage], 2 * TILE);
 #pragma unroll
         for (int half = 0; half < DP / 64; ++half) {
           tma_load(dst + half * kStep * 128, &map_y1, half * 64, begin, head, b, &y_full[stage]);
-          tma_load(dst + Shape::kStream + half * kStep * 128, &map_y2, half * 64, begin, head, b, &y_full[stage]);
+          tma_load(dst + TILE + half * kStep * 128, &map_y2, half * 64, begin, head, b, &y_full[stage]);
         }
       }
       if (!ok) {   // the copies in flight land before the block may end
@@ -398,60 +421,80 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
   } else if (warp == kMmaWarp) {
     const int width16 = (P.dim + 15) / 16;
     const uint32_t accumulate = tc_instruction<DT>(width16 * 16, true);
-    if (steps > 0) ok = wait_warp(&x_full, 0);
-    for (int t = 0; t <= steps && ok; ++t) {
-      if (t < steps) {   // s and dp of step t
-        const int stage = t % STAGES;
-        int begin, end, head;
-        step_rows(t, begin, end, head);
-        const int rows16 = (end - begin + 15) / 16, tail = rows16 * 16 - (end - begin);
-        ok = wait_warp(&y_full[stage], (t / STAGES) & 1);
-        if (!ok) break;
-        const int at = STREAM0 + stage * 2 * Shape::kStream;
-        if (tail > 0) {   // weight 0, contents unknown: see the forward
-          for (int i = lane; i < tail * (DP / 8); i += 32) {
-            const int row = end - begin + i / (DP / 8), c = i % (DP / 8);
-            uint8_t* dst = aligned + at + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(dst + Shape::kStream) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async();
-          __syncwarp();
+    const uint64_t x1 = tc_columns(base), x2 = tc_columns(base + TILE);
+    auto rows_of = [&](int t) {
+      int begin, end, head;
+      step_rows(t, begin, end, head);
+      return end - begin;
+    };
+    // acc = x y^T of one step
+    auto product = [&](uint32_t acc, uint64_t x, uint32_t at, int rows, uint64_t* done) {
+      if (elect_one()) {
+        const uint32_t instruction = tc_instruction<DT>((rows + 15) / 16 * 16, false);
+        const uint64_t y = tc_columns(at);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          if (k < width16) tc_mma(acc, x + tc_column_step(kTcRows, k), y + tc_column_step(kStep, k), instruction, k > 0);
+        tc_commit(done);
+      }
+      __syncwarp();
+    };
+    // acc += w y of one step; w lies in two halves of 64 columns
+    auto sum = [&](uint32_t acc, uint32_t w, uint32_t at, int rows, bool add, uint64_t* done) {
+      if (elect_one()) {
+        const uint64_t y = tc_rows(at, kStep);
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k)
+          if (k * 16 < rows)
+            tc_mma_tmem(acc, w + (k >> 2) * 64 + (k & 3) * 8, y + tc_row_step(k), accumulate, add || k > 0);
+        if (done != nullptr) tc_commit(done);
+      }
+      __syncwarp();
+    };
+    // Waits for the rows of step t and clears those between its end and the end of its group of
+    // 16: their weights are 0, but 0 * NaN must not reach a sum.
+    auto arrive = [&](int t, int rows) {
+      const int stage = t % STAGES;
+      if (!wait_warp(&y_full[stage], (t / STAGES) & 1)) return false;
+      const int tail = (rows + 15) / 16 * 16 - rows;
+      if (tail > 0) {
+        for (int i = lane; i < tail * (DP / 8); i += 32) {
+          const int row = rows + i / (DP / 8), c = i % (DP / 8);
+          uint8_t* dst = aligned + (2 + 2 * stage) * TILE + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + TILE) = make_uint4(0, 0, 0, 0);
         }
-        if (lane == 0) {
-          const uint32_t product = tc_instruction<DT>(rows16 * 16, false);
-          const uint32_t s = t_s + (t & 1) * kStep, dp = t_dp + (t & 1) * kStep;
-          for (int k = 0; k < width16; ++k)
-            tc_mma(s, tc_columns(base, kTcRows, k), tc_columns(base + at, kStep, k), product, k > 0);
-          for (int k = 0; k < width16; ++k)
-            tc_mma(dp, tc_columns(base + Shape::kKeep, kTcRows, k), tc_columns(base + at + Shape::kStream, kStep, k), product,
-                   k > 0);
-          tc_commit(&s_full[t & 1]);
-        }
+        fence_proxy_async();
         __syncwarp();
       }
-      if (t > 0) {       // the sums of step t - 1
-        const int u = t - 1, stage = u % STAGES;
-        int begin, end, head;
-        step_rows(u, begin, end, head);
-        const int rows16 = (end - begin + 15) / 16;
-        ok = wait_warp(&w_full[u & 1], (u >> 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t at = base + STREAM0 + stage * 2 * Shape::kStream;
-          const uint32_t p = t_s + (u & 1) * kStep, ds = t_dp + (u & 1) * kStep;
-          if constexpr (DKV)
-            for (int k = 0; k < rows16; ++k)
-              tc_mma_tmem(t_out2, p + k * 8, tc_rows(at + Shape::kStream, kStep, k), accumulate, u > 0 || k > 0);
-          for (int k = 0; k < rows16; ++k)
-            tc_mma_tmem(t_out1, ds + k * 8, tc_rows(at, kStep, k), accumulate, u > 0 || k > 0);
-          tc_commit(&y_free[stage]);
-        }
-        __syncwarp();
-      }
+      return true;
+    };
+    int rows = 0;
+    if (steps > 0) {
+      rows = rows_of(0);
+      ok = wait_warp(&x_full, 0) && arrive(0, rows);
+      if (ok) product(t_s, x1, base + 2 * TILE, rows, &s_full);
     }
-    if (lane == 0) tc_commit(&out_full);
+    for (int t = 0; t < steps && ok; ++t) {
+      const uint32_t at = base + (2 + 2 * (t % STAGES)) * TILE;
+      product(t_dp, x2, at + TILE, rows, &dp_full);
+      ok = wait_warp(&p_full, t & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if constexpr (DKV) sum(t_out2, t_s, at + TILE, rows, t > 0, nullptr);
+      const int now = rows;
+      if (t + 1 < steps) {
+        rows = rows_of(t + 1);
+        ok = arrive(t + 1, rows);
+        if (!ok) break;
+        product(t_s, x1, base + (2 + 2 * ((t + 1) % STAGES)) * TILE, rows, &s_full);
+      }
+      ok = wait_warp(&ds_full, t & 1);
+      if (!ok) break;
+      tc_fence_after();
+      sum(t_out1, t_dp, at, now, t > 0, &y_free[t % STAGES]);
+    }
+    if (elect_one()) tc_commit(&out_full);
     __syncwarp();
     if (!ok) wait_bar(&out_full, 0);
   } else {
@@ -490,16 +533,16 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     float ahead = 0.0f;
     auto fetch = [&](int t) {
       if constexpr (DKV) {
-        const int tid = threadIdx.x & 127, c = tid & 63;
+        const int tid = threadIdx.x & 127, c = group * 64 + (tid & 63);
         int begin, end, head;
         step_rows(t, begin, end, head);
         const int64_t stat = ((int64_t)b * P.heads + head) * P.queries + begin + c;
         ahead = begin + c < end ? (tid < 64 ? P.lse[stat] * kLog2eF : P.delta[stat]) : 0.0f;
       }
     };
-    if (group < steps) fetch(group);
+    if (steps > 0) fetch(0);
     const int p_first = P.offset + r0, p_last = P.offset + r1 - 1;
-    for (int t = group; t < steps; t += 2) {
+    for (int t = 0; t < steps; ++t) {
       int begin, end, head;
       step_rows(t, begin, end, head);
       ColumnMask mask;
@@ -510,9 +553,9 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         full = end - begin == kStep && end - 1 <= p_first &&
                (P.window == 0 || end <= P.sinks || p_last - begin < P.window);
       } else {
-        stats[group][(t >> 1) & 1][(threadIdx.x & 127) >> 6][threadIdx.x & 63] = ahead;
+        stats[group][t & 1][(threadIdx.x & 127) >> 6][threadIdx.x & 63] = ahead;
         named_barrier(1 + group, 128);
-        if (t + 2 < steps) fetch(t + 2);
+        if (t + 1 < steps) fetch(t + 1);
         const int key = r0 + row, first = P.offset + begin;
         const bool all = P.window == 0 || key < P.sinks;
         // (a window is at most 2^31 - 1 and positions stay below it, hence the 64-bit sum)
@@ -521,52 +564,90 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         full = end - begin == kStep && r0 + kTcRows <= length && r0 + kTcRows - 1 <= first &&
                (P.window == 0 || r0 + kTcRows <= P.sinks || P.offset + end - 1 - r0 < P.window);
       }
-      if (ok) ok = wait_bar(&s_full[t & 1], (t >> 1) & 1);   // as in the forward
+      // A wait that ran out is remembered and not waited for again (as in the forward).
+      if (ok) ok = wait_bar(&s_full, t & 1);
       __syncwarp();
       tc_fence_after();
+      float p[64];
+      {
+        uint32_t s0[32], s1[32];
+        tmem_load32(t_s + lanes + group * 64, s0);
+        tmem_load32(t_s + lanes + group * 64 + 32, s1);
+        tmem_wait_load();
+        if constexpr (!DKV) {   // s may be overwritten
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full);
+        }
 #pragma unroll
-      for (int c0 = 0; c0 < kStep; c0 += 32) {
-        float s[32], dp[32];
-        tmem_load32(t_s + lanes + group * kStep + c0, reinterpret_cast<uint32_t(&)[32]>(s));
-        tmem_load32(t_dp + lanes + group * kStep + c0, reinterpret_cast<uint32_t(&)[32]>(dp));
+        for (int c = 0; c < 32; ++c) {
+          p[c] = __uint_as_float(s0[c]);
+          p[32 + c] = __uint_as_float(s1[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        float4 ls = make_float4(lse, lse, lse, lse);
+        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&stats[group][t & 1][0][c]);
+        p[c] = ex2_approx(fmaf(p[c], P.scale_log2, -ls.x));
+        p[c + 1] = ex2_approx(fmaf(p[c + 1], P.scale_log2, -ls.y));
+        p[c + 2] = ex2_approx(fmaf(p[c + 2], P.scale_log2, -ls.z));
+        p[c + 3] = ex2_approx(fmaf(p[c + 3], P.scale_log2, -ls.w));
+      }
+      if (!full) {
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          const uint32_t seen = mask.word(group * 64 + c0);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) p[c0 + c] = seen >> c & 1 ? p[c0 + c] : 0.0f;
+        }
+      }
+      if constexpr (DKV) {
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(p[c0 + 2 * e], p[c0 + 2 * e + 1]);
+          tmem_store16(t_s + lanes + group * 64 + c0 / 2, w);
+        }
+        tmem_wait_store();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full);
+      }
+      if (ok) ok = wait_bar(&dp_full, t & 1);
+      __syncwarp();
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t d[32];
+        tmem_load32(t_dp + lanes + group * 64 + c0, d);
         tmem_wait_load();
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          float4 row_lse = make_float4(lse, lse, lse, lse), row_delta = make_float4(delta, delta, delta, delta);
-          if constexpr (DKV) {
-            row_lse = *reinterpret_cast<const float4*>(&stats[group][(t >> 1) & 1][0][c0 + c]);
-            row_delta = *reinterpret_cast<const float4*>(&stats[group][(t >> 1) & 1][1][c0 + c]);
-          }
-          const float ls[4] = {row_lse.x, row_lse.y, row_lse.z, row_lse.w};
-          const float de[4] = {row_delta.x, row_delta.y, row_delta.z, row_delta.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = ex2_approx(fmaf(s[c + e], P.scale_log2, -ls[e]));
-            s[c + e] = x;
-            dp[c + e] = x * (dp[c + e] - de[e]);
-          }
+          float4 de = make_float4(delta, delta, delta, delta);
+          if constexpr (DKV) de = *reinterpret_cast<const float4*>(&stats[group][t & 1][1][c0 + c]);
+          // Where P is 0 the key may be one that is not there, and dp anything.
+          const float a = p[c0 + c] * (__uint_as_float(d[c]) - de.x), e = p[c0 + c + 1] * (__uint_as_float(d[c + 1]) - de.y);
+          const float f = p[c0 + c + 2] * (__uint_as_float(d[c + 2]) - de.z),
+                      g = p[c0 + c + 3] * (__uint_as_float(d[c + 3]) - de.w);
+          w[(c0 + c) / 2] = pack2<DT>(a, e);
+          w[(c0 + c) / 2 + 1] = pack2<DT>(f, g);
         }
         if (!full) {
+          // Packed pairs of weight 0: 0 * NaN of a key that is not there is cleared as well.
+          const uint32_t seen = mask.word(group * 64 + c0);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const bool seen = mask(c0 + c);
-            s[c] = seen ? s[c] : 0.0f;
-            dp[c] = seen ? dp[c] : 0.0f;
-          }
+          for (int c = 0; c < 32; c += 2)
+            w[(c0 + c) / 2] &= (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u);
         }
-        uint32_t w[16];
-        if constexpr (DKV) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(s[2 * e], s[2 * e + 1]);
-          tmem_store16(t_s + lanes + group * kStep + c0 / 2, w);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(dp[2 * e], dp[2 * e + 1]);
-        tmem_store16(t_dp + lanes + group * kStep + c0 / 2, w);
       }
+      tmem_store32(t_dp + lanes + group * 64, w);
       tmem_wait_store();
       tc_fence_before();
-      mbar_arrive(&w_full[t & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_full);
     }
     if (ok && steps > 0) ok = wait_bar(&out_full, 0);
     __syncwarp();
@@ -673,7 +754,7 @@ static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
-  const dim3 grid((P.queries + kTcRows - 1) / kTcRows, P.heads, P.batch);
+  const unsigned grid = (unsigned)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
   attention_tc_forward<DT, DP><<<grid, kTcThreads, FwdShared<DP>::kBytes, s>>>(P, q, k, v);
   return launch_status("nt_attention_forward launch");
 }
@@ -681,26 +762,21 @@ static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
 template <int DT, int DP>
 static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   const char* who = "nt_attention_backward";
-  CUtensorMap keep[4], stream[4];   // q, g, k, v: 128 rows a box to keep, 64 to stream
+  CUtensorMap q, g, k, v;
   const int bytes = BwdShared<DP>::kBytes;
   int rc = large_smem(attention_tc_backward<DT, DP, false>, bytes, who);
   if (!rc) rc = large_smem(attention_tc_backward<DT, DP, true>, bytes, who);
-  for (int i = 0; i < 2 && !rc; ++i) {
-    CUtensorMap* m = i ? stream : keep;
-    const int rows = i ? kStep : kTcRows;
-    rc = make_map(&m[0], DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, rows, who);
-    if (!rc) rc = make_map(&m[1], DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, rows, who);
-    if (!rc) rc = make_map(&m[2], DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, rows, who);
-    if (!rc) rc = make_map(&m[3], DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, rows, who);
-  }
+  if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&g, DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
-  attention_tc_backward<DT, DP, false><<<dim3((P.queries + kTcRows - 1) / kTcRows, P.heads, P.batch), kTcThreads, bytes, s>>>(
-      P, keep[0], keep[1], stream[2], stream[3]);
+  const unsigned rows = (unsigned)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
+  attention_tc_backward<DT, DP, false><<<rows, kTcThreads, bytes, s>>>(P, q, g, k, v);
   rc = launch_status("nt_attention_backward launch");
   if (rc) return rc;
   const int tiles = (P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1);
-  attention_tc_backward<DT, DP, true><<<dim3(tiles, P.kv_heads, P.batch), kTcThreads, bytes, s>>>(
-      P, keep[2], keep[3], stream[0], stream[1]);
+  attention_tc_backward<DT, DP, true><<<(unsigned)tiles * P.kv_heads * P.batch, kTcThreads, bytes, s>>>(P, k, v, q, g);
   return launch_status("nt_attention_backward launch");
 }
 

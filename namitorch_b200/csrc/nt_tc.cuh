@@ -16,11 +16,16 @@
 
 namespace nt {
 
-// A wait that stays in the hardware's own suspended state on its first try and watches the
-// clock only after that.
+// A wait bounded by the SM's cycle counter: the waits between warps are a few hundred cycles, and
+// a read of %globaltimer costs as much (wait_stage of nt_bulk.cuh).
+constexpr long long kWaitLimitCycles = 4000000000ll;   // about 2 s
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
-  return wait_stage(bar, parity);
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - t0 > kWaitLimitCycles) return false;
+  }
+  return true;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -94,13 +99,22 @@ __device__ __forceinline__ uint64_t tc_descriptor(uint32_t addr, uint32_t leadin
   return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
-// 16 columns from `step` of a tile of `rows` rows, read along the columns.
-__device__ __forceinline__ uint64_t tc_columns(uint32_t tile, int rows, int step) {
-  return tc_descriptor(tile + (step >> 2) * rows * 128 + (step & 3) * 32, 16, 1024);
+// A tile of `rows` rows read along its columns, and what 16-column step k adds to its address.
+__device__ __forceinline__ uint64_t tc_columns(uint32_t tile) { return tc_descriptor(tile, 16, 1024); }
+__device__ __forceinline__ constexpr uint64_t tc_column_step(int rows, int k) {
+  return (uint64_t)(((k >> 2) * rows * 128 + (k & 3) * 32) >> 4);
 }
-// 16 rows from `step` of a tile of `rows` rows, read along the rows.
-__device__ __forceinline__ uint64_t tc_rows(uint32_t tile, int rows, int step) {
-  return tc_descriptor(tile + step * 2048, rows * 128, 1024);
+// The same read along its rows; 16-row step k.
+__device__ __forceinline__ uint64_t tc_rows(uint32_t tile, int rows) { return tc_descriptor(tile, rows * 128, 1024); }
+__device__ __forceinline__ constexpr uint64_t tc_row_step(int k) { return (uint64_t)(k * 2048 >> 4); }
+
+// True in one lane of the (whole, converged) warp. The compiler takes code under it as one
+// thread's, so the operands of the matrix instructions stay in uniform registers: under an
+// ordinary lane test each instruction took about 100 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(chosen));
+  return chosen != 0;
 }
 
 // float32 accumulator of 128 rows and n columns (a multiple of 16); a and b are both float16 or
