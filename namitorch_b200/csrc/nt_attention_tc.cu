@@ -313,25 +313,40 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 constexpr int kStep = kTcQueryStep;
 constexpr uint32_t kBwdColumns = 512;
 
+constexpr int kBwdThreads = 352;       // 8 computing warps, 1 copying, 1 issuing products, 1 for lse and delta
+constexpr int kStatWarp = 10;
+
+// Shared memory: x1, x2, the ring of y1 (three: s of the next step starts before out1 of this one
+// has ended), the ring of y2 (two) and the control block.
 template <int DP> struct BwdShared {
-  static constexpr int kTile = kTcRows * DP * 2;      // x1, x2, y1 or y2
-  static constexpr int kStages = DP == 64 ? 4 : 2;
-  static constexpr int kBytes = (2 + 2 * kStages) * kTile + 1024;
+  static constexpr int kTile = kTcRows * DP * 2;
+  static constexpr int kRing1 = 3, kRing2 = 2;
+  static constexpr int kY1 = 2 * kTile, kY2 = (2 + kRing1) * kTile, kControl = (2 + kRing1 + kRing2) * kTile;
+  struct Control {
+    float stats[2][2][kStep];          // ring of two; lse (times log2 e), delta
+    uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, dp_full, p_full, ds_full,
+        stat_full[2], stat_free[2], out_full;
+    uint32_t tmem;
+  };
+  static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
 static_assert(kStep == kTcRows, "rows kept and rows streamed have one shape");
+static_assert(BwdShared<128>::kBytes <= 227 * 1024, "one block per SM");
+
+// Phase of slot use n of a ring of `size`.
+__device__ __forceinline__ uint32_t ring_phase(int n, int size) { return (uint32_t)(n / size) & 1u; }
 
 template <int DT, int DP, bool DKV>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_x1,
                       const __grid_constant__ CUtensorMap map_x2, const __grid_constant__ CUtensorMap map_y1,
                       const __grid_constant__ CUtensorMap map_y2) {
-  constexpr int TILE = BwdShared<DP>::kTile, STAGES = BwdShared<DP>::kStages;
-  extern __shared__ uint8_t raw[];
-  __shared__ uint64_t x_full, y_full[STAGES], y_free[STAGES], s_full, dp_full, p_full, ds_full, out_full;
-  __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float stats[2][2][2][64];   // group, parity of its step, lse / delta, column
-  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  uint8_t* aligned = raw + (base - smem_u32(raw));
+  using Shape = BwdShared<DP>;
+  constexpr int TILE = Shape::kTile, RING1 = Shape::kRing1, RING2 = Shape::kRing2;
+  // No static shared memory: the dynamic block starts where shared memory does, 1024 bytes in.
+  extern __shared__ __align__(1024) uint8_t aligned[];
+  typename Shape::Control& ctl = *reinterpret_cast<typename Shape::Control*>(aligned + Shape::kControl);
+  const uint32_t base = smem_u32(aligned);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Blocks in the order of their work: the last queries, or the first keys, of every head first.
   const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch, tiles = gridDim.x / pairs;
@@ -363,75 +378,121 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     from = (uint32_t)(total * part / parts);
     steps = (int)(total * (part + 1) / parts - from);
   }
-  auto step_rows = [&](int t, int& begin, int& end, int& head) {
-    if constexpr (!DKV) {
-      key_range.block(t, kStep, begin, end);
-      head = h0 / P.group;
+  // Rows [begin, end) of `head` that step t streams; for the gradients of keys, counted on.
+  struct Step {
+    int begin, end, head, at;
+  };
+  auto start = [&](Step& s) {
+    if constexpr (DKV) {
+      s.head = h0 * P.group + (int)(from / (uint32_t)max(per_head, 1));
+      s.at = (int)(from % (uint32_t)max(per_head, 1));
+      s.begin = query_range.lo + s.at * kStep;
+      s.end = min(query_range.hi, s.begin + kStep);
     } else {
-      const uint32_t n = from + t;
-      head = h0 * P.group + (int)(n / (uint32_t)per_head);
-      begin = query_range.lo + (int)(n % (uint32_t)per_head) * kStep;
-      end = min(query_range.hi, begin + kStep);
+      s.head = h0 / P.group;
+      s.at = 0;
+      key_range.block(0, kStep, s.begin, s.end);
+    }
+  };
+  auto advance = [&](Step& s) {
+    ++s.at;
+    if constexpr (DKV) {
+      if (s.at == per_head) {
+        s.at = 0;
+        ++s.head;
+      }
+      s.begin = query_range.lo + s.at * kStep;
+      s.end = min(query_range.hi, s.begin + kStep);
+    } else {
+      key_range.block(s.at, kStep, s.begin, s.end);
     }
   };
 
-  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kBwdColumns);
+  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kBwdColumns);
   if (threadIdx.x == 0) {
-    mbar_init(&x_full, 1); mbar_init(&out_full, 1);
+    mbar_init(&ctl.x_full, 1); mbar_init(&ctl.out_full, 1);
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i) { mbar_init(&y_full[i], 1); mbar_init(&y_free[i], 1); }
-    mbar_init(&s_full, 1); mbar_init(&dp_full, 1); mbar_init(&p_full, 8); mbar_init(&ds_full, 8);
+    for (int i = 0; i < RING1; ++i) { mbar_init(&ctl.y1_full[i], 1); mbar_init(&ctl.y1_free[i], 1); }
+#pragma unroll
+    for (int i = 0; i < RING2; ++i) {
+      mbar_init(&ctl.y2_full[i], 1); mbar_init(&ctl.y2_free[i], 1);
+      mbar_init(&ctl.stat_full[i], 1); mbar_init(&ctl.stat_free[i], 8);
+    }
+    mbar_init(&ctl.s_full, 1); mbar_init(&ctl.dp_full, 1); mbar_init(&ctl.p_full, 8); mbar_init(&ctl.ds_full, 8);
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = ctl.tmem;
   const uint32_t t_s = tmem, t_dp = tmem + kStep, t_out1 = tmem + 2 * kStep, t_out2 = t_out1 + DP;
   bool ok = true;
 
   if (warp == kCopyWarp) {
     if (lane == 0 && steps > 0) {
-      mbar_arrive_expect_tx(&x_full, 2 * TILE);
+      auto load = [&](const CUtensorMap* map, int at, int token, int head, uint64_t* bar) {
 #pragma unroll
-      for (int half = 0; half < DP / 64; ++half) {
-        tma_load(aligned + half * kTcRows * 128, &map_x1, half * 64, r0, h0, b, &x_full);
-        tma_load(aligned + TILE + half * kTcRows * 128, &map_x2, half * 64, r0, h0, b, &x_full);
-      }
-      int t = 0;
-      for (; t < steps; ++t) {
-        const int stage = t % STAGES;
-        if (t >= STAGES) ok = wait_bar(&y_free[stage], (t / STAGES - 1) & 1);
+        for (int half = 0; half < DP / 64; ++half)
+          tma_load(aligned + at + half * kTcRows * 128, map, half * 64, token, head, b, bar);
+      };
+      mbar_arrive_expect_tx(&ctl.x_full, 2 * TILE);
+      load(&map_x1, 0, r0, h0, &ctl.x_full);
+      load(&map_x2, TILE, r0, h0, &ctl.x_full);
+      Step s;
+      start(s);
+      int n1 = 0, n2 = 0;
+      for (int t = 0; t < steps; ++t, advance(s)) {
+        if (t >= RING1) ok = wait_bar(&ctl.y1_free[t % RING1], ring_phase(t - RING1, RING1));
         if (!ok) break;
-        int begin, end, head;
-        step_rows(t, begin, end, head);
-        uint8_t* dst = aligned + (2 + 2 * stage) * TILE;
-        mbar_arrive_expect_tx(&y_full[stage], 2 * TILE);
-#pragma unroll
-        for (int half = 0; half < DP / 64; ++half) {
-          tma_load(dst + half * kStep * 128, &map_y1, half * 64, begin, head, b, &y_full[stage]);
-          tma_load(dst + TILE + half * kStep * 128, &map_y2, half * 64, begin, head, b, &y_full[stage]);
-        }
+        mbar_arrive_expect_tx(&ctl.y1_full[t % RING1], TILE);
+        load(&map_y1, Shape::kY1 + t % RING1 * TILE, s.begin, s.head, &ctl.y1_full[t % RING1]);
+        n1 = t + 1;
+        if (t >= RING2) ok = wait_bar(&ctl.y2_free[t % RING2], ring_phase(t - RING2, RING2));
+        if (!ok) break;
+        mbar_arrive_expect_tx(&ctl.y2_full[t % RING2], TILE);
+        load(&map_y2, Shape::kY2 + t % RING2 * TILE, s.begin, s.head, &ctl.y2_full[t % RING2]);
+        n2 = t + 1;
       }
       if (!ok) {   // the copies in flight land before the block may end
-        wait_bar(&x_full, 0);
-        for (int i = t > STAGES ? t - STAGES : 0; i < t; ++i) wait_bar(&y_full[i % STAGES], (i / STAGES) & 1);
+        wait_bar(&ctl.x_full, 0);
+        for (int i = max(0, n1 - RING1); i < n1; ++i) wait_bar(&ctl.y1_full[i % RING1], ring_phase(i, RING1));
+        for (int i = max(0, n2 - RING2); i < n2; ++i) wait_bar(&ctl.y2_full[i % RING2], ring_phase(i, RING2));
+      }
+    }
+  } else if (warp == kStatWarp) {
+    if constexpr (DKV) {
+      Step s;
+      start(s);
+      for (int t = 0; t < steps; ++t, advance(s)) {
+        const int64_t stat = ((int64_t)b * P.heads + s.head) * P.queries + s.begin;
+        float lse[kStep / 32], delta[kStep / 32];
+#pragma unroll
+        for (int i = 0; i < kStep / 32; ++i) {
+          const int c = i * 32 + lane;
+          const bool in = s.begin + c < s.end;
+          lse[i] = in ? P.lse[stat + c] * kLog2eF : 0.0f;
+          delta[i] = in ? P.delta[stat + c] : 0.0f;
+        }
+        if (t >= 2) ok = wait_warp(&ctl.stat_free[t & 1], ring_phase(t - 2, 2));
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kStep / 32; ++i) {
+          ctl.stats[t & 1][0][i * 32 + lane] = lse[i];
+          ctl.stats[t & 1][1][i * 32 + lane] = delta[i];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.stat_full[t & 1]);
       }
     }
   } else if (warp == kMmaWarp) {
     const int width16 = (P.dim + 15) / 16;
     const uint32_t accumulate = tc_instruction<DT>(width16 * 16, true);
     const uint64_t x1 = tc_columns(base), x2 = tc_columns(base + TILE);
-    auto rows_of = [&](int t) {
-      int begin, end, head;
-      step_rows(t, begin, end, head);
-      return end - begin;
-    };
     // acc = x y^T of one step
-    auto product = [&](uint32_t acc, uint64_t x, uint32_t at, int rows, uint64_t* done) {
+    auto product = [&](uint32_t acc, uint64_t x, int at, int rows, uint64_t* done) {
       if (elect_one()) {
         const uint32_t instruction = tc_instruction<DT>((rows + 15) / 16 * 16, false);
-        const uint64_t y = tc_columns(at);
+        const uint64_t y = tc_columns(base + at);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
           if (k < width16) tc_mma(acc, x + tc_column_step(kTcRows, k), y + tc_column_step(kStep, k), instruction, k > 0);
@@ -439,30 +500,27 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       }
       __syncwarp();
     };
-    // acc += w y of one step; w lies in two halves of 64 columns
-    auto sum = [&](uint32_t acc, uint32_t w, uint32_t at, int rows, bool add, uint64_t* done) {
+    // acc += w y of one step, which ends its use of y; w lies in two halves of 64 columns
+    auto sum = [&](uint32_t acc, uint32_t w, int at, int rows, bool add, uint64_t* done) {
       if (elect_one()) {
-        const uint64_t y = tc_rows(at, kStep);
+        const uint64_t y = tc_rows(base + at, kStep);
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)
           if (k * 16 < rows)
             tc_mma_tmem(acc, w + (k >> 2) * 64 + (k & 3) * 8, y + tc_row_step(k), accumulate, add || k > 0);
-        if (done != nullptr) tc_commit(done);
+        tc_commit(done);
       }
       __syncwarp();
     };
-    // Waits for the rows of step t and clears those between its end and the end of its group of
-    // 16: their weights are 0, but 0 * NaN must not reach a sum.
-    auto arrive = [&](int t, int rows) {
-      const int stage = t % STAGES;
-      if (!wait_warp(&y_full[stage], (t / STAGES) & 1)) return false;
+    // Waits for a tile and clears its rows between the step's end and the end of its group of 16:
+    // their weights are 0, but 0 * NaN must not reach a sum.
+    auto arrive = [&](uint64_t* bar, uint32_t phase, int at, int rows) {
+      if (!wait_warp(bar, phase)) return false;
       const int tail = (rows + 15) / 16 * 16 - rows;
       if (tail > 0) {
         for (int i = lane; i < tail * (DP / 8); i += 32) {
           const int row = rows + i / (DP / 8), c = i % (DP / 8);
-          uint8_t* dst = aligned + (2 + 2 * stage) * TILE + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16;
-          *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + TILE) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(aligned + at + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();
         __syncwarp();
@@ -470,33 +528,43 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       return true;
     };
     int rows = 0;
+    Step s;
     if (steps > 0) {
-      rows = rows_of(0);
-      ok = wait_warp(&x_full, 0) && arrive(0, rows);
-      if (ok) product(t_s, x1, base + 2 * TILE, rows, &s_full);
+      start(s);
+      rows = s.end - s.begin;
+      ok = wait_warp(&ctl.x_full, 0) && arrive(&ctl.y1_full[0], 0, Shape::kY1, rows);
+      if (ok) product(t_s, x1, Shape::kY1, rows, &ctl.s_full);
     }
     for (int t = 0; t < steps && ok; ++t) {
-      const uint32_t at = base + (2 + 2 * (t % STAGES)) * TILE;
-      product(t_dp, x2, at + TILE, rows, &dp_full);
-      ok = wait_warp(&p_full, t & 1);
+      const int y1 = Shape::kY1 + t % RING1 * TILE, y2 = Shape::kY2 + t % RING2 * TILE;
+      ok = arrive(&ctl.y2_full[t % RING2], ring_phase(t, RING2), y2, rows);
+      if (!ok) break;
+      product(t_dp, x2, y2, rows, &ctl.dp_full);
+      if constexpr (!DKV) {   // nothing else reads y2
+        if (elect_one()) tc_commit(&ctl.y2_free[t % RING2]);
+        __syncwarp();
+      }
+      ok = wait_warp(&ctl.p_full, t & 1);
       if (!ok) break;
       tc_fence_after();
-      if constexpr (DKV) sum(t_out2, t_s, at + TILE, rows, t > 0, nullptr);
+      if constexpr (DKV) sum(t_out2, t_s, y2, rows, t > 0, &ctl.y2_free[t % RING2]);
       const int now = rows;
       if (t + 1 < steps) {
-        rows = rows_of(t + 1);
-        ok = arrive(t + 1, rows);
+        advance(s);
+        rows = s.end - s.begin;
+        const int next = Shape::kY1 + (t + 1) % RING1 * TILE;
+        ok = arrive(&ctl.y1_full[(t + 1) % RING1], ring_phase(t + 1, RING1), next, rows);
         if (!ok) break;
-        product(t_s, x1, base + (2 + 2 * ((t + 1) % STAGES)) * TILE, rows, &s_full);
+        product(t_s, x1, next, rows, &ctl.s_full);
       }
-      ok = wait_warp(&ds_full, t & 1);
+      ok = wait_warp(&ctl.ds_full, t & 1);
       if (!ok) break;
       tc_fence_after();
-      sum(t_out1, t_dp, at, now, t > 0, &y_free[t % STAGES]);
+      sum(t_out1, t_dp, y1, now, t > 0, &ctl.y1_free[t % RING1]);
     }
-    if (elect_one()) tc_commit(&out_full);
+    if (elect_one()) tc_commit(&ctl.out_full);
     __syncwarp();
-    if (!ok) wait_bar(&out_full, 0);
+    if (!ok) wait_bar(&ctl.out_full, 0);
   } else {
     const int group = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
@@ -523,49 +591,31 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         }
         lse = P.lse[stat] * kLog2eF;
       }
-      float* halves = &stats[0][0][0][0];
+      float* halves = &ctl.stats[0][0][0];
       halves[group * kTcRows + row] = d;
       named_barrier(1, 256);
       delta = halves[row] + halves[kTcRows + row];
       if (live && group == 0) P.delta[stat] = delta;
     }
-    // DKV: lse and delta belong to the columns; a thread fetches one of them ahead of its step.
-    float ahead = 0.0f;
-    auto fetch = [&](int t) {
-      if constexpr (DKV) {
-        const int tid = threadIdx.x & 127, c = group * 64 + (tid & 63);
-        int begin, end, head;
-        step_rows(t, begin, end, head);
-        const int64_t stat = ((int64_t)b * P.heads + head) * P.queries + begin + c;
-        ahead = begin + c < end ? (tid < 64 ? P.lse[stat] * kLog2eF : P.delta[stat]) : 0.0f;
-      }
-    };
-    if (steps > 0) fetch(0);
-    const int p_first = P.offset + r0, p_last = P.offset + r1 - 1;
-    for (int t = 0; t < steps; ++t) {
-      int begin, end, head;
-      step_rows(t, begin, end, head);
-      ColumnMask mask;
-      bool full;
-      if constexpr (!DKV) {
-        const int p = P.offset + r0 + row;
-        mask = {P.window == 0 ? 0 : p - P.window + 1 - begin, min(end, p + 1) - begin, P.sinks - begin};
-        full = end - begin == kStep && end - 1 <= p_first &&
-               (P.window == 0 || end <= P.sinks || p_last - begin < P.window);
-      } else {
-        stats[group][t & 1][(threadIdx.x & 127) >> 6][threadIdx.x & 63] = ahead;
-        named_barrier(1 + group, 128);
-        if (t + 1 < steps) fetch(t + 1);
-        const int key = r0 + row, first = P.offset + begin;
-        const bool all = P.window == 0 || key < P.sinks;
-        // (a window is at most 2^31 - 1 and positions stay below it, hence the 64-bit sum)
-        const int64_t last = all ? (int64_t)kStep : (int64_t)key + P.window - first;
-        mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
-        full = end - begin == kStep && r0 + kTcRows <= length && r0 + kTcRows - 1 <= first &&
-               (P.window == 0 || r0 + kTcRows <= P.sinks || P.offset + end - 1 - r0 < P.window);
-      }
+    // Steps without a masked pair: those whose rows are all there and lie within these bounds.
+    int full_lo, full_hi;
+    if constexpr (!DKV) {
+      full_lo = P.window == 0 ? 0 : P.offset + r1 - P.window;   // first key the last query sees
+      full_hi = P.offset + r0;                                   // last key the first query sees
+    } else {
+      // (a window is at most 2^31 - 1 and positions stay below it, hence the 64-bit sum)
+      const int64_t last = P.window == 0 || r0 + kTcRows <= P.sinks ? INT32_MAX : (int64_t)r0 + P.window - 1 - P.offset;
+      full_lo = r0 + kTcRows - 1 - P.offset;                     // first query that sees the last key
+      full_hi = r0 + kTcRows > length ? -1 : (int)(last < INT32_MAX ? last : INT32_MAX);
+    }
+    Step step;
+    if (steps > 0) start(step);
+    for (int t = 0; t < steps; ++t, advance(step)) {
+      const int begin = step.begin, end = step.end;
+      const bool full = end - begin == kStep && end - 1 <= full_hi && (begin >= full_lo || (!DKV && end <= P.sinks));
       // A wait that ran out is remembered and not waited for again (as in the forward).
-      if (ok) ok = wait_bar(&s_full, t & 1);
+      if (ok && DKV) ok = wait_bar(&ctl.stat_full[t & 1], ring_phase(t, 2));
+      if (ok) ok = wait_bar(&ctl.s_full, t & 1);
       __syncwarp();
       tc_fence_after();
       float p[64];
@@ -577,7 +627,7 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         if constexpr (!DKV) {   // s may be overwritten
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full);
+          if (lane == 0) mbar_arrive(&ctl.p_full);
         }
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
@@ -588,18 +638,29 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 #pragma unroll
       for (int c = 0; c < 64; c += 4) {
         float4 ls = make_float4(lse, lse, lse, lse);
-        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&stats[group][t & 1][0][c]);
+        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][group * 64 + c]);
         p[c] = ex2_approx(fmaf(p[c], P.scale_log2, -ls.x));
         p[c + 1] = ex2_approx(fmaf(p[c + 1], P.scale_log2, -ls.y));
         p[c + 2] = ex2_approx(fmaf(p[c + 2], P.scale_log2, -ls.z));
         p[c + 3] = ex2_approx(fmaf(p[c + 3], P.scale_log2, -ls.w));
       }
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
       if (!full) {
+        ColumnMask mask;
+        if constexpr (!DKV) {
+          const int pos = P.offset + r0 + row;
+          mask = {P.window == 0 ? 0 : pos - P.window + 1 - begin, min(end, pos + 1) - begin, P.sinks - begin};
+        } else {
+          const int key = r0 + row, first = P.offset + begin;
+          const int64_t last = P.window == 0 || key < P.sinks ? (int64_t)kStep : (int64_t)key + P.window - first;
+          mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
+        }
+        seen[0] = mask.word(group * 64);
+        seen[1] = mask.word(group * 64 + 32);
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
-          const uint32_t seen = mask.word(group * 64 + c0);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) p[c0 + c] = seen >> c & 1 ? p[c0 + c] : 0.0f;
+          for (int c = 0; c < 32; ++c) p[c0 + c] = seen[c0 / 32] >> c & 1 ? p[c0 + c] : 0.0f;
         }
       }
       if constexpr (DKV) {
@@ -613,9 +674,9 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         tmem_wait_store();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full);
+        if (lane == 0) mbar_arrive(&ctl.p_full);
       }
-      if (ok) ok = wait_bar(&dp_full, t & 1);
+      if (ok) ok = wait_bar(&ctl.dp_full, t & 1);
       __syncwarp();
       tc_fence_after();
       uint32_t w[32];
@@ -627,8 +688,7 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           float4 de = make_float4(delta, delta, delta, delta);
-          if constexpr (DKV) de = *reinterpret_cast<const float4*>(&stats[group][t & 1][1][c0 + c]);
-          // Where P is 0 the key may be one that is not there, and dp anything.
+          if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * 64 + c0 + c]);
           const float a = p[c0 + c] * (__uint_as_float(d[c]) - de.x), e = p[c0 + c + 1] * (__uint_as_float(d[c + 1]) - de.y);
           const float f = p[c0 + c + 2] * (__uint_as_float(d[c + 2]) - de.z),
                       g = p[c0 + c + 3] * (__uint_as_float(d[c + 3]) - de.w);
@@ -636,20 +696,22 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
           w[(c0 + c) / 2 + 1] = pack2<DT>(f, g);
         }
         if (!full) {
-          // Packed pairs of weight 0: 0 * NaN of a key that is not there is cleared as well.
-          const uint32_t seen = mask.word(group * 64 + c0);
+          // dp of a key that is not there may be NaN: 0 * NaN is cleared here.
 #pragma unroll
           for (int c = 0; c < 32; c += 2)
-            w[(c0 + c) / 2] &= (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u);
+            w[(c0 + c) / 2] &= (seen[c0 / 32] >> c & 1 ? 0xffffu : 0u) | (seen[c0 / 32] >> (c + 1) & 1 ? 0xffff0000u : 0u);
         }
       }
       tmem_store32(t_dp + lanes + group * 64, w);
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full);
+      if (lane == 0) {
+        mbar_arrive(&ctl.ds_full);
+        if constexpr (DKV) mbar_arrive(&ctl.stat_free[t & 1]);
+      }
     }
-    if (ok && steps > 0) ok = wait_bar(&out_full, 0);
+    if (ok && steps > 0) ok = wait_bar(&ctl.out_full, 0);
     __syncwarp();
     tc_fence_after();
     // DKV: the first group stores dk, the second dv; else half of dq's columns each.
@@ -772,11 +834,11 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
   const unsigned rows = (unsigned)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
-  attention_tc_backward<DT, DP, false><<<rows, kTcThreads, bytes, s>>>(P, q, g, k, v);
+  attention_tc_backward<DT, DP, false><<<rows, kBwdThreads, bytes, s>>>(P, q, g, k, v);
   rc = launch_status("nt_attention_backward launch");
   if (rc) return rc;
   const int tiles = (P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1);
-  attention_tc_backward<DT, DP, true><<<(unsigned)tiles * P.kv_heads * P.batch, kTcThreads, bytes, s>>>(P, k, v, q, g);
+  attention_tc_backward<DT, DP, true><<<(unsigned)tiles * P.kv_heads * P.batch, kBwdThreads, bytes, s>>>(P, k, v, q, g);
   return launch_status("nt_attention_backward launch");
 }
 
