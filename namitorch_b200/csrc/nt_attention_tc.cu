@@ -1,14 +1,11 @@
 // Sliding-window attention on the fifth-generation tensor cores, for float16 and bfloat16 rows
 // that are whole 16-byte vectors. The mathematics and the masks are those of nt_attention.cu.
 //
-// Forward: a block owns 128 queries of one head and walks its visible keys 128 at a time. One
-// warp copies tiles, one issues the products, eight do the softmax: two threads share a query's
-// row, 64 columns each. S = q k^T accumulates in TMEM; the weights go back to TMEM over S as
-// 16-bit values and are the first operand of o += w v. Two blocks share an SM, so one's products
-// run under the other's exponentials.
-//
-// Backward: two passes of one kernel (see attention_tc_backward), each with S and dP computed
-// again. Sums that cross blocks exist only for the sink keys and are added in order afterwards.
+// One block per SM: one warp copies tiles, one issues the products, sixteen compute. Scores
+// accumulate in TMEM; the weights go back to TMEM over them as 16-bit values and are the first
+// operand of the second product. The backward is two passes of one kernel, each with S and dP
+// computed again; sums that cross blocks exist only for the sink keys and are added in order
+// afterwards.
 //
 // Roundings below 32 bits: the weights and dS are rounded to the inputs' type because the second
 // products take their operand in it; every sum, maximum and statistic is float32.
@@ -20,20 +17,11 @@
 namespace nt {
 
 constexpr int kTcRows = 128;
-constexpr int kTcThreads = 320;        // 8 computing warps, 1 copying, 1 issuing products
-constexpr int kCopyWarp = 8, kMmaWarp = 9;
-constexpr uint32_t kFwdColumns = 256;  // TMEM: S (and the weights over it) 128, output up to 128
+constexpr int kComputeWarps = 16;      // of forward and backward; four of them share 128 rows
+constexpr int kCopyWarp = 16, kMmaWarp = 17;
+constexpr int kFwdThreads = 18 * 32;
+constexpr uint32_t kTmemColumns = 512;
 constexpr float kRescaleLog2 = 8.0f;
-
-// A wait of a whole warp, which goes on or gives up as one.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, wait_bar(bar, parity));
-}
-
-template <int DP> struct FwdShared {
-  static constexpr int kTile = kTcRows * DP * 2;
-  static constexpr int kBytes = 3 * kTile + 1024;
-};
 
 // Which columns of a tile a row sees: c < end and (c >= begin or c < sink). word(c0) has bit e set
 // for column c0 + e, so that a masked tile costs one bit test and one select per element.
@@ -47,161 +35,237 @@ struct ColumnMask {
   }
 };
 
+// A wait of a whole warp, which goes on or gives up as one.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity));
+}
+// Phase of slot use n of a ring of `size`.
+__device__ __forceinline__ uint32_t ring_phase(int n, int size) { return (uint32_t)(n / size) & 1u; }
+
+// Rows [rows, next multiple of 16) of a tile are cleared: their weights are 0, but what lies there
+// may be anything, and 0 * NaN must not reach a sum. One warp.
+template <int DP>
+__device__ __forceinline__ void clear_tail(uint8_t* tile, int rows, int lane) {
+  const int tail = (rows + 15) / 16 * 16 - rows;
+  if (tail == 0) return;
+  for (int i = lane; i < tail * (DP / 8); i += 32) {
+    const int row = rows + i / (DP / 8), c = i % (DP / 8);
+    *reinterpret_cast<uint4*>(tile + (c / 8) * kTcRows * 128 + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+  __syncwarp();
+}
+
+// ---- forward -------------------------------------------------------------------------
+// A block owns 2 x 128 queries of one head, which share the key and value tiles (a tile fetched
+// for 128 queries alone would ask the L2 for 64 KB per 1024 cycles of products). Warps 0-7 do the
+// softmax of the first 128 rows, 8-15 of the second: two threads share a row, 64 columns each. The
+// products of one half run under the exponentials of the other:
+//   s0(0) s1(0) | o0 += w0(0) v, s0(1) | o1 += w1(0) v, s1(1) | o0 += w0(1) v, ...
+// TMEM: s0, s1 (the weights over them), o0, o1.
+template <int DP> struct FwdShared {
+  static constexpr int kTile = kTcRows * DP * 2;
+  static constexpr int kRing = 2;
+  static constexpr int kK = 2 * kTile, kV = (2 + kRing) * kTile, kControl = (2 + 2 * kRing) * kTile;
+  struct Control {
+    float exchange[2][2][2][kTcRows];   // half of the queries, parity of the tile, half of the columns, row
+    uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[2], w_full[2], o_full;
+    uint32_t tmem;
+  };
+  static constexpr int kBytes = kControl + (int)sizeof(Control);
+};
+
 template <int DT, int DP>
-__global__ void __launch_bounds__(kTcThreads, 2)
+__global__ void __launch_bounds__(kFwdThreads, 1)
 attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-  extern __shared__ uint8_t raw[];
-  __shared__ uint64_t q_full, k_full, k_free, v_full, v_free, s_full, w_full, o_full;
-  __shared__ uint32_t tmem_slot;
-  __shared__ float exchange[2][2][kTcRows];
-  constexpr int TILE = FwdShared<DP>::kTile;
-  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  uint8_t* aligned = raw + (base - smem_u32(raw));
-  const uint32_t sq = base, sk = base + TILE, sv = base + 2 * TILE;
+  using Shape = FwdShared<DP>;
+  constexpr int TILE = Shape::kTile, RING = Shape::kRing;
+  // No static shared memory: the dynamic block starts where shared memory does, 1024 bytes in.
+  extern __shared__ __align__(1024) uint8_t aligned[];
+  typename Shape::Control& ctl = *reinterpret_cast<typename Shape::Control*>(aligned + Shape::kControl);
+  const uint32_t base = smem_u32(aligned);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Blocks in the order of their work: the last queries of every head first.
   const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / pairs;
   const int b = blockIdx.x % pairs / P.heads, h = blockIdx.x % P.heads, hk = h / P.group;
-  const int i0 = (tiles - 1 - blockIdx.x / pairs) * kTcRows, i1 = min(P.queries, i0 + kTcRows);
+  const int i0 = (tiles - 1 - blockIdx.x / pairs) * 2 * kTcRows, i1 = min(P.queries, i0 + 2 * kTcRows);
   const int length = attn_length(P, b);
   const AttnKeys range(P, length, i0, i1);
   const int blocks = range.blocks(kTcRows);
+  // Whether a query of half g sees a key of [begin, end) (half 1 may be past the last query).
+  const AttnKeys range0(P, length, i0, min(i1, i0 + kTcRows)), range1(P, length, min(i1, i0 + kTcRows), i1);
+  auto active = [&](int g, int begin, int end) {
+    const AttnKeys& r = g ? range1 : range0;
+    return (g == 0 || i1 > i0 + kTcRows) && ((begin < r.hi && end > r.lo) || begin < r.sink_end);
+  };
 
-  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, kFwdColumns);
+  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, 1); mbar_init(&k_full, 1); mbar_init(&k_free, 1); mbar_init(&v_full, 1); mbar_init(&v_free, 1);
-    mbar_init(&s_full, 1); mbar_init(&w_full, 8); mbar_init(&o_full, 1);
+    mbar_init(&ctl.q_full, 1); mbar_init(&ctl.o_full, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.k_full[i], 1); mbar_init(&ctl.k_free[i], 1); mbar_init(&ctl.v_full[i], 1); mbar_init(&ctl.v_free[i], 1);
+      mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], kComputeWarps / 2);
+    }
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t t_s = tmem, t_o = tmem + kTcRows;
+  const uint32_t tmem = ctl.tmem;
   bool ok = true;
 
   if (warp == kCopyWarp) {
     if (lane == 0 && blocks > 0) {
-      auto load = [&](const CUtensorMap* map, int offset, int token, int head, uint64_t* bar) {
-        mbar_arrive_expect_tx(bar, TILE);
+      auto load = [&](const CUtensorMap* map, int at, int token, int head, uint64_t* bar) {
 #pragma unroll
         for (int half = 0; half < DP / 64; ++half)
-          tma_load(aligned + offset + half * kTcRows * 128, map, half * 64, token, head, b, bar);
+          tma_load(aligned + at + half * kTcRows * 128, map, half * 64, token, head, b, bar);
       };
-      load(&map_q, 0, i0, h, &q_full);
-      int issued = 0;
-      for (int j = 0; j < blocks && ok; ++j) {
+      // The second half's rows may all lie past the last query: the copy then writes zeros.
+      mbar_arrive_expect_tx(&ctl.q_full, 2 * TILE);
+      load(&map_q, 0, i0, h, &ctl.q_full);
+      load(&map_q, TILE, i0 + kTcRows, h, &ctl.q_full);
+      int n1 = 0, n2 = 0;
+      for (int j = 0; j < blocks; ++j) {
         int begin, end;
         range.block(j, kTcRows, begin, end);
-        if (j > 0) ok = wait_bar(&k_free, (j - 1) & 1);
+        if (j >= RING) ok = wait_bar(&ctl.k_free[j % RING], ring_phase(j - RING, RING));
         if (!ok) break;
-        load(&map_k, TILE, begin, hk, &k_full);
-        if (j > 0) ok = wait_bar(&v_free, (j - 1) & 1);
-        if (!ok) { wait_bar(&k_full, j & 1); break; }
-        load(&map_v, 2 * TILE, begin, hk, &v_full);
-        issued = j + 1;
+        mbar_arrive_expect_tx(&ctl.k_full[j % RING], TILE);
+        load(&map_k, Shape::kK + j % RING * TILE, begin, hk, &ctl.k_full[j % RING]);
+        n1 = j + 1;
+        if (j >= RING) ok = wait_bar(&ctl.v_free[j % RING], ring_phase(j - RING, RING));
+        if (!ok) break;
+        mbar_arrive_expect_tx(&ctl.v_full[j % RING], TILE);
+        load(&map_v, Shape::kV + j % RING * TILE, begin, hk, &ctl.v_full[j % RING]);
+        n2 = j + 1;
       }
       if (!ok) {   // the copies in flight land before the block may end
-        wait_bar(&q_full, 0);
-        if (issued > 0) { wait_bar(&k_full, (issued - 1) & 1); wait_bar(&v_full, (issued - 1) & 1); }
+        wait_bar(&ctl.q_full, 0);
+        for (int i = max(0, n1 - RING); i < n1; ++i) wait_bar(&ctl.k_full[i % RING], ring_phase(i, RING));
+        for (int i = max(0, n2 - RING); i < n2; ++i) wait_bar(&ctl.v_full[i % RING], ring_phase(i, RING));
       }
     }
   } else if (warp == kMmaWarp) {
     const int width16 = (P.dim + 15) / 16;
     const uint32_t pv = tc_instruction<DT>(width16 * 16, true);
-    const uint64_t dq = tc_columns(sq), dk = tc_columns(sk), dv = tc_rows(sv, kTcRows);
-    if (blocks > 0) ok = wait_warp(&q_full, 0);
-    for (int j = 0; j < blocks && ok; ++j) {
-      int begin, end;
-      range.block(j, kTcRows, begin, end);
-      const int keys16 = (end - begin + 15) / 16;
-      ok = wait_warp(&k_full, j & 1);
-      if (!ok) break;
+    auto scores = [&](int g, int at, int rows) {
       if (elect_one()) {
-        const uint32_t qk = tc_instruction<DT>(keys16 * 16, false);
+        const uint32_t qk = tc_instruction<DT>((rows + 15) / 16 * 16, false);
+        const uint64_t q = tc_columns(base + g * TILE), k = tc_columns(base + at);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
-          if (s < width16) tc_mma(t_s, dq + tc_column_step(kTcRows, s), dk + tc_column_step(kTcRows, s), qk, s > 0);
-        tc_commit(&s_full);
-        tc_commit(&k_free);
+          if (s < width16)
+            tc_mma(tmem + g * kTcRows, q + tc_column_step(kTcRows, s), k + tc_column_step(kTcRows, s), qk, s > 0);
+        tc_commit(&ctl.s_full[g]);
       }
       __syncwarp();
-      ok = wait_warp(&v_full, j & 1);
-      if (!ok) break;
-      // Rows between the last visible key and the end of its group of 16 have weight 0 but may
-      // hold anything: 0 * NaN must not reach the sum.
-      const int tail = keys16 * 16 - (end - begin);
-      if (tail > 0) {
-        for (int i = lane; i < tail * (DP / 8); i += 32) {
-          const int row = end - begin + i / (DP / 8), c = i % (DP / 8);
-          *reinterpret_cast<uint4*>(aligned + 2 * TILE + (c / 8) * kTcRows * 128 + row * 128 + (c % 8) * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async();
-        __syncwarp();
-      }
-      ok = wait_warp(&w_full, j & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (elect_one()) {
-#pragma unroll
-        for (int s = 0; s < kTcRows / 16; ++s)
-          if (s < keys16) tc_mma_tmem(t_o, t_s + s * 8, dv + tc_row_step(s), pv, j > 0 || s > 0);
-        tc_commit(&v_free);
-      }
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) tc_commit(bar);
       __syncwarp();
+    };
+    int done[2] = {0, 0};   // tiles of each half
+    int begin = 0, end = 0;
+    if (blocks > 0) {
+      range.block(0, kTcRows, begin, end);
+      ok = wait_warp(&ctl.q_full, 0) && wait_warp(&ctl.k_full[0], 0);
+      if (ok) {
+        if (active(0, begin, end)) scores(0, Shape::kK, end - begin);
+        if (active(1, begin, end)) scores(1, Shape::kK, end - begin);
+        commit(&ctl.k_free[0]);
+      }
     }
-    if (elect_one()) tc_commit(&o_full);
-    __syncwarp();
-    if (!ok) wait_bar(&o_full, 0);   // no product is in flight when TMEM is given back
+    for (int j = 0; j < blocks && ok; ++j) {
+      int next_begin = 0, next_end = 0;
+      const int slot = j % RING, next = (j + 1) % RING;
+      if (j + 1 < blocks) {
+        range.block(j + 1, kTcRows, next_begin, next_end);
+        ok = wait_warp(&ctl.k_full[next], ring_phase(j + 1, RING));
+      }
+      ok = ok && wait_warp(&ctl.v_full[slot], ring_phase(j, RING));
+      if (!ok) break;
+      clear_tail<DP>(aligned + Shape::kV + slot * TILE, end - begin, lane);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (active(g, begin, end)) {
+          ok = ok && wait_warp(&ctl.w_full[g], done[g] & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t v = tc_rows(base + Shape::kV + slot * TILE, kTcRows);
+#pragma unroll
+            for (int s = 0; s < kTcRows / 16; ++s)   // the weights lie in two halves of 64 columns
+              if (s * 16 < end - begin)
+                tc_mma_tmem(tmem + 2 * kTcRows + g * DP, tmem + g * kTcRows + (s >> 2) * 64 + (s & 3) * 8,
+                            v + tc_row_step(s), pv, done[g] > 0 || s > 0);
+          }
+          __syncwarp();
+          ++done[g];
+        }
+        if (j + 1 < blocks && active(g, next_begin, next_end))
+          scores(g, Shape::kK + next * TILE, next_end - next_begin);
+      }
+      if (!ok) break;
+      commit(&ctl.v_free[slot]);
+      if (j + 1 < blocks) commit(&ctl.k_free[next]);
+      begin = next_begin;
+      end = next_end;
+    }
+    commit(&ctl.o_full);
+    if (!ok) wait_bar(&ctl.o_full, 0);   // no product is in flight when TMEM is given back
   } else {
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int g = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // lane 32 (w % 4) in the address's upper half
-    const int p = P.offset + i0 + row;
-    const int p_first = P.offset + i0, p_last = P.offset + i1 - 1;
-    const int sinks = range.sink_blocks(kTcRows);
+    const uint32_t t_s = tmem + g * kTcRows + lanes + half * 64;
+    const uint32_t t_o = tmem + 2 * kTcRows + g * DP + lanes + half * (DP / 2);
+    const int q0 = i0 + g * kTcRows, q1 = min(i1, q0 + kTcRows);
+    const int p = P.offset + q0 + row;
+    const int full_lo = P.window == 0 ? 0 : P.offset + q1 - P.window;   // first key the last query sees
+    const int full_hi = P.offset + q0;                                   // last key the first query sees
+    const int pair = 1 + g * 4 + (warp & 3);
     float m = -INFINITY, l = 0.0f;
+    int done = 0;
     for (int j = 0; j < blocks; ++j) {
       int begin, end;
       range.block(j, kTcRows, begin, end);
+      if (!active(g, begin, end)) continue;
       // A wait that ran out is remembered and not waited for again; the warp still takes part in
       // every barrier, so that no other warp is left waiting for it.
-      if (ok) ok = wait_bar(&s_full, j & 1);
+      if (ok) ok = wait_bar(&ctl.s_full[g], done & 1);
       __syncwarp();
       tc_fence_after();
-      uint32_t r0[32], r1[32];
-      tmem_load32(t_s + lanes + half * 64, r0);
-      tmem_load32(t_s + lanes + half * 64 + 32, r1);
-      tmem_wait_load();
-      float s[64];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        s[c] = __uint_as_float(r0[c]);
-        s[32 + c] = __uint_as_float(r1[c]);
-      }
-      const bool full = end - begin == kTcRows && end - 1 <= p_first &&
-                        (P.window == 0 || j < sinks || p_last - begin < P.window);
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+      const bool full = end - begin == kTcRows && end - 1 <= full_hi && (begin >= full_lo || end <= P.sinks);
       if (!full) {
-        const ColumnMask mask{P.window == 0 ? 0 : p - P.window + 1 - begin - half * 64, min(end, p + 1) - begin - half * 64,
-                              P.sinks - begin - half * 64};
+        const ColumnMask mask{P.window == 0 ? 0 : p - P.window + 1 - begin, min(end, p + 1) - begin, P.sinks - begin};
+        seen[0] = mask.word(half * 64);
+        seen[1] = mask.word(half * 64 + 32);
+      }
+      // The scores are read twice: once for the maximum, once for the weights. 64 of them held in
+      // between would not fit the registers of 18 warps.
+      float top = -INFINITY;
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          const uint32_t seen = mask.word(c0);
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t s[32];
+        tmem_load32(t_s + c0, s);
+        tmem_wait_load();
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (full) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[c0 + c] = seen >> c & 1 ? s[c0 + c] : -INFINITY;
+          for (int c = 0; c < 32; ++c) t[c & 3] = fmaxf(t[c & 3], __uint_as_float(s[c]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            t[c & 3] = fmaxf(t[c & 3], seen[c0 / 32] >> c & 1 ? __uint_as_float(s[c]) : -INFINITY);
         }
+        top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
       }
-      float top = s[0], top1 = s[1];
-#pragma unroll
-      for (int c = 2; c < 64; c += 2) {
-        top = fmaxf(top, s[c]);
-        top1 = fmaxf(top1, s[c + 1]);
-      }
-      top = fmaxf(top, top1);
-      exchange[j & 1][half][row] = top;
-      named_barrier(1 + (warp & 3), 64);
-      top = fmaxf(top, exchange[j & 1][half ^ 1][row]);
+      ctl.exchange[g][done & 1][half][row] = top;
+      named_barrier(pair, 64);
+      top = fmaxf(top, ctl.exchange[g][done & 1][half ^ 1][row]);
       // The maximum only has to keep the weights in range, so the old one stays until the new is
       // 2^8 above it: the output is then rescaled for a few of the first tiles of a row only.
       const bool raise = top > m && !((top - m) * P.scale_log2 <= kRescaleLog2);
@@ -209,64 +273,71 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
         const float f = raise ? ex2_approx((m - top) * P.scale_log2) : 1.0f;
         if (raise) m = top;
         l *= f;
-        if (j > 0) {
-          // Products complete in order: S of this tile is there, so o of the last one is too.
-#pragma unroll
+        if (done > 0) {
+          // Products complete in order: s of this tile is there, so o of the last one is too.
+#pragma unroll 1
           for (int c = 0; c < DP / 2; c += 32) {
             uint32_t o[32];
-            tmem_load32(t_o + lanes + half * (DP / 2) + c, o);
+            tmem_load32(t_o + c, o);
             tmem_wait_load();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_store32(t_o + lanes + half * (DP / 2) + c, o);
+            tmem_store32(t_o + c, o);
           }
         }
       }
       float shift = m == -INFINITY ? 0.0f : m;
-      if (__any_sync(0xffffffffu, isinf(shift * P.scale_log2))) {
-        // Scores near the ends of float32: subtract before scaling.
+      // Scores near the ends of float32 are subtracted before they are scaled.
+      const bool extreme = __any_sync(0xffffffffu, isinf(shift * P.scale_log2));
+      const float minus = extreme ? 0.0f : -shift * P.scale_log2, before = extreme ? shift : 0.0f;
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < 64; ++c) s[c] -= shift;
-        shift = 0.0f;
-      }
-      const float minus = -shift * P.scale_log2;
-      float sum0 = 0.0f, sum1 = 0.0f;
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t s[32], w[16];
+        tmem_load32(t_s + c0, s);
+        tmem_wait_load();
+        if (extreme) {
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        uint32_t w[16];
+          for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) - before);
+        }
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) s[c] = seen[c0 / 32] >> c & 1 ? s[c] : 0xff800000u;
+        }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = ex2_approx(fmaf(s[c + 2 * e], P.scale_log2, minus));
-          const float y = ex2_approx(fmaf(s[c + 2 * e + 1], P.scale_log2, minus));
-          sum0 += x;
-          sum1 += y;
+          const float x = ex2_approx(fmaf(__uint_as_float(s[2 * e]), P.scale_log2, minus));
+          const float y = ex2_approx(fmaf(__uint_as_float(s[2 * e + 1]), P.scale_log2, minus));
+          sum[0] += x;
+          sum[1] += y;
           w[e] = pack2<DT>(x, y);
         }
-        tmem_store16(t_s + lanes + half * 32 + c / 2, w);
+        tmem_store16(t_s + c0 / 2, w);   // over scores that both reads are done with
       }
-      l += sum0 + sum1;
+      l += sum[0] + sum[1];
+      ++done;
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&w_full);
+      if (lane == 0) mbar_arrive(&ctl.w_full[g]);
     }
-    if (ok && blocks > 0) ok = wait_bar(&o_full, 0);
+    if (ok && blocks > 0) ok = wait_bar(&ctl.o_full, 0);
     __syncwarp();
     tc_fence_after();
-    exchange[blocks & 1][half][row] = l;
-    named_barrier(1 + (warp & 3), 64);
+    ctl.exchange[g][done & 1][half][row] = l;
+    named_barrier(pair, 64);
     // Halves in a fixed order, so that both threads of a row have the same sum.
-    l = exchange[blocks & 1][0][row] + exchange[blocks & 1][1][row];
+    l = ctl.exchange[g][done & 1][0][row] + ctl.exchange[g][done & 1][1][row];
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const bool live = i0 + row < i1;
-    uint16_t* out = static_cast<uint16_t*>(P.o) + P.os.at(b, h, i0 + row) + half * (DP / 2);
-    uint16_t* low = P.o_low == nullptr ? nullptr
-                                       : static_cast<uint16_t*>(P.o_low) + P.os.at(b, h, i0 + row) + half * (DP / 2);
+    const bool live = q0 + row < q1;
+    const int64_t at = P.os.at(b, h, q0 + row) + half * (DP / 2);
+    uint16_t* out = static_cast<uint16_t*>(P.o) + at;
+    uint16_t* low = P.o_low == nullptr ? nullptr : static_cast<uint16_t*>(P.o_low) + at;
 #pragma unroll
     for (int c = 0; c < DP / 2; c += 32) {
       uint32_t o[32];
-      if (blocks > 0) {
-        tmem_load32(t_o + lanes + half * (DP / 2) + c, o);
+      if (done > 0) {
+        tmem_load32(t_o + c, o);
         tmem_wait_load();
       } else {
 #pragma unroll
@@ -290,13 +361,13 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       }
     }
     if (live && half == 0 && P.lse != nullptr)
-      P.lse[((int64_t)b * P.heads + h) * P.queries + i0 + row] =
+      P.lse[((int64_t)b * P.heads + h) * P.queries + q0 + row] =
           l == 0.0f ? -INFINITY : fmaf(m, P.scale, log2f(l) * kLn2F);
   }
   if (!ok && P.error != nullptr) atomicOr(P.error, 1);
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_free(tmem, kFwdColumns);
+  if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -307,14 +378,15 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 // DKV = false: rows are queries (x1 = q, x2 = g; y1 = k, y2 = v): out1 = dq; delta = sum(g o) is
 // computed on the way in and stored. DKV = true: rows are keys (x1 = k, x2 = v; y1 = q, y2 = g):
 // out1 = dk, out2 = dv, over the heads of the group.
-// s, dp and the two outputs fill TMEM, so nothing has a second buffer; the order of the products
-// hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1) while
-// dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Two groups of four warps take 64 columns each.
+// With DKV s, dp and the two outputs fill TMEM, so nothing has a second buffer; the order of the
+// products hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1)
+// while dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Without it dp has two buffers and
+// dp(t + 1) does not wait for out1(t). Four groups of four warps take 32 columns each.
 constexpr int kStep = kTcQueryStep;
-constexpr uint32_t kBwdColumns = 512;
+constexpr int kColumns = kStep / 4;    // of a computing thread
 
-constexpr int kBwdThreads = 352;       // 8 computing warps, 1 copying, 1 issuing products, 1 for lse and delta
-constexpr int kStatWarp = 10;
+constexpr int kBwdThreads = 19 * 32;   // the warps of the forward and one for lse and delta
+constexpr int kStatWarp = 18;
 
 // Shared memory: x1, x2, the ring of y1 (three: s of the next step starts before out1 of this one
 // has ended), the ring of y2 (two) and the control block.
@@ -324,17 +396,16 @@ template <int DP> struct BwdShared {
   static constexpr int kY1 = 2 * kTile, kY2 = (2 + kRing1) * kTile, kControl = (2 + kRing1 + kRing2) * kTile;
   struct Control {
     float stats[2][2][kStep];          // ring of two; lse (times log2 e), delta
-    uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, dp_full, p_full, ds_full,
+    uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, p_full,
+        dp_full[2], ds_full[2],            // by the step's parity: dp(t + 1) may be there before dp(t) was waited for
         stat_full[2], stat_free[2], out_full;
+    float delta[kTcRows];
     uint32_t tmem;
   };
   static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
 static_assert(kStep == kTcRows, "rows kept and rows streamed have one shape");
 static_assert(BwdShared<128>::kBytes <= 227 * 1024, "one block per SM");
-
-// Phase of slot use n of a ring of `size`.
-__device__ __forceinline__ uint32_t ring_phase(int n, int size) { return (uint32_t)(n / size) & 1u; }
 
 template <int DT, int DP, bool DKV>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -408,7 +479,7 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     }
   };
 
-  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kBwdColumns);
+  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
   if (threadIdx.x == 0) {
     mbar_init(&ctl.x_full, 1); mbar_init(&ctl.out_full, 1);
 #pragma unroll
@@ -416,16 +487,20 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 #pragma unroll
     for (int i = 0; i < RING2; ++i) {
       mbar_init(&ctl.y2_full[i], 1); mbar_init(&ctl.y2_free[i], 1);
-      mbar_init(&ctl.stat_full[i], 1); mbar_init(&ctl.stat_free[i], 8);
+      mbar_init(&ctl.stat_full[i], 1); mbar_init(&ctl.stat_free[i], kComputeWarps);
     }
-    mbar_init(&ctl.s_full, 1); mbar_init(&ctl.dp_full, 1); mbar_init(&ctl.p_full, 8); mbar_init(&ctl.ds_full, 8);
+    mbar_init(&ctl.s_full, 1); mbar_init(&ctl.p_full, kComputeWarps);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctl.dp_full[i], 1); mbar_init(&ctl.ds_full[i], kComputeWarps); }
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl.tmem;
+  // Columns: s, dp, out1 and, with DKV, out2, else the second buffer of dp.
   const uint32_t t_s = tmem, t_dp = tmem + kStep, t_out1 = tmem + 2 * kStep, t_out2 = t_out1 + DP;
+  auto t_dp_of = [&](int t) { return DKV || (t & 1) == 0 ? t_dp : t_out1 + DP; };
   bool ok = true;
 
   if (warp == kCopyWarp) {
@@ -500,31 +575,21 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       }
       __syncwarp();
     };
-    // acc += w y of one step, which ends its use of y; w lies in two halves of 64 columns
+    // acc += w y of one step, which ends its use of y; w lies in four quarters, each over its scores
     auto sum = [&](uint32_t acc, uint32_t w, int at, int rows, bool add, uint64_t* done) {
       if (elect_one()) {
         const uint64_t y = tc_rows(base + at, kStep);
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k)
           if (k * 16 < rows)
-            tc_mma_tmem(acc, w + (k >> 2) * 64 + (k & 3) * 8, y + tc_row_step(k), accumulate, add || k > 0);
+            tc_mma_tmem(acc, w + (k >> 1) * kColumns + (k & 1) * 8, y + tc_row_step(k), accumulate, add || k > 0);
         tc_commit(done);
       }
       __syncwarp();
     };
-    // Waits for a tile and clears its rows between the step's end and the end of its group of 16:
-    // their weights are 0, but 0 * NaN must not reach a sum.
     auto arrive = [&](uint64_t* bar, uint32_t phase, int at, int rows) {
       if (!wait_warp(bar, phase)) return false;
-      const int tail = (rows + 15) / 16 * 16 - rows;
-      if (tail > 0) {
-        for (int i = lane; i < tail * (DP / 8); i += 32) {
-          const int row = rows + i / (DP / 8), c = i % (DP / 8);
-          *reinterpret_cast<uint4*>(aligned + at + (c / 8) * kStep * 128 + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async();
-        __syncwarp();
-      }
+      clear_tail<DP>(aligned + at, rows, lane);
       return true;
     };
     int rows = 0;
@@ -535,19 +600,23 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       ok = wait_warp(&ctl.x_full, 0) && arrive(&ctl.y1_full[0], 0, Shape::kY1, rows);
       if (ok) product(t_s, x1, Shape::kY1, rows, &ctl.s_full);
     }
-    for (int t = 0; t < steps && ok; ++t) {
-      const int y1 = Shape::kY1 + t % RING1 * TILE, y2 = Shape::kY2 + t % RING2 * TILE;
-      ok = arrive(&ctl.y2_full[t % RING2], ring_phase(t, RING2), y2, rows);
-      if (!ok) break;
-      product(t_dp, x2, y2, rows, &ctl.dp_full);
+    auto second = [&](int t, int rows) {   // dp(t)
+      const int y2 = Shape::kY2 + t % RING2 * TILE;
+      if (!arrive(&ctl.y2_full[t % RING2], ring_phase(t, RING2), y2, rows)) return false;
+      product(t_dp_of(t), x2, y2, rows, &ctl.dp_full[t & 1]);
       if constexpr (!DKV) {   // nothing else reads y2
         if (elect_one()) tc_commit(&ctl.y2_free[t % RING2]);
         __syncwarp();
       }
-      ok = wait_warp(&ctl.p_full, t & 1);
+      return true;
+    };
+    if (!DKV && steps > 0 && ok) ok = second(0, rows);
+    for (int t = 0; t < steps && ok; ++t) {
+      if constexpr (DKV) ok = second(t, rows);
+      ok = ok && wait_warp(&ctl.p_full, t & 1);
       if (!ok) break;
       tc_fence_after();
-      if constexpr (DKV) sum(t_out2, t_s, y2, rows, t > 0, &ctl.y2_free[t % RING2]);
+      if constexpr (DKV) sum(t_out2, t_s, Shape::kY2 + t % RING2 * TILE, rows, t > 0, &ctl.y2_free[t % RING2]);
       const int now = rows;
       if (t + 1 < steps) {
         advance(s);
@@ -556,46 +625,52 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         ok = arrive(&ctl.y1_full[(t + 1) % RING1], ring_phase(t + 1, RING1), next, rows);
         if (!ok) break;
         product(t_s, x1, next, rows, &ctl.s_full);
+        if constexpr (!DKV) ok = second(t + 1, rows);
       }
-      ok = wait_warp(&ctl.ds_full, t & 1);
+      ok = ok && wait_warp(&ctl.ds_full[t & 1], ring_phase(t, 2));
       if (!ok) break;
       tc_fence_after();
-      sum(t_out1, t_dp, y1, now, t > 0, &ctl.y1_free[t % RING1]);
+      sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * TILE, now, t > 0, &ctl.y1_free[t % RING1]);
     }
     if (elect_one()) tc_commit(&ctl.out_full);
     __syncwarp();
     if (!ok) wait_bar(&ctl.out_full, 0);
   } else {
-    const int group = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t at_s = t_s + lanes + quarter * kColumns;
     float lse = 0.0f, delta = 0.0f;
     if constexpr (!DKV) {
-      // delta of the row: each of its two threads sums half of the columns.
-      const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0 + row;
-      const bool live = r0 + row < r1;
-      float d = 0.0f;
-      if (live) {
-        const uint16_t* g = static_cast<const uint16_t*>(P.g) + P.gs.at(b, h0, r0 + row);
-        const uint16_t* o = static_cast<const uint16_t*>(P.o) + P.os.at(b, h0, r0 + row);
-        const uint16_t* low = P.o_low == nullptr ? nullptr : static_cast<const uint16_t*>(P.o_low) + P.os.at(b, h0, r0 + row);
+      // delta: each warp sums 8 rows, as many lanes to a row as it has 16-byte vectors.
+      constexpr int LPR = DP / 8, RPW = 32 / LPR;
+      const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0;
 #pragma unroll
-        for (int c = 0; c < DP / 2; c += 8) {
-          const int at = group * (DP / 2) + c;
-          if (at >= P.dim) break;
+      for (int i = 0; i < kTcRows / kComputeWarps; i += RPW) {
+        const int r = warp * (kTcRows / kComputeWarps) + i + lane / LPR, c = lane % LPR * 8;
+        float d = 0.0f;
+        if (r0 + r < r1 && c < P.dim) {
           float x[8], y[8], z[8];
-          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g + at)), x);
-          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(o + at)), y);
-          if (low != nullptr) unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(low + at)), z);
+          const int64_t o = P.os.at(b, h0, r0 + r) + c;
+          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.g) + P.gs.at(b, h0, r0 + r) + c)), x);
+          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o) + o)), y);
+          if (P.o_low != nullptr) {
+            unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o_low) + o)), z);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d = fmaf(x[e], low != nullptr ? y[e] + z[e] : y[e], d);
+            for (int e = 0; e < 8; ++e) y[e] += z[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
         }
-        lse = P.lse[stat] * kLog2eF;
+#pragma unroll
+        for (int w = LPR / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+        if (lane % LPR == 0) {
+          ctl.delta[r] = d;
+          if (r0 + r < r1) P.delta[stat + r] = d;
+        }
       }
-      float* halves = &ctl.stats[0][0][0];
-      halves[group * kTcRows + row] = d;
-      named_barrier(1, 256);
-      delta = halves[row] + halves[kTcRows + row];
-      if (live && group == 0) P.delta[stat] = delta;
+      if (r0 + row < r1) lse = P.lse[stat + row] * kLog2eF;
+      named_barrier(1, kComputeWarps * 32);
+      delta = ctl.delta[row];
     }
     // Steps without a masked pair: those whose rows are all there and lie within these bounds.
     int full_lo, full_hi;
@@ -618,33 +693,24 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       if (ok) ok = wait_bar(&ctl.s_full, t & 1);
       __syncwarp();
       tc_fence_after();
-      float p[64];
-      {
-        uint32_t s0[32], s1[32];
-        tmem_load32(t_s + lanes + group * 64, s0);
-        tmem_load32(t_s + lanes + group * 64 + 32, s1);
-        tmem_wait_load();
-        if constexpr (!DKV) {   // s may be overwritten
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&ctl.p_full);
-        }
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          p[c] = __uint_as_float(s0[c]);
-          p[32 + c] = __uint_as_float(s1[c]);
-        }
+      float p[kColumns];
+      tmem_load32(at_s, reinterpret_cast<uint32_t(&)[32]>(p));
+      tmem_wait_load();
+      if constexpr (!DKV) {   // s may be overwritten
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.p_full);
       }
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
+      for (int c = 0; c < kColumns; c += 4) {
         float4 ls = make_float4(lse, lse, lse, lse);
-        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][group * 64 + c]);
+        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][quarter * kColumns + c]);
         p[c] = ex2_approx(fmaf(p[c], P.scale_log2, -ls.x));
         p[c + 1] = ex2_approx(fmaf(p[c + 1], P.scale_log2, -ls.y));
         p[c + 2] = ex2_approx(fmaf(p[c + 2], P.scale_log2, -ls.z));
         p[c + 3] = ex2_approx(fmaf(p[c + 3], P.scale_log2, -ls.w));
       }
-      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+      uint32_t seen = 0xffffffffu;
       if (!full) {
         ColumnMask mask;
         if constexpr (!DKV) {
@@ -655,87 +721,75 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
           const int64_t last = P.window == 0 || key < P.sinks ? (int64_t)kStep : (int64_t)key + P.window - first;
           mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
         }
-        seen[0] = mask.word(group * 64);
-        seen[1] = mask.word(group * 64 + 32);
+        seen = mask.word(quarter * kColumns);
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) p[c0 + c] = seen[c0 / 32] >> c & 1 ? p[c0 + c] : 0.0f;
-        }
+        for (int c = 0; c < kColumns; ++c) p[c] = seen >> c & 1 ? p[c] : 0.0f;
       }
+      uint32_t w[kColumns / 2];
       if constexpr (DKV) {
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 32) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack2<DT>(p[c0 + 2 * e], p[c0 + 2 * e + 1]);
-          tmem_store16(t_s + lanes + group * 64 + c0 / 2, w);
-        }
+        for (int e = 0; e < kColumns / 2; ++e) w[e] = pack2<DT>(p[2 * e], p[2 * e + 1]);
+        tmem_store16(at_s, w);
         tmem_wait_store();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_full);
       }
-      if (ok) ok = wait_bar(&ctl.dp_full, t & 1);
+      if (ok) ok = wait_bar(&ctl.dp_full[t & 1], ring_phase(t, 2));
       __syncwarp();
       tc_fence_after();
-      uint32_t w[32];
+      const uint32_t at_dp = t_dp_of(t) + lanes + quarter * kColumns;
+      uint32_t d[kColumns];
+      tmem_load32(at_dp, d);
+      tmem_wait_load();
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t d[32];
-        tmem_load32(t_dp + lanes + group * 64 + c0, d);
-        tmem_wait_load();
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          float4 de = make_float4(delta, delta, delta, delta);
-          if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * 64 + c0 + c]);
-          const float a = p[c0 + c] * (__uint_as_float(d[c]) - de.x), e = p[c0 + c + 1] * (__uint_as_float(d[c + 1]) - de.y);
-          const float f = p[c0 + c + 2] * (__uint_as_float(d[c + 2]) - de.z),
-                      g = p[c0 + c + 3] * (__uint_as_float(d[c + 3]) - de.w);
-          w[(c0 + c) / 2] = pack2<DT>(a, e);
-          w[(c0 + c) / 2 + 1] = pack2<DT>(f, g);
-        }
-        if (!full) {
-          // dp of a key that is not there may be NaN: 0 * NaN is cleared here.
-#pragma unroll
-          for (int c = 0; c < 32; c += 2)
-            w[(c0 + c) / 2] &= (seen[c0 / 32] >> c & 1 ? 0xffffu : 0u) | (seen[c0 / 32] >> (c + 1) & 1 ? 0xffff0000u : 0u);
-        }
+      for (int c = 0; c < kColumns; c += 4) {
+        float4 de = make_float4(delta, delta, delta, delta);
+        if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][quarter * kColumns + c]);
+        w[c / 2] = pack2<DT>(p[c] * (__uint_as_float(d[c]) - de.x), p[c + 1] * (__uint_as_float(d[c + 1]) - de.y));
+        w[c / 2 + 1] = pack2<DT>(p[c + 2] * (__uint_as_float(d[c + 2]) - de.z), p[c + 3] * (__uint_as_float(d[c + 3]) - de.w));
       }
-      tmem_store32(t_dp + lanes + group * 64, w);
+      if (!full) {
+        // dp of a key that is not there may be NaN: 0 * NaN is cleared here.
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 2)
+          w[c / 2] &= (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u);
+      }
+      tmem_store16(at_dp, w);
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&ctl.ds_full);
+        mbar_arrive(&ctl.ds_full[t & 1]);
         if constexpr (DKV) mbar_arrive(&ctl.stat_free[t & 1]);
       }
     }
     if (ok && steps > 0) ok = wait_bar(&ctl.out_full, 0);
     __syncwarp();
     tc_fence_after();
-    // DKV: the first group stores dk, the second dv; else half of dq's columns each.
+    // DKV: the first two quarters store dk, the others dv, half of the columns each; else all four
+    // store dq, a quarter of the columns each.
     const bool live = r0 + row < r1;
-    constexpr int WIDTH = DKV ? DP : DP / 2;
-    const int c_first = DKV ? 0 : group * WIDTH;
-    const uint32_t t_out = (DKV && group == 1 ? t_out2 : t_out1) + lanes + c_first;
-    const float f = DKV && group == 1 ? 1.0f : P.scale;
+    constexpr int WIDTH = DKV ? DP / 2 : DP / 4, CHUNK = WIDTH < 32 ? WIDTH : 32;
+    const int which = DKV ? quarter >> 1 : 0, c_first = (DKV ? quarter & 1 : quarter) * WIDTH;
+    const uint32_t t_out = (which ? t_out2 : t_out1) + lanes + c_first;
+    const float f = which ? 1.0f : P.scale;
 #pragma unroll
-    for (int c = 0; c < WIDTH; c += 32) {
-      uint32_t v[32];
+    for (int c = 0; c < WIDTH; c += CHUNK) {
+      uint32_t v[CHUNK];
       if (steps > 0) {
-        tmem_load32(t_out + c, v);
+        tmem_load(t_out + c, v);
         tmem_wait_load();
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0u;
+        for (int e = 0; e < CHUNK; ++e) v[e] = 0u;
       }
       if (parts == 1) {
-        void* dst = DKV ? (group == 0 ? P.dk : P.dv) : P.dq;
-        const AttnStrides& st = DKV ? (group == 0 ? P.dks : P.dvs) : P.dqs;
+        void* dst = DKV ? (which ? P.dv : P.dk) : P.dq;
+        const AttnStrides& st = DKV ? (which ? P.dvs : P.dks) : P.dqs;
         uint16_t* out = static_cast<uint16_t*>(dst) + st.at(b, h0, r0 + row) + c_first + c;
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
+        for (int e = 0; e < CHUNK; e += 8) {
           if (!live || c_first + c + e >= P.dim) continue;
           uint32_t q[4];
 #pragma unroll
@@ -745,11 +799,11 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         }
       } else {
         // [batch, key head, sink block, part, 2, 128, dim]
-        float* out = P.partial + (((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + group) *
-                                     kTcRows * P.dim + (int64_t)row * P.dim + c;
+        float* out = P.partial + (((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + which) *
+                                     kTcRows * P.dim + (int64_t)row * P.dim + c_first + c;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          if (c + e >= P.dim) continue;
+        for (int e = 0; e < CHUNK; e += 4) {
+          if (c_first + c + e >= P.dim) continue;
           *reinterpret_cast<float4*>(out + e) =
               make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f,
                           __uint_as_float(v[e + 3]) * f);
@@ -760,7 +814,7 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
   if (!ok && P.error != nullptr) atomicOr(P.error, 1);
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_free(tmem, kBwdColumns);
+  if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -816,8 +870,8 @@ static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
-  const unsigned grid = (unsigned)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
-  attention_tc_forward<DT, DP><<<grid, kTcThreads, FwdShared<DP>::kBytes, s>>>(P, q, k, v);
+  const unsigned grid = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
+  attention_tc_forward<DT, DP><<<grid, kFwdThreads, FwdShared<DP>::kBytes, s>>>(P, q, k, v);
   return launch_status("nt_attention_forward launch");
 }
 

@@ -270,7 +270,7 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     softmax(scale * query @ key.T) over the keys it sees, ``scale`` 1 / sqrt(head_dim) by
     default; a query that sees none gives zeros. What ``key`` and ``value`` hold at or past
     ``lengths[b]`` (an integer tensor [batch], clamped to the keys) has no effect; a NaN or an
-    infinity that some query sees can reach other queries of its block of 128.
+    infinity that some query sees can reach other queries of its block of 256.
 
     Differentiable in query, key and value; sums run in float32 in a fixed order."""
     window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
