@@ -10,6 +10,7 @@
 // Roundings below 32 bits: the weights and dS are rounded to the inputs' type because the second
 // products take their operand in it; every sum, maximum and statistic is float32.
 #include <cmath>
+#include <utility>
 
 #include "nt_attention.cuh"
 #include "nt_tc.cuh"
@@ -41,6 +42,11 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
 }
 // Phase of slot use n of a ring of `size`.
 __device__ __forceinline__ uint32_t ring_phase(int n, int size) { return (uint32_t)(n / size) & 1u; }
+
+template <int N, int... C>
+__device__ __forceinline__ void exponentials(float (&x)[N], std::integer_sequence<int, C...>) {
+  ((x[C] = ex2_mixed<C>(x[C])), ...);
+}
 
 // Rows [rows, next multiple of 16) of a tile are cleared: their weights are 0, but what lies there
 // may be anything, and 0 * NaN must not reach a sum. One warp.
@@ -300,17 +306,19 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 #pragma unroll
           for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) - before);
         }
+        float x[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = fmaf(__uint_as_float(s[c]), P.scale_log2, minus);
+        exponentials(x, std::make_integer_sequence<int, 32>{});
         if (!full) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = seen[c0 / 32] >> c & 1 ? s[c] : 0xff800000u;
+          for (int c = 0; c < 32; ++c) x[c] = seen[c0 / 32] >> c & 1 ? x[c] : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = ex2_approx(fmaf(__uint_as_float(s[2 * e]), P.scale_log2, minus));
-          const float y = ex2_approx(fmaf(__uint_as_float(s[2 * e + 1]), P.scale_log2, minus));
-          sum[0] += x;
-          sum[1] += y;
-          w[e] = pack2<DT>(x, y);
+          sum[0] += x[2 * e];
+          sum[1] += x[2 * e + 1];
+          w[e] = pack2<DT>(x[2 * e], x[2 * e + 1]);
         }
         tmem_store16(t_s + c0 / 2, w);   // over scores that both reads are done with
       }
@@ -329,37 +337,42 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     // Halves in a fixed order, so that both threads of a row have the same sum.
     l = ctl.exchange[g][done & 1][0][row] + ctl.exchange[g][done & 1][1][row];
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const bool live = q0 + row < q1;
-    const int64_t at = P.os.at(b, h, q0 + row) + half * (DP / 2);
-    uint16_t* out = static_cast<uint16_t*>(P.o) + at;
-    uint16_t* low = P.o_low == nullptr ? nullptr : static_cast<uint16_t*>(P.o_low) + at;
+    // The queries' tiles are free now: 32 rows x half of the columns of each warp.
+    constexpr int WIDTH = DP / 2, CH = WIDTH / 8;
+    uint8_t* stage = aligned + warp * 32 * WIDTH * 2;
+    const int row0 = q0 + (warp & 3) * 32, rows = q1 - row0, vectors = (P.dim - half * WIDTH + 7) / 8;
+    const int64_t at = (P.os.at(b, h, row0) + half * WIDTH) * 2;
 #pragma unroll
-    for (int c = 0; c < DP / 2; c += 32) {
-      uint32_t o[32];
-      if (done > 0) {
-        tmem_load32(t_o + c, o);
-        tmem_wait_load();
-      } else {
+    for (int which = 0; which < 2; ++which) {
+      char* dst = static_cast<char*>(which ? P.o_low : P.o);
+      if (dst == nullptr) continue;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0u;
-      }
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        if (!live || half * (DP / 2) + c + e >= P.dim) continue;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // A row without keys is 0 whatever the accumulator holds.
-          const float x = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k]) * f;
-          const float y = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k + 1]) * f;
-          hi[k] = pack2<DT>(x, y);
-          const float2 r = unpack2<DT>(hi[k]);
-          lo[k] = pack2<DT>(x - r.x, y - r.y);
+      for (int c = 0; c < WIDTH; c += 32) {
+        uint32_t o[32];
+        if (done > 0) {
+          tmem_load32(t_o + c, o);
+          tmem_wait_load();
         }
-        *reinterpret_cast<uint4*>(out + c + e) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (low != nullptr) *reinterpret_cast<uint4*>(low + c + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // A row without keys is 0 whatever the accumulator holds.
+            const float x = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k]) * f;
+            const float y = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k + 1]) * f;
+            v[k] = pack2<DT>(x, y);
+            if (which) {
+              const float2 r = unpack2<DT>(v[k]);
+              v[k] = pack2<DT>(x - r.x, y - r.y);
+            }
+          }
+          stage_vector<CH>(stage, lane, (c + e) / 8, make_uint4(v[0], v[1], v[2], v[3]));
+        }
       }
+      store_staged<CH>(stage, lane, dst + at, P.os.t * 2, rows, vectors);
     }
+    const bool live = q0 + row < q1;
     if (live && half == 0 && P.lse != nullptr)
       P.lse[((int64_t)b * P.heads + h) * P.queries + q0 + row] =
           l == 0.0f ? -INFINITY : fmaf(m, P.scale, log2f(l) * kLn2F);
@@ -705,11 +718,12 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       for (int c = 0; c < kColumns; c += 4) {
         float4 ls = make_float4(lse, lse, lse, lse);
         if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][quarter * kColumns + c]);
-        p[c] = ex2_approx(fmaf(p[c], P.scale_log2, -ls.x));
-        p[c + 1] = ex2_approx(fmaf(p[c + 1], P.scale_log2, -ls.y));
-        p[c + 2] = ex2_approx(fmaf(p[c + 2], P.scale_log2, -ls.z));
-        p[c + 3] = ex2_approx(fmaf(p[c + 3], P.scale_log2, -ls.w));
+        p[c] = fmaf(p[c], P.scale_log2, -ls.x);
+        p[c + 1] = fmaf(p[c + 1], P.scale_log2, -ls.y);
+        p[c + 2] = fmaf(p[c + 2], P.scale_log2, -ls.z);
+        p[c + 3] = fmaf(p[c + 3], P.scale_log2, -ls.w);
       }
+      exponentials(p, std::make_integer_sequence<int, kColumns>{});
       uint32_t seen = 0xffffffffu;
       if (!full) {
         ColumnMask mask;
@@ -769,45 +783,59 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     tc_fence_after();
     // DKV: the first two quarters store dk, the others dv, half of the columns each; else all four
     // store dq, a quarter of the columns each.
-    const bool live = r0 + row < r1;
     constexpr int WIDTH = DKV ? DP / 2 : DP / 4, CHUNK = WIDTH < 32 ? WIDTH : 32;
     const int which = DKV ? quarter >> 1 : 0, c_first = (DKV ? quarter & 1 : quarter) * WIDTH;
     const uint32_t t_out = (which ? t_out2 : t_out1) + lanes + c_first;
     const float f = which ? 1.0f : P.scale;
+    const int row0 = r0 + (warp & 3) * 32;
+    // The tiles of x1 and x2 are free now.
+    uint8_t* stage = aligned + warp * 4096;
+    if (parts == 1) {
+      constexpr int CH = WIDTH / 8;
 #pragma unroll
-    for (int c = 0; c < WIDTH; c += CHUNK) {
-      uint32_t v[CHUNK];
-      if (steps > 0) {
-        tmem_load(t_out + c, v);
-        tmem_wait_load();
-      } else {
+      for (int c = 0; c < WIDTH; c += CHUNK) {
+        uint32_t v[CHUNK];
+        if (steps > 0) {
+          tmem_load(t_out + c, v);
+          tmem_wait_load();
+        } else {
 #pragma unroll
-        for (int e = 0; e < CHUNK; ++e) v[e] = 0u;
-      }
-      if (parts == 1) {
-        void* dst = DKV ? (which ? P.dv : P.dk) : P.dq;
-        const AttnStrides& st = DKV ? (which ? P.dvs : P.dks) : P.dqs;
-        uint16_t* out = static_cast<uint16_t*>(dst) + st.at(b, h0, r0 + row) + c_first + c;
+          for (int e = 0; e < CHUNK; ++e) v[e] = 0u;
+        }
 #pragma unroll
         for (int e = 0; e < CHUNK; e += 8) {
-          if (!live || c_first + c + e >= P.dim) continue;
           uint32_t q[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             q[k] = pack2<DT>(__uint_as_float(v[e + 2 * k]) * f, __uint_as_float(v[e + 2 * k + 1]) * f);
-          *reinterpret_cast<uint4*>(out + e) = make_uint4(q[0], q[1], q[2], q[3]);
+          stage_vector<CH>(stage, lane, (c + e) / 8, make_uint4(q[0], q[1], q[2], q[3]));
         }
-      } else {
-        // [batch, key head, sink block, part, 2, 128, dim]
-        float* out = P.partial + (((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + which) *
-                                     kTcRows * P.dim + (int64_t)row * P.dim + c_first + c;
+      }
+      char* dst = static_cast<char*>(DKV ? (which ? P.dv : P.dk) : P.dq);
+      const AttnStrides& st = DKV ? (which ? P.dvs : P.dks) : P.dqs;
+      store_staged<CH>(stage, lane, dst + (st.at(b, h0, row0) + c_first) * 2, st.t * 2, r1 - row0, (P.dim - c_first + 7) / 8);
+    } else {
+      // float32 [batch, key head, sink block, part, 2, 128, dim]
+      char* dst = reinterpret_cast<char*>(
+          P.partial + ((((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + which) * kTcRows +
+                       (warp & 3) * 32) * P.dim + c_first);
+      constexpr int CH = CHUNK / 4;
 #pragma unroll
-        for (int e = 0; e < CHUNK; e += 4) {
-          if (c_first + c + e >= P.dim) continue;
-          *reinterpret_cast<float4*>(out + e) =
-              make_float4(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f, __uint_as_float(v[e + 2]) * f,
-                          __uint_as_float(v[e + 3]) * f);
+      for (int c = 0; c < WIDTH; c += CHUNK) {
+        uint32_t v[CHUNK];
+        if (steps > 0) {
+          tmem_load(t_out + c, v);
+          tmem_wait_load();
+        } else {
+#pragma unroll
+          for (int e = 0; e < CHUNK; ++e) v[e] = 0u;
         }
+#pragma unroll
+        for (int e = 0; e < CHUNK; e += 4)
+          stage_vector<CH>(stage, lane, e / 4,
+                           make_uint4(__float_as_uint(__uint_as_float(v[e]) * f), __float_as_uint(__uint_as_float(v[e + 1]) * f),
+                                      __float_as_uint(__uint_as_float(v[e + 2]) * f), __float_as_uint(__uint_as_float(v[e + 3]) * f)));
+        store_staged<CH>(stage, lane, dst + c * 4, (int64_t)P.dim * 4, 32, (P.dim - c_first - c + 3) / 4);
       }
     }
   }

@@ -170,5 +170,45 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^x on the FP32 pipe: x = n + f with n the nearest integer, 2^f for |f| <= 1/2 by the polynomial
+// of degree 4 with the least largest relative error (2.7e-6, far below a 16-bit weight's own
+// rounding), scaled by 2^n. Down to 2^-126, which stands for everything below; NaN stays NaN.
+__device__ __forceinline__ float ex2_polynomial(float x) {
+  x = max_nan(x, -126.0f);
+  const float t = x + 12582912.0f;   // 1.5 * 2^23: the integer ends up in the low bits
+  const float f = x - (t - 12582912.0f);
+  float p = fmaf(f, 0.009570100344717503f, 0.05591785907745361f);
+  p = fmaf(p, f, 0.240247443318367f);
+  p = fmaf(p, f, 0.6931217908859253f);
+  p = fmaf(p, f, 0.9999992847442627f);
+  return p * __int_as_float((__float_as_int(t) << 23) + 0x3f800000);
+}
+// Exponentials of a thread's columns: the special-function unit gives 16 a cycle and SM, fewer
+// than the tensor cores can use, so every fourth column goes to the FP32 pipe.
+template <int COLUMN>
+__device__ __forceinline__ float ex2_mixed(float x) {
+  return COLUMN % 4 == 3 ? ex2_polynomial(x) : ex2_approx(x);
+}
+
+// 32 rows of a warp, CH 16-byte vectors each, lane r holding row r, written to global memory with
+// whole row segments per instruction (a lane storing its own row would touch 32 lines at a time;
+// that took longer than the products of a short window). `stage`: CH * 512 bytes of this warp's.
+// Rows from `rows` on and vectors from `vectors` on are not stored.
+template <int CH>
+__device__ __forceinline__ void stage_vector(uint8_t* stage, int lane, int k, uint4 v) {
+  *reinterpret_cast<uint4*>(stage + (lane * CH + (k ^ (lane / (8 / CH) % CH))) * 16) = v;
+}
+template <int CH>
+__device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, char* dst, int64_t row_bytes, int rows, int vectors) {
+  __syncwarp();
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 32 / CH) {
+    const int r = r0 + lane / CH, k = lane % CH;
+    if (r < rows && k < vectors)
+      *reinterpret_cast<uint4*>(dst + r * row_bytes + k * 16) =
+          *reinterpret_cast<const uint4*>(stage + (r * CH + (k ^ (r / (8 / CH) % CH))) * 16);
+  }
+  __syncwarp();
+}
 
 }  // namespace nt
