@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -128,6 +129,10 @@ class NormArgs(C.Structure):
 
 NT_ATTENTION_MAX_HEAD_DIM = 128
 _Strides = C.c_int64 * 3
+# The argument blocks of the attention and dropout calls as one struct.pack (their fields in
+# order): building a ctypes Structure field by field costs several times a kernel launch.
+pack_attention = struct.Struct("@ii5q3P9qP3qfiP3qPPPPPP12qPNP").pack
+pack_dropout = struct.Struct("@iiqqdQQPPPPPPN").pack
 
 
 class AttentionArgs(C.Structure):
@@ -218,13 +223,14 @@ SIGNATURES: dict[str, tuple] = {
     "nt_norm_forward": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
     "nt_norm_backward": (C.c_int, [C.POINTER(NormArgs), C.c_void_p]),
     "nt_fused_elementwise": (C.c_int, [C.POINTER(FusedArgs), C.c_void_p]),
-    "nt_attention_workspace_size": (C.c_size_t, [C.POINTER(AttentionArgs)]),
-    "nt_attention_forward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
-    "nt_attention_backward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
-    "nt_attention_step": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    # (c_void_p takes the packed bytes as well as byref(AttentionArgs))
+    "nt_attention_workspace_size": (C.c_size_t, [C.c_void_p]),
+    "nt_attention_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_attention_backward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_attention_step": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nt_dropout_workspace_size": (C.c_size_t, [C.c_int64, C.c_int64]),
-    "nt_dropout_forward": (C.c_int, [C.POINTER(DropoutArgs), C.c_void_p]),
-    "nt_dropout_backward": (C.c_int, [C.POINTER(DropoutArgs), C.c_void_p]),
+    "nt_dropout_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_dropout_backward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nt_xent_workspace_size": (C.c_size_t, []),
     "nt_softmax_xent": (C.c_int, [C.POINTER(XentArgs), C.c_void_p]),
     "nt_xent_backward_scale": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int32,
@@ -238,6 +244,8 @@ _lock = threading.Lock()
 def load(path: str | os.PathLike | None = None):
     """Loads the shared library once and binds every declared symbol."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -304,6 +312,17 @@ def stream_handle(stream=None) -> int:
     if stream is None:
         stream = torch.cuda.current_stream()
     return int(stream.cuda_stream)
+
+
+def on_device(device, name: str, args: bytes, launches: int) -> None:
+    """``call`` with an argument block on the current stream of ``device``, which is made the
+    current device for the call when it is not."""
+    import torch
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(device):
+            return on_device(device, name, args, launches)
+    call(name, args, torch._C._cuda_getCurrentRawStream(index), launches=launches)
 
 
 def dtype_code(dtype) -> int:

@@ -29,9 +29,11 @@ def get_backend(value=None):
     """The CUDA backend of a tensor or device (namitorch/backends/__init__.py:32-48)."""
     import torch
 
-    from .cuda import CUDABackend
     if isinstance(value, torch.Tensor):
         device = value.device
+        known = _backends.get(device)
+        if known is not None:
+            return known
     elif value is None:
         device = torch.device("cuda", torch.cuda.current_device())
     else:
@@ -40,6 +42,7 @@ def get_backend(value=None):
         raise RuntimeError(f"namitorch_b200 has no {device.type} backend: its kernels run on CUDA devices only.")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
+    from .cuda import CUDABackend
     with _lock:
         if device not in _backends:
             _backends[device] = CUDABackend(device)

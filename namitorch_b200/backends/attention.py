@@ -14,25 +14,29 @@ import torch
 
 from .. import _native as N
 
+_CODES = {torch.float32: N.NT_F32, torch.float16: N.NT_F16, torch.bfloat16: N.NT_BF16}
+_NO_STRIDES = (0,) * 12
+
 
 def _rows(tensor):
-    """The tensor itself when the kernels take its layout, else a contiguous copy: a dense last
-    dimension, no broadcast dimension, and 16-byte aligned rows where the width allows them (a
-    tile copy needs them)."""
-    size = tensor.element_size()
-    if tensor.shape[-1] > 1 and tensor.stride(-1) != 1:
-        return tensor.contiguous()
-    aligned = tensor.shape[-1] * size % 16 == 0
-    if aligned and tensor.data_ptr() % 16:
-        return tensor.clone(memory_format=torch.contiguous_format)
-    for extent, stride in zip(tensor.shape[:-1], tensor.stride()[:-1]):
-        if extent > 1 and (stride == 0 or (aligned and stride * size % 16)):
-            return tensor.contiguous()
-    return tensor
+    """(tensor, address, strides of the first three dimensions): the tensor itself when the kernels
+    take its layout, else a contiguous copy. They take a dense last dimension, no broadcast
+    dimension, and 16-byte aligned rows where the width allows them (a tile copy needs them)."""
+    shape, strides, address, size = tensor.shape, tensor.stride(), tensor.data_ptr(), tensor.element_size()
+    aligned = shape[3] * size % 16 == 0
+    good = (shape[3] <= 1 or strides[3] == 1) and not (aligned and address % 16)
+    for i in range(3):
+        if shape[i] > 1 and (strides[i] == 0 or (aligned and strides[i] * size % 16)):
+            good = False
+    if not good:
+        tensor = tensor.clone(memory_format=torch.contiguous_format)
+        strides, address = tensor.stride(), tensor.data_ptr()
+    return tensor, address, strides[:3]
 
 
 def _heads_last(batch, heads, tokens, dim, like):
-    return torch.empty((batch, tokens, heads, dim), dtype=like.dtype, device=like.device).transpose(1, 2)
+    return torch.empty_strided((batch, heads, tokens, dim), (tokens * heads * dim, dim, heads * dim, 1),
+                               dtype=like.dtype, device=like.device)
 
 
 class AttentionCUDAKernels:
@@ -43,7 +47,7 @@ class AttentionCUDAKernels:
     def _error_word(self, device):
         if self._error is None:
             self._error = torch.zeros(1, dtype=torch.int32, device=device)
-        return self._error
+        return self._error.data_ptr()
 
     def check(self) -> None:
         """Raises if a bounded wait inside an attention kernel of this device has ever run out
@@ -51,64 +55,73 @@ class AttentionCUDAKernels:
         if self._error is not None and int(self._error.item()):
             raise RuntimeError("A wait inside an attention kernel ran out; the results of that call are incomplete.")
 
-    def _args(self, query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse):
-        batch, heads, queries, dim = query.shape
-        return N.AttentionArgs(
-            dtype=N.dtype_code(query.dtype), head_dim=dim, batch=batch, query_heads=heads, kv_heads=key.shape[1],
-            queries=queries, keys=key.shape[2], query=query.data_ptr(), key=key.data_ptr(), value=value.data_ptr(),
-            query_strides=query.stride()[:3], key_strides=key.stride()[:3], value_strides=value.stride()[:3],
-            lengths=None if lengths is None else lengths.data_ptr(), window=window, sinks=sinks,
-            query_offset=query_offset, scale=scale, output=output.data_ptr(), output_strides=output.stride()[:3],
-            output_low=None if low is None else low.data_ptr(), lse=None if lse is None else lse.data_ptr(), error=self._error_word(query.device).data_ptr())
-
     def forward(self, query, key, value, lengths=None, *, window=0, sinks=0, query_offset=0, scale, save=True):
         """(output, low, lse). With ``save``, what the backward needs besides the output: lse, float32
         [batch, heads, queries], and for 16-bit types ``low``, the part of the output that its
         rounding took away (the backward subtracts the row sum of gradient * output from dP; over a
         few keys the two nearly cancel, and the rounded output alone would cost the gradients twice
         the error of their own rounding)."""
-        query, key, value = _rows(query), _rows(key), _rows(value)
+        query, q, q_strides = _rows(query)
+        key, k, k_strides = _rows(key)
+        value, v, v_strides = _rows(value)
         batch, heads, queries, dim = query.shape
         output = _heads_last(batch, heads, queries, dim, query)
-        low = _heads_last(batch, heads, queries, dim, query) if save and query.dtype != torch.float32 else None
-        lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=query.device) if save else None
-        with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse)
-            N.call("nt_attention_forward", N.C.byref(args), N.stream_handle(), launches=int(batch * queries > 0))
+        low = lse = None
+        if save:
+            if query.dtype != torch.float32:
+                low = _heads_last(batch, heads, queries, dim, query)
+            lse = torch.empty((batch, heads, queries), dtype=torch.float32, device=query.device)
+        args = N.pack_attention(
+            _CODES[query.dtype], dim, batch, heads, key.shape[1], queries, key.shape[2], q, k, v, *q_strides, *k_strides,
+            *v_strides, 0 if lengths is None else lengths.data_ptr(), window, sinks, query_offset, scale, 0,
+            output.data_ptr(), *output.stride()[:3], 0 if low is None else low.data_ptr(),
+            0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, *_NO_STRIDES, 0, 0, self._error_word(query.device))
+        N.on_device(query.device, "nt_attention_forward", args, int(batch * queries > 0))
         return output, low, lse
 
     def backward(self, query, key, value, output, low, lse, gradient, lengths=None, *, window=0, sinks=0, query_offset=0,
                  scale):
         """(grad_query, grad_key, grad_value)."""
-        query, key, value, gradient = _rows(query), _rows(key), _rows(value), _rows(gradient)
+        query, q, q_strides = _rows(query)
+        key, k, k_strides = _rows(key)
+        value, v, v_strides = _rows(value)
+        gradient, g, g_strides = _rows(gradient)
         batch, heads, queries, dim = query.shape
         kv_heads, keys = key.shape[1], key.shape[2]
         dq = _heads_last(batch, heads, queries, dim, query)
         dk = _heads_last(batch, kv_heads, keys, dim, query)
         dv = _heads_last(batch, kv_heads, keys, dim, query)
-        with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, query_offset, scale, output, low, lse)
-            args.gradient, args.gradient_strides = gradient.data_ptr(), gradient.stride()[:3]
-            args.grad_query, args.grad_query_strides = dq.data_ptr(), dq.stride()[:3]
-            args.grad_key, args.grad_key_strides = dk.data_ptr(), dk.stride()[:3]
-            args.grad_value, args.grad_value_strides = dv.data_ptr(), dv.stride()[:3]
-            size = int(N.load().nt_attention_workspace_size(N.C.byref(args)))
-            workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
-            args.workspace, args.workspace_bytes = workspace.data_ptr(), size
-            statistics = (batch * heads * queries * 4 + 255) // 256 * 256
-            N.call("nt_attention_backward", N.C.byref(args), N.stream_handle(),
-                   launches=int(batch * queries > 0) + int(batch * keys > 0) + int(size > statistics))
+        kv_strides = dk.stride()[:3]
+
+        def pack(workspace, size):
+            return N.pack_attention(
+                _CODES[query.dtype], dim, batch, heads, kv_heads, queries, keys, q, k, v, *q_strides, *k_strides,
+                *v_strides, 0 if lengths is None else lengths.data_ptr(), window, sinks, query_offset, scale, 0,
+                output.data_ptr(), *output.stride()[:3], 0 if low is None else low.data_ptr(), lse.data_ptr(), g,
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *g_strides, *dq.stride()[:3], *kv_strides, *kv_strides,
+                workspace, size, self._error_word(query.device))
+
+        size = int(N.load().nt_attention_workspace_size(pack(0, 0)))
+        workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
+        statistics = (batch * heads * queries * 4 + 255) // 256 * 256
+        N.on_device(query.device, "nt_attention_backward", pack(workspace.data_ptr(), size),
+                    int(batch * queries > 0) + int(batch * keys > 0) + int(size > statistics))
         return dq, dk, dv
 
     def step(self, query, key_cache, value_cache, lengths, *, window=0, sinks=0, scale):
         """query [batch, heads, head_dim] -> [batch, heads, head_dim]."""
-        query, key, value = _rows(query).unsqueeze(2), _rows(key_cache), _rows(value_cache)
-        batch, heads, _, dim = query.shape
-        output = torch.empty((batch, heads, 1, dim), dtype=query.dtype, device=query.device)
-        with torch.cuda.device(query.device):
-            args = self._args(query, key, value, lengths, window, sinks, 0, scale, output, None, None)
-            N.call("nt_attention_step", N.C.byref(args), N.stream_handle(), launches=int(batch > 0))
-        return output.squeeze(2)
+        query = query.contiguous()
+        key, k, k_strides = _rows(key_cache)
+        value, v, v_strides = _rows(value_cache)
+        batch, heads, dim = query.shape
+        output = torch.empty_like(query)
+        strides = (heads * dim, dim, dim)
+        args = N.pack_attention(
+            _CODES[query.dtype], dim, batch, heads, key.shape[1], 1, key.shape[2], query.data_ptr(), k, v, *strides,
+            *k_strides, *v_strides, lengths.data_ptr(), window, sinks, 0, scale, 0, output.data_ptr(), *strides, 0, 0, 0,
+            0, 0, 0, *_NO_STRIDES, 0, 0, self._error_word(query.device))
+        N.on_device(query.device, "nt_attention_step", args, int(batch > 0))
+        return output
 
 
 __all__ = ["AttentionCUDAKernels"]

@@ -10,6 +10,8 @@ import torch
 
 from .. import _native as N
 
+_CODES = {torch.float32: N.NT_F32, torch.float16: N.NT_F16, torch.bfloat16: N.NT_BF16}
+
 
 class DropoutCUDAKernels:
     def __init__(self, backend=None):
@@ -22,14 +24,13 @@ class DropoutCUDAKernels:
         bias = None if bias is None else bias.contiguous()
         residual = None if residual is None else residual.contiguous()
         output = torch.empty_like(input)
-        if not input.numel():
-            return output
-        width = input.shape[-1]
-        args = N.DropoutArgs(dtype=N.dtype_code(input.dtype), rows=input.numel() // width, width=width, p=p, seed=seed,
-                             offset=offset, input=input.data_ptr(), bias=None if bias is None else bias.data_ptr(),
-                             residual=None if residual is None else residual.data_ptr(), output=output.data_ptr())
-        with torch.cuda.device(input.device):
-            N.call("nt_dropout_forward", N.C.byref(args), N.stream_handle())
+        count = input.numel()
+        if count:
+            width = input.shape[-1]
+            args = N.pack_dropout(_CODES[input.dtype], 0, count // width, width, p, seed, offset, input.data_ptr(),
+                                  0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                                  output.data_ptr(), 0, 0, 0)
+            N.on_device(input.device, "nt_dropout_forward", args, 1)
         return output
 
     @staticmethod
@@ -44,13 +45,10 @@ class DropoutCUDAKernels:
             return dx, db
         size = int(N.load().nt_dropout_workspace_size(rows, width)) if needs[1] else 0
         workspace = torch.empty(size, dtype=torch.uint8, device=gradient.device) if size else None
-        args = N.DropoutArgs(dtype=N.dtype_code(gradient.dtype), rows=rows, width=width, p=p, seed=seed, offset=offset,
-                             input=gradient.data_ptr(), output=None if dx is None else dx.data_ptr(),
-                             grad_bias=None if db is None else db.data_ptr(),
-                             workspace=None if workspace is None else workspace.data_ptr(), workspace_bytes=size)
-        with torch.cuda.device(gradient.device):
-            N.call("nt_dropout_backward", N.C.byref(args), N.stream_handle(),
-                   launches=int(rows > 0) * (1 + int(needs[1])))
+        args = N.pack_dropout(_CODES[gradient.dtype], 0, rows, width, p, seed, offset, gradient.data_ptr(), 0, 0,
+                              0 if dx is None else dx.data_ptr(), 0 if db is None else db.data_ptr(),
+                              0 if workspace is None else workspace.data_ptr(), size)
+        N.on_device(gradient.device, "nt_dropout_backward", args, int(rows > 0) * (1 + int(needs[1])))
         return dx, db
 
 

@@ -562,19 +562,13 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
 
 // ---- launches ------------------------------------------------------------------------
 
-static int smem_limit(const void* kernel, size_t bytes, const char* what) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == cudaSuccess ? NT_OK : cuda_fail(e, what);
-}
-
 template <int DT, int DP>
 static int launch_forward(const AttnParams& P, cudaStream_t s) {
   const size_t bytes = (size_t)(2 * kRows * (DP + 4) + kRows * kWeightStride) * 4;
-  auto kernel = attention_forward_kernel<DT, DP>;
-  int rc = smem_limit((const void*)kernel, bytes, "nt_attention_forward");
+  const int rc = large_smem<attention_forward_kernel<DT, DP>>(bytes, "nt_attention_forward");
   if (rc) return rc;
   const dim3 grid((P.queries + kRows - 1) / kRows, P.heads, P.batch);
-  kernel<<<grid, kSimtThreads, bytes, s>>>(P);
+  attention_forward_kernel<DT, DP><<<grid, kSimtThreads, bytes, s>>>(P);
   return launch_status("nt_attention_forward launch");
 }
 
@@ -583,8 +577,8 @@ static int launch_backward(const AttnParams& P, cudaStream_t s) {
   const size_t bytes = (size_t)(4 * kRows * (DP + 4) + 2 * kRows * kWeightStride) * 4;
   auto dq = attention_backward_kernel<DT, DP, false>;
   auto dkv = attention_backward_kernel<DT, DP, true>;
-  int rc = smem_limit((const void*)dq, bytes, "nt_attention_backward");
-  if (!rc) rc = smem_limit((const void*)dkv, bytes, "nt_attention_backward");
+  int rc = large_smem<attention_backward_kernel<DT, DP, false>>(bytes, "nt_attention_backward");
+  if (!rc) rc = large_smem<attention_backward_kernel<DT, DP, true>>(bytes, "nt_attention_backward");
   if (rc) return rc;
   if (P.queries > 0) {
     dq<<<dim3((P.queries + kRows - 1) / kRows, P.heads, P.batch), kSimtThreads, bytes, s>>>(P);

@@ -882,18 +882,13 @@ static int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStri
   return NT_OK;
 }
 
-template <typename K>
-static int large_smem(K kernel, int bytes, const char* who) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == cudaSuccess ? NT_OK : cuda_fail(e, who);
-}
-
 template <int DT, int DP>
 static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
   const char* who = "nt_attention_forward";
   CUtensorMap q, k, v;
-  // A runtime call first: the map encoder is a driver call and needs a context on this thread.
-  int rc = large_smem(attention_tc_forward<DT, DP>, FwdShared<DP>::kBytes, who);
+  // A runtime call first: the map encoder is a driver call and needs a context on this thread
+  // (cudaGetDevice alone does not make one on a thread that has made no other call).
+  int rc = large_smem<attention_tc_forward<DT, DP>>(FwdShared<DP>::kBytes, who);
   if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
@@ -908,8 +903,8 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   const char* who = "nt_attention_backward";
   CUtensorMap q, g, k, v;
   const int bytes = BwdShared<DP>::kBytes;
-  int rc = large_smem(attention_tc_backward<DT, DP, false>, bytes, who);
-  if (!rc) rc = large_smem(attention_tc_backward<DT, DP, true>, bytes, who);
+  int rc = large_smem<attention_tc_backward<DT, DP, false>>(bytes, who);
+  if (!rc) rc = large_smem<attention_tc_backward<DT, DP, true>>(bytes, who);
   if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&g, DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);

@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "namitorch_b200.h"
 #include <nvtx3/nvToolsExt.h>
 
@@ -30,6 +32,21 @@ int current_sm_count();
 inline int launch_status(const char* what) {
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return cuda_fail(err, what);
+  return NT_OK;
+}
+
+// Raises a kernel's limit of dynamic shared memory, once per device.
+template <auto Kernel>
+inline int large_smem(size_t bytes, const char* what) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return cuda_fail(err, what);
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return NT_OK;
+  err = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err != cudaSuccess) return cuda_fail(err, what);
+  done.fetch_or(bit, std::memory_order_relaxed);
   return NT_OK;
 }
 

@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from .. import _native as N
+from ..backends import get_backend
 from ..flat import xent_workspace
 
 _REDUCTIONS = {"none": N.NT_REDUCTION_NONE, "mean": N.NT_REDUCTION_MEAN, "sum": N.NT_REDUCTION_SUM}
@@ -189,6 +190,8 @@ def linear(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 
 def _count(name: str, value, low: int = 0) -> int:
+    if type(value) is int and value >= low:
+        return value
     if isinstance(value, (bool, np.bool_)) or not isinstance(value, Integral):
         raise TypeError(f"{name} must be an integer.")
     if value < low:
@@ -196,38 +199,43 @@ def _count(name: str, value, low: int = 0) -> int:
     return int(value)
 
 
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
 def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale):
-    for name, tensor, want in (("query", query, rank), ("key", key, 4), ("value", value, 4)):
-        if not isinstance(tensor, torch.Tensor):
-            raise TypeError(f"Attention {name} must be a NamiTorch Tensor.")
-        if tensor.dim() != want:
-            raise ValueError(f"Attention {name} must have rank {want}, got shape {tuple(tensor.shape)}.")
-    batch, heads, dim = query.shape[0], query.shape[1], query.shape[-1]
-    if key.shape != value.shape or key.shape[0] != batch or key.shape[3] != dim:
+    if not (isinstance(query, torch.Tensor) and isinstance(key, torch.Tensor) and isinstance(value, torch.Tensor)):
+        raise TypeError("Attention query, key and value must be NamiTorch Tensors.")
+    if query.dim() != rank or key.dim() != 4 or value.dim() != 4:
+        raise ValueError(f"Attention query must have rank {rank}, key and value rank 4, got shapes "
+                         f"{tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}.")
+    shape, kv_shape = query.shape, key.shape
+    batch, heads, dim = shape[0], shape[1], shape[-1]
+    if kv_shape != value.shape or kv_shape[0] != batch or kv_shape[3] != dim:
         raise ValueError(f"Attention key and value must have shape [{batch}, kv_heads, keys, {dim}], got "
-                         f"{tuple(key.shape)} and {tuple(value.shape)}.")
+                         f"{tuple(kv_shape)} and {tuple(value.shape)}.")
     if not 1 <= dim <= N.NT_ATTENTION_MAX_HEAD_DIM:
         raise ValueError(f"Attention head dimension must be in [1, {N.NT_ATTENTION_MAX_HEAD_DIM}], got {dim}.")
-    if heads < 1 or key.shape[1] < 1 or heads % key.shape[1]:
-        raise ValueError(f"Attention needs a whole number of query heads per key head, got {heads} and {key.shape[1]}.")
-    if query.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError(f"Attention supports float32, float16 and bfloat16 tensors, got {query.dtype}.")
-    if key.dtype != query.dtype or value.dtype != query.dtype:
-        raise TypeError(f"Attention query, key and value must have one dtype, got {query.dtype}, {key.dtype} and "
+    if heads < 1 or kv_shape[1] < 1 or heads % kv_shape[1]:
+        raise ValueError(f"Attention needs a whole number of query heads per key head, got {heads} and {kv_shape[1]}.")
+    dtype, device = query.dtype, query.device
+    if dtype not in _DTYPES:
+        raise TypeError(f"Attention supports float32, float16 and bfloat16 tensors, got {dtype}.")
+    if key.dtype != dtype or value.dtype != dtype:
+        raise TypeError(f"Attention query, key and value must have one dtype, got {dtype}, {key.dtype} and "
                         f"{value.dtype}.")
-    if query.device.type != "cuda" or key.device != query.device or value.device != query.device:
+    if device.type != "cuda" or key.device != device or value.device != device:
         raise RuntimeError("namitorch_b200 attention runs on one CUDA device; move query, key and value there first.")
     window = 0 if window is None else _count("window", window, 1)
     sinks = _count("sinks", sinks)
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError("Attention lengths must be an int32 or int64 Tensor or None.")
-        if tuple(lengths.shape) != (batch,):
+        if lengths.shape != (batch,):
             raise ValueError(f"Attention lengths must have shape {(batch,)}, got {tuple(lengths.shape)}.")
-        if lengths.device != query.device:
+        if lengths.device != device:
             raise RuntimeError("Attention lengths must be on the device of the query.")
         if lengths.dtype != torch.int32 or not lengths.is_contiguous():
-            lengths = lengths.clamp(0, key.shape[2]).to(torch.int32).contiguous()
+            lengths = lengths.clamp(0, kv_shape[2]).to(torch.int32).contiguous()
     if scale is None:
         scale = dim ** -0.5
     else:
@@ -242,7 +250,6 @@ def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale)
 class _SlidingWindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, lengths, options):
-        from ..backends import get_backend
         output, low, lse = get_backend(query).attention.forward(query, key, value, lengths, **options)
         ctx.save_for_backward(query, key, value, output, low, lse, lengths)
         ctx.options = options
@@ -250,7 +257,6 @@ class _SlidingWindowAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        from ..backends import get_backend
         query, key, value, output, low, lse, lengths = ctx.saved_tensors
         grads = get_backend(query).attention.backward(query, key, value, output, low, lse, grad_output, lengths,
                                                       **ctx.options)
@@ -278,7 +284,6 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
                "scale": scale}
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _SlidingWindowAttention.apply(query, key, value, lengths, options)
-    from ..backends import get_backend
     return get_backend(query).attention.forward(query, key, value, lengths, save=False, **options)[0]
 
 
@@ -293,7 +298,6 @@ def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, 
     if lengths is None:
         raise TypeError("Attention lengths must be an int32 or int64 Tensor.")
     window, sinks, lengths, scale = _attention_arguments(query, key_cache, value_cache, 3, window, sinks, lengths, scale)
-    from ..backends import get_backend
     return get_backend(query).attention.step(query, key_cache, value_cache, lengths, window=window, sinks=sinks,
                                              scale=scale)
 
@@ -301,13 +305,11 @@ def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, bias, residual, p, seed, offset):
-        from ..backends import get_backend
         ctx.call = (p, seed, offset)
         return get_backend(input).dropout.forward(input, p, seed=seed, offset=offset, bias=bias, residual=residual)
 
     @staticmethod
     def backward(ctx, grad_output):
-        from ..backends import get_backend
         p, seed, offset = ctx.call
         need_input, need_bias, need_residual = ctx.needs_input_grad[:3]
         grad_input, grad_bias = get_backend(grad_output).dropout.backward(
@@ -327,7 +329,7 @@ def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: 
     nothing is dropped."""
     if not isinstance(input, torch.Tensor):
         raise TypeError("dropout input must be a NamiTorch Tensor.")
-    if input.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if input.dtype not in _DTYPES:
         raise TypeError(f"dropout supports float32, float16 and bfloat16 tensors, got {input.dtype}.")
     if input.dim() < 1:
         raise ValueError("dropout input must have rank >= 1.")
@@ -353,7 +355,11 @@ def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: 
             raise RuntimeError(f"dropout {name} must be on the device of the input.")
     if input.device.type != "cuda":
         raise RuntimeError("namitorch_b200 dropout runs on a CUDA device; move the input there first.")
-    return _Dropout.apply(input, bias, residual, float(p) if training else 0.0, int(seed), int(offset))
+    p = float(p) if training else 0.0
+    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(input, bias, residual, p, int(seed), int(offset))
+    return get_backend(input).dropout.forward(input, p, seed=int(seed), offset=int(offset), bias=bias, residual=residual)
 
 
 __all__ = ["cross_entropy", "dropout", "linear", "sliding_window_attention", "sliding_window_attention_step",
