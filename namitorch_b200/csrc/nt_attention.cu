@@ -1,5 +1,5 @@
-// Sliding-window attention with sinks: the C entry points, the kernels for float32 (and for
-// 16-bit rows that are no whole 16-byte vectors) and the one-token step.
+// Sliding-window attention with sinks: the C entry points and the kernels for float32 (and for
+// 16-bit rows that are no whole 16-byte vectors).
 //
 //   S = scale q k^T over the visible keys,  m = max S,  l = sum exp(S - m),
 //   o = sum exp(S - m) v / l,  lse = m + ln l
@@ -370,196 +370,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
   }
 }
 
-// ---- one token over a cache ----------------------------------------------------------
-// Bound: HBM, one read of the visible keys and values. A cluster of blocks shares one
-// (sequence, key head, HG query heads): each block takes a contiguous piece of the visible keys,
-// each warp rows of it, LPR lanes of 16 bytes to a row. Every lane group keeps its own running
-// maximum, sum and output; they are joined over the warp by shuffles, over the block in shared
-// memory and over the cluster in distributed shared memory, always in the same order.
-constexpr int kStepThreads = 256;
-constexpr int kStepWarps = kStepThreads / 32;
-constexpr int kStepRows = 4;   // rows in flight per lane group
-constexpr int kStepMaxCluster = 8;
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
-  uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p)), remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
-  return v;
-}
-
-template <int DT, int LPR, int HG>
-__global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __grid_constant__ AttnParams P) {
-  using T = typename Elem<DT>::T;
-  constexpr int EPV = 16 / (int)sizeof(T);
-  constexpr int DP = LPR * EPV;
-  constexpr int RPL = 32 / LPR;
-  __shared__ float part_ml[kStepWarps][HG][2];
-  __shared__ float part_acc[kStepWarps][HG][DP];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int sub = lane / LPR, col = lane % LPR * EPV;
-  const int splits = gridDim.x, rank = blockIdx.x;
-  const int passes = P.group / HG;
-  const int hk = blockIdx.y / passes, h0 = hk * P.group + blockIdx.y % passes * HG;
-  const int b = blockIdx.z;
-  const int length = attn_length(P, b);
-  int lo = P.window == 0 ? 0 : max(0, length - P.window);
-  const int sink_end = min(P.sinks, lo);
-  const int visible = sink_end + length - lo;
-  const int chunk = (visible + splits - 1) / splits;
-  const int from = min(visible, rank * chunk), to = min(visible, from + chunk);
-  const int skip = lo - sink_end;    // visible key n >= sink_end is row n + skip
-
-  float q[HG][EPV], acc[HG][EPV], m[HG], l[HG];
-#pragma unroll
-  for (int g = 0; g < HG; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) {
-      acc[g][e] = 0.0f;
-      q[g][e] = col + e < P.dim ? load1<DT>(P.q, P.qs.at(b, h0 + g, 0) + col + e) : 0.0f;
-    }
-  }
-  const T* kb = static_cast<const T*>(P.k) + P.ks.at(b, hk, 0) + col;
-  const T* vb = static_cast<const T*>(P.v) + P.vs.at(b, hk, 0) + col;
-  auto load = [&](const T* base, int64_t stride, int n, uint4& raw) {
-    raw = make_uint4(0, 0, 0, 0);
-    if (n < to && col < P.dim) {
-      const int64_t row = n < sink_end ? n : n + skip;
-      const T* src = base + row * stride;
-      if (P.vec) {
-        raw = __ldcs(reinterpret_cast<const uint4*>(src));
-      } else {
-        T* out = reinterpret_cast<T*>(&raw);
-#pragma unroll
-        for (int e = 0; e < EPV; ++e)
-          if (col + e < P.dim) out[e] = src[e];
-      }
-    }
-  };
-  constexpr int STRIDE = kStepWarps * RPL;
-  for (int n0 = from + warp * RPL + sub; n0 - sub < to; n0 += STRIDE * kStepRows) {
-    uint4 kr[kStepRows], vr[kStepRows];
-#pragma unroll
-    for (int r = 0; r < kStepRows; ++r) load(kb, P.ks.t, n0 + r * STRIDE, kr[r]);
-#pragma unroll
-    for (int r = 0; r < kStepRows; ++r) load(vb, P.vs.t, n0 + r * STRIDE, vr[r]);
-    float s[kStepRows][HG];
-#pragma unroll
-    for (int r = 0; r < kStepRows; ++r) {
-      float kf[EPV];
-      unpack16<DT>(kr[r], kf);
-#pragma unroll
-      for (int g = 0; g < HG; ++g) {
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) d = fmaf(q[g][e], kf[e], d);
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        s[r][g] = n0 + r * STRIDE < to ? d : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < HG; ++g) {
-      float top = m[g];
-#pragma unroll
-      for (int r = 0; r < kStepRows; ++r) top = fmaxf(top, s[r][g]);
-      const float shift = top == -INFINITY ? 0.0f : top;
-      const float old = exp2f((m[g] - shift) * P.scale_log2);
-      m[g] = top;
-      l[g] *= old;
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) acc[g][e] *= old;
-#pragma unroll
-      for (int r = 0; r < kStepRows; ++r) {
-        s[r][g] = exp2f((s[r][g] - shift) * P.scale_log2);
-        l[g] += s[r][g];
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kStepRows; ++r) {
-      float vf[EPV];
-      unpack16<DT>(vr[r], vf);
-#pragma unroll
-      for (int g = 0; g < HG; ++g)
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) acc[g][e] = fmaf(s[r][g], vf[e], acc[g][e]);
-    }
-  }
-  // Join the lane groups of a warp, then the warps.
-#pragma unroll
-  for (int g = 0; g < HG; ++g) {
-    float top = m[g];
-#pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float f = top == -INFINITY ? 0.0f : exp2f((m[g] - top) * P.scale_log2);
-    l[g] *= f;
-#pragma unroll
-    for (int e = 0; e < EPV; ++e) acc[g][e] *= f;
-#pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-      l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
-    }
-    if (sub == 0) {
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) part_acc[warp][g][col + e] = acc[g][e];
-      if (lane == 0) {
-        part_ml[warp][g][0] = top;
-        part_ml[warp][g][1] = l[g];
-      }
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < HG * DP; i += kStepThreads) {
-    const int g = i / DP, c = i % DP;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) top = fmaxf(top, part_ml[w][g][0]);
-    float sum = 0.0f, a = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) {
-      const float f = top == -INFINITY ? 0.0f : exp2f((part_ml[w][g][0] - top) * P.scale_log2);
-      sum = fmaf(part_ml[w][g][1], f, sum);
-      a = fmaf(part_acc[w][g][c], f, a);
-    }
-    part_acc[0][g][c] = a;   // only this thread reads column c
-    if (splits == 1) {
-      if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
-    } else {
-      part_acc[1][g][c] = c == 0 ? top : sum;   // statistics of the block: columns 0 and 1
-    }
-  }
-  if (splits == 1) return;
-  __syncthreads();
-  cluster_sync_all();
-  for (int i = rank * kStepThreads + threadIdx.x; i < HG * DP; i += splits * kStepThreads) {
-    const int g = i / DP, c = i % DP;
-    float top = -INFINITY;
-    for (int r = 0; r < splits; ++r) top = fmaxf(top, load_cluster(&part_acc[1][g][0], r));
-    float sum = 0.0f, a = 0.0f;
-    for (int r = 0; r < splits; ++r) {
-      const float t = load_cluster(&part_acc[1][g][0], r);
-      const float f = top == -INFINITY ? 0.0f : exp2f((t - top) * P.scale_log2);
-      sum = fmaf(load_cluster(&part_acc[1][g][1], r), f, sum);
-      a = fmaf(load_cluster(&part_acc[0][g][c], r), f, a);
-    }
-    if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
-  }
-  cluster_sync_all();   // a block's shared memory stays until every block has read it
-}
-
 // ---- launches ------------------------------------------------------------------------
 
 template <int DT, int DP>
@@ -589,44 +399,6 @@ static int launch_backward(const AttnParams& P, cudaStream_t s) {
   if (tiles == 0) return NT_OK;
   dkv<<<dim3(tiles + P.sink_tiles * (P.parts - 1), P.kv_heads, P.batch), kSimtThreads, bytes, s>>>(P);
   return launch_status("nt_attention_backward launch");
-}
-
-template <int DT, int LPR, int HG>
-static int launch_step(const AttnParams& P, cudaStream_t s) {
-  const int passes = P.group / HG;
-  // Visible keys at most; blocks of one cluster share them, at least 64 keys to a block.
-  const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
-  const int64_t units = (int64_t)P.batch * P.kv_heads * passes;
-  int splits = 1;
-  while (splits < kStepMaxCluster && units * splits < 2 * current_sm_count() && most > 64 * splits) splits *= 2;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(splits, P.kv_heads * passes, P.batch);
-  config.blockDim = dim3(kStepThreads);
-  config.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = splits;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  config.attrs = &attr;
-  config.numAttrs = splits > 1 ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&config, attention_step_kernel<DT, LPR, HG>, P);
-  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_step launch"); }
-  return launch_status("nt_attention_step launch");
-}
-
-template <int DT, int LPR>
-static int dispatch_step_heads(const AttnParams& P, cudaStream_t s) {
-  if (P.group % 8 == 0) return launch_step<DT, LPR, 8>(P, s);
-  if (P.group % 4 == 0) return launch_step<DT, LPR, 4>(P, s);
-  if (P.group % 2 == 0) return launch_step<DT, LPR, 2>(P, s);
-  return launch_step<DT, LPR, 1>(P, s);
-}
-
-template <int DT>
-static int dispatch_step(const AttnParams& P, cudaStream_t s) {
-  constexpr int EPV = DT == NT_F32 ? 4 : 8;
-  if (P.dim <= 64) return dispatch_step_heads<DT, 64 / EPV>(P, s);
-  return dispatch_step_heads<DT, 128 / EPV>(P, s);
 }
 
 template <int DT>
@@ -837,12 +609,7 @@ int nt_attention_step(const nt_attention_args* args, void* stream) {
   }
   AttnParams P = attention_params(a);
   P.vec = vector_key(a, a.key, a.key_strides) && vector_key(a, a.value, a.value_strides);
-  cudaStream_t s = as_stream(stream);
-  switch (a.dtype) {
-    case NT_F32: return dispatch_step<NT_F32>(P, s);
-    case NT_F16: return dispatch_step<NT_F16>(P, s);
-    default: return dispatch_step<NT_BF16>(P, s);
-  }
+  return attention_step_launch(P, a.dtype, as_stream(stream));
 }
 
 }  // extern "C"

@@ -2,6 +2,8 @@
 // keys (of a block of queries) and of queries (of a block of keys) that hold every visible pair.
 #pragma once
 
+#include <cuda.h>
+
 #include "nt_common.cuh"
 
 namespace nt {
@@ -78,9 +80,15 @@ struct AttnQueries {
   }
 };
 
+// nt_attention_map.cu: tensor map (column, token, head, batch) of a 16-bit tensor with boxes of 64
+// columns x `rows` tokens, 128-byte swizzle, zeros outside.
+int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st, int dim, int tokens, int heads, int batch,
+             int rows, const char* who);
+// nt_attention_step.cu: one token per sequence.
+int attention_step_launch(const AttnParams& P, int dtype, cudaStream_t s);
 // nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
 constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
-constexpr int kTcQueryStep = 128;   // queries it takes at a time
+constexpr int kTcQueryStep = 128;  // queries it takes at a time
 int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 

@@ -1,0 +1,518 @@
+// Sliding-window attention of one new token per sequence over a cache of keys and values.
+//
+// Bound: HBM, one read of the visible keys and values (2 head_dim elements a key and key head
+// against 4 head_dim products per query head). The visible keys are the sinks [0, sink_end) and the
+// window [lo, length); number n of them is row n or n + skip. A cluster of blocks shares one
+// (sequence, key head, up to 8 query heads): each block takes a contiguous piece of the visible
+// keys, each warp pieces of that, with a running maximum, sum and output of its own; they are
+// joined over the block in shared memory and over the cluster in distributed shared memory, always
+// in the same order.
+#include <cmath>
+
+#include "nt_attention.cuh"
+#include "nt_tc.cuh"
+
+namespace nt {
+
+constexpr int kStepMaxCluster = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
+  uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p)), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+  return v;
+}
+
+// The block's piece [from, to) of the visible keys of its sequence.
+struct StepKeys {
+  int sink_end, skip, from, to;
+  __device__ __forceinline__ StepKeys(const AttnParams& P, int length, int rank, int splits) {
+    const int lo = P.window == 0 ? 0 : max(0, length - P.window);
+    sink_end = min(P.sinks, lo);
+    const int visible = sink_end + length - lo;
+    const int chunk = (visible + splits - 1) / splits;
+    from = min(visible, rank * chunk);
+    to = min(visible, from + chunk);
+    skip = lo - sink_end;
+  }
+  __device__ __forceinline__ int64_t row(int n) const { return n < sink_end ? n : (int64_t)n + skip; }
+};
+
+// Joins the partial results of the block's warps (maximum and sum in ml[warp][head][2], output in
+// acc[warp][head][DP], unnormalised) and of the cluster's blocks and stores the output. `acc` is in
+// shared memory at the same place in every block.
+template <int DT, int DP, int WARPS, int HEADS>
+__device__ __forceinline__ void join_step(const AttnParams& P, float* acc, const float* ml, int heads, int b, int h0, int splits,
+                                          int rank) {
+  constexpr int THREADS = WARPS * 32, STRIDE = HEADS * DP;
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * DP; i += THREADS) {
+    const int g = i / DP, c = i % DP;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[(w * HEADS + g) * 2]);
+    float sum = 0.0f, a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = top == -INFINITY ? 0.0f : exp2f((ml[(w * HEADS + g) * 2] - top) * P.scale_log2);
+      sum = fmaf(ml[(w * HEADS + g) * 2 + 1], f, sum);
+      a = fmaf(acc[w * STRIDE + i], f, a);
+    }
+    if (splits == 1) {
+      if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
+    } else {
+      acc[i] = a;                             // only this thread reads column i of the partial outputs
+      acc[STRIDE + i] = c == 0 ? top : sum;   // statistics of the block: columns 0 and 1
+    }
+  }
+  if (splits == 1) return;
+  __syncthreads();
+  cluster_sync_all();
+  for (int i = rank * THREADS + threadIdx.x; i < heads * DP; i += splits * THREADS) {
+    const int g = i / DP, c = i % DP;
+    float top = -INFINITY;
+    for (int r = 0; r < splits; ++r) top = fmaxf(top, load_cluster(acc + STRIDE + g * DP, r));
+    float sum = 0.0f, a = 0.0f;
+    for (int r = 0; r < splits; ++r) {
+      const float f = top == -INFINITY ? 0.0f : exp2f((load_cluster(acc + STRIDE + g * DP, r) - top) * P.scale_log2);
+      sum = fmaf(load_cluster(acc + STRIDE + g * DP + 1, r), f, sum);
+      a = fmaf(load_cluster(acc + i, r), f, a);
+    }
+    if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
+  }
+  cluster_sync_all();   // a block's shared memory stays until every block has read it
+}
+
+// ---- 16-bit rows of whole 16-byte vectors ------------------------------------------------
+// A warp owns a ring of 16-key stages that tiled copies fill, 2 KB each (copies of single rows, 256
+// bytes, came at one per 30 cycles and SM, a third of the bandwidth); the 128-byte swizzle spreads
+// the eight rows that an ldmatrix reads over the banks. The products are the small matrix
+// instructions, with the keys as their 16 rows and the query heads as their 8 columns: S^T = K q^T,
+// O^T += V^T P^T. (A tcgen05 product has 128 rows; a group of query heads has one to eight.) P^T is
+// the accumulator of the first as the second operand of the other, transposed between the lanes in
+// registers. The weights are rounded to the type of the values for the second product.
+constexpr int kRingWarps = 4;
+constexpr int kRingKeys = 16;
+
+template <int DP> struct StepShared {
+  static constexpr int kTile = kRingKeys * DP * 2;      // keys or values
+  static constexpr int kStages = DP == 128 ? 3 : 6;
+  static constexpr int kRing = kStages * 2 * kTile;
+  static constexpr int kBytes = kRingWarps * kRing + 1024;
+  static_assert(kRingWarps * 8 * DP * 4 <= kBytes - 1024, "the partial outputs take the rings' place");
+};
+
+// The block's pieces of 16 keys: those of the sinks, then those of the window.
+struct StepPieces {
+  int sink_end, lo, length, sinks, from, to;
+  __device__ __forceinline__ StepPieces(const AttnParams& P, int n, int rank, int splits) : length(n) {
+    lo = P.window == 0 ? 0 : max(0, n - P.window);
+    sink_end = min(P.sinks, lo);
+    sinks = (sink_end + kRingKeys - 1) / kRingKeys;
+    const int pieces = sinks + (n - lo + kRingKeys - 1) / kRingKeys;
+    const int chunk = (pieces + splits - 1) / splits;
+    from = min(pieces, rank * chunk);
+    to = min(pieces, from + chunk);
+  }
+  __device__ __forceinline__ void piece(int i, int& row, int& rows) const {
+    row = i < sinks ? i * kRingKeys : lo + (i - sinks) * kRingKeys;
+    rows = min(kRingKeys, (i < sinks ? sink_end : length) - row);
+  }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_transposed(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void mma16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (DT == NT_BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(kRingWarps * 32)
+attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v) {
+  using Shape = StepShared<DP>;
+  constexpr int STAGES = Shape::kStages, TILE = Shape::kTile;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[kRingWarps][STAGES];
+  __shared__ float ml[kRingWarps][8][2];
+  // The same place in every block of the cluster.
+  uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int passes = (P.group + 7) / 8;
+  const int hk = blockIdx.y / passes, first = blockIdx.y % passes * 8;
+  const int h0 = hk * P.group + first, heads = min(8, P.group - first);
+  const int b = blockIdx.z;
+  const StepPieces pieces(P, attn_length(P, b), rank, splits);
+  uint8_t* mine = ring + warp * Shape::kRing;
+
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) mbar_init(&full[warp][s], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+
+  const int blocks = pieces.to - pieces.from;
+  const int count = blocks > warp ? (blocks - warp + kRingWarps - 1) / kRingWarps : 0;   // of this warp
+  auto fill = [&](int i) {
+    if (lane == 0) {
+      int row, rows;
+      pieces.piece(pieces.from + warp + i * kRingWarps, row, rows);
+      uint64_t* bar = &full[warp][i % STAGES];
+      uint8_t* dst = mine + i % STAGES * 2 * TILE;
+      mbar_arrive_expect_tx(bar, 2 * TILE);
+#pragma unroll
+      for (int half = 0; half < DP / 64; ++half) {
+        tma_load(dst + half * kRingKeys * 128, &map_k, half * 64, row, hk, b, bar);
+        tma_load(dst + TILE + half * kRingKeys * 128, &map_v, half * 64, row, hk, b, bar);
+      }
+    }
+  };
+  for (int i = 0; i < min(count, STAGES); ++i) fill(i);
+
+  const int steps = (P.dim + 15) / 16;
+  uint32_t q[DP / 16][2];
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = k * 16 + e * 8 + 2 * t;
+      uint32_t v = 0;
+      if (g < heads) {
+        const uint16_t* src = static_cast<const uint16_t*>(P.q) + P.qs.at(b, h0 + g, 0);
+        v = (c < P.dim ? src[c] : 0u) | (uint32_t)(c + 1 < P.dim ? src[c + 1] : 0u) << 16;
+      }
+      q[k][e] = v;
+    }
+  float acc[DP / 16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[k][e] = 0.0f;
+
+  bool ok = true;
+  int i = 0;
+  for (; i < count; ++i) {
+    ok = __all_sync(0xffffffffu, wait_bar(&full[warp][i % STAGES], (i / STAGES) & 1));
+    if (!ok) break;
+    uint8_t* stage = mine + i % STAGES * 2 * TILE;
+    int row, rows;
+    pieces.piece(pieces.from + warp + i * kRingWarps, row, rows);
+    if (rows < kRingKeys) {
+      // What lies past the last visible key may be anything; its weight is 0, but 0 * NaN must not
+      // reach the sum.
+      for (int n = lane; n < (kRingKeys - rows) * (DP / 8); n += 32)
+        *reinterpret_cast<uint4*>(stage + TILE + n % (DP / 64) * kRingKeys * 128 + (rows + n / (DP / 8)) * 128 +
+                                  n / (DP / 64) % 8 * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();   // the next copy into this stage comes after it
+      __syncwarp();
+    }
+    // Lane's row of the four 8 x 8 matrices of a 16 x 16 tile, and the 16-byte vector of its columns,
+    // where the swizzle put it.
+    const uint32_t at_k = smem_u32(stage) + (lane & 15) * 128;
+    const uint32_t at_v = smem_u32(stage) + TILE + ((lane >> 4) * 8 + (lane & 7)) * 128;
+    const int vec_k = lane >> 4, vec_v = lane >> 3 & 1, swap = lane & 7;
+    auto column = [&](int k, int vec) {
+      return (uint32_t)((k >> 2) * kRingKeys * 128 + ((((k & 3) * 2 + vec) ^ swap) << 4));
+    };
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+      if (k < steps) {
+        uint32_t a[4];
+        ldmatrix4(at_k + column(k, vec_k), a);
+        mma16x8x16<DT>(s, a, q[k][0], q[k][1]);
+      }
+    // s: keys g and g + 8, heads 2 t and 2 t + 1.
+    if (g >= rows) s[0] = s[1] = -INFINITY;
+    if (g + 8 >= rows) s[2] = s[3] = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float top = fmaxf(s[e], s[e + 2]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmaxf(top, m[e]);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      const float old = ex2_approx((m[e] - shift) * P.scale_log2);
+      m[e] = top;
+      s[e] = ex2_approx((s[e] - shift) * P.scale_log2);
+      s[e + 2] = ex2_approx((s[e + 2] - shift) * P.scale_log2);
+      l[e] = fmaf(l[e], old, s[e] + s[e + 2]);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        acc[k][e] *= old;
+        acc[k][e + 2] *= old;
+      }
+    }
+    const uint32_t p0 = transpose8x8(pack2<DT>(s[0], s[1])), p1 = transpose8x8(pack2<DT>(s[2], s[3]));
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+      if (k < steps) {
+        uint32_t a[4];
+        ldmatrix4_transposed(at_v + column(k, vec_v), a);
+        mma16x8x16<DT>(acc[k], a, p0, p1);
+      }
+    __syncwarp();
+    if (i + STAGES < count) fill(i + STAGES);
+  }
+  if (!ok) {   // the copies in flight land before the block may end
+    for (int n = i; n < min(count, i + STAGES); ++n) wait_bar(&full[warp][n % STAGES], (n / STAGES) & 1);
+    if (lane == 0 && P.error != nullptr) atomicOr(P.error, 1);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], o);
+  __syncthreads();   // every warp is done with its ring
+  float* part = reinterpret_cast<float*>(ring) + warp * 8 * DP;
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[(2 * t + (e & 1)) * DP + k * 16 + g + (e >> 1) * 8] = acc[k][e];
+  if (g == 0) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      ml[warp][2 * t + e][0] = m[e];
+      ml[warp][2 * t + e][1] = l[e];
+    }
+  }
+  join_step<DT, DP, kRingWarps, 8>(P, reinterpret_cast<float*>(ring), &ml[0][0][0], heads, b, h0, splits, rank);
+}
+
+// ---- float32, and 16-bit rows of any layout ------------------------------------------------
+// Lanes of 16 bytes share a row (LPR of them); every lane group keeps its own running maximum, sum
+// and output for HG query heads, joined over the warp by shuffles.
+constexpr int kStepThreads = 256;
+constexpr int kStepWarps = kStepThreads / 32;
+constexpr int kStepRows = 4;   // rows in flight per lane group
+
+template <int DT, int LPR, int HG>
+__global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __grid_constant__ AttnParams P) {
+  using T = typename Elem<DT>::T;
+  constexpr int EPV = 16 / (int)sizeof(T);
+  constexpr int DP = LPR * EPV;
+  constexpr int RPL = 32 / LPR;
+  __shared__ float part_ml[kStepWarps][HG][2];
+  __shared__ __align__(16) float part_acc[kStepWarps][HG][DP];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int sub = lane / LPR, col = lane % LPR * EPV;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const int passes = P.group / HG;
+  const int hk = blockIdx.y / passes, h0 = hk * P.group + blockIdx.y % passes * HG;
+  const int b = blockIdx.z;
+  const StepKeys keys(P, attn_length(P, b), rank, splits);
+  const int from = keys.from, to = keys.to;
+
+  float q[HG][EPV], acc[HG][EPV], m[HG], l[HG];
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    m[g] = -INFINITY;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) {
+      acc[g][e] = 0.0f;
+      q[g][e] = col + e < P.dim ? load1<DT>(P.q, P.qs.at(b, h0 + g, 0) + col + e) : 0.0f;
+    }
+  }
+  const T* kb = static_cast<const T*>(P.k) + P.ks.at(b, hk, 0) + col;
+  const T* vb = static_cast<const T*>(P.v) + P.vs.at(b, hk, 0) + col;
+  auto load = [&](const T* base, int64_t stride, int n, uint4& raw) {
+    raw = make_uint4(0, 0, 0, 0);
+    if (n < to && col < P.dim) {
+      const T* src = base + keys.row(n) * stride;
+      if (P.vec) {
+        raw = __ldcs(reinterpret_cast<const uint4*>(src));
+      } else {
+        T* out = reinterpret_cast<T*>(&raw);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e)
+          if (col + e < P.dim) out[e] = src[e];
+      }
+    }
+  };
+  constexpr int STRIDE = kStepWarps * RPL;
+  for (int n0 = from + warp * RPL + sub; n0 - sub < to; n0 += STRIDE * kStepRows) {
+    uint4 kr[kStepRows], vr[kStepRows];
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) load(kb, P.ks.t, n0 + r * STRIDE, kr[r]);
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) load(vb, P.vs.t, n0 + r * STRIDE, vr[r]);
+    float s[kStepRows][HG];
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) {
+      float kf[EPV];
+      unpack16<DT>(kr[r], kf);
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        float d = 0.0f;
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) d = fmaf(q[g][e], kf[e], d);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        s[r][g] = n0 + r * STRIDE < to ? d : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < HG; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int r = 0; r < kStepRows; ++r) top = fmaxf(top, s[r][g]);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      const float old = exp2f((m[g] - shift) * P.scale_log2);
+      m[g] = top;
+      l[g] *= old;
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) acc[g][e] *= old;
+#pragma unroll
+      for (int r = 0; r < kStepRows; ++r) {
+        s[r][g] = exp2f((s[r][g] - shift) * P.scale_log2);
+        l[g] += s[r][g];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r) {
+      float vf[EPV];
+      unpack16<DT>(vr[r], vf);
+#pragma unroll
+      for (int g = 0; g < HG; ++g)
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) acc[g][e] = fmaf(s[r][g], vf[e], acc[g][e]);
+    }
+  }
+  // Join the lane groups of a warp, then the warps.
+#pragma unroll
+  for (int g = 0; g < HG; ++g) {
+    float top = m[g];
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = top == -INFINITY ? 0.0f : exp2f((m[g] - top) * P.scale_log2);
+    l[g] *= f;
+#pragma unroll
+    for (int e = 0; e < EPV; ++e) acc[g][e] *= f;
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) acc[g][e] += __shfl_xor_sync(0xffffffffu, acc[g][e], o);
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int e = 0; e < EPV; ++e) part_acc[warp][g][col + e] = acc[g][e];
+      if (lane == 0) {
+        part_ml[warp][g][0] = top;
+        part_ml[warp][g][1] = l[g];
+      }
+    }
+  }
+  join_step<DT, DP, kStepWarps, HG>(P, &part_acc[0][0][0], &part_ml[0][0][0], HG, b, h0, splits, rank);
+}
+
+// Blocks of one cluster share the visible keys: enough of them that `want` blocks run on the device,
+// with at least `least` keys to a block.
+static int step_splits(const AttnParams& P, int64_t units, int want, int least) {
+  const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
+  int splits = 1;
+  while (splits < kStepMaxCluster && units * splits < want && most > (int64_t)least * splits) splits *= 2;
+  return splits;
+}
+
+template <typename K, typename... Maps>
+static int launch_step(K kernel, const AttnParams& P, int splits, int heads, int threads, size_t bytes, cudaStream_t s,
+                       const Maps&... maps) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(splits, heads, P.batch);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = splits > 1 ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&config, kernel, P, maps...);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_step launch"); }
+  return launch_status("nt_attention_step launch");
+}
+
+template <int DT, int DP>
+static int launch_ring(const AttnParams& P, cudaStream_t s) {
+  const char* who = "nt_attention_step";
+  CUtensorMap k, v;
+  int rc = large_smem<attention_step_ring_kernel<DT, DP>>(StepShared<DP>::kBytes, who);
+  if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
+  if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
+  if (rc) return rc;
+  const int heads = P.kv_heads * ((P.group + 7) / 8);
+  const int splits = step_splits(P, (int64_t)P.batch * heads, 3 * current_sm_count(), kRingWarps * kRingKeys);
+  return launch_step(attention_step_ring_kernel<DT, DP>, P, splits, heads, kRingWarps * 32, StepShared<DP>::kBytes, s, k, v);
+}
+
+template <int DT, int LPR, int HG>
+static int launch_simt(const AttnParams& P, cudaStream_t s) {
+  const int heads = P.kv_heads * (P.group / HG);
+  const int splits = step_splits(P, (int64_t)P.batch * heads, 2 * current_sm_count(), 64);
+  return launch_step(attention_step_kernel<DT, LPR, HG>, P, splits, heads, kStepThreads, 0, s);
+}
+
+template <int DT, int LPR>
+static int dispatch_heads(const AttnParams& P, cudaStream_t s) {
+  if (P.group % 4 == 0) return launch_simt<DT, LPR, 4>(P, s);
+  if (P.group % 2 == 0) return launch_simt<DT, LPR, 2>(P, s);
+  return launch_simt<DT, LPR, 1>(P, s);
+}
+
+template <int DT>
+static int dispatch_step(const AttnParams& P, cudaStream_t s) {
+  if constexpr (DT != NT_F32) {
+    if (P.vec && P.keys > 0) return P.dim <= 64 ? launch_ring<DT, 64>(P, s) : launch_ring<DT, 128>(P, s);
+  }
+  constexpr int EPV = DT == NT_F32 ? 4 : 8;
+  return P.dim <= 64 ? dispatch_heads<DT, 64 / EPV>(P, s) : dispatch_heads<DT, 128 / EPV>(P, s);
+}
+
+int attention_step_launch(const AttnParams& P, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case NT_F32: return dispatch_step<NT_F32>(P, s);
+    case NT_F16: return dispatch_step<NT_F16>(P, s);
+    default: return dispatch_step<NT_BF16>(P, s);
+  }
+}
+
+}  // namespace nt

@@ -847,47 +847,10 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 
 // ---- host ------------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
-
-// (column, token, head, batch) of one tensor, boxes of 64 columns x `rows` tokens, zeros outside.
-static int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st, int dim, int tokens, int heads,
-                    int batch, int rows, const char* who) {
-  EncodeTiled encode = encode_tiled();
-  if (!encode) { set_error("%s: the driver has no cuTensorMapEncodeTiled", who); return NT_ECUDA; }
-  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
-  // The stride of a dimension of one element is never used, but has to be a valid one.
-  const cuuint64_t row_bytes = ((cuuint64_t)dim * 2 + 15) / 16 * 16;
-  const cuuint64_t strides[3] = {tokens > 1 ? (cuuint64_t)st.t * 2 : row_bytes, heads > 1 ? (cuuint64_t)st.h * 2 : row_bytes,
-                                 batch > 1 ? (cuuint64_t)st.b * 2 : row_bytes};
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, ones[4] = {1, 1, 1, 1};
-  const CUresult rc = encode(map, dtype == NT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                             const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (rc != CUDA_SUCCESS) { set_error("%s: cuTensorMapEncodeTiled failed (%d)", who, (int)rc); return NT_ECUDA; }
-  return NT_OK;
-}
-
 template <int DT, int DP>
 static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
   const char* who = "nt_attention_forward";
   CUtensorMap q, k, v;
-  // A runtime call first: the map encoder is a driver call and needs a context on this thread
-  // (cudaGetDevice alone does not make one on a thread that has made no other call).
   int rc = large_smem<attention_tc_forward<DT, DP>>(FwdShared<DP>::kBytes, who);
   if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
