@@ -443,12 +443,14 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
   join_step<DT, DP, kStepWarps, HG>(P, &part_acc[0][0][0], &part_ml[0][0][0], HG, b, h0, splits, rank);
 }
 
-// Blocks of one cluster share the visible keys: enough of them that `want` blocks run on the device,
-// with at least `least` keys to a block.
-static int step_splits(const AttnParams& P, int64_t units, int want, int least) {
+// Blocks of one cluster share the visible keys: as many as the device runs at once (`most_blocks`:
+// a second wave of short pieces costs more than the idle SMs of one; 32 sequences with 4 key heads
+// and a 4096-key window take 39 us in clusters of 2 and 47 in clusters of 4), with at least `least`
+// keys to a block.
+static int step_splits(const AttnParams& P, int64_t units, int most_blocks, int least) {
   const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
   int splits = 1;
-  while (splits < kStepMaxCluster && units * splits < want && most > (int64_t)least * splits) splits *= 2;
+  while (splits < kStepMaxCluster && units * splits * 2 <= most_blocks && most > (int64_t)least * splits) splits *= 2;
   return splits;
 }
 
@@ -480,7 +482,7 @@ static int launch_ring(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
   if (rc) return rc;
   const int heads = P.kv_heads * ((P.group + 7) / 8);
-  const int splits = step_splits(P, (int64_t)P.batch * heads, 3 * current_sm_count(), kRingWarps * kRingKeys);
+  const int splits = step_splits(P, (int64_t)P.batch * heads, 2 * current_sm_count(), kRingWarps * kRingKeys);
   return launch_step(attention_step_ring_kernel<DT, DP>, P, splits, heads, kRingWarps * 32, StepShared<DP>::kBytes, s, k, v);
 }
 

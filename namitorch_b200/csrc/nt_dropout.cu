@@ -48,7 +48,7 @@ __device__ __forceinline__ uint4 philox7(uint64_t counter, const DropoutParams& 
 constexpr int kDropoutColumns = 8;
 constexpr int kDropoutThreads = 256;
 // Partial rows of the bias gradient (row slots of the grid) at most.
-constexpr int64_t kDropoutMaxSlots = 512;
+constexpr int64_t kDropoutMaxSlots = 1024;
 
 // The keep factors (0 or 1 / (1 - p)) of the V columns from flat element e0. On the vector path
 // e0 is a multiple of 8; otherwise a thread's columns start anywhere in a counter's four words,
@@ -142,10 +142,9 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.0f;
   if (live > 0) {
-    for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < P.rows; row += (int64_t)gridDim.y * blockDim.y) {
-      const int64_t e0 = row * P.width + c0;
-      float g[V], f[V];
-      load_columns<DT, VEC>(P.x, e0, live, g);
+    const int64_t stride = (int64_t)gridDim.y * blockDim.y;
+    auto body = [&](int64_t e0, float (&g)[V]) {
+      float f[V];
       keep_factors<VEC>(e0, P, f);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
@@ -153,6 +152,21 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
         if constexpr (AFFINE) acc[k] += g[k];
       }
       if (P.y != nullptr) store_columns<DT, VEC>(P.y, e0, live, g);
+    };
+    int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y;
+    for (; row + stride < P.rows; row += 2 * stride) {   // two rows in flight
+      const int64_t e0 = row * P.width + c0, e1 = e0 + stride * P.width;
+      float g0[V], g1[V];
+      load_columns<DT, VEC>(P.x, e0, live, g0);
+      load_columns<DT, VEC>(P.x, e1, live, g1);
+      body(e0, g0);
+      body(e1, g1);
+    }
+    if (row < P.rows) {
+      const int64_t e0 = row * P.width + c0;
+      float g[V];
+      load_columns<DT, VEC>(P.x, e0, live, g);
+      body(e0, g);
     }
   }
   if constexpr (AFFINE) {
@@ -170,9 +184,9 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
   }
 }
 
-// Column sums of the partial rows: lane j of a column adds partial rows j, j + 8, ... in order,
-// then the eight lane sums are added in lane order.
-constexpr int kReduceLanes = 8;
+// Column sums of the partial rows: lane j of a column adds partial rows j, j + 32, ... in order,
+// then the lane sums are added in lane order.
+constexpr int kReduceLanes = 32;
 template <int DT>
 __global__ void __launch_bounds__(32 * kReduceLanes)
 dropout_bias_reduce_kernel(const float* partial, int64_t slots, int64_t width, void* out) {
@@ -180,6 +194,7 @@ dropout_bias_reduce_kernel(const float* partial, int64_t slots, int64_t width, v
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
   float s = 0.0f;
   if (c < width)
+#pragma unroll 4
     for (int64_t k = threadIdx.y; k < slots; k += kReduceLanes) s += partial[k * width + c];
   lanes[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
@@ -196,22 +211,22 @@ struct DropoutGrid {
 
 // Blocks of CX x RY threads over [rows, width / 8]: rows wider than 256 threads are cut into
 // equal parts, narrow ones share a block; the grid holds as many row slots as fit on the
-// device at eight blocks per SM.
-static DropoutGrid dropout_grid(int64_t rows, int64_t width) {
+// device at `per_sm` blocks per SM.
+static DropoutGrid dropout_grid(int64_t rows, int64_t width, int per_sm) {
   const int64_t groups = (width + kDropoutColumns - 1) / kDropoutColumns;
   const int64_t parts = (groups + kDropoutThreads - 1) / kDropoutThreads;
   const int64_t cx = (groups + parts - 1) / parts;
   const int64_t ry = kDropoutThreads / cx;
-  int64_t slots = ((int64_t)current_sm_count() * 8 + parts - 1) / parts;
+  int64_t slots = ((int64_t)current_sm_count() * per_sm + parts - 1) / parts;
   if (slots > (rows + ry - 1) / ry) slots = (rows + ry - 1) / ry;
-  if (slots > kDropoutMaxSlots) slots = kDropoutMaxSlots;
+  if (slots > 65535) slots = 65535;
   if (slots < 1) slots = 1;
   return {dim3((unsigned)parts, (unsigned)slots), dim3((unsigned)cx, (unsigned)ry)};
 }
 
 template <int DT>
 static int launch_dropout_forward(const DropoutParams& P, bool vec, cudaStream_t s) {
-  const DropoutGrid g = dropout_grid(P.rows, P.width);
+  const DropoutGrid g = dropout_grid(P.rows, P.width, 8);
   if (vec) dropout_forward_kernel<DT, true><<<g.grid, g.block, 0, s>>>(P);
   else dropout_forward_kernel<DT, false><<<g.grid, g.block, 0, s>>>(P);
   return launch_status("nt_dropout_forward launch");
@@ -219,7 +234,8 @@ static int launch_dropout_forward(const DropoutParams& P, bool vec, cudaStream_t
 
 template <int DT>
 static int launch_dropout_backward(const DropoutParams& P, bool vec, void* grad_bias, cudaStream_t s) {
-  const DropoutGrid g = dropout_grid(P.rows, P.width);
+  DropoutGrid g = dropout_grid(P.rows, P.width, 4);
+  if (g.grid.y > kDropoutMaxSlots) g.grid.y = kDropoutMaxSlots;
   if (grad_bias == nullptr) {
     if (vec) dropout_backward_kernel<DT, true, false><<<g.grid, g.block, 0, s>>>(P);
     else dropout_backward_kernel<DT, false, false><<<g.grid, g.block, 0, s>>>(P);
