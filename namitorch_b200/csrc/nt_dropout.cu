@@ -23,21 +23,19 @@ struct DropoutParams {
   int64_t width;
   uint32_t threshold;
   float scale;
-  uint32_t key0, key1, offset0, offset1;
+  uint32_t offset0, offset1;
+  uint32_t keys[7][2];   // of the rounds: operands in constant memory, nothing to compute per call
 };
 
 __device__ __forceinline__ uint4 philox7(uint64_t counter, const DropoutParams& P) {
   uint32_t a = (uint32_t)counter, b = (uint32_t)(counter >> 32), c = P.offset0, d = P.offset1;
-  uint32_t k0 = P.key0, k1 = P.key1;
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
     const uint64_t x = (uint64_t)a * 0xD2511F53u, y = (uint64_t)c * 0xCD9E8D57u;
-    a = (uint32_t)(y >> 32) ^ b ^ k0;
+    a = (uint32_t)(y >> 32) ^ b ^ P.keys[r][0];
     b = (uint32_t)y;
-    c = (uint32_t)(x >> 32) ^ d ^ k1;
+    c = (uint32_t)(x >> 32) ^ d ^ P.keys[r][1];
     d = (uint32_t)x;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(a, b, c, d);
 }
@@ -50,21 +48,21 @@ constexpr int kDropoutThreads = 256;
 // Partial rows of the bias gradient (row slots of the grid) at most.
 constexpr int64_t kDropoutMaxSlots = 1024;
 
-// The keep factors (0 or 1 / (1 - p)) of the V columns from flat element e0. On the vector path
-// e0 is a multiple of 8; otherwise a thread's columns start anywhere in a counter's four words,
+// Which of the V columns from flat element e0 are kept. On the vector path e0 is a multiple of 8;
+// otherwise a thread's columns start anywhere in a counter's four words,
 // and one more counter than V / 4 covers them.
 template <bool VEC>
-__device__ __forceinline__ void keep_factors(int64_t e0, const DropoutParams& P, float (&f)[kDropoutColumns]) {
+__device__ __forceinline__ void keep_columns(int64_t e0, const DropoutParams& P, bool (&keep)[kDropoutColumns]) {
   constexpr int V = kDropoutColumns;
   const uint64_t counter = (uint64_t)e0 >> 2;
   if constexpr (VEC) {
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
       const uint4 w = philox7(counter + c, P);
-      f[4 * c] = w.x < P.threshold ? 0.0f : P.scale;
-      f[4 * c + 1] = w.y < P.threshold ? 0.0f : P.scale;
-      f[4 * c + 2] = w.z < P.threshold ? 0.0f : P.scale;
-      f[4 * c + 3] = w.w < P.threshold ? 0.0f : P.scale;
+      keep[4 * c] = w.x >= P.threshold;
+      keep[4 * c + 1] = w.y >= P.threshold;
+      keep[4 * c + 2] = w.z >= P.threshold;
+      keep[4 * c + 3] = w.w >= P.threshold;
     }
   } else {
     uint32_t w[V + 4];
@@ -77,7 +75,7 @@ __device__ __forceinline__ void keep_factors(int64_t e0, const DropoutParams& P,
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const uint32_t lo = shift & 1 ? w[k + 1] : w[k], hi = shift & 1 ? w[k + 3] : w[k + 2];
-      f[k] = (shift & 2 ? hi : lo) < P.threshold ? 0.0f : P.scale;
+      keep[k] = (shift & 2 ? hi : lo) >= P.threshold;
     }
   }
 }
@@ -112,19 +110,22 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_forward_kernel(const 
   float b[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) b[k] = P.bias != nullptr && k < live ? load1<DT>(P.bias, c0 + k) : 0.0f;
-  for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < P.rows; row += (int64_t)gridDim.y * blockDim.y) {
+  const int64_t stride = (int64_t)gridDim.y * blockDim.y;
+#pragma unroll 2
+  for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < P.rows; row += stride) {
     const int64_t e0 = row * P.width + c0;
-    float x[V], r[V], f[V];
+    float x[V], r[V];
+    bool keep[V];
     load_columns<DT, VEC>(P.x, e0, live, x);
     if (P.residual != nullptr) load_columns<DT, VEC>(P.residual, e0, live, r);
     else {
 #pragma unroll
       for (int k = 0; k < V; ++k) r[k] = 0.0f;
     }
-    keep_factors<VEC>(e0, P, f);
+    keep_columns<VEC>(e0, P, keep);
     // A dropped element contributes exactly 0, whatever x holds (0 * inf would be NaN).
 #pragma unroll
-    for (int k = 0; k < V; ++k) r[k] += f[k] == 0.0f ? 0.0f : (x[k] + b[k]) * f[k];
+    for (int k = 0; k < V; ++k) r[k] = keep[k] ? fmaf(x[k] + b[k], P.scale, r[k]) : r[k];
     store_columns<DT, VEC>(P.y, e0, live, r);
   }
 }
@@ -144,11 +145,11 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
   if (live > 0) {
     const int64_t stride = (int64_t)gridDim.y * blockDim.y;
     auto body = [&](int64_t e0, float (&g)[V]) {
-      float f[V];
-      keep_factors<VEC>(e0, P, f);
+      bool keep[V];
+      keep_columns<VEC>(e0, P, keep);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        g[k] = f[k] == 0.0f ? 0.0f : g[k] * f[k];
+        g[k] = keep[k] ? g[k] * P.scale : 0.0f;
         if constexpr (AFFINE) acc[k] += g[k];
       }
       if (P.y != nullptr) store_columns<DT, VEC>(P.y, e0, live, g);
@@ -210,44 +211,62 @@ struct DropoutGrid {
 };
 
 // Blocks of CX x RY threads over [rows, width / 8]: rows wider than 256 threads are cut into
-// equal parts, narrow ones share a block; the grid holds as many row slots as fit on the
-// device at `per_sm` blocks per SM.
-static DropoutGrid dropout_grid(int64_t rows, int64_t width, int per_sm) {
+// equal parts, narrow ones share a block; the grid holds as many row slots as the device runs at
+// once, at most `most`.
+template <typename K>
+static DropoutGrid dropout_grid(K kernel, int64_t rows, int64_t width, int64_t most) {
   const int64_t groups = (width + kDropoutColumns - 1) / kDropoutColumns;
   const int64_t parts = (groups + kDropoutThreads - 1) / kDropoutThreads;
   const int64_t cx = (groups + parts - 1) / parts;
   const int64_t ry = kDropoutThreads / cx;
-  int64_t slots = ((int64_t)current_sm_count() * per_sm + parts - 1) / parts;
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, (int)(cx * ry), 0) != cudaSuccess || per_sm < 1) per_sm = 4;
+  int64_t slots = (int64_t)current_sm_count() * per_sm / parts;
   if (slots > (rows + ry - 1) / ry) slots = (rows + ry - 1) / ry;
-  if (slots > 65535) slots = 65535;
+  if (slots > most) slots = most;
   if (slots < 1) slots = 1;
   return {dim3((unsigned)parts, (unsigned)slots), dim3((unsigned)cx, (unsigned)ry)};
 }
 
-template <int DT>
-static int launch_dropout_forward(const DropoutParams& P, bool vec, cudaStream_t s) {
-  const DropoutGrid g = dropout_grid(P.rows, P.width, 8);
-  if (vec) dropout_forward_kernel<DT, true><<<g.grid, g.block, 0, s>>>(P);
-  else dropout_forward_kernel<DT, false><<<g.grid, g.block, 0, s>>>(P);
+template <int DT, bool VEC>
+static int launch_dropout_forward(const DropoutParams& P, cudaStream_t s) {
+  const DropoutGrid g = dropout_grid(dropout_forward_kernel<DT, VEC>, P.rows, P.width, 65535);
+  dropout_forward_kernel<DT, VEC><<<g.grid, g.block, 0, s>>>(P);
   return launch_status("nt_dropout_forward launch");
 }
 
-template <int DT>
-static int launch_dropout_backward(const DropoutParams& P, bool vec, void* grad_bias, cudaStream_t s) {
-  DropoutGrid g = dropout_grid(P.rows, P.width, 4);
-  if (g.grid.y > kDropoutMaxSlots) g.grid.y = kDropoutMaxSlots;
+template <int DT, bool VEC>
+static int launch_dropout_backward(const DropoutParams& P, void* grad_bias, cudaStream_t s) {
   if (grad_bias == nullptr) {
-    if (vec) dropout_backward_kernel<DT, true, false><<<g.grid, g.block, 0, s>>>(P);
-    else dropout_backward_kernel<DT, false, false><<<g.grid, g.block, 0, s>>>(P);
+    const DropoutGrid g = dropout_grid(dropout_backward_kernel<DT, VEC, false>, P.rows, P.width, 65535);
+    dropout_backward_kernel<DT, VEC, false><<<g.grid, g.block, 0, s>>>(P);
     return launch_status("nt_dropout_backward launch");
   }
-  if (vec) dropout_backward_kernel<DT, true, true><<<g.grid, g.block, 0, s>>>(P);
-  else dropout_backward_kernel<DT, false, true><<<g.grid, g.block, 0, s>>>(P);
+  const DropoutGrid g = dropout_grid(dropout_backward_kernel<DT, VEC, true>, P.rows, P.width, kDropoutMaxSlots);
+  dropout_backward_kernel<DT, VEC, true><<<g.grid, g.block, 0, s>>>(P);
   int rc = launch_status("nt_dropout_backward launch");
   if (rc) return rc;
   dropout_bias_reduce_kernel<DT><<<(unsigned)((P.width + 31) / 32), dim3(32, kReduceLanes), 0, s>>>(
       P.partial, g.grid.y, P.width, grad_bias);
   return launch_status("nt_dropout_backward (reduce) launch");
+}
+
+template <bool VEC>
+static int dispatch_dropout_forward(const DropoutParams& P, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case NT_F32: return launch_dropout_forward<NT_F32, VEC>(P, s);
+    case NT_F16: return launch_dropout_forward<NT_F16, VEC>(P, s);
+    default: return launch_dropout_forward<NT_BF16, VEC>(P, s);
+  }
+}
+
+template <bool VEC>
+static int dispatch_dropout_backward(const DropoutParams& P, int dtype, void* grad_bias, cudaStream_t s) {
+  switch (dtype) {
+    case NT_F32: return launch_dropout_backward<NT_F32, VEC>(P, grad_bias, s);
+    case NT_F16: return launch_dropout_backward<NT_F16, VEC>(P, grad_bias, s);
+    default: return launch_dropout_backward<NT_BF16, VEC>(P, grad_bias, s);
+  }
 }
 
 static int check_dropout(const nt_dropout_args& a, const char* who, DropoutParams* P) {
@@ -261,8 +280,10 @@ static int check_dropout(const nt_dropout_args& a, const char* who, DropoutParam
   P->width = a.width;
   P->threshold = (uint32_t)floor(a.p * 4294967296.0);
   P->scale = (float)(1.0 / (1.0 - a.p));
-  P->key0 = (uint32_t)a.seed;
-  P->key1 = (uint32_t)(a.seed >> 32);
+  for (uint32_t r = 0; r < 7; ++r) {
+    P->keys[r][0] = (uint32_t)a.seed + r * 0x9E3779B9u;
+    P->keys[r][1] = (uint32_t)(a.seed >> 32) + r * 0xBB67AE85u;
+  }
   P->offset0 = (uint32_t)a.offset;
   P->offset1 = (uint32_t)(a.offset >> 32);
   return NT_OK;
@@ -292,11 +313,7 @@ int nt_dropout_forward(const nt_dropout_args* args, void* stream) {
   const bool vec = a.width % kDropoutColumns == 0 && aligned16(a.input) && aligned16(a.output) &&
                    (!a.residual || aligned16(a.residual));
   cudaStream_t s = as_stream(stream);
-  switch (a.dtype) {
-    case NT_F32: return launch_dropout_forward<NT_F32>(P, vec, s);
-    case NT_F16: return launch_dropout_forward<NT_F16>(P, vec, s);
-    default: return launch_dropout_forward<NT_BF16>(P, vec, s);
-  }
+  return vec ? dispatch_dropout_forward<true>(P, a.dtype, s) : dispatch_dropout_forward<false>(P, a.dtype, s);
 }
 
 int nt_dropout_backward(const nt_dropout_args* args, void* stream) {
@@ -323,11 +340,8 @@ int nt_dropout_backward(const nt_dropout_args* args, void* stream) {
   }
   P.x = a.input; P.y = a.output; P.partial = static_cast<float*>(a.workspace);
   const bool vec = a.width % kDropoutColumns == 0 && aligned16(a.input) && (!a.output || aligned16(a.output));
-  switch (a.dtype) {
-    case NT_F32: return launch_dropout_backward<NT_F32>(P, vec, a.grad_bias, s);
-    case NT_F16: return launch_dropout_backward<NT_F16>(P, vec, a.grad_bias, s);
-    default: return launch_dropout_backward<NT_BF16>(P, vec, a.grad_bias, s);
-  }
+  return vec ? dispatch_dropout_backward<true>(P, a.dtype, a.grad_bias, s)
+             : dispatch_dropout_backward<false>(P, a.dtype, a.grad_bias, s);
 }
 
 }  // extern "C"
