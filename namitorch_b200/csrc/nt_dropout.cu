@@ -45,6 +45,7 @@ __device__ __forceinline__ uint4 philox7(uint64_t counter, const DropoutParams& 
 // columns: the bias is loaded once and the bias gradient summed in registers.
 constexpr int kDropoutColumns = 8;
 constexpr int kDropoutThreads = 256;
+constexpr int kAhead = 4;
 // Partial rows of the bias gradient (row slots of the grid) at most.
 constexpr int64_t kDropoutMaxSlots = 1024;
 
@@ -155,15 +156,27 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
       if (P.y != nullptr) store_columns<DT, VEC>(P.y, e0, live, g);
     };
     int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y;
-    for (; row + stride < P.rows; row += 2 * stride) {   // two rows in flight
-      const int64_t e0 = row * P.width + c0, e1 = e0 + stride * P.width;
-      float g0[V], g1[V];
-      load_columns<DT, VEC>(P.x, e0, live, g0);
-      load_columns<DT, VEC>(P.x, e1, live, g1);
-      body(e0, g0);
-      body(e1, g1);
+    if constexpr (VEC) {
+      // kAhead rows in flight, packed as they came.
+      constexpr int N = DT == NT_F32 ? 2 : 1;
+      for (; row + (kAhead - 1) * stride < P.rows; row += kAhead * stride) {
+        uint4 raw[kAhead][N];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            raw[i][k] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::T*>(P.x) +
+                                                              (row + i * stride) * P.width + c0) + k);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          float g[V];
+#pragma unroll
+          for (int k = 0; k < N; ++k) unpack16<DT>(raw[i][k], g + k * (V / N));
+          body((row + i * stride) * P.width + c0, g);
+        }
+      }
     }
-    if (row < P.rows) {
+    for (; row < P.rows; row += stride) {
       const int64_t e0 = row * P.width + c0;
       float g[V];
       load_columns<DT, VEC>(P.x, e0, live, g);
