@@ -22,7 +22,7 @@ constexpr int kComputeWarps = 16;      // of forward and backward; four of them 
 constexpr int kCopyWarp = 16, kMmaWarp = 17;
 constexpr int kFwdThreads = 18 * 32;
 constexpr uint32_t kTmemColumns = 512;
-constexpr float kRescaleLog2 = 8.0f;
+constexpr float kRaiseSum = 8192.0f;
 
 // Which columns of a tile a row sees: c < end and (c >= begin or c < sink). word(c0) has bit e set
 // for column c0 + e, so that a masked tile costs one bit test and one select per element.
@@ -45,7 +45,7 @@ __device__ __forceinline__ uint32_t ring_phase(int n, int size) { return (uint32
 
 template <int N, int... C>
 __device__ __forceinline__ void exponentials(float (&x)[N], std::integer_sequence<int, C...>) {
-  ((x[C] = ex2_mixed<C>(x[C])), ...);
+  (ex2_mixed<C>(x[2 * C], x[2 * C + 1]), ...);
 }
 
 // Rows [rows, next multiple of 16) of a tile are cleared: their weights are 0, but what lies there
@@ -74,8 +74,8 @@ template <int DP> struct FwdShared {
   static constexpr int kRing = 2;
   static constexpr int kK = 2 * kTile, kV = (2 + kRing) * kTile, kControl = (2 + 2 * kRing) * kTile;
   struct Control {
-    float exchange[2][2][2][kTcRows];   // half of the queries, parity of the tile, half of the columns, row
-    uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[2], w_full[2], o_full;
+    float exchange[2][2][2][kTcRows];   // half of the queries, use (maximum, sum), half of the columns, row
+    uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[2], w_full[2], o_full[2];
     uint32_t tmem;
   };
   static constexpr int kBytes = kControl + (int)sizeof(Control);
@@ -108,11 +108,11 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 
   if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
   if (threadIdx.x == 0) {
-    mbar_init(&ctl.q_full, 1); mbar_init(&ctl.o_full, 1);
+    mbar_init(&ctl.q_full, 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.k_full[i], 1); mbar_init(&ctl.k_free[i], 1); mbar_init(&ctl.v_full[i], 1); mbar_init(&ctl.v_free[i], 1);
-      mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], kComputeWarps / 2);
+      mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], kComputeWarps / 2); mbar_init(&ctl.o_full[i], 1);
     }
     fence_mbar_init();
   }
@@ -174,6 +174,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       __syncwarp();
     };
     int done[2] = {0, 0};   // tiles of each half
+    bool finished[2] = {false, false};
     int begin = 0, end = 0;
     if (blocks > 0) {
       range.block(0, kTcRows, begin, end);
@@ -211,8 +212,13 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
           __syncwarp();
           ++done[g];
         }
-        if (j + 1 < blocks && active(g, next_begin, next_end))
+        if (j + 1 < blocks && active(g, next_begin, next_end)) {
           scores(g, Shape::kK + next * TILE, next_end - next_begin);
+        } else if (g == 0 && j + 2 == blocks) {
+          // The first half sees nothing of the last tile (of causal attention): its output is ready.
+          commit(&ctl.o_full[0]);
+          finished[0] = true;
+        }
       }
       if (!ok) break;
       commit(&ctl.v_free[slot]);
@@ -220,8 +226,9 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       begin = next_begin;
       end = next_end;
     }
-    commit(&ctl.o_full);
-    if (!ok) wait_bar(&ctl.o_full, 0);   // no product is in flight when TMEM is given back
+    if (!finished[0]) commit(&ctl.o_full[0]);
+    if (!finished[1]) commit(&ctl.o_full[1]);
+    if (!ok) wait_bar(&ctl.o_full[1], 0);   // no product is in flight when TMEM is given back
   } else {
     const int g = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // lane 32 (w % 4) in the address's upper half
@@ -232,7 +239,8 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     const int full_lo = P.window == 0 ? 0 : P.offset + q1 - P.window;   // first key the last query sees
     const int full_hi = P.offset + q0;                                   // last key the first query sees
     const int pair = 1 + g * 4 + (warp & 3);
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f, shift = 0.0f, minus = 0.0f;
+    bool extreme = false;
     int done = 0;
     for (int j = 0; j < blocks; ++j) {
       int begin, end;
@@ -250,94 +258,97 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
         seen[0] = mask.word(half * 64);
         seen[1] = mask.word(half * 64 + 32);
       }
-      // The scores are read twice: once for the maximum, once for the weights. 64 of them held in
-      // between would not fit the registers of 18 warps.
-      float top = -INFINITY;
+      // The reference maximum only has to keep the weights in range, so the one of the first tile
+      // stays until a row's weights of one tile sum to more than 2^13 (float16 holds 2^15). In the
+      // first tile, in that rare case, and where a row sees its first key, the two warps of the rows
+      // agree on a new maximum, rescale the output and form the weights (again).
+      bool again = done == 0;
+      while (true) {
+        if (again) {
+          float top = -INFINITY;
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t s[32];
-        tmem_load32(t_s + c0, s);
-        tmem_wait_load();
-        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (full) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) t[c & 3] = fmaxf(t[c & 3], __uint_as_float(s[c]));
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            t[c & 3] = fmaxf(t[c & 3], seen[c0 / 32] >> c & 1 ? __uint_as_float(s[c]) : -INFINITY);
-        }
-        top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-      }
-      ctl.exchange[g][done & 1][half][row] = top;
-      named_barrier(pair, 64);
-      top = fmaxf(top, ctl.exchange[g][done & 1][half ^ 1][row]);
-      // The maximum only has to keep the weights in range, so the old one stays until the new is
-      // 2^8 above it: the output is then rescaled for a few of the first tiles of a row only.
-      const bool raise = top > m && !((top - m) * P.scale_log2 <= kRescaleLog2);
-      if (__any_sync(0xffffffffu, raise)) {
-        const float f = raise ? ex2_approx((m - top) * P.scale_log2) : 1.0f;
-        if (raise) m = top;
-        l *= f;
-        if (done > 0) {
-          // Products complete in order: s of this tile is there, so o of the last one is too.
-#pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 32) {
-            uint32_t o[32];
-            tmem_load32(t_o + c, o);
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            uint32_t s[32];
+            tmem_load32(t_s + c0, s);
             tmem_wait_load();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_store32(t_o + c, o);
+            for (int c = 0; c < 32; ++c) top = fmaxf(top, seen[c0 / 32] >> c & 1 ? __uint_as_float(s[c]) : -INFINITY);
+          }
+          ctl.exchange[g][0][half][row] = top;
+          named_barrier(pair, 64);
+          top = fmaxf(m, fmaxf(top, ctl.exchange[g][0][half ^ 1][row]));
+          const float f = top == -INFINITY ? 1.0f : ex2_approx((m - top) * P.scale_log2);
+          m = top;
+          l *= f;
+          if (done > 0) {
+            // Products complete in order: s of this tile is there, so o of the last one is too.
+#pragma unroll 1
+            for (int c = 0; c < DP / 2; c += 32) {
+              uint32_t o[32];
+              tmem_load32(t_o + c, o);
+              tmem_wait_load();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_store32(t_o + c, o);
+            }
+          }
+          shift = m == -INFINITY ? 0.0f : m;
+          // Scores near the ends of float32 are subtracted before they are scaled.
+          extreme = __any_sync(0xffffffffu, isinf(shift * P.scale_log2));
+          minus = extreme ? 0.0f : -shift * P.scale_log2;
+        }
+        Pair sum(0.0f, 0.0f);
+        uint32_t w[32];
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t s[32];
+          tmem_load32(t_s + c0, s);
+          tmem_wait_load();
+          if (extreme) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) - shift);
+          }
+          float x[32];
+          const Pair scale2(P.scale_log2, P.scale_log2), minus2(minus, minus);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2)
+            fma2(Pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, minus2).get(x[c], x[c + 1]);
+          exponentials(x, std::make_integer_sequence<int, 16>{});
+          if (!full) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = seen[c0 / 32] >> c & 1 ? x[c] : 0.0f;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            sum = add2(sum, Pair(x[c], x[c + 1]));
+            w[(c0 + c) / 2] = pack2<DT>(x[c], x[c + 1]);
           }
         }
+        float a, b;
+        sum.get(a, b);
+        if (!again) {
+          again = named_barrier_or(pair, 64, a + b > kRaiseSum || (m == -INFINITY && (seen[0] | seen[1])));
+          if (again) continue;
+        }
+        tmem_store32(t_s, w);   // over scores that are no longer needed
+        l += a + b;
+        break;
       }
-      float shift = m == -INFINITY ? 0.0f : m;
-      // Scores near the ends of float32 are subtracted before they are scaled.
-      const bool extreme = __any_sync(0xffffffffu, isinf(shift * P.scale_log2));
-      const float minus = extreme ? 0.0f : -shift * P.scale_log2, before = extreme ? shift : 0.0f;
-      float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t s[32], w[16];
-        tmem_load32(t_s + c0, s);
-        tmem_wait_load();
-        if (extreme) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) - before);
-        }
-        float x[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = fmaf(__uint_as_float(s[c]), P.scale_log2, minus);
-        exponentials(x, std::make_integer_sequence<int, 32>{});
-        if (!full) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) x[c] = seen[c0 / 32] >> c & 1 ? x[c] : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sum[0] += x[2 * e];
-          sum[1] += x[2 * e + 1];
-          w[e] = pack2<DT>(x[2 * e], x[2 * e + 1]);
-        }
-        tmem_store16(t_s + c0 / 2, w);   // over scores that both reads are done with
-      }
-      l += sum[0] + sum[1];
       ++done;
       tmem_wait_store();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl.w_full[g]);
     }
-    if (ok && blocks > 0) ok = wait_bar(&ctl.o_full, 0);
+    if (ok && blocks > 0) ok = wait_bar(&ctl.o_full[g], 0);
     __syncwarp();
     tc_fence_after();
-    ctl.exchange[g][done & 1][half][row] = l;
+    ctl.exchange[g][1][half][row] = l;
     named_barrier(pair, 64);
     // Halves in a fixed order, so that both threads of a row have the same sum.
-    l = ctl.exchange[g][done & 1][0][row] + ctl.exchange[g][done & 1][1][row];
+    l = ctl.exchange[g][1][0][row] + ctl.exchange[g][1][1][row];
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    // The queries' tiles are free now: 32 rows x half of the columns of each warp.
+    // The half's tile of queries is free now: 32 rows x half of the columns of each warp.
     constexpr int WIDTH = DP / 2, CH = WIDTH / 8;
     uint8_t* stage = aligned + warp * 32 * WIDTH * 2;
     const int row0 = q0 + (warp & 3) * 32, rows = q1 - row0, vectors = (P.dim - half * WIDTH + 7) / 8;
@@ -408,7 +419,7 @@ template <int DP> struct BwdShared {
   static constexpr int kRing1 = 3, kRing2 = 2;
   static constexpr int kY1 = 2 * kTile, kY2 = (2 + kRing1) * kTile, kControl = (2 + kRing1 + kRing2) * kTile;
   struct Control {
-    float stats[2][2][kStep];          // ring of two; lse (times log2 e), delta
+    float stats[2][2][kStep];          // ring of two; lse (times log2 e) and delta, both negative
     uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, p_full,
         dp_full[2], ds_full[2],            // by the step's parity: dp(t + 1) may be there before dp(t) was waited for
         stat_full[2], stat_free[2], out_full;
@@ -558,8 +569,8 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         for (int i = 0; i < kStep / 32; ++i) {
           const int c = i * 32 + lane;
           const bool in = s.begin + c < s.end;
-          lse[i] = in ? P.lse[stat + c] * kLog2eF : 0.0f;
-          delta[i] = in ? P.delta[stat + c] : 0.0f;
+          lse[i] = in ? -P.lse[stat + c] * kLog2eF : 0.0f;
+          delta[i] = in ? -P.delta[stat + c] : 0.0f;
         }
         if (t >= 2) ok = wait_warp(&ctl.stat_free[t & 1], ring_phase(t - 2, 2));
         if (!ok) break;
@@ -681,9 +692,9 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
           if (r0 + r < r1) P.delta[stat + r] = d;
         }
       }
-      if (r0 + row < r1) lse = P.lse[stat + row] * kLog2eF;
+      if (r0 + row < r1) lse = -P.lse[stat + row] * kLog2eF;
       named_barrier(1, kComputeWarps * 32);
-      delta = ctl.delta[row];
+      delta = -ctl.delta[row];
     }
     // Steps without a masked pair: those whose rows are all there and lie within these bounds.
     int full_lo, full_hi;
@@ -714,16 +725,15 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctl.p_full);
       }
+      const Pair scale2(P.scale_log2, P.scale_log2);
 #pragma unroll
       for (int c = 0; c < kColumns; c += 4) {
-        float4 ls = make_float4(lse, lse, lse, lse);
+        float4 ls = make_float4(lse, lse, lse, lse);   // negative
         if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][quarter * kColumns + c]);
-        p[c] = fmaf(p[c], P.scale_log2, -ls.x);
-        p[c + 1] = fmaf(p[c + 1], P.scale_log2, -ls.y);
-        p[c + 2] = fmaf(p[c + 2], P.scale_log2, -ls.z);
-        p[c + 3] = fmaf(p[c + 3], P.scale_log2, -ls.w);
+        fma2(Pair(p[c], p[c + 1]), scale2, Pair(ls.x, ls.y)).get(p[c], p[c + 1]);
+        fma2(Pair(p[c + 2], p[c + 3]), scale2, Pair(ls.z, ls.w)).get(p[c + 2], p[c + 3]);
       }
-      exponentials(p, std::make_integer_sequence<int, kColumns>{});
+      exponentials(p, std::make_integer_sequence<int, kColumns / 2>{});
       uint32_t seen = 0xffffffffu;
       if (!full) {
         ColumnMask mask;
@@ -758,10 +768,13 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
       tmem_wait_load();
 #pragma unroll
       for (int c = 0; c < kColumns; c += 4) {
-        float4 de = make_float4(delta, delta, delta, delta);
+        float4 de = make_float4(delta, delta, delta, delta);   // negative
         if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][quarter * kColumns + c]);
-        w[c / 2] = pack2<DT>(p[c] * (__uint_as_float(d[c]) - de.x), p[c + 1] * (__uint_as_float(d[c + 1]) - de.y));
-        w[c / 2 + 1] = pack2<DT>(p[c + 2] * (__uint_as_float(d[c + 2]) - de.z), p[c + 3] * (__uint_as_float(d[c + 3]) - de.w));
+        float a, e;
+        mul2(Pair(p[c], p[c + 1]), add2(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
+        w[c / 2] = pack2<DT>(a, e);
+        mul2(Pair(p[c + 2], p[c + 3]), add2(Pair(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), Pair(de.z, de.w))).get(a, e);
+        w[c / 2 + 1] = pack2<DT>(a, e);
       }
       if (!full) {
         // dp of a key that is not there may be NaN: 0 * NaN is cleared here.

@@ -170,24 +170,72 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x on the FP32 pipe: x = n + f with n the nearest integer, 2^f for |f| <= 1/2 by the polynomial
-// of degree 4 with the least largest relative error (2.7e-6, far below a 16-bit weight's own
-// rounding), scaled by 2^n. Down to 2^-126, which stands for everything below; NaN stays NaN.
-__device__ __forceinline__ float ex2_polynomial(float x) {
-  x = max_nan(x, -126.0f);
-  const float t = x + 12582912.0f;   // 1.5 * 2^23: the integer ends up in the low bits
-  const float f = x - (t - 12582912.0f);
-  float p = fmaf(f, 0.009570100344717503f, 0.05591785907745361f);
-  p = fmaf(p, f, 0.240247443318367f);
-  p = fmaf(p, f, 0.6931217908859253f);
-  p = fmaf(p, f, 0.9999992847442627f);
-  return p * __int_as_float((__float_as_int(t) << 23) + 0x3f800000);
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-// Exponentials of a thread's columns: the special-function unit gives 16 a cycle and SM, fewer
-// than the tensor cores can use, so every fourth column goes to the FP32 pipe.
-template <int COLUMN>
-__device__ __forceinline__ float ex2_mixed(float x) {
-  return COLUMN % 4 == 3 ? ex2_polynomial(x) : ex2_approx(x);
+
+// Two float32 operations in one instruction.
+struct Pair {
+  uint64_t bits;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(bits)); }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+
+// 2^x of two values on the FP32 pipe: x = n + f with n the nearest integer, 2^f for |f| <= 1/2 by the
+// polynomial of degree 4 with the least largest relative error (2.7e-6, far below a 16-bit
+// weight's own rounding), scaled by 2^n. From 2^-126, which stands for everything below, to 2^126,
+// which does for everything above; NaN stays NaN.
+__device__ __forceinline__ void ex2_polynomial(float& x, float& y) {
+  const Pair v(min_nan(max_nan(x, -126.0f), 126.0f), min_nan(max_nan(y, -126.0f), 126.0f));
+  const Pair t = add2(v, Pair(12582912.0f, 12582912.0f));   // 1.5 * 2^23: the integer ends up in the low bits
+  const Pair f = add2(v, fma2(t, Pair(-1.0f, -1.0f), Pair(12582912.0f, 12582912.0f)));
+  Pair p = fma2(f, Pair(0.009570100344717503f, 0.009570100344717503f), Pair(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, Pair(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, Pair(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, Pair(0.9999992847442627f, 0.9999992847442627f));
+  float a, b;
+  t.get(a, b);
+  mul2(p, Pair(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000)))
+      .get(x, y);
+}
+// Exponentials of two neighbouring columns: the special-function unit gives 16 a cycle and SM, fewer
+// than the tensor cores can use, so every fourth pair goes to the FP32 pipe.
+template <int PAIR>
+__device__ __forceinline__ void ex2_mixed(float& x, float& y) {
+  if constexpr (PAIR % 4 == 3) {
+    ex2_polynomial(x, y);
+  } else {
+    x = ex2_approx(x);
+    y = ex2_approx(y);
+  }
+}
+// True in every thread of the barrier when `any` was in one.
+__device__ __forceinline__ bool named_barrier_or(int id, int threads, bool any) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)any), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
 }
 
 // 32 rows of a warp, CH 16-byte vectors each, lane r holding row r, written to global memory with
