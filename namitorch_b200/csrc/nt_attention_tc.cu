@@ -106,8 +106,20 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     return (g == 0 || i1 > i0 + kTcRows) && ((begin < r.hi && end > r.lo) || begin < r.sink_end);
   };
 
+  // The copying warp sets up the barriers and issues the first copies while the rest is set up.
+  auto load = [&](const CUtensorMap& map, int at, int token, int head, uint64_t* bar) {
+#pragma unroll
+    for (int half = 0; half < DP / 64; ++half)
+      tma_load(aligned + at + half * kTcRows * 128, &map, half * 64, token, head, b, bar);
+  };
+  auto fill = [&](const CUtensorMap& map, int at, uint64_t* full, int j) {
+    int begin, end;
+    range.block(j, kTcRows, begin, end);
+    mbar_arrive_expect_tx(&full[j % RING], TILE);
+    load(map, at + j % RING * TILE, begin, hk, &full[j % RING]);
+  };
   if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
-  if (threadIdx.x == 0) {
+  if (warp == kCopyWarp && lane == 0) {
     mbar_init(&ctl.q_full, 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -115,6 +127,14 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], kComputeWarps / 2); mbar_init(&ctl.o_full[i], 1);
     }
     fence_mbar_init();
+    if (blocks > 0) {
+      // The second half's rows may all lie past the last query: the copy then writes zeros.
+      mbar_arrive_expect_tx(&ctl.q_full, 2 * TILE);
+      load(map_q, 0, i0, h, &ctl.q_full);
+      fill(map_k, Shape::kK, ctl.k_full, 0);
+      load(map_q, TILE, i0 + kTcRows, h, &ctl.q_full);
+      fill(map_v, Shape::kV, ctl.v_full, 0);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -124,28 +144,15 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 
   if (warp == kCopyWarp) {
     if (lane == 0 && blocks > 0) {
-      auto load = [&](const CUtensorMap* map, int at, int token, int head, uint64_t* bar) {
-#pragma unroll
-        for (int half = 0; half < DP / 64; ++half)
-          tma_load(aligned + at + half * kTcRows * 128, map, half * 64, token, head, b, bar);
-      };
-      // The second half's rows may all lie past the last query: the copy then writes zeros.
-      mbar_arrive_expect_tx(&ctl.q_full, 2 * TILE);
-      load(&map_q, 0, i0, h, &ctl.q_full);
-      load(&map_q, TILE, i0 + kTcRows, h, &ctl.q_full);
-      int n1 = 0, n2 = 0;
-      for (int j = 0; j < blocks; ++j) {
-        int begin, end;
-        range.block(j, kTcRows, begin, end);
+      int n1 = 1, n2 = 1;
+      for (int j = 1; j < blocks; ++j) {
         if (j >= RING) ok = wait_bar(&ctl.k_free[j % RING], ring_phase(j - RING, RING));
         if (!ok) break;
-        mbar_arrive_expect_tx(&ctl.k_full[j % RING], TILE);
-        load(&map_k, Shape::kK + j % RING * TILE, begin, hk, &ctl.k_full[j % RING]);
+        fill(map_k, Shape::kK, ctl.k_full, j);
         n1 = j + 1;
         if (j >= RING) ok = wait_bar(&ctl.v_free[j % RING], ring_phase(j - RING, RING));
         if (!ok) break;
-        mbar_arrive_expect_tx(&ctl.v_full[j % RING], TILE);
-        load(&map_v, Shape::kV + j % RING * TILE, begin, hk, &ctl.v_full[j % RING]);
+        fill(map_v, Shape::kV, ctl.v_full, j);
         n2 = j + 1;
       }
       if (!ok) {   // the copies in flight land before the block may end
@@ -399,9 +406,11 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 //   s = x1 y1^T, dp = x2 y2^T (TMEM, float32);  P = exp(scale s - lse), dS = P (dp - delta)
 //   out1 += dS y1, and with DKV out2 += P y2, with P and dS over s and dp in TMEM as the
 //   products' first operand.
-// DKV = false: rows are queries (x1 = q, x2 = g; y1 = k, y2 = v): out1 = dq; delta = sum(g o) is
-// computed on the way in and stored. DKV = true: rows are keys (x1 = k, x2 = v; y1 = q, y2 = g):
-// out1 = dk, out2 = dv, over the heads of the group.
+// DKV = false: rows are queries (x1 = q, x2 = g; y1 = k, y2 = v): out1 = dq. DKV = true: rows are keys
+// (x1 = k, x2 = v; y1 = q, y2 = g): out1 = dk, out2 = dv, over the heads of the group. Both kinds of
+// blocks are one launch, the key blocks (the longer ones) first, so that the other kind fills the
+// SMs that the last of them leave idle. delta = sum(g o) comes from a kernel before it, whose end
+// only the warps that read delta wait for.
 // With DKV s, dp and the two outputs fill TMEM, so nothing has a second buffer; the order of the
 // products hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1)
 // while dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Without it dp has two buffers and
@@ -423,7 +432,6 @@ template <int DP> struct BwdShared {
     uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, p_full,
         dp_full[2], ds_full[2],            // by the step's parity: dp(t + 1) may be there before dp(t) was waited for
         stat_full[2], stat_free[2], out_full;
-    float delta[kTcRows];
     uint32_t tmem;
   };
   static constexpr int kBytes = kControl + (int)sizeof(Control);
@@ -431,11 +439,36 @@ template <int DP> struct BwdShared {
 static_assert(kStep == kTcRows, "rows kept and rows streamed have one shape");
 static_assert(BwdShared<128>::kBytes <= 227 * 1024, "one block per SM");
 
+// delta of every query: as many lanes to a row as it has 16-byte vectors.
+template <int DT, int DP>
+__global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ AttnParams P) {
+  constexpr int LPR = DP / 8, ROWS = 256 / LPR;
+  grid_dependents_go();
+  const int b = blockIdx.z, h = blockIdx.y, c = threadIdx.x % LPR * 8;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
+  float d = 0.0f;
+  if (row < P.queries && c < P.dim) {
+    float x[8], y[8], z[8];
+    const int64_t o = P.os.at(b, h, row) + c;
+    unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.g) + P.gs.at(b, h, row) + c)), x);
+    unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o) + o)), y);
+    if (P.o_low != nullptr) {
+      unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o_low) + o)), z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] += z[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
+  }
+#pragma unroll
+  for (int w = LPR / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+  if (threadIdx.x % LPR == 0 && row < P.queries) P.delta[((int64_t)b * P.heads + h) * P.queries + row] = d;
+}
+
 template <int DT, int DP, bool DKV>
-__global__ void __launch_bounds__(kBwdThreads, 1)
-attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_x1,
-                      const __grid_constant__ CUtensorMap map_x2, const __grid_constant__ CUtensorMap map_y1,
-                      const __grid_constant__ CUtensorMap map_y2) {
+__device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t block, const CUtensorMap& map_x1,
+                                               const CUtensorMap& map_x2, const CUtensorMap& map_y1,
+                                               const CUtensorMap& map_y2) {
   using Shape = BwdShared<DP>;
   constexpr int TILE = Shape::kTile, RING1 = Shape::kRing1, RING2 = Shape::kRing2;
   // No static shared memory: the dynamic block starts where shared memory does, 1024 bytes in.
@@ -444,16 +477,16 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
   const uint32_t base = smem_u32(aligned);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Blocks in the order of their work: the last queries, or the first keys, of every head first.
-  const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch, tiles = gridDim.x / pairs;
-  const int b = blockIdx.x % pairs / heads, h0 = blockIdx.x % heads;   // query head of dq, key head of dk and dv
-  const int index = blockIdx.x / pairs;
+  const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch;
+  const int b = block % pairs / heads, h0 = block % heads;   // query head of dq, key head of dk and dv
+  const int index = block / pairs;
   const int length = attn_length(P, b);
 
   // The block's rows [r0, r1) and the steps it walks.
   int r0, r1, part = 0, parts = 1, tile = 0, steps, per_head = 1;
   uint32_t from = 0;
   if constexpr (!DKV) {
-    r0 = (tiles - 1 - index) * kTcRows;
+    r0 = ((P.queries + kTcRows - 1) / kTcRows - 1 - index) * kTcRows;
     r1 = min(P.queries, r0 + kTcRows);
   } else {
     const int split = P.sink_tiles * P.parts;
@@ -503,8 +536,22 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     }
   };
 
+  // The copying warp sets up the barriers and issues the first copies while the rest is set up.
+  auto load = [&](const CUtensorMap& map, int at, int token, int head, uint64_t* bar) {
+#pragma unroll
+    for (int half = 0; half < DP / 64; ++half)
+      tma_load(aligned + at + half * kTcRows * 128, &map, half * 64, token, head, b, bar);
+  };
+  auto fill1 = [&](int t, const Step& s) {
+    mbar_arrive_expect_tx(&ctl.y1_full[t % RING1], TILE);
+    load(map_y1, Shape::kY1 + t % RING1 * TILE, s.begin, s.head, &ctl.y1_full[t % RING1]);
+  };
+  auto fill2 = [&](int t, const Step& s) {
+    mbar_arrive_expect_tx(&ctl.y2_full[t % RING2], TILE);
+    load(map_y2, Shape::kY2 + t % RING2 * TILE, s.begin, s.head, &ctl.y2_full[t % RING2]);
+  };
   if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
-  if (threadIdx.x == 0) {
+  if (warp == kCopyWarp && lane == 0) {
     mbar_init(&ctl.x_full, 1); mbar_init(&ctl.out_full, 1);
 #pragma unroll
     for (int i = 0; i < RING1; ++i) { mbar_init(&ctl.y1_full[i], 1); mbar_init(&ctl.y1_free[i], 1); }
@@ -517,6 +564,15 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 #pragma unroll
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl.dp_full[i], 1); mbar_init(&ctl.ds_full[i], kComputeWarps); }
     fence_mbar_init();
+    if (steps > 0) {
+      Step s;
+      start(s);
+      mbar_arrive_expect_tx(&ctl.x_full, 2 * TILE);
+      load(map_x1, 0, r0, h0, &ctl.x_full);
+      fill1(0, s);
+      load(map_x2, TILE, r0, h0, &ctl.x_full);
+      fill2(0, s);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -529,27 +585,18 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
 
   if (warp == kCopyWarp) {
     if (lane == 0 && steps > 0) {
-      auto load = [&](const CUtensorMap* map, int at, int token, int head, uint64_t* bar) {
-#pragma unroll
-        for (int half = 0; half < DP / 64; ++half)
-          tma_load(aligned + at + half * kTcRows * 128, map, half * 64, token, head, b, bar);
-      };
-      mbar_arrive_expect_tx(&ctl.x_full, 2 * TILE);
-      load(&map_x1, 0, r0, h0, &ctl.x_full);
-      load(&map_x2, TILE, r0, h0, &ctl.x_full);
       Step s;
       start(s);
-      int n1 = 0, n2 = 0;
-      for (int t = 0; t < steps; ++t, advance(s)) {
+      int n1 = 1, n2 = 1;
+      for (int t = 1; t < steps; ++t) {
+        advance(s);
         if (t >= RING1) ok = wait_bar(&ctl.y1_free[t % RING1], ring_phase(t - RING1, RING1));
         if (!ok) break;
-        mbar_arrive_expect_tx(&ctl.y1_full[t % RING1], TILE);
-        load(&map_y1, Shape::kY1 + t % RING1 * TILE, s.begin, s.head, &ctl.y1_full[t % RING1]);
+        fill1(t, s);
         n1 = t + 1;
         if (t >= RING2) ok = wait_bar(&ctl.y2_free[t % RING2], ring_phase(t - RING2, RING2));
         if (!ok) break;
-        mbar_arrive_expect_tx(&ctl.y2_full[t % RING2], TILE);
-        load(&map_y2, Shape::kY2 + t % RING2 * TILE, s.begin, s.head, &ctl.y2_full[t % RING2]);
+        fill2(t, s);
         n2 = t + 1;
       }
       if (!ok) {   // the copies in flight land before the block may end
@@ -560,6 +607,7 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     }
   } else if (warp == kStatWarp) {
     if constexpr (DKV) {
+      grid_dependency_wait();
       Step s;
       start(s);
       for (int t = 0; t < steps; ++t, advance(s)) {
@@ -665,36 +713,12 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
     const uint32_t at_s = t_s + lanes + quarter * kColumns;
     float lse = 0.0f, delta = 0.0f;
     if constexpr (!DKV) {
-      // delta: each warp sums 8 rows, as many lanes to a row as it has 16-byte vectors.
-      constexpr int LPR = DP / 8, RPW = 32 / LPR;
-      const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0;
-#pragma unroll
-      for (int i = 0; i < kTcRows / kComputeWarps; i += RPW) {
-        const int r = warp * (kTcRows / kComputeWarps) + i + lane / LPR, c = lane % LPR * 8;
-        float d = 0.0f;
-        if (r0 + r < r1 && c < P.dim) {
-          float x[8], y[8], z[8];
-          const int64_t o = P.os.at(b, h0, r0 + r) + c;
-          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.g) + P.gs.at(b, h0, r0 + r) + c)), x);
-          unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o) + o)), y);
-          if (P.o_low != nullptr) {
-            unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o_low) + o)), z);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] += z[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
-        }
-#pragma unroll
-        for (int w = LPR / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-        if (lane % LPR == 0) {
-          ctl.delta[r] = d;
-          if (r0 + r < r1) P.delta[stat + r] = d;
-        }
+      grid_dependency_wait();
+      if (r0 + row < r1) {
+        const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0 + row;
+        lse = -P.lse[stat] * kLog2eF;
+        delta = -P.delta[stat];
       }
-      if (r0 + row < r1) lse = -P.lse[stat + row] * kLog2eF;
-      named_barrier(1, kComputeWarps * 32);
-      delta = -ctl.delta[row];
     }
     // Steps without a masked pair: those whose rows are all there and lie within these bounds.
     int full_lo, full_hi;
@@ -858,6 +882,16 @@ attention_tc_backward(const __grid_constant__ AttnParams P, const __grid_constan
   if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
 }
 
+// Blocks 0 .. key_blocks - 1 own keys, the others queries.
+template <int DT, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attention_tc_backward(const __grid_constant__ AttnParams P, uint32_t key_blocks, const __grid_constant__ CUtensorMap map_q,
+                      const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v) {
+  if (blockIdx.x < key_blocks) backward_block<DT, DP, true>(P, blockIdx.x, map_k, map_v, map_q, map_g);
+  else backward_block<DT, DP, false>(P, blockIdx.x - key_blocks, map_q, map_g, map_k, map_v);
+}
+
 // ---- host ------------------------------------------------------------------------------
 
 template <int DT, int DP>
@@ -879,19 +913,32 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   const char* who = "nt_attention_backward";
   CUtensorMap q, g, k, v;
   const int bytes = BwdShared<DP>::kBytes;
-  int rc = large_smem<attention_tc_backward<DT, DP, false>>(bytes, who);
-  if (!rc) rc = large_smem<attention_tc_backward<DT, DP, true>>(bytes, who);
+  int rc = large_smem<attention_tc_backward<DT, DP>>(bytes, who);
   if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&g, DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
-  const unsigned rows = (unsigned)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
-  attention_tc_backward<DT, DP, false><<<rows, kBwdThreads, bytes, s>>>(P, q, g, k, v);
+  constexpr int ROWS = 256 / (DP / 8);
+  attention_delta_kernel<DT, DP><<<dim3((P.queries + ROWS - 1) / ROWS, P.heads, P.batch), 256, 0, s>>>(P);
   rc = launch_status("nt_attention_backward launch");
   if (rc) return rc;
-  const int tiles = (P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1);
-  attention_tc_backward<DT, DP, true><<<(unsigned)tiles * P.kv_heads * P.batch, kBwdThreads, bytes, s>>>(P, k, v, q, g);
+  const uint32_t query_blocks = (uint32_t)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
+  const uint32_t key_blocks =
+      (uint32_t)((P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1)) * P.kv_heads * P.batch;
+  // Its blocks may start while the kernel before it ends.
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(key_blocks + query_blocks);
+  config.blockDim = dim3(kBwdThreads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&config, attention_tc_backward<DT, DP>, P, key_blocks, q, g, k, v);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_backward launch"); }
   return launch_status("nt_attention_backward launch");
 }
 
