@@ -348,26 +348,23 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   }
 }
 
-// dk and dv of the sink blocks: the parts added in order. One thread per element; `tile_rows`
-// keys a block.
+// dk and dv of the split key blocks (of `tile_rows` keys): the parts added in order, one thread per
+// element. Grid: pieces of 256 elements of dk or dv of a block, in that order; then blocks, then
+// batch x key head.
 template <int DT>
 __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnParams P, int tile_rows) {
-  const int64_t per_tile = (int64_t)2 * tile_rows * P.dim;
-  const int64_t total = (int64_t)P.batch * P.kv_heads * P.sink_tiles * per_tile;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t block = e / per_tile, in = e % per_tile;
-    const int which = (int)(in / ((int64_t)tile_rows * P.dim));
-    const int row = (int)(in / P.dim % tile_rows), c = (int)(in % P.dim);
-    const int key = (int)(block % P.sink_tiles) * tile_rows + row;
-    if (key >= P.keys) continue;
-    const int64_t bh = block / P.sink_tiles;
-    const float* src = P.partial + block * P.parts * per_tile + in;
-    float s = 0.0f;
-    for (int k = 0; k < P.parts; ++k) s += src[k * per_tile];
-    const int b = (int)(bh / P.kv_heads), hk = (int)(bh % P.kv_heads);
-    if (which == 0) store1<DT>(P.dk, P.dks.at(b, hk, key) + c, s);
-    else store1<DT>(P.dv, P.dvs.at(b, hk, key) + c, s);
-  }
+  const int size = tile_rows * P.dim, pieces = (size + 255) / 256;
+  const int e = blockIdx.x % pieces * 256 + threadIdx.x, which = blockIdx.x / pieces % 2;
+  const int block = blockIdx.x / pieces / 2, tile = block % P.sink_tiles, pair = block / P.sink_tiles;
+  const int b = pair / P.kv_heads, hk = pair % P.kv_heads;
+  const int key = tile * tile_rows + e / P.dim, c = e % P.dim;
+  if (e >= size || key >= P.keys) return;
+  const float* src = P.partial + ((int64_t)block * P.parts * 2 + which) * size + e;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int k = 0; k < P.parts; ++k) s += src[(int64_t)k * 2 * size];
+  if (which == 0) store1<DT>(P.dk, P.dks.at(b, hk, key) + c, s);
+  else store1<DT>(P.dv, P.dvs.at(b, hk, key) + c, s);
 }
 
 // ---- launches ------------------------------------------------------------------------
@@ -408,7 +405,8 @@ static int dispatch_forward(const AttnParams& P, cudaStream_t s) {
 template <int DT>
 static int launch_join(const AttnParams& P, int tile_rows, cudaStream_t s) {
   if (P.parts == 1 || P.sink_tiles == 0) return NT_OK;
-  attention_join_kernel<DT><<<(unsigned)(current_sm_count() * 4), 256, 0, s>>>(P, tile_rows);
+  const unsigned pieces = (tile_rows * P.dim + 255) / 256;
+  attention_join_kernel<DT><<<pieces * 2 * P.sink_tiles * P.batch * P.kv_heads, 256, 0, s>>>(P, tile_rows);
   return launch_status("nt_attention_backward (join) launch");
 }
 template <int DT>
@@ -432,11 +430,17 @@ static size_t delta_bytes(const nt_attention_args& a) {
   return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
 }
 
+// The window where it hides a key: 0 where it covers every position (below `positions`) or every key
+// is a sink.
+static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
+  return a.window >= positions || a.sinks >= a.keys ? 0 : a.window;
+}
+
 static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows) {
-  if (a.window <= 0 || a.sinks <= 0 || a.keys == 0) return 0;
-  const int64_t sinks = a.sinks < a.keys ? a.sinks : a.keys;
-  const int64_t tiles = (sinks + tile_rows - 1) / tile_rows;
-  const int64_t parts = sink_parts(a.queries, a.window < a.keys ? a.window : a.keys, a.query_heads / a.kv_heads, tile_rows, step_rows);
+  const int64_t window = effective_window(a, a.query_offset + a.queries);
+  if (window == 0 || a.sinks == 0) return 0;
+  const int64_t tiles = (a.sinks + tile_rows - 1) / tile_rows;
+  const int64_t parts = sink_parts(a.queries, window, a.query_heads / a.kv_heads, tile_rows, step_rows);
   if (parts == 1) return 0;
   return (size_t)a.batch * a.kv_heads * tiles * parts * 2 * tile_rows * a.head_dim * 4;
 }
@@ -492,7 +496,8 @@ static bool vector_key(const nt_attention_args& a, const void* p, const int64_t*
   return vector_rows(a, p, s, a.kv_heads, a.keys);
 }
 
-static AttnParams attention_params(const nt_attention_args& a) {
+// `positions`: every query stands below it.
+static AttnParams attention_params(const nt_attention_args& a, int64_t positions) {
   AttnParams P{};
   P.q = a.query; P.k = a.key; P.v = a.value; P.g = a.gradient; P.o = a.output;
   P.dq = a.grad_query; P.dk = a.grad_key; P.dv = a.grad_value;
@@ -502,9 +507,8 @@ static AttnParams attention_params(const nt_attention_args& a) {
   P.o_low = a.output_low; P.lse = a.lse; P.lengths = a.lengths; P.error = a.error;
   P.batch = (int)a.batch; P.heads = (int)a.query_heads; P.kv_heads = (int)a.kv_heads;
   P.group = (int)(a.query_heads / a.kv_heads); P.queries = (int)a.queries; P.keys = (int)a.keys; P.dim = a.head_dim;
-  // Positions stay below 2^31 - 1, so a window or a sink count past that hides or shows the same keys.
-  P.window = (int)(a.window < INT_MAX ? a.window : INT_MAX);
-  P.sinks = a.window == 0 ? 0 : (int)(a.sinks < a.keys ? a.sinks : a.keys);
+  P.window = (int)effective_window(a, positions);
+  P.sinks = P.window == 0 ? 0 : (int)a.sinks;
   P.offset = (int)a.query_offset;
   P.scale = a.scale;
   P.scale_log2 = a.scale * kLog2eF;
@@ -535,7 +539,7 @@ int nt_attention_forward(const nt_attention_args* args, void* stream) {
     set_error("nt_attention_forward: NULL query/key/value/output");
     return NT_EINVAL;
   }
-  AttnParams P = attention_params(a);
+  AttnParams P = attention_params(a, a.query_offset + a.queries);
   P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
           vector_key(a, a.value, a.value_strides);
   cudaStream_t s = as_stream(stream);
@@ -569,19 +573,18 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
     set_error("nt_attention_backward: needs a 16-byte aligned workspace of %zu bytes (got %zu)", need, a.workspace_bytes);
     return NT_EINVAL;
   }
-  AttnParams P = attention_params(a);
+  AttnParams P = attention_params(a, a.query_offset + a.queries);
   P.delta = static_cast<float*>(a.workspace);
   P.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + delta_bytes(a));
   P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
           vector_key(a, a.value, a.value_strides) && vector_query(a, a.gradient, a.gradient_strides) &&
           vector_query(a, a.output, a.output_strides);
-  const int64_t window = a.window < a.keys ? a.window : a.keys;
   const bool tc = a.dtype != NT_F32 && a.keys > 0 && a.queries > 0 && P.vec &&
                   vector_query(a, a.output_low, a.output_strides) && vector_query(a, a.grad_query, a.grad_query_strides) &&
                   vector_key(a, a.grad_key, a.grad_key_strides) && vector_key(a, a.grad_value, a.grad_value_strides);
   const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? kTcQueryStep : kRows;
   P.sink_tiles = (P.sinks + tile_rows - 1) / tile_rows;
-  P.parts = P.sink_tiles ? sink_parts(a.queries, window, P.group, tile_rows, step_rows) : 1;
+  P.parts = P.sink_tiles ? sink_parts(a.queries, P.window, P.group, tile_rows, step_rows) : 1;
   cudaStream_t s = as_stream(stream);
   if (tc) {
     rc = attention_tc_backward_launch(P, a.dtype, s);
@@ -607,7 +610,7 @@ int nt_attention_step(const nt_attention_args* args, void* stream) {
     set_error("nt_attention_step: NULL query/key/value/lengths/output");
     return NT_EINVAL;
   }
-  AttnParams P = attention_params(a);
+  AttnParams P = attention_params(a, a.keys);
   P.vec = vector_key(a, a.key, a.key_strides) && vector_key(a, a.value, a.value_strides);
   return attention_step_launch(P, a.dtype, as_stream(stream));
 }

@@ -34,6 +34,7 @@ struct AttnParams {
   // Backward over key blocks: the first `sink_tiles` blocks hold sinks, which every later query
   // sees, so their queries are cut into `parts` pieces.
   int sink_tiles, parts;
+  int splits;        // forward: blocks of a cluster that share a block of queries
   float scale, scale_log2;
 };
 

@@ -16,22 +16,6 @@ namespace nt {
 
 constexpr int kStepMaxCluster = 8;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
-  uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p)), remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
-  return v;
-}
-
 // The block's piece [from, to) of the visible keys of its sequence.
 struct StepKeys {
   int sink_end, skip, from, to;

@@ -69,19 +69,25 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int rows, int lane) {
 // products of one half run under the exponentials of the other:
 //   s0(0) s1(0) | o0 += w0(0) v, s0(1) | o1 += w1(0) v, s1(1) | o0 += w0(1) v, ...
 // TMEM: s0, s1 (the weights over them), o0, o1.
+// SPLIT: where there are too few blocks of queries for the device, a cluster of blocks shares the
+// tiles of one; each leaves its unnormalised output, maxima and sums in its shared memory, and they
+// are joined from there, rows dealt to the blocks, always in the same order.
 template <int DP> struct FwdShared {
   static constexpr int kTile = kTcRows * DP * 2;
   static constexpr int kRing = 2;
   static constexpr int kK = 2 * kTile, kV = (2 + kRing) * kTile, kControl = (2 + 2 * kRing) * kTile;
   struct Control {
     float exchange[2][2][2][kTcRows];   // half of the queries, use (maximum, sum), half of the columns, row
+    float statistics[2 * kTcRows][2];   // SPLIT: maximum and sum
     uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[2], w_full[2], o_full[2];
     uint32_t tmem;
   };
+  static constexpr int kPartRow = DP + 4;   // floats; SPLIT: a row of the unnormalised output
+  static_assert(2 * kTcRows * kPartRow * 4 <= kControl, "the output takes the tiles' place");
   static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
 
-template <int DT, int DP>
+template <int DT, int DP, bool SPLIT>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -93,12 +99,16 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   const uint32_t base = smem_u32(aligned);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Blocks in the order of their work: the last queries of every head first.
-  const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / pairs;
-  const int b = blockIdx.x % pairs / P.heads, h = blockIdx.x % P.heads, hk = h / P.group;
-  const int i0 = (tiles - 1 - blockIdx.x / pairs) * 2 * kTcRows, i1 = min(P.queries, i0 + 2 * kTcRows);
+  const int splits = SPLIT ? P.splits : 1, rank = SPLIT ? (int)cluster_rank() : 0;
+  const uint32_t block = blockIdx.x / splits;
+  const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / splits / pairs;
+  const int b = block % pairs / P.heads, h = block % P.heads, hk = h / P.group;
+  const int i0 = (tiles - 1 - block / pairs) * 2 * kTcRows, i1 = min(P.queries, i0 + 2 * kTcRows);
   const int length = attn_length(P, b);
   const AttnKeys range(P, length, i0, i1);
-  const int blocks = range.blocks(kTcRows);
+  // The block's tiles: all, or its share.
+  const int all = range.blocks(kTcRows), first = all * rank / splits, blocks = all * (rank + 1) / splits - first;
+  auto tile_of = [&](int j, int& begin, int& end) { range.block(first + j, kTcRows, begin, end); };
   // Whether a query of half g sees a key of [begin, end) (half 1 may be past the last query).
   const AttnKeys range0(P, length, i0, min(i1, i0 + kTcRows)), range1(P, length, min(i1, i0 + kTcRows), i1);
   auto active = [&](int g, int begin, int end) {
@@ -114,7 +124,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   };
   auto fill = [&](const CUtensorMap& map, int at, uint64_t* full, int j) {
     int begin, end;
-    range.block(j, kTcRows, begin, end);
+    tile_of(j, begin, end);
     mbar_arrive_expect_tx(&full[j % RING], TILE);
     load(map, at + j % RING * TILE, begin, hk, &full[j % RING]);
   };
@@ -184,7 +194,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     bool finished[2] = {false, false};
     int begin = 0, end = 0;
     if (blocks > 0) {
-      range.block(0, kTcRows, begin, end);
+      tile_of(0, begin, end);
       ok = wait_warp(&ctl.q_full, 0) && wait_warp(&ctl.k_full[0], 0);
       if (ok) {
         if (active(0, begin, end)) scores(0, Shape::kK, end - begin);
@@ -196,7 +206,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       int next_begin = 0, next_end = 0;
       const int slot = j % RING, next = (j + 1) % RING;
       if (j + 1 < blocks) {
-        range.block(j + 1, kTcRows, next_begin, next_end);
+        tile_of(j + 1, next_begin, next_end);
         ok = wait_warp(&ctl.k_full[next], ring_phase(j + 1, RING));
       }
       ok = ok && wait_warp(&ctl.v_full[slot], ring_phase(j, RING));
@@ -251,7 +261,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     int done = 0;
     for (int j = 0; j < blocks; ++j) {
       int begin, end;
-      range.block(j, kTcRows, begin, end);
+      tile_of(j, begin, end);
       if (!active(g, begin, end)) continue;
       // A wait that ran out is remembered and not waited for again; the warp still takes part in
       // every barrier, so that no other warp is left waiting for it.
@@ -354,51 +364,113 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     named_barrier(pair, 64);
     // Halves in a fixed order, so that both threads of a row have the same sum.
     l = ctl.exchange[g][1][0][row] + ctl.exchange[g][1][1][row];
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    // The half's tile of queries is free now: 32 rows x half of the columns of each warp.
-    constexpr int WIDTH = DP / 2, CH = WIDTH / 8;
-    uint8_t* stage = aligned + warp * 32 * WIDTH * 2;
-    const int row0 = q0 + (warp & 3) * 32, rows = q1 - row0, vectors = (P.dim - half * WIDTH + 7) / 8;
-    const int64_t at = (P.os.at(b, h, row0) + half * WIDTH) * 2;
+    if constexpr (SPLIT) {
+      if (ok && blocks > 0) ok = wait_bar(&ctl.o_full[g ^ 1], 0);   // every tile is free
+      __syncwarp();
+      const int r = g * kTcRows + row;
+      if (done > 0) {
+        float* part = reinterpret_cast<float*>(aligned) + r * Shape::kPartRow + half * (DP / 2);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      char* dst = static_cast<char*>(which ? P.o_low : P.o);
-      if (dst == nullptr) continue;
-#pragma unroll
-      for (int c = 0; c < WIDTH; c += 32) {
-        uint32_t o[32];
-        if (done > 0) {
+        for (int c = 0; c < DP / 2; c += 32) {
+          uint32_t o[32];
           tmem_load32(t_o + c, o);
           tmem_wait_load();
-        }
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          uint32_t v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // A row without keys is 0 whatever the accumulator holds.
-            const float x = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k]) * f;
-            const float y = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k + 1]) * f;
-            v[k] = pack2<DT>(x, y);
-            if (which) {
-              const float2 r = unpack2<DT>(v[k]);
-              v[k] = pack2<DT>(x - r.x, y - r.y);
-            }
-          }
-          stage_vector<CH>(stage, lane, (c + e) / 8, make_uint4(v[0], v[1], v[2], v[3]));
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
-      store_staged<CH>(stage, lane, dst + at, P.os.t * 2, rows, vectors);
+      if (half == 0) {
+        ctl.statistics[r][0] = m;
+        ctl.statistics[r][1] = l;
+      }
+    } else {
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
+      // The half's tile of queries is free now: 32 rows x half of the columns of each warp.
+      constexpr int WIDTH = DP / 2, CH = WIDTH / 8;
+      uint8_t* stage = aligned + warp * 32 * WIDTH * 2;
+      const int row0 = q0 + (warp & 3) * 32, rows = q1 - row0, vectors = (P.dim - half * WIDTH + 7) / 8;
+      const int64_t at = (P.os.at(b, h, row0) + half * WIDTH) * 2;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        char* dst = static_cast<char*>(which ? P.o_low : P.o);
+        if (dst == nullptr) continue;
+#pragma unroll
+        for (int c = 0; c < WIDTH; c += 32) {
+          uint32_t o[32];
+          if (done > 0) {
+            tmem_load32(t_o + c, o);
+            tmem_wait_load();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // A row without keys is 0 whatever the accumulator holds.
+              const float x = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k]) * f;
+              const float y = f == 0.0f ? 0.0f : __uint_as_float(o[e + 2 * k + 1]) * f;
+              v[k] = pack2<DT>(x, y);
+              if (which) {
+                const float2 r = unpack2<DT>(v[k]);
+                v[k] = pack2<DT>(x - r.x, y - r.y);
+              }
+            }
+            stage_vector<CH>(stage, lane, (c + e) / 8, make_uint4(v[0], v[1], v[2], v[3]));
+          }
+        }
+        store_staged<CH>(stage, lane, dst + at, P.os.t * 2, rows, vectors);
+      }
+      const bool live = q0 + row < q1;
+      if (live && half == 0 && P.lse != nullptr)
+        P.lse[((int64_t)b * P.heads + h) * P.queries + q0 + row] =
+            l == 0.0f ? -INFINITY : fmaf(m, P.scale, log2f(l) * kLn2F);
     }
-    const bool live = q0 + row < q1;
-    if (live && half == 0 && P.lse != nullptr)
-      P.lse[((int64_t)b * P.heads + h) * P.queries + q0 + row] =
-          l == 0.0f ? -INFINITY : fmaf(m, P.scale, log2f(l) * kLn2F);
   }
   if (!ok && P.error != nullptr) atomicOr(P.error, 1);
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
+  if constexpr (SPLIT) {
+    cluster_sync_all();
+    constexpr int N = DP / 32;   // columns of a lane
+    const float* part = reinterpret_cast<const float*>(aligned);
+    for (int r = rank + splits * warp; warp < kComputeWarps && r < i1 - i0; r += splits * kComputeWarps) {
+      float top = -INFINITY, l = 0.0f, o[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = 0.0f;
+      for (int k = 0; k < splits; ++k) top = fmaxf(top, load_cluster(&ctl.statistics[r][0], k));
+      for (int k = 0; k < splits; ++k) {
+        const float m = load_cluster(&ctl.statistics[r][0], k);
+        const float f = m == -INFINITY ? 0.0f : ex2_approx((m - top) * P.scale_log2);
+        l = fmaf(load_cluster(&ctl.statistics[r][1], k), f, l);
+        if (f == 0.0f) continue;   // its part may not have been written
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fmaf(load_cluster(part + r * Shape::kPartRow + lane * N + e, k), f, o[e]);
+      }
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
+      uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+      for (int e = 0; e < N; e += 2) {
+        const float x = f == 0.0f ? 0.0f : o[e] * f, y = f == 0.0f ? 0.0f : o[e + 1] * f;
+        hi[e / 2] = pack2<DT>(x, y);
+        const float2 v = unpack2<DT>(hi[e / 2]);
+        lo[e / 2] = pack2<DT>(x - v.x, y - v.y);
+      }
+      if (lane * N < P.dim) {
+        const int64_t at = P.os.at(b, h, i0 + r) + lane * N;
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+          reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + at)[e] = hi[e];
+          if (P.o_low != nullptr) reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o_low) + at)[e] = lo[e];
+        }
+      }
+      if (lane == 0 && P.lse != nullptr)
+        P.lse[((int64_t)b * P.heads + h) * P.queries + i0 + r] =
+            l == 0.0f ? -INFINITY : fmaf(top, P.scale, log2f(l) * kLn2F);
+    }
+    cluster_sync_all();   // a block's shared memory stays until every block has read it
+  }
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -894,18 +966,43 @@ attention_tc_backward(const __grid_constant__ AttnParams P, uint32_t key_blocks,
 
 // ---- host ------------------------------------------------------------------------------
 
-template <int DT, int DP>
-static int launch_tc_forward(const AttnParams& P, cudaStream_t s) {
+template <int DT, int DP, bool SPLIT>
+static int launch_tc_forward(const AttnParams& P, unsigned blocks, cudaStream_t s) {
   const char* who = "nt_attention_forward";
   CUtensorMap q, k, v;
-  int rc = large_smem<attention_tc_forward<DT, DP>>(FwdShared<DP>::kBytes, who);
+  int rc = large_smem<attention_tc_forward<DT, DP, SPLIT>>(FwdShared<DP>::kBytes, who);
   if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
   if (rc) return rc;
-  const unsigned grid = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
-  attention_tc_forward<DT, DP><<<grid, kFwdThreads, FwdShared<DP>::kBytes, s>>>(P, q, k, v);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(blocks * (SPLIT ? P.splits : 1));
+  config.blockDim = dim3(kFwdThreads);
+  config.dynamicSmemBytes = FwdShared<DP>::kBytes;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = SPLIT ? P.splits : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = SPLIT ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&config, attention_tc_forward<DT, DP, SPLIT>, P, q, k, v);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, who); }
   return launch_status("nt_attention_forward launch");
+}
+
+// Blocks of a cluster that share the tiles of one block of queries: as many as the device runs at
+// once, with two tiles at least to each (512 queries of 16 heads after 7680 keys, window 2048: 39 us
+// in 32 blocks, SPLITUS in clusters of 4).
+template <int DT, int DP>
+static int dispatch_tc_forward(AttnParams P, cudaStream_t s) {
+  const unsigned blocks = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
+  int64_t keys = (int64_t)P.offset + P.queries < P.keys ? (int64_t)P.offset + P.queries : P.keys;
+  if (P.window > 0 && (int64_t)P.window + 2 * kTcRows + P.sinks < keys) keys = (int64_t)P.window + 2 * kTcRows + P.sinks;
+  P.splits = 1;
+  while (P.splits < 8 && (int64_t)blocks * P.splits * 2 <= current_sm_count() && keys >= (int64_t)4 * P.splits * kTcRows)
+    P.splits *= 2;
+  return P.splits > 1 ? launch_tc_forward<DT, DP, true>(P, blocks, s) : launch_tc_forward<DT, DP, false>(P, blocks, s);
 }
 
 template <int DT, int DP>
@@ -943,8 +1040,8 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
 }
 
 int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s) {
-  if (dtype == NT_BF16) return P.dim <= 64 ? launch_tc_forward<NT_BF16, 64>(P, s) : launch_tc_forward<NT_BF16, 128>(P, s);
-  return P.dim <= 64 ? launch_tc_forward<NT_F16, 64>(P, s) : launch_tc_forward<NT_F16, 128>(P, s);
+  if (dtype == NT_BF16) return P.dim <= 64 ? dispatch_tc_forward<NT_BF16, 64>(P, s) : dispatch_tc_forward<NT_BF16, 128>(P, s);
+  return P.dim <= 64 ? dispatch_tc_forward<NT_F16, 64>(P, s) : dispatch_tc_forward<NT_F16, 128>(P, s);
 }
 
 int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s) {
