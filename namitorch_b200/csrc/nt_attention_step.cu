@@ -14,8 +14,6 @@
 
 namespace nt {
 
-constexpr int kStepMaxCluster = 8;
-
 // The block's piece [from, to) of the visible keys of its sequence.
 struct StepKeys {
   int sink_end, skip, from, to;
@@ -61,17 +59,13 @@ __device__ __forceinline__ void join_step(const AttnParams& P, float* acc, const
   if (splits == 1) return;
   __syncthreads();
   cluster_sync_all();
-  for (int i = rank * THREADS + threadIdx.x; i < heads * DP; i += splits * THREADS) {
+  for (int i = (rank * THREADS + threadIdx.x) * 4; i < heads * DP; i += splits * THREADS * 4) {
     const int g = i / DP, c = i % DP;
-    float top = -INFINITY;
-    for (int r = 0; r < splits; ++r) top = fmaxf(top, load_cluster(acc + STRIDE + g * DP, r));
-    float sum = 0.0f, a = 0.0f;
-    for (int r = 0; r < splits; ++r) {
-      const float f = top == -INFINITY ? 0.0f : exp2f((load_cluster(acc + STRIDE + g * DP, r) - top) * P.scale_log2);
-      sum = fmaf(load_cluster(acc + STRIDE + g * DP + 1, r), f, sum);
-      a = fmaf(load_cluster(acc + i, r), f, a);
-    }
-    if (c < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c, sum == 0.0f ? 0.0f : a / sum);
+    const JoinedRow row = join_row(acc + i, acc + STRIDE + g * DP, splits, P.scale_log2);
+    const float x[4] = {row.o.x, row.o.y, row.o.z, row.o.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < P.dim) store1<DT>(P.o, P.os.at(b, h0 + g, 0) + c + e, row.sum == 0.0f ? 0.0f : x[e] / row.sum);
   }
   cluster_sync_all();   // a block's shared memory stays until every block has read it
 }
@@ -434,7 +428,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
 static int step_splits(const AttnParams& P, int64_t units, int most_blocks, int least) {
   const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
   int splits = 1;
-  while (splits < kStepMaxCluster && units * splits * 2 <= most_blocks && most > (int64_t)least * splits) splits *= 2;
+  while (splits < kMaxSplits && units * splits * 2 <= most_blocks && most > (int64_t)least * splits) splits *= 2;
   return splits;
 }
 

@@ -433,41 +433,27 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
   if constexpr (SPLIT) {
     cluster_sync_all();
-    constexpr int N = DP / 32;   // columns of a lane
+    constexpr int LPR = DP / 4, RPW = 32 / LPR;   // four columns a lane
     const float* part = reinterpret_cast<const float*>(aligned);
-    for (int r = rank + splits * warp; warp < kComputeWarps && r < i1 - i0; r += splits * kComputeWarps) {
-      float top = -INFINITY, l = 0.0f, o[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = 0.0f;
-      for (int k = 0; k < splits; ++k) top = fmaxf(top, load_cluster(&ctl.statistics[r][0], k));
-      for (int k = 0; k < splits; ++k) {
-        const float m = load_cluster(&ctl.statistics[r][0], k);
-        const float f = m == -INFINITY ? 0.0f : ex2_approx((m - top) * P.scale_log2);
-        l = fmaf(load_cluster(&ctl.statistics[r][1], k), f, l);
-        if (f == 0.0f) continue;   // its part may not have been written
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = fmaf(load_cluster(part + r * Shape::kPartRow + lane * N + e, k), f, o[e]);
-      }
-      const float f = l == 0.0f ? 0.0f : 1.0f / l;
-      uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        const float x = f == 0.0f ? 0.0f : o[e] * f, y = f == 0.0f ? 0.0f : o[e + 1] * f;
-        hi[e / 2] = pack2<DT>(x, y);
-        const float2 v = unpack2<DT>(hi[e / 2]);
-        lo[e / 2] = pack2<DT>(x - v.x, y - v.y);
-      }
-      if (lane * N < P.dim) {
-        const int64_t at = P.os.at(b, h, i0 + r) + lane * N;
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) {
-          reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o) + at)[e] = hi[e];
-          if (P.o_low != nullptr) reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(P.o_low) + at)[e] = lo[e];
+    for (int r0 = (rank + splits * warp) * RPW; warp < kComputeWarps && r0 < i1 - i0; r0 += splits * kComputeWarps * RPW) {
+      const int r = r0 + lane / LPR, c = lane % LPR * 4;
+      if (r >= i1 - i0) continue;
+      const JoinedRow row = join_row(part + r * Shape::kPartRow + c, ctl.statistics[r], splits, P.scale_log2);
+      const float f = row.sum == 0.0f ? 0.0f : 1.0f / row.sum;
+      const float x[4] = {row.o.x * f, row.o.y * f, row.o.z * f, row.o.w * f};
+      if (c < P.dim) {
+        const int64_t at = P.os.at(b, h, i0 + r) + c;
+        const uint2 hi = make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.o) + at) = hi;
+        if (P.o_low != nullptr) {
+          const float2 v = unpack2<DT>(hi.x), w = unpack2<DT>(hi.y);
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.o_low) + at) =
+              make_uint2(pack2<DT>(x[0] - v.x, x[1] - v.y), pack2<DT>(x[2] - w.x, x[3] - w.y));
         }
       }
-      if (lane == 0 && P.lse != nullptr)
+      if (c == 0 && P.lse != nullptr)
         P.lse[((int64_t)b * P.heads + h) * P.queries + i0 + r] =
-            l == 0.0f ? -INFINITY : fmaf(top, P.scale, log2f(l) * kLn2F);
+            row.sum == 0.0f ? -INFINITY : fmaf(row.top, P.scale, log2f(row.sum) * kLn2F);
     }
     cluster_sync_all();   // a block's shared memory stays until every block has read it
   }
@@ -993,14 +979,14 @@ static int launch_tc_forward(const AttnParams& P, unsigned blocks, cudaStream_t 
 
 // Blocks of a cluster that share the tiles of one block of queries: as many as the device runs at
 // once, with two tiles at least to each (512 queries of 16 heads after 7680 keys, window 2048: 39 us
-// in 32 blocks, SPLITUS in clusters of 4).
+// in 32 blocks, 23 in clusters of 4).
 template <int DT, int DP>
 static int dispatch_tc_forward(AttnParams P, cudaStream_t s) {
   const unsigned blocks = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
   int64_t keys = (int64_t)P.offset + P.queries < P.keys ? (int64_t)P.offset + P.queries : P.keys;
   if (P.window > 0 && (int64_t)P.window + 2 * kTcRows + P.sinks < keys) keys = (int64_t)P.window + 2 * kTcRows + P.sinks;
   P.splits = 1;
-  while (P.splits < 8 && (int64_t)blocks * P.splits * 2 <= current_sm_count() && keys >= (int64_t)4 * P.splits * kTcRows)
+  while (P.splits < kMaxSplits && (int64_t)blocks * P.splits * 2 <= current_sm_count() && keys >= (int64_t)4 * P.splits * kTcRows)
     P.splits *= 2;
   return P.splits > 1 ? launch_tc_forward<DT, DP, true>(P, blocks, s) : launch_tc_forward<DT, DP, false>(P, blocks, s);
 }

@@ -48,6 +48,53 @@ __device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ float4 load_cluster4(const float* p, uint32_t rank) {
+  uint32_t local = static_cast<uint32_t>(__cvta_generic_to_shared(p)), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote));
+  return v;
+}
+constexpr int kMaxSplits = 8;   // blocks of a portable cluster
+
+// Four columns of a row whose parts lie in `splits` blocks: unnormalised output at `part`, maximum
+// and sum at `statistic`. Every load is issued before the first is used (one at a time they cost a
+// trip to the other SM each). Adds the parts in rank order; a part of weight 0 may not be there.
+struct JoinedRow {
+  float4 o;
+  float top, sum;
+};
+__device__ __forceinline__ JoinedRow join_row(const float* part, const float* statistic, int splits, float scale_log2) {
+  float m[kMaxSplits], l[kMaxSplits];
+  float4 v[kMaxSplits];
+#pragma unroll
+  for (int k = 0; k < kMaxSplits; ++k) {
+    m[k] = -INFINITY;
+    l[k] = 0.0f;
+    v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (k < splits) {
+      m[k] = load_cluster(statistic, k);
+      l[k] = load_cluster(statistic + 1, k);
+      v[k] = load_cluster4(part, k);
+    }
+  }
+  JoinedRow r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+#pragma unroll
+  for (int k = 0; k < kMaxSplits; ++k) r.top = fmaxf(r.top, m[k]);
+#pragma unroll
+  for (int k = 0; k < kMaxSplits; ++k) {
+    const float f = m[k] == -INFINITY ? 0.0f : exp2f((m[k] - r.top) * scale_log2);
+    r.sum = fmaf(l[k], f, r.sum);
+    if (f != 0.0f) {
+      r.o.x = fmaf(v[k].x, f, r.o.x);
+      r.o.y = fmaf(v[k].y, f, r.o.y);
+      r.o.z = fmaf(v[k].z, f, r.o.z);
+      r.o.w = fmaf(v[k].w, f, r.o.w);
+    }
+  }
+  return r;
+}
+
 // Programmatic dependent launch: the next kernel's blocks may start from here on; wait for the end of
 // the kernel before (no wait where there is no such dependence).
 __device__ __forceinline__ void grid_dependents_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
