@@ -135,8 +135,10 @@ __global__ void __launch_bounds__(kSimtThreads) attention_forward_kernel(const _
   float* kv = q + kRows * (DP + 4);
   float* w = kv + kRows * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int b = blockIdx.z, h = blockIdx.y, hk = h / P.group;
-  const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows, i1 = min(P.queries, i0 + kRows);
+  // Blocks in the order of their work: the last queries of every head first.
+  const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / pairs;
+  const int b = blockIdx.x % pairs / P.heads, h = blockIdx.x % P.heads, hk = h / P.group;
+  const int i0 = (tiles - 1 - blockIdx.x / pairs) * kRows, i1 = min(P.queries, i0 + kRows);
   const int length = attn_length(P, b);
   const AttnKeys range(P, length, i0, i1);
   const int es = sizeof(typename Elem<DT>::T);
@@ -224,7 +226,9 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   __shared__ float row_lse[kRows], row_delta[kRows];
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int es = sizeof(typename Elem<DT>::T);
-  const int b = blockIdx.z;
+  // Blocks in the order of their work: the last queries, or the first keys, of every head first.
+  const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch;
+  const int b = blockIdx.x % pairs / heads, index = blockIdx.x / pairs;
   const int length = attn_length(P, b);
   const char *qb = static_cast<const char*>(P.q), *kb = static_cast<const char*>(P.k), *vb = static_cast<const char*>(P.v),
              *gb = static_cast<const char*>(P.g);
@@ -235,8 +239,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     for (int u = 0; u < DP / 64; ++u) out1[i][u] = out2[i][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
   if constexpr (!DKV) {
-    const int h = blockIdx.y, hk = h / P.group;
-    const int i0 = (gridDim.x - 1 - blockIdx.x) * kRows, i1 = min(P.queries, i0 + kRows);
+    const int h = blockIdx.x % heads, hk = h / P.group;
+    const int i0 = ((P.queries + kRows - 1) / kRows - 1 - index) * kRows, i1 = min(P.queries, i0 + kRows);
     const AttnKeys range(P, length, i0, i1);
     load_tile<DT, DP>(x1, qb + P.qs.at(b, h, 0) * es, P.qs.t, i0, i1, P.dim, P.vec);
     load_tile<DT, DP>(x2, gb + P.gs.at(b, h, 0) * es, P.gs.t, i0, i1, P.dim, P.vec);
@@ -285,11 +289,11 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     for (int i = 0; i < 4; ++i)
       if (i0 + 4 * ty + i < i1) store_row4<DT, DP>(P.dq, P.dqs.at(b, h, i0 + 4 * ty + i), tx, P.dim, out1[i], P.scale);
   } else {
-    const int hk = blockIdx.y;
-    const int split = P.sink_tiles * P.parts;
-    const int tile = (int)blockIdx.x < split ? (int)blockIdx.x / P.parts : (int)blockIdx.x - split + P.sink_tiles;
-    const int part = (int)blockIdx.x < split ? (int)blockIdx.x % P.parts : 0;
-    const int parts = (int)blockIdx.x < split ? P.parts : 1;
+    const int hk = blockIdx.x % heads;
+    const int split = P.split_tiles * P.parts;
+    const int tile = index < split ? index / P.parts : index - split + P.split_tiles;
+    const int part = index < split ? index % P.parts : 0;
+    const int parts = index < split ? P.parts : 1;
     const int k0 = tile * kRows, k1 = min(P.keys, k0 + kRows);
     const AttnQueries range(P, length, k0, k1);
     load_tile<DT, DP>(x1, kb + P.ks.at(b, hk, 0) * es, P.ks.t, k0, k1, P.dim, P.vec);
@@ -336,8 +340,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
         store_row4<DT, DP>(P.dv, P.dvs.at(b, hk, row), tx, P.dim, out2[i], 1.0f);
       }
     } else {
-      // [batch, kv head, sink block, part, 2, 64, dim]
-      const int64_t at = ((((int64_t)b * P.kv_heads + hk) * P.sink_tiles + tile) * parts + part) * 2 * kRows * P.dim;
+      // [batch, kv head, split block, part, 2, 64, dim]
+      const int64_t at = ((((int64_t)b * P.kv_heads + hk) * P.split_tiles + tile) * parts + part) * 2 * kRows * P.dim;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t r = 4 * ty + i;
@@ -348,23 +352,31 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   }
 }
 
-// dk and dv of the split key blocks (of `tile_rows` keys): the parts added in order, one thread per
-// element. Grid: pieces of 256 elements of dk or dv of a block, in that order; then blocks, then
+// dk and dv of the split key blocks (of `tile_rows` keys): the parts added in order, four elements a
+// thread. Grid: pieces of 1024 elements of dk or dv of a block, in that order; then blocks, then
 // batch x key head.
 template <int DT>
 __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnParams P, int tile_rows) {
-  const int size = tile_rows * P.dim, pieces = (size + 255) / 256;
-  const int e = blockIdx.x % pieces * 256 + threadIdx.x, which = blockIdx.x / pieces % 2;
-  const int block = blockIdx.x / pieces / 2, tile = block % P.sink_tiles, pair = block / P.sink_tiles;
+  const int size = tile_rows * P.dim, pieces = (size + 1023) / 1024;   // (size is a multiple of 64)
+  const int e = (blockIdx.x % pieces * 256 + threadIdx.x) * 4, which = blockIdx.x / pieces % 2;
+  const int block = blockIdx.x / pieces / 2, tile = block % P.split_tiles, pair = block / P.split_tiles;
   const int b = pair / P.kv_heads, hk = pair % P.kv_heads;
-  const int key = tile * tile_rows + e / P.dim, c = e % P.dim;
-  if (e >= size || key >= P.keys) return;
+  if (e >= size || tile * tile_rows + e / P.dim >= P.keys) return;
   const float* src = P.partial + ((int64_t)block * P.parts * 2 + which) * size + e;
-  float s = 0.0f;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int k = 0; k < P.parts; ++k) s += src[(int64_t)k * 2 * size];
-  if (which == 0) store1<DT>(P.dk, P.dks.at(b, hk, key) + c, s);
-  else store1<DT>(P.dv, P.dvs.at(b, hk, key) + c, s);
+  for (int k = 0; k < P.parts; ++k) {
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)k * 2 * size));
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const float out[4] = {s.x, s.y, s.z, s.w};
+  void* dst = which == 0 ? P.dk : P.dv;
+  const AttnStrides& st = which == 0 ? P.dks : P.dvs;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = tile * tile_rows + (e + i) / P.dim;
+    if (key < P.keys) store1<DT>(dst, st.at(b, hk, key) + (e + i) % P.dim, out[i]);
+  }
 }
 
 // ---- launches ------------------------------------------------------------------------
@@ -374,7 +386,7 @@ static int launch_forward(const AttnParams& P, cudaStream_t s) {
   const size_t bytes = (size_t)(2 * kRows * (DP + 4) + kRows * kWeightStride) * 4;
   const int rc = large_smem<attention_forward_kernel<DT, DP>>(bytes, "nt_attention_forward");
   if (rc) return rc;
-  const dim3 grid((P.queries + kRows - 1) / kRows, P.heads, P.batch);
+  const unsigned grid = (unsigned)((P.queries + kRows - 1) / kRows) * P.heads * P.batch;
   attention_forward_kernel<DT, DP><<<grid, kSimtThreads, bytes, s>>>(P);
   return launch_status("nt_attention_forward launch");
 }
@@ -388,13 +400,13 @@ static int launch_backward(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = large_smem<attention_backward_kernel<DT, DP, true>>(bytes, "nt_attention_backward");
   if (rc) return rc;
   if (P.queries > 0) {
-    dq<<<dim3((P.queries + kRows - 1) / kRows, P.heads, P.batch), kSimtThreads, bytes, s>>>(P);
+    dq<<<(unsigned)((P.queries + kRows - 1) / kRows) * P.heads * P.batch, kSimtThreads, bytes, s>>>(P);
     rc = launch_status("nt_attention_backward launch");
     if (rc) return rc;
   }
   const int tiles = (P.keys + kRows - 1) / kRows;
   if (tiles == 0) return NT_OK;
-  dkv<<<dim3(tiles + P.sink_tiles * (P.parts - 1), P.kv_heads, P.batch), kSimtThreads, bytes, s>>>(P);
+  dkv<<<(unsigned)(tiles + P.split_tiles * (P.parts - 1)) * P.kv_heads * P.batch, kSimtThreads, bytes, s>>>(P);
   return launch_status("nt_attention_backward launch");
 }
 
@@ -404,9 +416,9 @@ static int dispatch_forward(const AttnParams& P, cudaStream_t s) {
 }
 template <int DT>
 static int launch_join(const AttnParams& P, int tile_rows, cudaStream_t s) {
-  if (P.parts == 1 || P.sink_tiles == 0) return NT_OK;
-  const unsigned pieces = (tile_rows * P.dim + 255) / 256;
-  attention_join_kernel<DT><<<pieces * 2 * P.sink_tiles * P.batch * P.kv_heads, 256, 0, s>>>(P, tile_rows);
+  if (P.parts == 1 || P.split_tiles == 0) return NT_OK;
+  const unsigned pieces = (tile_rows * P.dim + 1023) / 1024;
+  attention_join_kernel<DT><<<pieces * 2 * P.split_tiles * P.batch * P.kv_heads, 256, 0, s>>>(P, tile_rows);
   return launch_status("nt_attention_backward (join) launch");
 }
 template <int DT>
@@ -415,34 +427,51 @@ static int dispatch_backward(const AttnParams& P, cudaStream_t s) {
   return rc ? rc : launch_join<DT>(P, kRows, s);
 }
 
-// Pieces of the queries of a sink key block: an ordinary key block sees the queries of its own
-// width and one window, a sink block all later ones. A piece is no longer than an ordinary
-// block's work, nor shorter than 16 steps.
-static int sink_parts(int64_t queries, int64_t window, int64_t group, int64_t tile_rows, int64_t step_rows) {
-  const int64_t most = (queries + step_rows - 1) / step_rows * group;
-  int64_t piece = ((tile_rows + window - 1 + step_rows - 1) / step_rows + 1) * group;
-  if (piece < 16) piece = 16;
-  const int64_t parts = (most + piece - 1) / piece;
-  return (int)(parts < 1 ? 1 : parts);
-}
-
-static size_t delta_bytes(const nt_attention_args& a) {
-  return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
-}
-
 // The window where it hides a key: 0 where it covers every position (below `positions`) or every key
 // is a sink.
 static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
   return a.window >= positions || a.sinks >= a.keys ? 0 : a.window;
 }
 
+// Which key blocks of the backward (the first `tiles`) have their queries cut into `parts` pieces,
+// whose sums are joined by a kernel of their own. Counted in steps of one block of queries:
+// - a sink block sees every later query, an ordinary one those of its own width and one window; a
+//   sink block's piece is no longer than an ordinary block's work, nor shorter than 16 steps;
+// - where the longest ordinary block is more than an SM's share of all steps (few key heads, many
+//   query heads to each, long rows), every key block is cut, to half of that share (4 query heads on
+//   one key head, 6508 tokens, no window, forward and backward: 407 us uncut, 225 cut).
+struct KeySplit {
+  int tiles, parts;
+};
+static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_rows) {
+  auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+  const int64_t window = effective_window(a, a.query_offset + a.queries), group = a.query_heads / a.kv_heads;
+  const int64_t tiles = up(a.keys, tile_rows), steps = up(a.queries, step_rows);
+  if (tiles == 0 || steps == 0) return {0, 1};
+  int64_t ordinary = window == 0 ? steps : up(tile_rows + window - 1, step_rows) + 1;
+  if (ordinary > steps) ordinary = steps;
+  // Both passes; without a window about half of the blocks' pairs lie past the diagonal.
+  const int64_t share = tiles * ordinary * a.query_heads * a.batch * (window == 0 ? 1 : 2) / current_sm_count();
+  const int64_t longest = ordinary * group, most = steps * group;
+  const bool sinks = window > 0 && a.sinks > 0;
+  if (longest >= 16 && longest > share) {
+    const int64_t piece = share / 2 > 8 ? share / 2 : 8;
+    const int64_t parts = up(sinks ? most : longest, piece);
+    return {(int)tiles, (int)(parts < 32 ? parts : 32)};
+  }
+  if (!sinks) return {0, 1};
+  const int64_t parts = up(most, longest > 16 ? longest : 16);
+  return {(int)up(a.sinks, tile_rows), (int)parts};
+}
+
+static size_t delta_bytes(const nt_attention_args& a) {
+  return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
+}
+
 static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows) {
-  const int64_t window = effective_window(a, a.query_offset + a.queries);
-  if (window == 0 || a.sinks == 0) return 0;
-  const int64_t tiles = (a.sinks + tile_rows - 1) / tile_rows;
-  const int64_t parts = sink_parts(a.queries, window, a.query_heads / a.kv_heads, tile_rows, step_rows);
-  if (parts == 1) return 0;
-  return (size_t)a.batch * a.kv_heads * tiles * parts * 2 * tile_rows * a.head_dim * 4;
+  const KeySplit split = key_split(a, tile_rows, step_rows);
+  if (split.parts == 1) return 0;
+  return (size_t)a.batch * a.kv_heads * split.tiles * split.parts * 2 * tile_rows * a.head_dim * 4;
 }
 
 static int check_attention(const nt_attention_args& a, const char* who) {
@@ -583,8 +612,9 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
                   vector_query(a, a.output_low, a.output_strides) && vector_query(a, a.grad_query, a.grad_query_strides) &&
                   vector_key(a, a.grad_key, a.grad_key_strides) && vector_key(a, a.grad_value, a.grad_value_strides);
   const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? kTcQueryStep : kRows;
-  P.sink_tiles = (P.sinks + tile_rows - 1) / tile_rows;
-  P.parts = P.sink_tiles ? sink_parts(a.queries, P.window, P.group, tile_rows, step_rows) : 1;
+  const KeySplit split = key_split(a, tile_rows, step_rows);
+  P.split_tiles = split.parts > 1 ? split.tiles : 0;
+  P.parts = split.parts;
   cudaStream_t s = as_stream(stream);
   if (tc) {
     rc = attention_tc_backward_launch(P, a.dtype, s);

@@ -23,7 +23,7 @@ struct AttnParams {
   AttnStrides qs, ks, vs, gs, os, dqs, dks, dvs;
   float* lse;        // [batch, heads, queries]
   float* delta;      // [batch, heads, queries]: sum over head_dim of g * o
-  float* partial;    // backward: partial gradients of the sink key blocks, or NULL
+  float* partial;    // backward: partial gradients of the split key blocks
   const int32_t* lengths;
   int32_t* error;
   int batch, heads, kv_heads, group, queries, keys, dim;
@@ -31,9 +31,9 @@ struct AttnParams {
   int sinks;         // 0 without a window
   int offset;
   int vec;           // rows are 16-byte aligned runs of whole 16-byte vectors
-  // Backward over key blocks: the first `sink_tiles` blocks hold sinks, which every later query
-  // sees, so their queries are cut into `parts` pieces.
-  int sink_tiles, parts;
+  // Backward over key blocks: the queries of the first `split_tiles` blocks are cut into `parts`
+  // pieces.
+  int split_tiles, parts;
   int splits;        // forward: blocks of a cluster that share a block of queries
   float scale, scale_log2;
 };

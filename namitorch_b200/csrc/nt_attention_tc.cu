@@ -4,7 +4,7 @@
 // One block per SM: one warp copies tiles, one issues the products, sixteen compute. Scores
 // accumulate in TMEM; the weights go back to TMEM over them as 16-bit values and are the first
 // operand of the second product. The backward is two passes of one kernel, each with S and dP
-// computed again; sums that cross blocks exist only for the sink keys and are added in order
+// computed again; sums that cross blocks exist only for split key blocks and are added in order
 // afterwards.
 //
 // Roundings below 32 bits: the weights and dS are rounded to the inputs' type because the second
@@ -547,8 +547,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     r0 = ((P.queries + kTcRows - 1) / kTcRows - 1 - index) * kTcRows;
     r1 = min(P.queries, r0 + kTcRows);
   } else {
-    const int split = P.sink_tiles * P.parts;
-    tile = index < split ? index / P.parts : index - split + P.sink_tiles;
+    const int split = P.split_tiles * P.parts;
+    tile = index < split ? index / P.parts : index - split + P.split_tiles;
     part = index < split ? index % P.parts : 0;
     parts = index < split ? P.parts : 1;
     r0 = tile * kTcRows;
@@ -910,9 +910,9 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       const AttnStrides& st = DKV ? (which ? P.dvs : P.dks) : P.dqs;
       store_staged<CH>(stage, lane, dst + (st.at(b, h0, row0) + c_first) * 2, st.t * 2, r1 - row0, (P.dim - c_first + 7) / 8);
     } else {
-      // float32 [batch, key head, sink block, part, 2, 128, dim]
+      // float32 [batch, key head, split block, part, 2, 128, dim]
       char* dst = reinterpret_cast<char*>(
-          P.partial + ((((((int64_t)b * P.kv_heads + h0) * P.sink_tiles + tile) * parts + part) * 2 + which) * kTcRows +
+          P.partial + ((((((int64_t)b * P.kv_heads + h0) * P.split_tiles + tile) * parts + part) * 2 + which) * kTcRows +
                        (warp & 3) * 32) * P.dim + c_first);
       constexpr int CH = CHUNK / 4;
 #pragma unroll
@@ -977,16 +977,22 @@ static int launch_tc_forward(const AttnParams& P, unsigned blocks, cudaStream_t 
   return launch_status("nt_attention_forward launch");
 }
 
-// Blocks of a cluster that share the tiles of one block of queries: as many as the device runs at
-// once, with two tiles at least to each (512 queries of 16 heads after 7680 keys, window 2048: 39 us
-// in 32 blocks, 23 in clusters of 4).
+// Blocks of a cluster that share the tiles of one block of queries: more of them while the longest
+// block is more than 1.5 times an SM's share of all tiles, with two tiles at least to each (512
+// queries of 16 heads after 7680 keys, window 2048: 39 us in 32 blocks, 23 in clusters of 4). Clusters
+// of 8 only where they all run at once: a second wave of them waits for 8 free SMs side by side (58 us).
 template <int DT, int DP>
 static int dispatch_tc_forward(AttnParams P, cudaStream_t s) {
   const unsigned blocks = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
-  int64_t keys = (int64_t)P.offset + P.queries < P.keys ? (int64_t)P.offset + P.queries : P.keys;
-  if (P.window > 0 && (int64_t)P.window + 2 * kTcRows + P.sinks < keys) keys = (int64_t)P.window + 2 * kTcRows + P.sinks;
+  const int64_t end = (int64_t)P.offset + P.queries;
+  int64_t longest = end < P.keys ? end : P.keys, mean = longest;
+  if (P.window > 0 && (int64_t)P.window + 2 * kTcRows + P.sinks < longest) longest = mean = (int64_t)P.window + 2 * kTcRows + P.sinks;
+  else if (P.offset + P.queries / 2 < mean) mean = P.offset + P.queries / 2;
+  const int sms = current_sm_count();
   P.splits = 1;
-  while (P.splits < kMaxSplits && (int64_t)blocks * P.splits * 2 <= current_sm_count() && keys >= (int64_t)4 * P.splits * kTcRows)
+  while (P.splits < kMaxSplits && longest >= (int64_t)4 * P.splits * kTcRows &&
+         longest * sms * 2 > 3 * (int64_t)blocks * mean * P.splits &&
+         (P.splits < 4 || (int64_t)blocks * P.splits * 2 <= sms))
     P.splits *= 2;
   return P.splits > 1 ? launch_tc_forward<DT, DP, true>(P, blocks, s) : launch_tc_forward<DT, DP, false>(P, blocks, s);
 }
@@ -1008,7 +1014,7 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   if (rc) return rc;
   const uint32_t query_blocks = (uint32_t)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
   const uint32_t key_blocks =
-      (uint32_t)((P.keys + kTcKeyRows - 1) / kTcKeyRows + P.sink_tiles * (P.parts - 1)) * P.kv_heads * P.batch;
+      (uint32_t)((P.keys + kTcKeyRows - 1) / kTcKeyRows + P.split_tiles * (P.parts - 1)) * P.kv_heads * P.batch;
   // Its blocks may start while the kernel before it ends.
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(key_blocks + query_blocks);
