@@ -131,7 +131,8 @@ NT_ATTENTION_MAX_HEAD_DIM = 128
 _Strides = C.c_int64 * 3
 # The argument blocks of the attention and dropout calls as one struct.pack (their fields in
 # order): building a ctypes Structure field by field costs several times a kernel launch.
-pack_attention = struct.Struct("@ii5q3P9qP3qfiP3qPPPPPP12qPNP").pack
+pack_attention = struct.Struct("@ii5q3P9qP3qfiP3qPPPPPP12q").pack
+pack_attention_scratch = struct.Struct("@PNP").pack   # workspace, its bytes, error word: the last three fields
 pack_dropout = struct.Struct("@iiqqdQQPPPPPPN").pack
 
 
@@ -317,12 +318,16 @@ def stream_handle(stream=None) -> int:
 def on_device(device, name: str, args: bytes, launches: int) -> None:
     """``call`` with an argument block on the current stream of ``device``, which is made the
     current device for the call when it is not."""
+    global launch_count
     import torch
     index = device.index
     if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
             return on_device(device, name, args, launches)
-    call(name, args, torch._C._cuda_getCurrentRawStream(index), launches=launches)
+    status = getattr(_lib or load(), name)(args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status, name)
+    launch_count += launches
 
 
 def dtype_code(dtype) -> int:

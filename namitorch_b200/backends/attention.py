@@ -16,6 +16,7 @@ from .. import _native as N
 
 _CODES = {torch.float32: N.NT_F32, torch.float16: N.NT_F16, torch.bfloat16: N.NT_BF16}
 _NO_STRIDES = (0,) * 12
+_NO_SCRATCH = N.pack_attention_scratch(0, 0, 0)
 
 
 def _rows(tensor):
@@ -75,7 +76,8 @@ class AttentionCUDAKernels:
             _CODES[query.dtype], dim, batch, heads, key.shape[1], queries, key.shape[2], q, k, v, *q_strides, *k_strides,
             *v_strides, 0 if lengths is None else lengths.data_ptr(), window, sinks, query_offset, scale, 0,
             output.data_ptr(), *output.stride()[:3], 0 if low is None else low.data_ptr(),
-            0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, *_NO_STRIDES, 0, 0, self._error_word(query.device))
+            0 if lse is None else lse.data_ptr(), 0, 0, 0, 0, *_NO_STRIDES)
+        args += N.pack_attention_scratch(0, 0, self._error_word(query.device))
         N.on_device(query.device, "nt_attention_forward", args, int(batch * queries > 0))
         return output, low, lse
 
@@ -92,19 +94,16 @@ class AttentionCUDAKernels:
         dk = _heads_last(batch, kv_heads, keys, dim, query)
         dv = _heads_last(batch, kv_heads, keys, dim, query)
         kv_strides = dk.stride()[:3]
-
-        def pack(workspace, size):
-            return N.pack_attention(
-                _CODES[query.dtype], dim, batch, heads, kv_heads, queries, keys, q, k, v, *q_strides, *k_strides,
-                *v_strides, 0 if lengths is None else lengths.data_ptr(), window, sinks, query_offset, scale, 0,
-                output.data_ptr(), *output.stride()[:3], 0 if low is None else low.data_ptr(), lse.data_ptr(), g,
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *g_strides, *dq.stride()[:3], *kv_strides, *kv_strides,
-                workspace, size, self._error_word(query.device))
-
-        size = int(N.load().nt_attention_workspace_size(pack(0, 0)))
+        args = N.pack_attention(
+            _CODES[query.dtype], dim, batch, heads, kv_heads, queries, keys, q, k, v, *q_strides, *k_strides, *v_strides,
+            0 if lengths is None else lengths.data_ptr(), window, sinks, query_offset, scale, 0, output.data_ptr(),
+            *output.stride()[:3], 0 if low is None else low.data_ptr(), lse.data_ptr(), g, dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), *g_strides, *dq.stride()[:3], *kv_strides, *kv_strides)
+        size = N.load().nt_attention_workspace_size(args + _NO_SCRATCH)
         workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
+        args += N.pack_attention_scratch(workspace.data_ptr(), size, self._error_word(query.device))
         statistics = (batch * heads * queries * 4 + 255) // 256 * 256
-        N.on_device(query.device, "nt_attention_backward", pack(workspace.data_ptr(), size),
+        N.on_device(query.device, "nt_attention_backward", args,
                     int(batch * queries > 0) + int(batch * keys > 0) + int(size > statistics))
         return dq, dk, dv
 
@@ -119,7 +118,7 @@ class AttentionCUDAKernels:
         args = N.pack_attention(
             _CODES[query.dtype], dim, batch, heads, key.shape[1], 1, key.shape[2], query.data_ptr(), k, v, *strides,
             *k_strides, *v_strides, lengths.data_ptr(), window, sinks, 0, scale, 0, output.data_ptr(), *strides, 0, 0, 0,
-            0, 0, 0, *_NO_STRIDES, 0, 0, self._error_word(query.device))
+            0, 0, 0, *_NO_STRIDES) + N.pack_attention_scratch(0, 0, self._error_word(query.device))
         N.on_device(query.device, "nt_attention_step", args, int(batch > 0))
         return output
 
