@@ -83,11 +83,34 @@ constexpr int kRingKeys = 16;
 
 template <int DP> struct StepShared {
   static constexpr int kTile = kRingKeys * DP * 2;      // keys or values
-  static constexpr int kStages = DP == 128 ? 3 : 6;
+  // (More in flight is slower: the DRAM sees as many streams as there are warps. 8 sequences up to 32768
+  // keys took 64.5 us with 2 stages, 67 with 3, 109 with 6.)
+  static constexpr int kStages = DP == 128 ? 2 : 4;
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kBytes = kRingWarps * kRing + 1024;
   static_assert(kRingWarps * 8 * DP * 4 <= kBytes - 1024, "the partial outputs take the rings' place");
 };
+
+// Sequence of the blocks with index z: the longest first, so that the last ones to start are short and
+// the blocks that share an SM differ (the lengths are known on the device alone). Every block ranks
+// them for itself, in `scratch`; more than kRankedBatch of them stay in their order.
+constexpr int kRankedBatch = 256;
+__device__ __forceinline__ int ranked_sequence(const AttnParams& P, int z, int* scratch, int* found) {
+  if (P.batch == 1 || P.batch > kRankedBatch) return z;
+  for (int i = threadIdx.x; i < P.batch; i += blockDim.x) {
+    const int n = attn_length(P, i);
+    scratch[i] = P.window == 0 ? n : min(n, P.window + P.sinks);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < P.batch; i += blockDim.x) {
+    const int n = scratch[i];
+    int rank = 0;
+    for (int j = 0; j < P.batch; ++j) rank += scratch[j] > n || (scratch[j] == n && j < i);
+    if (rank == z) *found = i;
+  }
+  __syncthreads();
+  return *found;
+}
 
 // The block's pieces of 16 keys: those of the sinks, then those of the window.
 struct StepPieces {
@@ -147,6 +170,7 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kRingWarps][STAGES];
   __shared__ float ml[kRingWarps][8][2];
+  __shared__ int sequence;
   // The same place in every block of the cluster.
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -155,7 +179,7 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
   const int passes = (P.group + 7) / 8;
   const int hk = blockIdx.y / passes, first = blockIdx.y % passes * 8;
   const int h0 = hk * P.group + first, heads = min(8, P.group - first);
-  const int b = blockIdx.z;
+  const int b = ranked_sequence(P, blockIdx.z, reinterpret_cast<int*>(ring), &sequence);
   const StepPieces pieces(P, attn_length(P, b), rank, splits);
   uint8_t* mine = ring + warp * Shape::kRing;
 
@@ -163,6 +187,7 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) mbar_init(&full[warp][s], 1);
     fence_mbar_init();
+    fence_proxy_async();   // the ranking used the ring's place
   }
   __syncwarp();
 
@@ -424,11 +449,13 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
 // Blocks of one cluster share the visible keys: as many as the device runs at once (`most_blocks`:
 // a second wave of short pieces costs more than the idle SMs of one; 32 sequences with 4 key heads
 // and a 4096-key window take 39 us in clusters of 2 and 47 in clusters of 4), with at least `least`
-// keys to a block.
+// keys to a block. Clusters of 16 are past what every device promises; where this one runs none of
+// that size the launch falls back to 8.
+constexpr int kStepMaxSplits = 16;
 static int step_splits(const AttnParams& P, int64_t units, int most_blocks, int least) {
   const int64_t most = P.window == 0 ? P.keys : (int64_t)P.window + P.sinks < P.keys ? (int64_t)P.window + P.sinks : P.keys;
   int splits = 1;
-  while (splits < kMaxSplits && units * splits * 2 <= most_blocks && most > (int64_t)least * splits) splits *= 2;
+  while (splits < kStepMaxSplits && units * splits * 2 <= most_blocks && most > (int64_t)least * splits) splits *= 2;
   return splits;
 }
 
@@ -446,6 +473,14 @@ static int launch_step(K kernel, const AttnParams& P, int splits, int heads, int
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   config.attrs = &attr;
   config.numAttrs = splits > 1 ? 1 : 0;
+  if (splits > kMaxSplits) {
+    int clusters = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters < 1) {
+      cudaGetLastError();
+      config.gridDim.x = attr.val.clusterDim.x = kMaxSplits;
+    }
+  }
   cudaError_t e = cudaLaunchKernelEx(&config, kernel, P, maps...);
   if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_step launch"); }
   return launch_status("nt_attention_step launch");
@@ -460,7 +495,7 @@ static int launch_ring(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
   if (rc) return rc;
   const int heads = P.kv_heads * ((P.group + 7) / 8);
-  const int splits = step_splits(P, (int64_t)P.batch * heads, 2 * current_sm_count(), kRingWarps * kRingKeys);
+  const int splits = step_splits(P, (int64_t)P.batch * heads, 3 * current_sm_count(), kRingWarps * kRingKeys);
   return launch_step(attention_step_ring_kernel<DT, DP>, P, splits, heads, kRingWarps * 32, StepShared<DP>::kBytes, s, k, v);
 }
 

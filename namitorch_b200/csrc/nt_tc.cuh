@@ -58,38 +58,46 @@ __device__ __forceinline__ float4 load_cluster4(const float* p, uint32_t rank) {
 constexpr int kMaxSplits = 8;   // blocks of a portable cluster
 
 // Four columns of a row whose parts lie in `splits` blocks: unnormalised output at `part`, maximum
-// and sum at `statistic`. Every load is issued before the first is used (one at a time they cost a
-// trip to the other SM each). Adds the parts in rank order; a part of weight 0 may not be there.
+// and sum at `statistic`. Eight blocks' loads are issued before the first is used (one at a time they
+// cost a trip to the other SM each). Adds the parts in rank order; a part of weight 0 may not be
+// there.
 struct JoinedRow {
   float4 o;
   float top, sum;
 };
 __device__ __forceinline__ JoinedRow join_row(const float* part, const float* statistic, int splits, float scale_log2) {
-  float m[kMaxSplits], l[kMaxSplits];
-  float4 v[kMaxSplits];
-#pragma unroll
-  for (int k = 0; k < kMaxSplits; ++k) {
-    m[k] = -INFINITY;
-    l[k] = 0.0f;
-    v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (k < splits) {
-      m[k] = load_cluster(statistic, k);
-      l[k] = load_cluster(statistic + 1, k);
-      v[k] = load_cluster4(part, k);
-    }
-  }
   JoinedRow r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
+  for (int k0 = 0; k0 < splits; k0 += 8) {
+    float m[8], l[8];
+    float4 v[8];
 #pragma unroll
-  for (int k = 0; k < kMaxSplits; ++k) r.top = fmaxf(r.top, m[k]);
+    for (int k = 0; k < 8; ++k) {
+      m[k] = -INFINITY;
+      l[k] = 0.0f;
+      v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (k0 + k < splits) {
+        m[k] = load_cluster(statistic, k0 + k);
+        l[k] = load_cluster(statistic + 1, k0 + k);
+        v[k] = load_cluster4(part, k0 + k);
+      }
+    }
+    float top = r.top;
 #pragma unroll
-  for (int k = 0; k < kMaxSplits; ++k) {
-    const float f = m[k] == -INFINITY ? 0.0f : exp2f((m[k] - r.top) * scale_log2);
-    r.sum = fmaf(l[k], f, r.sum);
-    if (f != 0.0f) {
-      r.o.x = fmaf(v[k].x, f, r.o.x);
-      r.o.y = fmaf(v[k].y, f, r.o.y);
-      r.o.z = fmaf(v[k].z, f, r.o.z);
-      r.o.w = fmaf(v[k].w, f, r.o.w);
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, m[k]);
+    const float old = r.top == -INFINITY ? 0.0f : exp2f((r.top - top) * scale_log2);
+    r.top = top;
+    r.sum *= old;
+    if (old != 0.0f) { r.o.x *= old; r.o.y *= old; r.o.z *= old; r.o.w *= old; }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = m[k] == -INFINITY ? 0.0f : exp2f((m[k] - top) * scale_log2);
+      r.sum = fmaf(l[k], f, r.sum);
+      if (f != 0.0f) {
+        r.o.x = fmaf(v[k].x, f, r.o.x);
+        r.o.y = fmaf(v[k].y, f, r.o.y);
+        r.o.z = fmaf(v[k].z, f, r.o.z);
+        r.o.w = fmaf(v[k].w, f, r.o.w);
+      }
     }
   }
   return r;
