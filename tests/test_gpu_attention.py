@@ -302,3 +302,27 @@ def test_refusals_on_the_device(cuda_device):
         F.sliding_window_attention_step(q, k, k, n)
     with pytest.raises(RuntimeError, match="CUDA"):
         F.sliding_window_attention(q, k.cpu(), k)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,window,sinks", [(64, 2, 0), (128, 2, 1), (64, 3, 0), (128, 16, 0), (128, 17, 0), (64, 100, 0)])
+def test_gradients_of_narrow_windows_keep_their_precision(cuda_device, dt, dim, window, sinks):
+    """Beside the result's own rounding one operand is rounded, of the same size and independent of it:
+    at most sqrt(2) times the error of rounding the exact gradient, and 1.5 with the sample's spread."""
+    q, k, v, g = (_make((1, 4, 1500, dim), dt, s) for s in (1, 2, 3, 4))
+    leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(F.sliding_window_attention(*leaves, window=window, sinks=sinks), leaves, g.cuda())
+    wanted = O.backward(*(_np(t) for t in (q, k, v, g)), window=window, sinks=sinks, lengths=None, offset=0, scale=None)
+    for got, want in zip(grads, wanted):
+        rounded = _np(torch.from_numpy(want).to(TORCH[dt]))
+        assert np.linalg.norm(_np(got) - want) <= 1.5 * np.linalg.norm(rounded - want)
+
+
+@pytest.mark.parametrize("dt", list(TORCH))
+def test_masked_keys_of_a_narrow_window(cuda_device, dt):
+    q, g = _make((2, 4, 180, 64), dt, 1).cuda(), _make((2, 4, 180, 64), dt, 2).cuda()
+    k, v = _make((2, 2, 200, 64), dt, 3).cuda(), _make((2, 2, 200, 64), dt, 4).cuda()
+    for b, n in enumerate((133, 1)):
+        k[b, :, n:], v[b, :, n:] = float("nan"), float("-inf")
+    _, (_, dk, dv) = _check(q, k, v, g, dt, lengths=(133, 1), window=4, sinks=1)
+    assert torch.all(dk[0, :, 133:] == 0) and torch.all(dv[1, :, 1:] == 0)
