@@ -247,6 +247,19 @@ def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale)
     return window, sinks, lengths, scale
 
 
+class _Once(torch.autograd.Function):
+    """Gradients tied to what they were computed from, so that a second derivative is an error
+    rather than a term left out."""
+    @staticmethod
+    def forward(ctx, name, grads, *sources):
+        ctx.name = name
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} can be differentiated only once.")
+
+
 class _SlidingWindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, lengths, options):
@@ -260,6 +273,8 @@ class _SlidingWindowAttention(torch.autograd.Function):
         query, key, value, output, low, lse, lengths = ctx.saved_tensors
         grads = get_backend(query).attention.backward(query, key, value, output, low, lse, grad_output, lengths,
                                                       **ctx.options)
+        if torch.is_grad_enabled():                    # create_graph=True
+            grads = _Once.apply("sliding_window_attention", grads, query, key, value, grad_output)
         return (*grads, None, None)
 
 
@@ -278,7 +293,7 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     ``lengths[b]`` (an integer tensor [batch], clamped to the keys) has no effect; a NaN or an
     infinity that some query sees can reach other queries of its block of 256.
 
-    Differentiable in query, key and value; sums run in float32 in a fixed order."""
+    Differentiable once in query, key and value; sums run in float32 in a fixed order."""
     window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
     options = {"window": window, "sinks": sinks, "query_offset": _count("query_position_offset", query_position_offset),
                "scale": scale}
@@ -314,6 +329,8 @@ class _Dropout(torch.autograd.Function):
         need_input, need_bias, need_residual = ctx.needs_input_grad[:3]
         grad_input, grad_bias = get_backend(grad_output).dropout.backward(
             grad_output, p, seed=seed, offset=offset, needs=(need_input, need_bias))
+        if torch.is_grad_enabled():                    # create_graph=True
+            grad_input, grad_bias = _Once.apply("dropout", (grad_input, grad_bias), grad_output)
         return grad_input, grad_bias, grad_output if need_residual else None, None, None, None
 
 

@@ -326,3 +326,50 @@ def test_masked_keys_of_a_narrow_window(cuda_device, dt):
         k[b, :, n:], v[b, :, n:] = float("nan"), float("-inf")
     _, (_, dk, dv) = _check(q, k, v, g, dt, lengths=(133, 1), window=4, sinks=1)
     assert torch.all(dk[0, :, 133:] == 0) and torch.all(dv[1, :, 1:] == 0)
+
+
+def test_a_graph_replays_what_the_calls_compute(cuda_device):
+    """Forward, backward and the one-token step captured once and replayed on new inputs and lengths."""
+    shape = dict(q=(2, 8, 600, 64), k=(2, 2, 600, 64), v=(2, 2, 600, 64), g=(2, 8, 600, 64), one=(2, 8, 64))
+    inputs = {name: _make(s, "bf16", i).cuda() for i, (name, s) in enumerate(shape.items())}
+    lengths = torch.tensor([600, 411], dtype=torch.int32, device="cuda")
+
+    def run(t, n):
+        leaves = [t[name].detach().requires_grad_() for name in "qkv"]
+        out = F.sliding_window_attention(*leaves, window=90, sinks=4, lengths=n)
+        kept = F.dropout(out, 0.3, seed=7, offset=9)
+        grads = torch.autograd.grad(kept, leaves, t["g"])
+        step = F.sliding_window_attention_step(t["one"], t["k"], t["v"], n, window=90, sinks=4)
+        return [out.detach(), kept.detach(), *grads, step]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(inputs, lengths)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = run(inputs, lengths)
+    for seed, n in ((20, (600, 411)), (30, (3, 0))):
+        for i, (name, s) in enumerate(shape.items()):
+            inputs[name].copy_(_make(s, "bf16", seed + i))
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in results]
+        for a, b in zip(got, run(inputs, lengths)):
+            assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused(cuda_device):
+    q, k, v = (_make((1, 2, 40, 64), "f32", s).cuda().requires_grad_() for s in (1, 2, 3))
+    want = torch.autograd.grad(F.sliding_window_attention(q, k, v).sum(), (q, k, v))
+    grads = torch.autograd.grad(F.sliding_window_attention(q, k, v).sum(), (q, k, v), create_graph=True)
+    for a, b in zip(want, grads):
+        assert torch.equal(a, b)
+    for grad in grads:
+        with pytest.raises(RuntimeError, match="only once"):
+            torch.autograd.grad(grad.sum() + k.sum(), k, retain_graph=True)
+    grad, = torch.autograd.grad(F.dropout(q, 0.5, seed=1).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        torch.autograd.grad(grad.sum(), q)
