@@ -290,10 +290,8 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
       if (i0 + 4 * ty + i < i1) store_row4<DT, DP>(P.dq, P.dqs.at(b, h, i0 + 4 * ty + i), tx, P.dim, out1[i], P.scale);
   } else {
     const int hk = blockIdx.x % heads;
-    const int split = P.split_tiles * P.parts;
-    const int tile = index < split ? index / P.parts : index - split + P.split_tiles;
-    const int part = index < split ? index % P.parts : 0;
-    const int parts = index < split ? P.parts : 1;
+    const AttnPiece piece(P, index);
+    const int tile = piece.tile, part = piece.part, parts = piece.parts;
     const int k0 = tile * kRows, k1 = min(P.keys, k0 + kRows);
     const AttnQueries range(P, length, k0, k1);
     load_tile<DT, DP>(x1, kb + P.ks.at(b, hk, 0) * es, P.ks.t, k0, k1, P.dim, P.vec);
@@ -341,7 +339,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
       }
     } else {
       // [batch, kv head, split block, part, 2, 64, dim]
-      const int64_t at = ((((int64_t)b * P.kv_heads + hk) * P.split_tiles + tile) * parts + part) * 2 * kRows * P.dim;
+      const int64_t at = (((int64_t)b * P.kv_heads + hk) * attn_joined(P, (P.keys + kRows - 1) / kRows) + index) * 2 * kRows * P.dim;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t r = 4 * ty + i;
@@ -352,20 +350,23 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   }
 }
 
-// dk and dv of the split key blocks (of `tile_rows` keys): the parts added in order, four elements a
-// thread. Grid: pieces of 1024 elements of dk or dv of a block, in that order; then blocks, then
-// batch x key head.
+// dk and dv of the key blocks (of `tile_rows` keys) that were cut: the parts added in order, four
+// elements a thread. Grid: runs of 1024 elements of dk or dv of a block, in that order; then blocks,
+// then batch x key head.
 template <int DT>
 __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ AttnParams P, int tile_rows) {
-  const int size = tile_rows * P.dim, pieces = (size + 1023) / 1024;   // (size is a multiple of 64)
-  const int e = (blockIdx.x % pieces * 256 + threadIdx.x) * 4, which = blockIdx.x / pieces % 2;
-  const int block = blockIdx.x / pieces / 2, tile = block % P.split_tiles, pair = block / P.split_tiles;
+  const int size = tile_rows * P.dim, runs = (size + 1023) / 1024;   // (size is a multiple of 64)
+  const int e = (blockIdx.x % runs * 256 + threadIdx.x) * 4, which = blockIdx.x / runs % 2;
+  const int tiles = (P.keys + tile_rows - 1) / tile_rows, cut = P.rest > 1 ? tiles : P.sink_tiles;
+  const int block = blockIdx.x / runs / 2, tile = block % cut, pair = block / cut;
+  const bool sink = tile < P.sink_tiles;
+  const int first = sink ? tile * P.parts : P.sink_tiles * P.parts + (tile - P.sink_tiles) * P.rest;
   const int b = pair / P.kv_heads, hk = pair % P.kv_heads;
   if (e >= size || tile * tile_rows + e / P.dim >= P.keys) return;
-  const float* src = P.partial + ((int64_t)block * P.parts * 2 + which) * size + e;
+  const float* src = P.partial + (((int64_t)pair * attn_joined(P, tiles) + first) * 2 + which) * size + e;
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int k = 0; k < P.parts; ++k) {
+  for (int k = 0; k < (sink ? P.parts : P.rest); ++k) {
     const float4 v = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)k * 2 * size));
     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
   }
@@ -406,7 +407,7 @@ static int launch_backward(const AttnParams& P, cudaStream_t s) {
   }
   const int tiles = (P.keys + kRows - 1) / kRows;
   if (tiles == 0) return NT_OK;
-  dkv<<<(unsigned)(tiles + P.split_tiles * (P.parts - 1)) * P.kv_heads * P.batch, kSimtThreads, bytes, s>>>(P);
+  dkv<<<(unsigned)attn_pieces(P, tiles) * P.kv_heads * P.batch, kSimtThreads, bytes, s>>>(P);
   return launch_status("nt_attention_backward launch");
 }
 
@@ -416,9 +417,10 @@ static int dispatch_forward(const AttnParams& P, cudaStream_t s) {
 }
 template <int DT>
 static int launch_join(const AttnParams& P, int tile_rows, cudaStream_t s) {
-  if (P.parts == 1 || P.split_tiles == 0) return NT_OK;
-  const unsigned pieces = (tile_rows * P.dim + 1023) / 1024;
-  attention_join_kernel<DT><<<pieces * 2 * P.split_tiles * P.batch * P.kv_heads, 256, 0, s>>>(P, tile_rows);
+  const unsigned runs = (tile_rows * P.dim + 1023) / 1024;
+  const unsigned cut = P.rest > 1 ? (P.keys + tile_rows - 1) / tile_rows : P.sink_tiles;
+  if (cut == 0) return NT_OK;
+  attention_join_kernel<DT><<<runs * 2 * cut * P.batch * P.kv_heads, 256, 0, s>>>(P, tile_rows);
   return launch_status("nt_attention_backward (join) launch");
 }
 template <int DT>
@@ -433,45 +435,50 @@ static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
   return a.window >= positions || a.sinks >= a.keys ? 0 : a.window;
 }
 
-// Which key blocks of the backward (the first `tiles`) have their queries cut into `parts` pieces,
-// whose sums are joined by a kernel of their own. Counted in steps of one block of queries:
-// - a sink block sees every later query, an ordinary one those of its own width and one window; a
-//   sink block's piece is no longer than an ordinary block's work, nor shorter than 16 steps;
+// Into how many pieces the backward cuts the queries of its key blocks; the pieces' sums are joined by
+// a kernel of their own. Counted in steps of one block of queries:
 // - where the longest ordinary block is more than an SM's share of all steps (few key heads, many
-//   query heads to each, long rows), every key block is cut, to half of that share (4 query heads on
-//   one key head, 6508 tokens, no window, forward and backward: 407 us uncut, 225 cut).
+//   query heads to each, long rows), every key block is cut, to half of that share (4 query heads of
+//   64 on one key head, 1000 tokens, window 100, 2 sequences, backward: 38 us uncut, 21 cut);
+// - a sink block sees every later query, an ordinary one those of its own width and one window: a
+//   sink block's piece is no longer than an ordinary block or piece, nor shorter than 16 steps where
+//   those are whole (3000 tokens, window 200, 4 sinks, 8 heads on 2: all cut alike 40 us, so 31).
 struct KeySplit {
-  int tiles, parts;
+  int sink_tiles, parts, rest;
 };
 static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_rows) {
   auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
   const int64_t window = effective_window(a, a.query_offset + a.queries), group = a.query_heads / a.kv_heads;
   const int64_t tiles = up(a.keys, tile_rows), steps = up(a.queries, step_rows);
-  if (tiles == 0 || steps == 0) return {0, 1};
+  if (tiles == 0 || steps == 0) return {0, 1, 1};
   int64_t ordinary = window == 0 ? steps : up(tile_rows + window - 1, step_rows) + 1;
   if (ordinary > steps) ordinary = steps;
   // Both passes; without a window about half of the blocks' pairs lie past the diagonal.
   const int64_t share = tiles * ordinary * a.query_heads * a.batch * (window == 0 ? 1 : 2) / current_sm_count();
-  const int64_t longest = ordinary * group, most = steps * group;
-  const bool sinks = window > 0 && a.sinks > 0;
+  const int64_t longest = ordinary * group;
+  int64_t piece = longest > 16 ? longest : 16, rest = 1;
   if (longest >= 16 && longest > share) {
-    const int64_t piece = share / 2 > 8 ? share / 2 : 8;
-    const int64_t parts = up(sinks ? most : longest, piece);
-    return {(int)tiles, (int)(parts < 32 ? parts : 32)};
+    piece = share / 2 > 8 ? share / 2 : 8;
+    rest = up(longest, piece) < 32 ? up(longest, piece) : 32;
   }
-  if (!sinks) return {0, 1};
-  const int64_t parts = up(most, longest > 16 ? longest : 16);
-  return {(int)up(a.sinks, tile_rows), (int)parts};
+  const int64_t parts = window > 0 && a.sinks > 0 ? up(steps * group, piece) : 1;
+  return {parts > 1 ? (int)up(a.sinks, tile_rows) : 0, (int)parts, (int)rest};
 }
 
 static size_t delta_bytes(const nt_attention_args& a) {
   return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
 }
 
+static void set_split(AttnParams& P, const KeySplit& split) {
+  P.sink_tiles = split.sink_tiles;
+  P.parts = split.parts;
+  P.rest = split.rest;
+}
+
 static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows) {
-  const KeySplit split = key_split(a, tile_rows, step_rows);
-  if (split.parts == 1) return 0;
-  return (size_t)a.batch * a.kv_heads * split.tiles * split.parts * 2 * tile_rows * a.head_dim * 4;
+  AttnParams P{};
+  set_split(P, key_split(a, tile_rows, step_rows));
+  return (size_t)a.batch * a.kv_heads * attn_joined(P, (int)((a.keys + tile_rows - 1) / tile_rows)) * 2 * tile_rows * a.head_dim * 4;
 }
 
 static int check_attention(const nt_attention_args& a, const char* who) {
@@ -488,7 +495,7 @@ static int check_attention(const nt_attention_args& a, const char* who) {
     set_error("%s: batch and heads must be below 65536, queries and keys below 2^30", who);
     return NT_EINVAL;
   }
-  if ((a.queries + kTcQueryStep - 1) / kTcQueryStep * (a.query_heads / a.kv_heads) > INT_MAX) {
+  if ((a.queries + kRows - 1) / kRows * (a.query_heads / a.kv_heads) > INT_MAX) {
     set_error("%s: too many queries for one key head", who);
     return NT_EINVAL;
   }
@@ -541,7 +548,7 @@ static AttnParams attention_params(const nt_attention_args& a, int64_t positions
   P.offset = (int)a.query_offset;
   P.scale = a.scale;
   P.scale_log2 = a.scale * kLog2eF;
-  P.parts = 1;
+  P.parts = P.rest = 1;
   return P;
 }
 
@@ -553,7 +560,7 @@ extern "C" {
 
 size_t nt_attention_workspace_size(const nt_attention_args* args) {
   if (!args || check_attention(*args, "nt_attention_workspace_size")) return 0;
-  const size_t a = partial_bytes(*args, kRows, kRows), b = partial_bytes(*args, kTcKeyRows, kTcQueryStep);
+  const size_t a = partial_bytes(*args, kRows, kRows), b = partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim));
   return delta_bytes(*args) + (a > b ? a : b);
 }
 
@@ -611,10 +618,8 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
   const bool tc = a.dtype != NT_F32 && a.keys > 0 && a.queries > 0 && P.vec &&
                   vector_query(a, a.output_low, a.output_strides) && vector_query(a, a.grad_query, a.grad_query_strides) &&
                   vector_key(a, a.grad_key, a.grad_key_strides) && vector_key(a, a.grad_value, a.grad_value_strides);
-  const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? kTcQueryStep : kRows;
-  const KeySplit split = key_split(a, tile_rows, step_rows);
-  P.split_tiles = split.parts > 1 ? split.tiles : 0;
-  P.parts = split.parts;
+  const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? tc_query_step(args->head_dim) : kRows;
+  set_split(P, key_split(a, tile_rows, step_rows));
   cudaStream_t s = as_stream(stream);
   if (tc) {
     rc = attention_tc_backward_launch(P, a.dtype, s);

@@ -31,9 +31,10 @@ struct AttnParams {
   int sinks;         // 0 without a window
   int offset;
   int vec;           // rows are 16-byte aligned runs of whole 16-byte vectors
-  // Backward over key blocks: the queries of the first `split_tiles` blocks are cut into `parts`
-  // pieces.
-  int split_tiles, parts;
+  // Backward over key blocks: the queries of the first `sink_tiles` blocks are cut into `parts`
+  // pieces, those of the others into `rest`. Pieces count on through the blocks of a key head; with
+  // rest = 1 the others have none, they are whole.
+  int sink_tiles, parts, rest;
   int splits;        // forward: blocks of a cluster that share a block of queries
   float scale, scale_log2;
 };
@@ -81,6 +82,24 @@ struct AttnQueries {
   }
 };
 
+// Key block and piece of block `index` of a key head.
+struct AttnPiece {
+  int tile, part, parts;
+  __device__ __forceinline__ AttnPiece(const AttnParams& P, int index) {
+    const int first = P.sink_tiles * P.parts;
+    parts = index < first ? P.parts : P.rest;
+    tile = index < first ? index / P.parts : P.sink_tiles + (index - first) / P.rest;
+    part = (index < first ? index : index - first) % parts;
+  }
+};
+// Pieces of all `tiles` key blocks of a key head, and those among them whose sums are joined.
+__host__ __device__ inline int attn_pieces(const AttnParams& P, int tiles) {
+  return P.sink_tiles * P.parts + (tiles - P.sink_tiles) * P.rest;
+}
+__host__ __device__ inline int attn_joined(const AttnParams& P, int tiles) {
+  return P.rest > 1 ? attn_pieces(P, tiles) : P.parts > 1 ? P.sink_tiles * P.parts : 0;
+}
+
 // nt_attention_map.cu: tensor map (column, token, head, batch) of a 16-bit tensor with boxes of 64
 // columns x `rows` tokens, 128-byte swizzle, zeros outside.
 int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st, int dim, int tokens, int heads, int batch,
@@ -89,7 +108,7 @@ int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st
 int attention_step_launch(const AttnParams& P, int dtype, cudaStream_t s);
 // nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
 constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
-constexpr int kTcQueryStep = 128;  // queries it takes at a time
+constexpr int tc_query_step(int dim) { return dim <= 64 ? 64 : 128; }   // queries it takes at a time
 int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 

@@ -465,7 +465,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 }
 
 // ---- backward ------------------------------------------------------------------------
-// One block keeps 128 rows x1, x2 and walks rows y1, y2 128 at a time:
+// One block keeps 128 rows x1, x2 and walks rows y1, y2 128 (heads of up to 64: 64) at a time:
 //   s = x1 y1^T, dp = x2 y2^T (TMEM, float32);  P = exp(scale s - lse), dS = P (dp - delta)
 //   out1 += dS y1, and with DKV out2 += P y2, with P and dS over s and dp in TMEM as the
 //   products' first operand.
@@ -477,19 +477,23 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 // With DKV s, dp and the two outputs fill TMEM, so nothing has a second buffer; the order of the
 // products hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1)
 // while dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Without it dp has two buffers and
-// dp(t + 1) does not wait for out1(t). Four groups of four warps take 32 columns each.
-constexpr int kStep = kTcQueryStep;
-constexpr int kColumns = kStep / 4;    // of a computing thread
+// dp(t + 1) does not wait for out1(t). Groups of four warps take 32 columns each.
+// Heads of up to 64 leave room for two blocks on an SM, with half of TMEM and steps of 64 rows each: one
+// begins and ends, or waits for its products, while the other computes (8 x 1024 tokens of 12 heads of
+// 64, window 256: 97 us with one block and steps of 128, 70 with two; 2 x 4096 of 16, causal: 317, 267).
+constexpr int kColumns = 32;           // of a computing thread
 
-constexpr int kBwdThreads = 19 * 32;   // the warps of the forward and one for lse and delta
-constexpr int kStatWarp = 18;
-
-// Shared memory: x1, x2, the ring of y1 (three: s of the next step starts before out1 of this one
-// has ended), the ring of y2 (two) and the control block.
+// The copying warp also fetches lse and delta of the rows that are walked. Shared memory: x1, x2, the
+// ring of y1 (three: s of the next step starts before out1 of this one has ended), the ring of y2 (two)
+// and the control block.
 template <int DP> struct BwdShared {
-  static constexpr int kTile = kTcRows * DP * 2;
+  static constexpr int kResident = DP <= 64 ? 2 : 1;   // blocks on an SM
+  static constexpr int kStep = tc_query_step(DP), kGroups = kStep / kColumns;
+  static constexpr int kWarps = 4 * kGroups, kCopyWarp = kWarps, kMmaWarp = kWarps + 1, kThreads = (kWarps + 2) * 32;
+  static constexpr int kTmem = kTmemColumns / kResident;
+  static constexpr int kTile = kTcRows * DP * 2, kPiece = kStep * DP * 2;
   static constexpr int kRing1 = 3, kRing2 = 2;
-  static constexpr int kY1 = 2 * kTile, kY2 = (2 + kRing1) * kTile, kControl = (2 + kRing1 + kRing2) * kTile;
+  static constexpr int kY1 = 2 * kTile, kY2 = kY1 + kRing1 * kPiece, kControl = kY2 + kRing2 * kPiece;
   struct Control {
     float stats[2][2][kStep];          // ring of two; lse (times log2 e) and delta, both negative
     uint64_t x_full, y1_full[kRing1], y1_free[kRing1], y2_full[kRing2], y2_free[kRing2], s_full, p_full,
@@ -499,8 +503,7 @@ template <int DP> struct BwdShared {
   };
   static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
-static_assert(kStep == kTcRows, "rows kept and rows streamed have one shape");
-static_assert(BwdShared<128>::kBytes <= 227 * 1024, "one block per SM");
+static_assert(BwdShared<128>::kBytes <= 227 * 1024 && BwdShared<64>::kBytes <= 113 * 1024, "blocks on an SM");
 
 // delta of every query: as many lanes to a row as it has 16-byte vectors.
 template <int DT, int DP>
@@ -533,7 +536,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
                                                const CUtensorMap& map_x2, const CUtensorMap& map_y1,
                                                const CUtensorMap& map_y2) {
   using Shape = BwdShared<DP>;
-  constexpr int TILE = Shape::kTile, RING1 = Shape::kRing1, RING2 = Shape::kRing2;
+  constexpr int TILE = Shape::kTile, PIECE = Shape::kPiece, RING1 = Shape::kRing1, RING2 = Shape::kRing2;
+  constexpr int kStep = Shape::kStep, kCopyWarp = Shape::kCopyWarp, kMmaWarp = Shape::kMmaWarp;
   // No static shared memory: the dynamic block starts where shared memory does, 1024 bytes in.
   extern __shared__ __align__(1024) uint8_t aligned[];
   typename Shape::Control& ctl = *reinterpret_cast<typename Shape::Control*>(aligned + Shape::kControl);
@@ -546,17 +550,16 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
   const int length = attn_length(P, b);
 
   // The block's rows [r0, r1) and the steps it walks.
-  int r0, r1, part = 0, parts = 1, tile = 0, steps, per_head = 1;
+  int r0, r1, part = 0, parts = 1, steps, per_head = 1;
   uint32_t from = 0;
   if constexpr (!DKV) {
     r0 = ((P.queries + kTcRows - 1) / kTcRows - 1 - index) * kTcRows;
     r1 = min(P.queries, r0 + kTcRows);
   } else {
-    const int split = P.split_tiles * P.parts;
-    tile = index < split ? index / P.parts : index - split + P.split_tiles;
-    part = index < split ? index % P.parts : 0;
-    parts = index < split ? P.parts : 1;
-    r0 = tile * kTcRows;
+    const AttnPiece piece(P, index);
+    part = piece.part;
+    parts = piece.parts;
+    r0 = piece.tile * kTcRows;
     r1 = min(P.keys, r0 + kTcRows);
   }
   const AttnKeys key_range(P, length, r0, r1);
@@ -600,20 +603,22 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
   };
 
   // The copying warp sets up the barriers and issues the first copies while the rest is set up.
-  auto load = [&](const CUtensorMap& map, int at, int token, int head, uint64_t* bar) {
+  auto load = [&](const CUtensorMap& map, int at, int token, int head, int rows, uint64_t* bar) {
 #pragma unroll
     for (int half = 0; half < DP / 64; ++half)
-      tma_load(aligned + at + half * kTcRows * 128, &map, half * 64, token, head, b, bar);
+#pragma unroll
+      for (int row = 0; row < rows; row += kStep)
+        tma_load(aligned + at + (half * rows + row) * 128, &map, half * 64, token + row, head, b, bar);
   };
   auto fill1 = [&](int t, const Step& s) {
-    mbar_arrive_expect_tx(&ctl.y1_full[t % RING1], TILE);
-    load(map_y1, Shape::kY1 + t % RING1 * TILE, s.begin, s.head, &ctl.y1_full[t % RING1]);
+    mbar_arrive_expect_tx(&ctl.y1_full[t % RING1], PIECE);
+    load(map_y1, Shape::kY1 + t % RING1 * PIECE, s.begin, s.head, kStep, &ctl.y1_full[t % RING1]);
   };
   auto fill2 = [&](int t, const Step& s) {
-    mbar_arrive_expect_tx(&ctl.y2_full[t % RING2], TILE);
-    load(map_y2, Shape::kY2 + t % RING2 * TILE, s.begin, s.head, &ctl.y2_full[t % RING2]);
+    mbar_arrive_expect_tx(&ctl.y2_full[t % RING2], PIECE);
+    load(map_y2, Shape::kY2 + t % RING2 * PIECE, s.begin, s.head, kStep, &ctl.y2_full[t % RING2]);
   };
-  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
+  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, Shape::kTmem);
   if (warp == kCopyWarp && lane == 0) {
     mbar_init(&ctl.x_full, 1); mbar_init(&ctl.out_full, 1);
 #pragma unroll
@@ -621,19 +626,19 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
 #pragma unroll
     for (int i = 0; i < RING2; ++i) {
       mbar_init(&ctl.y2_full[i], 1); mbar_init(&ctl.y2_free[i], 1);
-      mbar_init(&ctl.stat_full[i], 1); mbar_init(&ctl.stat_free[i], kComputeWarps);
+      mbar_init(&ctl.stat_full[i], 1); mbar_init(&ctl.stat_free[i], Shape::kWarps);
     }
-    mbar_init(&ctl.s_full, 1); mbar_init(&ctl.p_full, kComputeWarps);
+    mbar_init(&ctl.s_full, 1); mbar_init(&ctl.p_full, Shape::kWarps);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) { mbar_init(&ctl.dp_full[i], 1); mbar_init(&ctl.ds_full[i], kComputeWarps); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctl.dp_full[i], 1); mbar_init(&ctl.ds_full[i], Shape::kWarps); }
     fence_mbar_init();
     if (steps > 0) {
       Step s;
       start(s);
       mbar_arrive_expect_tx(&ctl.x_full, 2 * TILE);
-      load(map_x1, 0, r0, h0, &ctl.x_full);
+      load(map_x1, 0, r0, h0, kTcRows, &ctl.x_full);
       fill1(0, s);
-      load(map_x2, TILE, r0, h0, &ctl.x_full);
+      load(map_x2, TILE, r0, h0, kTcRows, &ctl.x_full);
       fill2(0, s);
     }
   }
@@ -647,52 +652,59 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
   bool ok = true;
 
   if (warp == kCopyWarp) {
-    if (lane == 0 && steps > 0) {
-      Step s;
-      start(s);
-      int n1 = 1, n2 = 1;
-      for (int t = 1; t < steps; ++t) {
-        advance(s);
-        if (t >= RING1) ok = wait_bar(&ctl.y1_free[t % RING1], ring_phase(t - RING1, RING1));
-        if (!ok) break;
-        fill1(t, s);
-        n1 = t + 1;
-        if (t >= RING2) ok = wait_bar(&ctl.y2_free[t % RING2], ring_phase(t - RING2, RING2));
-        if (!ok) break;
-        fill2(t, s);
-        n2 = t + 1;
-      }
-      if (!ok) {   // the copies in flight land before the block may end
-        wait_bar(&ctl.x_full, 0);
-        for (int i = max(0, n1 - RING1); i < n1; ++i) wait_bar(&ctl.y1_full[i % RING1], ring_phase(i, RING1));
-        for (int i = max(0, n2 - RING2); i < n2; ++i) wait_bar(&ctl.y2_full[i % RING2], ring_phase(i, RING2));
-      }
+    Step copied{}, read{};
+    if (steps > 0) {
+      start(copied);
+      read = copied;
     }
-  } else if (warp == kStatWarp) {
+    int n1 = min(steps, 1), n2 = n1;
+    auto copies = [&](int t) {
+      advance(copied);
+      if (t >= RING1) ok = wait_warp(&ctl.y1_free[t % RING1], ring_phase(t - RING1, RING1));
+      if (!ok) return;
+      if (lane == 0) fill1(t, copied);
+      n1 = t + 1;
+      if (t >= RING2) ok = wait_warp(&ctl.y2_free[t % RING2], ring_phase(t - RING2, RING2));
+      if (!ok) return;
+      if (lane == 0) fill2(t, copied);
+      n2 = t + 1;
+    };
+    auto statistics = [&](int t) {
+      const int64_t stat = ((int64_t)b * P.heads + read.head) * P.queries + read.begin;
+      float lse[kStep / 32], delta[kStep / 32];
+#pragma unroll
+      for (int i = 0; i < kStep / 32; ++i) {
+        const int c = i * 32 + lane;
+        const bool in = read.begin + c < read.end;
+        lse[i] = in ? -P.lse[stat + c] * kLog2eF : 0.0f;
+        delta[i] = in ? -P.delta[stat + c] : 0.0f;
+      }
+      advance(read);
+      if (t >= 2) ok = wait_warp(&ctl.stat_free[t & 1], ring_phase(t - 2, 2));
+      if (!ok) return;
+#pragma unroll
+      for (int i = 0; i < kStep / 32; ++i) {
+        ctl.stats[t & 1][0][i * 32 + lane] = lse[i];
+        ctl.stats[t & 1][1][i * 32 + lane] = delta[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.stat_full[t & 1]);
+    };
+    // Both rings hold two steps and more; statistics(t + 1) wait for dS(t - 1), copies(t + 2) for
+    // out1(t - 1) and out2(t): the order in which these end.
+    if (steps > 1) copies(1);
     if constexpr (DKV) {
       grid_dependency_wait();
-      Step s;
-      start(s);
-      for (int t = 0; t < steps; ++t, advance(s)) {
-        const int64_t stat = ((int64_t)b * P.heads + s.head) * P.queries + s.begin;
-        float lse[kStep / 32], delta[kStep / 32];
-#pragma unroll
-        for (int i = 0; i < kStep / 32; ++i) {
-          const int c = i * 32 + lane;
-          const bool in = s.begin + c < s.end;
-          lse[i] = in ? -P.lse[stat + c] * kLog2eF : 0.0f;
-          delta[i] = in ? -P.delta[stat + c] : 0.0f;
-        }
-        if (t >= 2) ok = wait_warp(&ctl.stat_free[t & 1], ring_phase(t - 2, 2));
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < kStep / 32; ++i) {
-          ctl.stats[t & 1][0][i * 32 + lane] = lse[i];
-          ctl.stats[t & 1][1][i * 32 + lane] = delta[i];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl.stat_full[t & 1]);
-      }
+      if (steps > 0) statistics(0);
+    }
+    for (int t = 0; t < steps && ok; ++t) {
+      if (DKV && t + 1 < steps) statistics(t + 1);
+      if (ok && t + 2 < steps) copies(t + 2);
+    }
+    if (!ok && lane == 0) {   // the copies in flight land before the block may end
+      wait_bar(&ctl.x_full, 0);
+      for (int i = max(0, n1 - RING1); i < n1; ++i) wait_bar(&ctl.y1_full[i % RING1], ring_phase(i, RING1));
+      for (int i = max(0, n2 - RING2); i < n2; ++i) wait_bar(&ctl.y2_full[i % RING2], ring_phase(i, RING2));
     }
   } else if (warp == kMmaWarp) {
     const int width16 = (P.dim + 15) / 16;
@@ -710,8 +722,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       }
       __syncwarp();
     };
-    // acc += w y of one step, which ends its use of y; w lies in four quarters, each over its scores, with
-    // its low parts, where there are any, beside it
+    // acc += w y of one step, which ends its use of y; w lies in pieces of 32 columns, each over its
+    // scores, with its low parts, where there are any, beside it
     auto sum = [&](uint32_t acc, uint32_t w, int at, int rows, bool add, bool low, uint64_t* done) {
       if (elect_one()) {
         const uint64_t y = tc_rows(base + at, kStep);
@@ -742,7 +754,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       if (ok) product(t_s, x1, Shape::kY1, rows, &ctl.s_full);
     }
     auto second = [&](int t, int rows) {   // dp(t)
-      const int y2 = Shape::kY2 + t % RING2 * TILE;
+      const int y2 = Shape::kY2 + t % RING2 * PIECE;
       if (!arrive(&ctl.y2_full[t % RING2], ring_phase(t, RING2), y2, rows)) return false;
       product(t_dp_of(t), x2, y2, rows, &ctl.dp_full[t & 1]);
       if constexpr (!DKV) {   // nothing else reads y2
@@ -757,12 +769,12 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       ok = ok && wait_warp(&ctl.p_full, t & 1);
       if (!ok) break;
       tc_fence_after();
-      if constexpr (DKV) sum(t_out2, t_s, Shape::kY2 + t % RING2 * TILE, rows, t > 0, false, &ctl.y2_free[t % RING2]);
+      if constexpr (DKV) sum(t_out2, t_s, Shape::kY2 + t % RING2 * PIECE, rows, t > 0, false, &ctl.y2_free[t % RING2]);
       const int now = rows;
       if (t + 1 < steps) {
         advance(s);
         rows = s.end - s.begin;
-        const int next = Shape::kY1 + (t + 1) % RING1 * TILE;
+        const int next = Shape::kY1 + (t + 1) % RING1 * PIECE;
         ok = arrive(&ctl.y1_full[(t + 1) % RING1], ring_phase(t + 1, RING1), next, rows);
         if (!ok) break;
         product(t_s, x1, next, rows, &ctl.s_full);
@@ -771,15 +783,15 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       ok = ok && wait_warp(&ctl.ds_full[t & 1], ring_phase(t, 2));
       if (!ok) break;
       tc_fence_after();
-      sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * TILE, now, t > 0, FINE, &ctl.y1_free[t % RING1]);
+      sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * PIECE, now, t > 0, FINE, &ctl.y1_free[t % RING1]);
     }
     if (elect_one()) tc_commit(&ctl.out_full);
     __syncwarp();
     if (!ok) wait_bar(&ctl.out_full, 0);
   } else {
-    const int quarter = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int group = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const uint32_t at_s = t_s + lanes + quarter * kColumns;
+    const uint32_t at_s = t_s + lanes + group * kColumns;
     float lse = 0.0f, delta = 0.0f;
     if constexpr (!DKV) {
       grid_dependency_wait();
@@ -822,7 +834,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
 #pragma unroll
       for (int c = 0; c < kColumns; c += 4) {
         float4 ls = make_float4(lse, lse, lse, lse);   // negative
-        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][quarter * kColumns + c]);
+        if constexpr (DKV) ls = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][0][group * kColumns + c]);
         fma2(Pair(p[c], p[c + 1]), scale2, Pair(ls.x, ls.y)).get(p[c], p[c + 1]);
         fma2(Pair(p[c + 2], p[c + 3]), scale2, Pair(ls.z, ls.w)).get(p[c + 2], p[c + 3]);
       }
@@ -838,7 +850,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
           const int64_t last = P.window == 0 || key < P.sinks ? (int64_t)kStep : (int64_t)key + P.window - first;
           mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
         }
-        seen = mask.word(quarter * kColumns);
+        seen = mask.word(group * kColumns);
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) p[c] = seen >> c & 1 ? p[c] : 0.0f;
       }
@@ -855,14 +867,14 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       if (ok) ok = wait_bar(&ctl.dp_full[t & 1], ring_phase(t, 2));
       __syncwarp();
       tc_fence_after();
-      const uint32_t at_dp = t_dp_of(t) + lanes + quarter * kColumns;
+      const uint32_t at_dp = t_dp_of(t) + lanes + group * kColumns;
       uint32_t d[kColumns];
       tmem_load32(at_dp, d);
       tmem_wait_load();
 #pragma unroll
       for (int c = 0; c < kColumns; c += 4) {
         float4 de = make_float4(delta, delta, delta, delta);   // negative
-        if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][quarter * kColumns + c]);
+        if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * kColumns + c]);
         float a, e;
         mul2(Pair(p[c], p[c + 1]), add2(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
         w[c / 2] = pack2<DT>(a, e);
@@ -880,7 +892,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
 #pragma unroll
         for (int c = 0; c < kColumns; c += 2) {
           float2 de = make_float2(delta, delta);
-          if constexpr (DKV) de = *reinterpret_cast<const float2*>(&ctl.stats[t & 1][1][quarter * kColumns + c]);
+          if constexpr (DKV) de = *reinterpret_cast<const float2*>(&ctl.stats[t & 1][1][group * kColumns + c]);
           const float2 hi = unpack2<DT>(w[c / 2]);
           // (a masked element's low part is cleared with its high part)
           const float a = seen >> c & 1 ? p[c] * (__uint_as_float(d[c]) + de.x) - hi.x : 0.0f;
@@ -900,10 +912,10 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     if (ok && steps > 0) ok = wait_bar(&ctl.out_full, 0);
     __syncwarp();
     tc_fence_after();
-    // DKV: the first two quarters store dk, the others dv, half of the columns each; else all four
-    // store dq, a quarter of the columns each.
-    constexpr int WIDTH = DKV ? DP / 2 : DP / 4, CHUNK = WIDTH < 32 ? WIDTH : 32;
-    const int which = DKV ? quarter >> 1 : 0, c_first = (DKV ? quarter & 1 : quarter) * WIDTH;
+    // DKV: the first half of the groups store dk, the others dv; else all store dq: an equal share of the
+    // columns each.
+    constexpr int SHARERS = DKV ? Shape::kGroups / 2 : Shape::kGroups, WIDTH = DP / SHARERS, CHUNK = WIDTH < 32 ? WIDTH : 32;
+    const int which = group / SHARERS, c_first = group % SHARERS * WIDTH;
     const uint32_t t_out = (which ? t_out2 : t_out1) + lanes + c_first;
     const float f = which ? 1.0f : P.scale;
     const int row0 = r0 + (warp & 3) * 32;
@@ -936,7 +948,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     } else {
       // float32 [batch, key head, split block, part, 2, 128, dim]
       char* dst = reinterpret_cast<char*>(
-          P.partial + ((((((int64_t)b * P.kv_heads + h0) * P.split_tiles + tile) * parts + part) * 2 + which) * kTcRows +
+          P.partial + (((((int64_t)b * P.kv_heads + h0) * attn_joined(P, (P.keys + kTcKeyRows - 1) / kTcKeyRows) + index) * 2 + which) * kTcRows +
                        (warp & 3) * 32) * P.dim + c_first);
       constexpr int CH = CHUNK / 4;
 #pragma unroll
@@ -961,18 +973,23 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
   if (!ok && P.error != nullptr) atomicOr(P.error, 1);
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
+  if (warp == kMmaWarp) tmem_free(tmem, Shape::kTmem);
 }
 
-// Blocks 0 .. key_blocks - 1 own keys, the others queries. FINE is a variant of its own because
-// the branch alone made every other call spill registers.
+// `key_blocks` blocks own keys, the others queries. The longer kind comes first: the key blocks, unless
+// all of them are cut (4 heads on one key head, 6508 tokens of 64: 138 us with the cut ones first, 103
+// with the query blocks). FINE is a variant of its own because the branch alone made every other call
+// spill registers.
 template <int DT, int DP, bool FINE>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdShared<DP>::kThreads, BwdShared<DP>::kResident)
 attention_tc_backward(const __grid_constant__ AttnParams P, uint32_t key_blocks, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v) {
-  if (blockIdx.x < key_blocks) backward_block<DT, DP, true, FINE>(P, blockIdx.x, map_k, map_v, map_q, map_g);
-  else backward_block<DT, DP, false, FINE>(P, blockIdx.x - key_blocks, map_q, map_g, map_k, map_v);
+  const bool keys_first = P.rest == 1;
+  const uint32_t split = keys_first ? key_blocks : gridDim.x - key_blocks;
+  const uint32_t index = blockIdx.x < split ? blockIdx.x : blockIdx.x - split;
+  if ((blockIdx.x < split) == keys_first) backward_block<DT, DP, true, FINE>(P, index, map_k, map_v, map_q, map_g);
+  else backward_block<DT, DP, false, FINE>(P, index, map_q, map_g, map_k, map_v);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -1028,10 +1045,10 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   CUtensorMap q, g, k, v;
   const int bytes = BwdShared<DP>::kBytes;
   int rc = large_smem<attention_tc_backward<DT, DP, FINE>>(bytes, who);
-  if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
-  if (!rc) rc = make_map(&g, DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, kTcRows, who);
-  if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
-  if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kTcRows, who);
+  if (!rc) rc = make_map(&q, DT, P.q, P.qs, P.dim, P.queries, P.heads, P.batch, BwdShared<DP>::kStep, who);
+  if (!rc) rc = make_map(&g, DT, P.g, P.gs, P.dim, P.queries, P.heads, P.batch, BwdShared<DP>::kStep, who);
+  if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, BwdShared<DP>::kStep, who);
+  if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, BwdShared<DP>::kStep, who);
   if (rc) return rc;
   constexpr int ROWS = 256 / (DP / 8);
   attention_delta_kernel<DT, DP><<<dim3((P.queries + ROWS - 1) / ROWS, P.heads, P.batch), 256, 0, s>>>(P);
@@ -1039,11 +1056,11 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   if (rc) return rc;
   const uint32_t query_blocks = (uint32_t)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;
   const uint32_t key_blocks =
-      (uint32_t)((P.keys + kTcKeyRows - 1) / kTcKeyRows + P.split_tiles * (P.parts - 1)) * P.kv_heads * P.batch;
+      (uint32_t)attn_pieces(P, (P.keys + kTcKeyRows - 1) / kTcKeyRows) * P.kv_heads * P.batch;
   // Its blocks may start while the kernel before it ends.
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(key_blocks + query_blocks);
-  config.blockDim = dim3(kBwdThreads);
+  config.blockDim = dim3(BwdShared<DP>::kThreads);
   config.dynamicSmemBytes = bytes;
   config.stream = s;
   cudaLaunchAttribute attr{};
