@@ -22,9 +22,6 @@
 namespace nt {
 
 constexpr int kTcRows = 128;
-constexpr int kComputeWarps = 16;      // of forward and backward; four of them share 128 rows
-constexpr int kCopyWarp = 16, kMmaWarp = 17;
-constexpr int kFwdThreads = 18 * 32;
 constexpr uint32_t kTmemColumns = 512;
 constexpr float kRaiseSum = 8192.0f;
 constexpr int64_t kFineKeys = 16;
@@ -68,36 +65,48 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int rows, int lane) {
 }
 
 // ---- forward -------------------------------------------------------------------------
-// A block owns 2 x 128 queries of one head, which share the key and value tiles (a tile fetched
-// for 128 queries alone would ask the L2 for 64 KB per 1024 cycles of products). Warps 0-7 do the
-// softmax of the first 128 rows, 8-15 of the second: two threads share a row, 64 columns each. The
-// products of one half run under the exponentials of the other:
+// o = sum_j exp(scale s_j - m) v_j / sum_j exp(scale s_j - m) in one pass over the keys, 128 at a time.
+// Heads of up to 128: a block owns two groups of 128 queries of one head, which share the key and value
+// tiles (a tile fetched for 128 queries alone would ask the L2 for 64 KB per 1024 cycles of products).
+// Eight warps do the softmax of a group: two threads share a row, 64 columns each. The products of one
+// group run under the exponentials of the other:
 //   s0(0) s1(0) | o0 += w0(0) v, s0(1) | o1 += w1(0) v, s1(1) | o0 += w0(1) v, ...
-// TMEM: s0, s1 (the weights over them), o0, o1.
+// TMEM: s0, s1 (the weights over them), o0, o1. (16 heads of 128, 4096 causal tokens: 70 us, 0.99
+// PFLOP/s of the visible pairs; with a window of 512 of 2 x 2048 tokens 43 us, where a block's start and
+// end, some 5 us of 20, are bare.)
+// Heads of up to 64: half of the bytes and of TMEM, so one group to a block and two blocks on an SM,
+// and the start and end of one lie under the other's work (8 x 1024 tokens of 12 heads, window 256: 40
+// us with two groups to a block, 34 so; 8192 tokens of 16 heads, window 128: 46, 34; 2 x 4096 causal of
+// 16: 119, 113).
 // SPLIT: where there are too few blocks of queries for the device, a cluster of blocks shares the
 // tiles of one; each leaves its unnormalised output, maxima and sums in its shared memory, and they
 // are joined from there, rows dealt to the blocks, always in the same order.
 template <int DP> struct FwdShared {
+  static constexpr int kGroups = DP <= 64 ? 1 : 2, kResident = 2 / kGroups;   // of 128 queries; blocks on an SM
+  static constexpr int kRows = kGroups * kTcRows;
+  static constexpr int kWarps = 8 * kGroups, kCopyWarp = kWarps, kMmaWarp = kWarps + 1, kThreads = (kWarps + 2) * 32;
+  static constexpr int kTmem = kTmemColumns / kResident;
   static constexpr int kTile = kTcRows * DP * 2;
   static constexpr int kRing = 2;
-  static constexpr int kK = 2 * kTile, kV = (2 + kRing) * kTile, kControl = (2 + 2 * kRing) * kTile;
+  static constexpr int kK = kGroups * kTile, kV = kK + kRing * kTile, kControl = kV + kRing * kTile;
   struct Control {
-    float exchange[2][2][2][kTcRows];   // half of the queries, use (maximum, sum), half of the columns, row
-    float statistics[2 * kTcRows][2];   // SPLIT: maximum and sum
-    uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[2], w_full[2], o_full[2];
+    float exchange[kGroups][2][2][kTcRows];   // group, use (maximum, sum), half of the columns, row
+    float statistics[kRows][2];   // SPLIT: maximum and sum
+    uint64_t q_full, k_full[kRing], k_free[kRing], v_full[kRing], v_free[kRing], s_full[kGroups], w_full[kGroups], o_full[kGroups];
     uint32_t tmem;
   };
   static constexpr int kPartRow = DP + 4;   // floats; SPLIT: a row of the unnormalised output
-  static_assert(2 * kTcRows * kPartRow * 4 <= kControl, "the output takes the tiles' place");
+  static_assert(kRows * kPartRow * 4 <= kControl, "the output takes the tiles' place");
   static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
 
 template <int DT, int DP, bool SPLIT>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(FwdShared<DP>::kThreads, FwdShared<DP>::kResident)
 attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Shape = FwdShared<DP>;
-  constexpr int TILE = Shape::kTile, RING = Shape::kRing;
+  constexpr int TILE = Shape::kTile, RING = Shape::kRing, GROUPS = Shape::kGroups, ROWS = Shape::kRows;
+  constexpr int kCopyWarp = Shape::kCopyWarp, kMmaWarp = Shape::kMmaWarp;
   // No static shared memory: the dynamic block starts where shared memory does, 1024 bytes in.
   extern __shared__ __align__(1024) uint8_t aligned[];
   typename Shape::Control& ctl = *reinterpret_cast<typename Shape::Control*>(aligned + Shape::kControl);
@@ -108,15 +117,16 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   const uint32_t block = blockIdx.x / splits;
   const uint32_t pairs = (uint32_t)P.heads * P.batch, tiles = gridDim.x / splits / pairs;
   const int b = block % pairs / P.heads, h = block % P.heads, hk = h / P.group;
-  const int i0 = (tiles - 1 - block / pairs) * 2 * kTcRows, i1 = min(P.queries, i0 + 2 * kTcRows);
+  const int i0 = (tiles - 1 - block / pairs) * ROWS, i1 = min(P.queries, i0 + ROWS);
   const int length = attn_length(P, b);
   const AttnKeys range(P, length, i0, i1);
   // The block's tiles: all, or its share.
   const int all = range.blocks(kTcRows), first = all * rank / splits, blocks = all * (rank + 1) / splits - first;
   auto tile_of = [&](int j, int& begin, int& end) { range.block(first + j, kTcRows, begin, end); };
-  // Whether a query of half g sees a key of [begin, end) (half 1 may be past the last query).
+  // Whether a query of group g sees a key of [begin, end) (group 1 may be past the last query).
   const AttnKeys range0(P, length, i0, min(i1, i0 + kTcRows)), range1(P, length, min(i1, i0 + kTcRows), i1);
   auto active = [&](int g, int begin, int end) {
+    if (GROUPS == 1) return true;
     const AttnKeys& r = g ? range1 : range0;
     return (g == 0 || i1 > i0 + kTcRows) && ((begin < r.hi && end > r.lo) || begin < r.sink_end);
   };
@@ -133,21 +143,24 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     mbar_arrive_expect_tx(&full[j % RING], TILE);
     load(map, at + j % RING * TILE, begin, hk, &full[j % RING]);
   };
-  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, kTmemColumns);
+  if (warp == kMmaWarp) tmem_alloc(&ctl.tmem, Shape::kTmem);
   if (warp == kCopyWarp && lane == 0) {
     mbar_init(&ctl.q_full, 1);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RING; ++i) {
       mbar_init(&ctl.k_full[i], 1); mbar_init(&ctl.k_free[i], 1); mbar_init(&ctl.v_full[i], 1); mbar_init(&ctl.v_free[i], 1);
-      mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], kComputeWarps / 2); mbar_init(&ctl.o_full[i], 1);
+    }
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      mbar_init(&ctl.s_full[i], 1); mbar_init(&ctl.w_full[i], 8); mbar_init(&ctl.o_full[i], 1);
     }
     fence_mbar_init();
     if (blocks > 0) {
-      // The second half's rows may all lie past the last query: the copy then writes zeros.
-      mbar_arrive_expect_tx(&ctl.q_full, 2 * TILE);
+      // The second group's rows may all lie past the last query: the copy then writes zeros.
+      mbar_arrive_expect_tx(&ctl.q_full, GROUPS * TILE);
       load(map_q, 0, i0, h, &ctl.q_full);
       fill(map_k, Shape::kK, ctl.k_full, 0);
-      load(map_q, TILE, i0 + kTcRows, h, &ctl.q_full);
+      if constexpr (GROUPS == 2) load(map_q, TILE, i0 + kTcRows, h, &ctl.q_full);
       fill(map_v, Shape::kV, ctl.v_full, 0);
     }
   }
@@ -195,15 +208,15 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       if (elect_one()) tc_commit(bar);
       __syncwarp();
     };
-    int done[2] = {0, 0};   // tiles of each half
-    bool finished[2] = {false, false};
+    int done[GROUPS] = {};   // tiles of each group
+    bool finished = false;   // group 0, before the last tile
     int begin = 0, end = 0;
     if (blocks > 0) {
       tile_of(0, begin, end);
       ok = wait_warp(&ctl.q_full, 0) && wait_warp(&ctl.k_full[0], 0);
       if (ok) {
         if (active(0, begin, end)) scores(0, Shape::kK, end - begin);
-        if (active(1, begin, end)) scores(1, Shape::kK, end - begin);
+        if (GROUPS == 2 && active(1, begin, end)) scores(1, Shape::kK, end - begin);
         commit(&ctl.k_free[0]);
       }
     }
@@ -218,7 +231,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       if (!ok) break;
       clear_tail<DP>(aligned + Shape::kV + slot * TILE, end - begin, lane);
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int g = 0; g < GROUPS; ++g) {
         if (active(g, begin, end)) {
           ok = ok && wait_warp(&ctl.w_full[g], done[g] & 1);
           if (!ok) break;
@@ -228,7 +241,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 #pragma unroll
             for (int s = 0; s < kTcRows / 16; ++s)   // the weights lie in two halves of 64 columns
               if (s * 16 < end - begin)
-                tc_mma_tmem(tmem + 2 * kTcRows + g * DP, tmem + g * kTcRows + (s >> 2) * 64 + (s & 3) * 8,
+                tc_mma_tmem(tmem + ROWS + g * DP, tmem + g * kTcRows + (s >> 2) * 64 + (s & 3) * 8,
                             v + tc_row_step(s), pv, done[g] > 0 || s > 0);
           }
           __syncwarp();
@@ -236,10 +249,10 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
         }
         if (j + 1 < blocks && active(g, next_begin, next_end)) {
           scores(g, Shape::kK + next * TILE, next_end - next_begin);
-        } else if (g == 0 && j + 2 == blocks) {
-          // The first half sees nothing of the last tile (of causal attention): its output is ready.
+        } else if (GROUPS == 2 && g == 0 && j + 2 == blocks) {
+          // The first group sees nothing of the last tile (of causal attention): its output is ready.
           commit(&ctl.o_full[0]);
-          finished[0] = true;
+          finished = true;
         }
       }
       if (!ok) break;
@@ -248,14 +261,14 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       begin = next_begin;
       end = next_end;
     }
-    if (!finished[0]) commit(&ctl.o_full[0]);
-    if (!finished[1]) commit(&ctl.o_full[1]);
-    if (!ok) wait_bar(&ctl.o_full[1], 0);   // no product is in flight when TMEM is given back
+    if (!finished) commit(&ctl.o_full[0]);
+    if constexpr (GROUPS == 2) commit(&ctl.o_full[1]);
+    if (!ok) wait_bar(&ctl.o_full[GROUPS - 1], 0);   // no product is in flight when TMEM is given back
   } else {
-    const int g = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+    const int g = GROUPS == 2 ? warp >> 3 : 0, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // lane 32 (w % 4) in the address's upper half
     const uint32_t t_s = tmem + g * kTcRows + lanes + half * 64;
-    const uint32_t t_o = tmem + 2 * kTcRows + g * DP + lanes + half * (DP / 2);
+    const uint32_t t_o = tmem + ROWS + g * DP + lanes + half * (DP / 2);
     const int q0 = i0 + g * kTcRows, q1 = min(i1, q0 + kTcRows);
     const int p = P.offset + q0 + row;
     const int full_lo = P.window == 0 ? 0 : P.offset + q1 - P.window;   // first key the last query sees
@@ -370,7 +383,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
     // Halves in a fixed order, so that both threads of a row have the same sum.
     l = ctl.exchange[g][1][0][row] + ctl.exchange[g][1][1][row];
     if constexpr (SPLIT) {
-      if (ok && blocks > 0) ok = wait_bar(&ctl.o_full[g ^ 1], 0);   // every tile is free
+      if (GROUPS == 2 && ok && blocks > 0) ok = wait_bar(&ctl.o_full[GROUPS - 1 - g], 0);   // every tile is free
       __syncwarp();
       const int r = g * kTcRows + row;
       if (done > 0) {
@@ -391,7 +404,7 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       }
     } else {
       const float f = l == 0.0f ? 0.0f : 1.0f / l;
-      // The half's tile of queries is free now: 32 rows x half of the columns of each warp.
+      // The group's tile of queries is free now: 32 rows x half of the columns of each warp.
       constexpr int WIDTH = DP / 2, CH = WIDTH / 8;
       uint8_t* stage = aligned + warp * 32 * WIDTH * 2;
       const int row0 = q0 + (warp & 3) * 32, rows = q1 - row0, vectors = (P.dim - half * WIDTH + 7) / 8;
@@ -435,12 +448,12 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
   if (!ok && P.error != nullptr) atomicOr(P.error, 1);
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tmem_free(tmem, kTmemColumns);
+  if (warp == kMmaWarp) tmem_free(tmem, Shape::kTmem);
   if constexpr (SPLIT) {
     cluster_sync_all();
     constexpr int LPR = DP / 4, RPW = 32 / LPR;   // four columns a lane
     const float* part = reinterpret_cast<const float*>(aligned);
-    for (int r0 = (rank + splits * warp) * RPW; warp < kComputeWarps && r0 < i1 - i0; r0 += splits * kComputeWarps * RPW) {
+    for (int r0 = (rank + splits * warp) * RPW; warp < Shape::kWarps && r0 < i1 - i0; r0 += splits * Shape::kWarps * RPW) {
       const int r = r0 + lane / LPR, c = lane % LPR * 4;
       if (r >= i1 - i0) continue;
       const JoinedRow row = join_row(part + r * Shape::kPartRow + c, ctl.statistics[r], splits, P.scale_log2);
@@ -1005,7 +1018,7 @@ static int launch_tc_forward(const AttnParams& P, unsigned blocks, cudaStream_t 
   if (rc) return rc;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(blocks * (SPLIT ? P.splits : 1));
-  config.blockDim = dim3(kFwdThreads);
+  config.blockDim = dim3(FwdShared<DP>::kThreads);
   config.dynamicSmemBytes = FwdShared<DP>::kBytes;
   config.stream = s;
   cudaLaunchAttribute attr{};
@@ -1020,20 +1033,22 @@ static int launch_tc_forward(const AttnParams& P, unsigned blocks, cudaStream_t 
 }
 
 // Blocks of a cluster that share the tiles of one block of queries: more of them while the longest
-// block is more than 1.5 times an SM's share of all tiles, with two tiles at least to each (512
+// block is more than 1.5 times an SM's share of all tiles (1.25 times where a second block on the SM slows
+// it: 6508 tokens, 4 heads of 64 on one, 68 us at 1.5, 58 at 1.25), with two tiles at least to each (512
 // queries of 16 heads after 7680 keys, window 2048: 39 us in 32 blocks, 23 in clusters of 4). Clusters
 // of 8 only where they all run at once: a second wave of them waits for 8 free SMs side by side (58 us).
 template <int DT, int DP>
 static int dispatch_tc_forward(AttnParams P, cudaStream_t s) {
-  const unsigned blocks = (unsigned)((P.queries + 2 * kTcRows - 1) / (2 * kTcRows)) * P.heads * P.batch;
+  constexpr int rows = FwdShared<DP>::kRows;
+  const unsigned blocks = (unsigned)((P.queries + rows - 1) / rows) * P.heads * P.batch;
   const int64_t end = (int64_t)P.offset + P.queries;
   int64_t longest = end < P.keys ? end : P.keys, mean = longest;
-  if (P.window > 0 && (int64_t)P.window + 2 * kTcRows + P.sinks < longest) longest = mean = (int64_t)P.window + 2 * kTcRows + P.sinks;
+  if (P.window > 0 && (int64_t)P.window + rows + P.sinks < longest) longest = mean = (int64_t)P.window + rows + P.sinks;
   else if (P.offset + P.queries / 2 < mean) mean = P.offset + P.queries / 2;
-  const int sms = current_sm_count();
+  const int sms = current_sm_count(), quarters = FwdShared<DP>::kResident == 2 ? 5 : 6;
   P.splits = 1;
   while (P.splits < kMaxSplits && longest >= (int64_t)4 * P.splits * kTcRows &&
-         longest * sms * 2 > 3 * (int64_t)blocks * mean * P.splits &&
+         longest * sms * 4 > quarters * (int64_t)blocks * mean * P.splits &&
          (P.splits < 4 || (int64_t)blocks * P.splits * 2 <= sms))
     P.splits *= 2;
   return P.splits > 1 ? launch_tc_forward<DT, DP, true>(P, blocks, s) : launch_tc_forward<DT, DP, false>(P, blocks, s);
