@@ -14,6 +14,7 @@
 #include <climits>
 
 #include "nt_attention.cuh"
+#include "nt_tc.cuh"
 
 namespace nt {
 
@@ -213,12 +214,31 @@ __global__ void __launch_bounds__(kSimtThreads) attention_forward_kernel(const _
   }
 }
 
-// One pass of the backward. DKV = false: a block owns 64 queries and walks the keys (x1 = q,
-// x2 = g; y1 = k, y2 = v), giving dq and writing delta. DKV = true: a block owns 64 keys and
-// walks the queries of its group's heads (x1 = k, x2 = v; y1 = q, y2 = g), giving dk and dv.
-// In both, s = x1 y1^T and dp = x2 y2^T, out1 = dS y1, and with DKV out2 = P y2.
+// delta = sum over the width of g o of every query, 16 lanes to a row.
+template <int DT>
+__global__ void __launch_bounds__(256) attention_rows_delta_kernel(const __grid_constant__ AttnParams P) {
+  grid_dependents_go();
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  float d = 0.0f;
+  if (row < P.queries) {
+    const int64_t g = P.gs.at(b, h, row), o = P.os.at(b, h, row);
+    for (int c = threadIdx.x % 16; c < P.dim; c += 16) {
+      float x = load1<DT>(P.o, o + c);
+      if (DT != NT_F32 && P.o_low != nullptr) x += load1<DT>(P.o_low, o + c);
+      d = fmaf(load1<DT>(P.g, g + c), x, d);
+    }
+  }
+  d = lanes16_sum(d);
+  if (threadIdx.x % 16 == 0 && row < P.queries) P.delta[((int64_t)b * P.heads + h) * P.queries + row] = d;
+}
+
+// A block of the backward. DKV = false: it owns 64 queries and walks the keys (x1 = q, x2 = g; y1 = k,
+// y2 = v), giving dq. DKV = true: it owns 64 keys and walks the queries of its group's heads (x1 = k,
+// x2 = v; y1 = q, y2 = g), giving dk and dv. In both, s = x1 y1^T and dp = x2 y2^T, out1 = dS y1, and
+// with DKV out2 = P y2.
 template <int DT, int DP, bool DKV>
-__global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const __grid_constant__ AttnParams P) {
+__device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t block) {
   extern __shared__ __align__(16) float smem[];
   constexpr int TILE = kRows * (DP + 4);
   float *x1 = smem, *x2 = x1 + TILE, *y1 = x2 + TILE, *y2 = y1 + TILE;
@@ -228,7 +248,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   const int es = sizeof(typename Elem<DT>::T);
   // Blocks in the order of their work: the last queries, or the first keys, of every head first.
   const uint32_t heads = DKV ? P.kv_heads : P.heads, pairs = heads * P.batch;
-  const int b = blockIdx.x % pairs / heads, index = blockIdx.x / pairs;
+  const int b = block % pairs / heads, index = block / pairs;
   const int length = attn_length(P, b);
   const char *qb = static_cast<const char*>(P.q), *kb = static_cast<const char*>(P.k), *vb = static_cast<const char*>(P.v),
              *gb = static_cast<const char*>(P.g);
@@ -239,28 +259,19 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     for (int u = 0; u < DP / 64; ++u) out1[i][u] = out2[i][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 
   if constexpr (!DKV) {
-    const int h = blockIdx.x % heads, hk = h / P.group;
+    const int h = block % heads, hk = h / P.group;
     const int i0 = ((P.queries + kRows - 1) / kRows - 1 - index) * kRows, i1 = min(P.queries, i0 + kRows);
     const AttnKeys range(P, length, i0, i1);
     load_tile<DT, DP>(x1, qb + P.qs.at(b, h, 0) * es, P.qs.t, i0, i1, P.dim, P.vec);
     load_tile<DT, DP>(x2, gb + P.gs.at(b, h, 0) * es, P.gs.t, i0, i1, P.dim, P.vec);
-    load_tile<DT, DP>(y1, static_cast<const char*>(P.o) + P.os.at(b, h, 0) * es, P.os.t, i0, i1, P.dim, P.vec);
-    const bool low = DT != NT_F32 && P.o_low != nullptr;
-    if (low) load_tile<DT, DP>(y2, static_cast<const char*>(P.o_low) + P.os.at(b, h, 0) * es, P.os.t, i0, i1, P.dim, P.vec);
-    __syncthreads();
+    grid_dependency_wait();
     const int64_t stat = ((int64_t)b * P.heads + h) * P.queries;
     float lse[4], delta[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 4 * ty + i;
-      float d = 0.0f;
-      for (int c = tx; c < P.dim; c += 16) {
-        const int at = r * (DP + 4) + c;
-        d = fmaf(x2[at], low ? y1[at] + y2[at] : y1[at], d);
-      }
-      delta[i] = lanes16_sum(d);
-      lse[i] = i0 + r < i1 ? P.lse[stat + i0 + r] * kLog2eF : 0.0f;
-      if (tx == 0 && i0 + r < i1) P.delta[stat + i0 + r] = delta[i];
+      const int r = i0 + 4 * ty + i;
+      lse[i] = r < i1 ? P.lse[stat + r] * kLog2eF : 0.0f;
+      delta[i] = r < i1 ? P.delta[stat + r] : 0.0f;
     }
     const int blocks = range.blocks(kRows);
     for (int t = 0; t < blocks; ++t) {
@@ -289,13 +300,14 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
     for (int i = 0; i < 4; ++i)
       if (i0 + 4 * ty + i < i1) store_row4<DT, DP>(P.dq, P.dqs.at(b, h, i0 + 4 * ty + i), tx, P.dim, out1[i], P.scale);
   } else {
-    const int hk = blockIdx.x % heads;
+    const int hk = block % heads;
     const AttnPiece piece(P, index);
     const int tile = piece.tile, part = piece.part, parts = piece.parts;
     const int k0 = tile * kRows, k1 = min(P.keys, k0 + kRows);
     const AttnQueries range(P, length, k0, k1);
     load_tile<DT, DP>(x1, kb + P.ks.at(b, hk, 0) * es, P.ks.t, k0, k1, P.dim, P.vec);
     load_tile<DT, DP>(x2, vb + P.vs.at(b, hk, 0) * es, P.vs.t, k0, k1, P.dim, P.vec);
+    grid_dependency_wait();
     const int steps = (range.hi - range.lo + kRows - 1) / kRows;
     const int64_t total = (int64_t)steps * P.group;
     const int64_t from = total * part / parts, to = total * (part + 1) / parts;
@@ -350,6 +362,20 @@ __global__ void __launch_bounds__(kSimtThreads) attention_backward_kernel(const 
   }
 }
 
+// Both kinds of blocks in one launch, so that one fills the SMs that the other leaves idle: `key_blocks`
+// own keys, the others queries; the longer kind comes first, the key blocks unless all of them are cut.
+// Bound by the FP32 pipe where there are blocks enough (4 x 1024 causal tokens of 4 heads of 128: 481 us,
+// 33 TFLOP/s of the tiles' products), else by the copies and products of one block after another.
+template <int DT, int DP>
+__global__ void __launch_bounds__(kSimtThreads, DP <= 64 ? 2 : 1)
+attention_backward_kernel(const __grid_constant__ AttnParams P, uint32_t key_blocks) {
+  const bool keys_first = P.rest == 1;
+  const uint32_t split = keys_first ? key_blocks : gridDim.x - key_blocks;
+  const uint32_t index = blockIdx.x < split ? blockIdx.x : blockIdx.x - split;
+  if ((blockIdx.x < split) == keys_first) backward_block<DT, DP, true>(P, index);
+  else backward_block<DT, DP, false>(P, index);
+}
+
 // dk and dv of the key blocks (of `tile_rows` keys) that were cut: the parts added in order, four
 // elements a thread. Grid: runs of 1024 elements of dk or dv of a block, in that order; then blocks,
 // then batch x key head.
@@ -394,21 +420,32 @@ static int launch_forward(const AttnParams& P, cudaStream_t s) {
 
 template <int DT, int DP>
 static int launch_backward(const AttnParams& P, cudaStream_t s) {
+  const char* who = "nt_attention_backward launch";
   const size_t bytes = (size_t)(4 * kRows * (DP + 4) + 2 * kRows * kWeightStride) * 4;
-  auto dq = attention_backward_kernel<DT, DP, false>;
-  auto dkv = attention_backward_kernel<DT, DP, true>;
-  int rc = large_smem<attention_backward_kernel<DT, DP, false>>(bytes, "nt_attention_backward");
-  if (!rc) rc = large_smem<attention_backward_kernel<DT, DP, true>>(bytes, "nt_attention_backward");
+  int rc = large_smem<attention_backward_kernel<DT, DP>>(bytes, "nt_attention_backward");
   if (rc) return rc;
   if (P.queries > 0) {
-    dq<<<(unsigned)((P.queries + kRows - 1) / kRows) * P.heads * P.batch, kSimtThreads, bytes, s>>>(P);
-    rc = launch_status("nt_attention_backward launch");
+    attention_rows_delta_kernel<DT><<<dim3((P.queries + 15) / 16, P.heads, P.batch), 256, 0, s>>>(P);
+    rc = launch_status(who);
     if (rc) return rc;
   }
-  const int tiles = (P.keys + kRows - 1) / kRows;
-  if (tiles == 0) return NT_OK;
-  dkv<<<(unsigned)attn_pieces(P, tiles) * P.kv_heads * P.batch, kSimtThreads, bytes, s>>>(P);
-  return launch_status("nt_attention_backward launch");
+  const uint32_t key_blocks = (uint32_t)attn_pieces(P, (P.keys + kRows - 1) / kRows) * P.kv_heads * P.batch;
+  const uint32_t query_blocks = (uint32_t)((P.queries + kRows - 1) / kRows) * P.heads * P.batch;
+  if (key_blocks + query_blocks == 0) return NT_OK;
+  // Its blocks may start while the kernel before it ends.
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(key_blocks + query_blocks);
+  config.blockDim = dim3(kSimtThreads);
+  config.dynamicSmemBytes = bytes;
+  config.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = P.queries > 0 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&config, attention_backward_kernel<DT, DP>, P, key_blocks);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, who); }
+  return launch_status(who);
 }
 
 template <int DT>
@@ -441,12 +478,16 @@ static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
 //   query heads to each, long rows), every key block is cut, to half of that share (4 query heads of
 //   64 on one key head, 1000 tokens, window 100, 2 sequences, backward: 38 us uncut, 21 cut);
 // - a sink block sees every later query, an ordinary one those of its own width and one window: a
-//   sink block's piece is no longer than an ordinary block or piece, nor shorter than 16 steps where
-//   those are whole (3000 tokens, window 200, 4 sinks, 8 heads on 2: all cut alike 40 us, so 31).
+//   sink block's piece is no longer than an ordinary block or piece (3000 tokens, window 200, 4 sinks, 8
+//   heads on 2: all cut alike 40 us, so 31).
+// A join costs some 4 us and a step 1 on the tensor cores but 10 on the FP32 pipe, so whole blocks are
+// those of up to 16 steps there and 2 here (float32, 2 x 1024 tokens of 8 heads, window 256, backward: 294
+// us with 16, 174 with 2; 300 tokens of 2 heads: 148, 62; both with the passes in one launch).
+constexpr int kTcLeastPiece = 16, kLeastPiece = 2;
 struct KeySplit {
   int sink_tiles, parts, rest;
 };
-static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_rows) {
+static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_rows, int least) {
   auto up = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
   const int64_t window = effective_window(a, a.query_offset + a.queries), group = a.query_heads / a.kv_heads;
   const int64_t tiles = up(a.keys, tile_rows), steps = up(a.queries, step_rows);
@@ -456,9 +497,9 @@ static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_ro
   // Both passes; without a window about half of the blocks' pairs lie past the diagonal.
   const int64_t share = tiles * ordinary * a.query_heads * a.batch * (window == 0 ? 1 : 2) / current_sm_count();
   const int64_t longest = ordinary * group;
-  int64_t piece = longest > 16 ? longest : 16, rest = 1;
-  if (longest >= 16 && longest > share) {
-    piece = share / 2 > 8 ? share / 2 : 8;
+  int64_t piece = longest > least ? longest : least, rest = 1;
+  if (longest >= least && longest > share) {
+    piece = share > least ? share / 2 : least / 2;
     rest = up(longest, piece) < 32 ? up(longest, piece) : 32;
   }
   const int64_t parts = window > 0 && a.sinks > 0 ? up(steps * group, piece) : 1;
@@ -475,9 +516,9 @@ static void set_split(AttnParams& P, const KeySplit& split) {
   P.rest = split.rest;
 }
 
-static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows) {
+static size_t partial_bytes(const nt_attention_args& a, int tile_rows, int step_rows, int least) {
   AttnParams P{};
-  set_split(P, key_split(a, tile_rows, step_rows));
+  set_split(P, key_split(a, tile_rows, step_rows, least));
   return (size_t)a.batch * a.kv_heads * attn_joined(P, (int)((a.keys + tile_rows - 1) / tile_rows)) * 2 * tile_rows * a.head_dim * 4;
 }
 
@@ -560,7 +601,8 @@ extern "C" {
 
 size_t nt_attention_workspace_size(const nt_attention_args* args) {
   if (!args || check_attention(*args, "nt_attention_workspace_size")) return 0;
-  const size_t a = partial_bytes(*args, kRows, kRows), b = partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim));
+  const size_t a = partial_bytes(*args, kRows, kRows, kLeastPiece);
+  const size_t b = partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim), kTcLeastPiece);
   return delta_bytes(*args) + (a > b ? a : b);
 }
 
@@ -618,8 +660,8 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
   const bool tc = a.dtype != NT_F32 && a.keys > 0 && a.queries > 0 && P.vec &&
                   vector_query(a, a.output_low, a.output_strides) && vector_query(a, a.grad_query, a.grad_query_strides) &&
                   vector_key(a, a.grad_key, a.grad_key_strides) && vector_key(a, a.grad_value, a.grad_value_strides);
-  const int tile_rows = tc ? kTcKeyRows : kRows, step_rows = tc ? tc_query_step(args->head_dim) : kRows;
-  set_split(P, key_split(a, tile_rows, step_rows));
+  const int tile_rows = tc ? kTcKeyRows : kRows;
+  set_split(P, tc ? key_split(a, kTcKeyRows, tc_query_step(a.head_dim), kTcLeastPiece) : key_split(a, kRows, kRows, kLeastPiece));
   cudaStream_t s = as_stream(stream);
   if (tc) {
     rc = attention_tc_backward_launch(P, a.dtype, s);

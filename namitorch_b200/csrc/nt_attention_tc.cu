@@ -1,8 +1,8 @@
 // Sliding-window attention on the fifth-generation tensor cores, for float16 and bfloat16 rows
 // that are whole 16-byte vectors. The mathematics and the masks are those of nt_attention.cu.
 //
-// One block per SM: one warp copies tiles, one issues the products, sixteen compute. Scores
-// accumulate in TMEM; the weights go back to TMEM over them as 16-bit values and are the first
+// One warp of a block copies tiles, one issues the products, the others (16; 8 where two blocks share
+// an SM) compute. Scores accumulate in TMEM; the weights go back to TMEM over them as 16-bit values and are the first
 // operand of the second product. The backward is two passes of one kernel, each with S and dP
 // computed again; sums that cross blocks exist only for split key blocks and are added in order
 // afterwards.
@@ -71,7 +71,7 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int rows, int lane) {
 // Eight warps do the softmax of a group: two threads share a row, 64 columns each. The products of one
 // group run under the exponentials of the other:
 //   s0(0) s1(0) | o0 += w0(0) v, s0(1) | o1 += w1(0) v, s1(1) | o0 += w0(1) v, ...
-// TMEM: s0, s1 (the weights over them), o0, o1. (16 heads of 128, 4096 causal tokens: 70 us, 0.99
+// TMEM: s0, s1 (the weights over them), o0, o1. (16 heads of 128, 4096 causal tokens: 70 us, 0.98
 // PFLOP/s of the visible pairs; with a window of 512 of 2 x 2048 tokens 43 us, where a block's start and
 // end, some 5 us of 20, are bare.)
 // Heads of up to 64: half of the bytes and of TMEM, so one group to a block and two blocks on an SM,
