@@ -2,7 +2,7 @@
 //
 // Bound: HBM, one read of the visible keys and values (2 head_dim elements a key and key head
 // against 4 head_dim products per query head). The visible keys are the sinks [0, sink_end) and the
-// window [lo, length); number n of them is row n or n + skip. A cluster of blocks shares one
+// window [lo, length); number n of them is row n or n + skip. Blocks of a cluster share one
 // (sequence, key head, up to 8 query heads): each block takes a contiguous piece of the visible
 // keys, each warp pieces of that, with a running maximum, sum and output of its own; they are
 // joined over the block in shared memory and over the cluster in distributed shared memory, always
@@ -30,11 +30,12 @@ struct StepKeys {
 };
 
 // Joins the partial results of the block's warps (maximum and sum in ml[warp][head][2], output in
-// acc[warp][head][DP], unnormalised) and of the cluster's blocks and stores the output. `acc` is in
-// shared memory at the same place in every block.
+// acc[warp][head][DP], unnormalised) and of the `splits` blocks from block `base` of the cluster on,
+// of which this one is number `rank`, and stores the output. `acc` is in shared memory at the same
+// place in every block.
 template <int DT, int DP, int WARPS, int HEADS>
 __device__ __forceinline__ void join_step(const AttnParams& P, float* acc, const float* ml, int heads, int b, int h0, int splits,
-                                          int rank) {
+                                          int rank, int base = 0) {
   constexpr int THREADS = WARPS * 32, STRIDE = HEADS * DP;
   __syncthreads();
   for (int i = threadIdx.x; i < heads * DP; i += THREADS) {
@@ -56,12 +57,12 @@ __device__ __forceinline__ void join_step(const AttnParams& P, float* acc, const
       acc[STRIDE + i] = c == 0 ? top : sum;   // statistics of the block: columns 0 and 1
     }
   }
-  if (splits == 1) return;
+  if (gridDim.x == 1) return;
   __syncthreads();
   cluster_sync_all();
-  for (int i = (rank * THREADS + threadIdx.x) * 4; i < heads * DP; i += splits * THREADS * 4) {
+  for (int i = (rank * THREADS + threadIdx.x) * 4; splits > 1 && i < heads * DP; i += splits * THREADS * 4) {
     const int g = i / DP, c = i % DP;
-    const JoinedRow row = join_row(acc + i, acc + STRIDE + g * DP, splits, P.scale_log2);
+    const JoinedRow row = join_row(acc + i, acc + STRIDE + g * DP, splits, P.scale_log2, base);
     const float x[4] = {row.o.x, row.o.y, row.o.z, row.o.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -84,19 +85,21 @@ constexpr int kRingKeys = 16;
 template <int DP> struct StepShared {
   static constexpr int kTile = kRingKeys * DP * 2;      // keys or values
   // (More in flight is slower: the DRAM sees as many streams as there are warps. 8 sequences up to 32768
-  // keys took 64.5 us with 2 stages, 67 with 3, 109 with 6.)
+  // keys took 64.5 us with 2 stages, 67 with 3, 109 with 6; all apart, before two shared a cluster.)
   static constexpr int kStages = DP == 128 ? 2 : 4;
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kBytes = kRingWarps * kRing + 1024;
   static_assert(kRingWarps * 8 * DP * 4 <= kBytes - 1024, "the partial outputs take the rings' place");
 };
 
-// Sequence of the blocks with index z: the longest first, so that the last ones to start are short and
-// the blocks that share an SM differ (the lengths are known on the device alone). Every block ranks
-// them for itself, in `scratch`; more than kRankedBatch of them stay in their order.
+// The sequence of number z, and with BOTH the one of number batch - 1 - z, the longest first: the last
+// blocks to start are short and the blocks that share an SM differ (the lengths are known on the device
+// alone). Every block ranks them for itself, in `scratch`; more than kRankedBatch of them stay in
+// their order.
 constexpr int kRankedBatch = 256;
+template <bool BOTH>
 __device__ __forceinline__ int ranked_sequence(const AttnParams& P, int z, int* scratch, int* found) {
-  if (P.batch == 1 || P.batch > kRankedBatch) return z;
+  if (!BOTH && (P.batch == 1 || P.batch > kRankedBatch)) return z;   // (a pair is one of a few sequences)
   for (int i = threadIdx.x; i < P.batch; i += blockDim.x) {
     const int n = attn_length(P, i);
     scratch[i] = P.window == 0 ? n : min(n, P.window + P.sinks);
@@ -106,13 +109,15 @@ __device__ __forceinline__ int ranked_sequence(const AttnParams& P, int z, int* 
     const int n = scratch[i];
     int rank = 0;
     for (int j = 0; j < P.batch; ++j) rank += scratch[j] > n || (scratch[j] == n && j < i);
-    if (rank == z) *found = i;
+    if (rank == z) found[0] = i;
+    if (BOTH && rank == P.batch - 1 - z) found[1] = i;
   }
   __syncthreads();
-  return *found;
+  return found[0];
 }
 
-// The block's pieces of 16 keys: those of the sinks, then those of the window.
+// The pieces of 16 visible keys of a sequence: those of the sinks, then those of the window; the block's
+// share of them is [from, to).
 struct StepPieces {
   int sink_end, lo, length, sinks, from, to;
   __device__ __forceinline__ StepPieces(const AttnParams& P, int n, int rank, int splits) : length(n) {
@@ -161,7 +166,9 @@ __device__ __forceinline__ void mma16x8x16(float (&c)[4], const uint32_t (&a)[4]
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DT, int DP>
+// PAIRED: a cluster serves two sequences, the longest with the shortest and so on, and deals its
+// blocks to them by their lengths.
+template <int DT, int DP, bool PAIRED>
 __global__ void __launch_bounds__(kRingWarps * 32)
 attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v) {
@@ -170,16 +177,31 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kRingWarps][STAGES];
   __shared__ float ml[kRingWarps][8][2];
-  __shared__ int sequence;
+  __shared__ int sequences[2];
   // The same place in every block of the cluster.
   uint8_t* ring = raw + (((smem_u32(raw) + 1023u) & ~1023u) - smem_u32(raw));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int splits = gridDim.x, rank = blockIdx.x;
   const int passes = (P.group + 7) / 8;
   const int hk = blockIdx.y / passes, first = blockIdx.y % passes * 8;
   const int h0 = hk * P.group + first, heads = min(8, P.group - first);
-  const int b = ranked_sequence(P, blockIdx.z, reinterpret_cast<int*>(ring), &sequence);
+  int b = ranked_sequence<PAIRED>(P, blockIdx.z, reinterpret_cast<int*>(ring), sequences), splits = gridDim.x, rank = blockIdx.x, base = 0;
+  if (PAIRED && sequences[1] != b) {
+    auto visible = [&](int b) {
+      const int n = attn_length(P, b);
+      return P.window == 0 ? n : min(n, P.window + P.sinks);
+    };
+    const int64_t one = visible(b), both = max((int64_t)1, one + visible(sequences[1]));
+    const int share = min(splits - 1, max(1, (int)((2 * one * splits + both) / (2 * both))));
+    if (rank >= share) {
+      b = sequences[1];
+      base = share;
+      rank -= share;
+      splits -= share;
+    } else {
+      splits = share;
+    }
+  }
   const StepPieces pieces(P, attn_length(P, b), rank, splits);
   uint8_t* mine = ring + warp * Shape::kRing;
 
@@ -315,7 +337,7 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
       ml[warp][2 * t + e][1] = l[e];
     }
   }
-  join_step<DT, DP, kRingWarps, 8>(P, reinterpret_cast<float*>(ring), &ml[0][0][0], heads, b, h0, splits, rank);
+  join_step<DT, DP, kRingWarps, 8>(P, reinterpret_cast<float*>(ring), &ml[0][0][0], heads, b, h0, splits, rank, base);
 }
 
 // ---- float32, and 16-bit rows of any layout ------------------------------------------------
@@ -460,10 +482,10 @@ static int step_splits(const AttnParams& P, int64_t units, int most_blocks, int 
 }
 
 template <typename K, typename... Maps>
-static int launch_step(K kernel, const AttnParams& P, int splits, int heads, int threads, size_t bytes, cudaStream_t s,
-                       const Maps&... maps) {
+static int launch_step(K kernel, const AttnParams& P, int splits, int heads, int sequences, int threads, size_t bytes,
+                       cudaStream_t s, const Maps&... maps) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(splits, heads, P.batch);
+  config.gridDim = dim3(splits, heads, sequences);
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = bytes;
   config.stream = s;
@@ -486,24 +508,35 @@ static int launch_step(K kernel, const AttnParams& P, int splits, int heads, int
   return launch_status("nt_attention_step launch");
 }
 
-template <int DT, int DP>
-static int launch_ring(const AttnParams& P, cudaStream_t s) {
+template <int DT, int DP, bool PAIRED>
+static int launch_ring(const AttnParams& P, int splits, int heads, cudaStream_t s) {
   const char* who = "nt_attention_step";
   CUtensorMap k, v;
-  int rc = large_smem<attention_step_ring_kernel<DT, DP>>(StepShared<DP>::kBytes, who);
+  int rc = large_smem<attention_step_ring_kernel<DT, DP, PAIRED>>(StepShared<DP>::kBytes, who);
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, kRingKeys, who);
   if (rc) return rc;
+  return launch_step(attention_step_ring_kernel<DT, DP, PAIRED>, P, splits, heads, PAIRED ? (P.batch + 1) / 2 : P.batch,
+                     kRingWarps * 32, StepShared<DP>::kBytes, s, k, v);
+}
+
+template <int DT, int DP>
+static int dispatch_ring(const AttnParams& P, cudaStream_t s) {
   const int heads = P.kv_heads * ((P.group + 7) / 8);
   const int splits = step_splits(P, (int64_t)P.batch * heads, 3 * current_sm_count(), kRingWarps * kRingKeys);
-  return launch_step(attention_step_ring_kernel<DT, DP>, P, splits, heads, kRingWarps * 32, StepShared<DP>::kBytes, s, k, v);
+  // Clusters of 8 become clusters of 16 for two sequences, whose lengths differ as a rule: 8 sequences of 16
+  // heads on 4, up to 32768 keys, 63 us apart and 56.5 paired (all of 32768: 84, 87); 4 of 32 on 8, up to
+  // 16384, 37 and 35. Smaller ones gain nothing: 32 sequences in clusters of 4 for two take 44, in
+  // clusters of 2 39.
+  return P.batch > 1 && splits == kStepMaxSplits / 2 ? launch_ring<DT, DP, true>(P, kStepMaxSplits, heads, s)
+                                                     : launch_ring<DT, DP, false>(P, splits, heads, s);
 }
 
 template <int DT, int LPR, int HG>
 static int launch_simt(const AttnParams& P, cudaStream_t s) {
   const int heads = P.kv_heads * (P.group / HG);
   const int splits = step_splits(P, (int64_t)P.batch * heads, 2 * current_sm_count(), 64);
-  return launch_step(attention_step_kernel<DT, LPR, HG>, P, splits, heads, kStepThreads, 0, s);
+  return launch_step(attention_step_kernel<DT, LPR, HG>, P, splits, heads, P.batch, kStepThreads, 0, s);
 }
 
 template <int DT, int LPR>
@@ -516,7 +549,7 @@ static int dispatch_heads(const AttnParams& P, cudaStream_t s) {
 template <int DT>
 static int dispatch_step(const AttnParams& P, cudaStream_t s) {
   if constexpr (DT != NT_F32) {
-    if (P.vec && P.keys > 0) return P.dim <= 64 ? launch_ring<DT, 64>(P, s) : launch_ring<DT, 128>(P, s);
+    if (P.vec && P.keys > 0) return P.dim <= 64 ? dispatch_ring<DT, 64>(P, s) : dispatch_ring<DT, 128>(P, s);
   }
   constexpr int EPV = DT == NT_F32 ? 4 : 8;
   return P.dim <= 64 ? dispatch_heads<DT, 64 / EPV>(P, s) : dispatch_heads<DT, 128 / EPV>(P, s);

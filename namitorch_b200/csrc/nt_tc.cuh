@@ -57,15 +57,16 @@ __device__ __forceinline__ float4 load_cluster4(const float* p, uint32_t rank) {
 }
 constexpr int kMaxSplits = 8;   // blocks of a portable cluster
 
-// Four columns of a row whose parts lie in `splits` blocks: unnormalised output at `part`, maximum
-// and sum at `statistic`. Eight blocks' loads are issued before the first is used (one at a time they
+// Four columns of a row whose parts lie in `splits` blocks from block `base` of the cluster on:
+// unnormalised output at `part`, maximum and sum at `statistic`. Eight blocks' loads are issued before the first is used (one at a time they
 // cost a trip to the other SM each). Adds the parts in rank order; a part of weight 0 may not be
 // there.
 struct JoinedRow {
   float4 o;
   float top, sum;
 };
-__device__ __forceinline__ JoinedRow join_row(const float* part, const float* statistic, int splits, float scale_log2) {
+__device__ __forceinline__ JoinedRow join_row(const float* part, const float* statistic, int splits, float scale_log2,
+                                             int base = 0) {
   JoinedRow r{make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f};
   for (int k0 = 0; k0 < splits; k0 += 8) {
     float m[8], l[8];
@@ -76,9 +77,9 @@ __device__ __forceinline__ JoinedRow join_row(const float* part, const float* st
       l[k] = 0.0f;
       v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (k0 + k < splits) {
-        m[k] = load_cluster(statistic, k0 + k);
-        l[k] = load_cluster(statistic + 1, k0 + k);
-        v[k] = load_cluster4(part, k0 + k);
+        m[k] = load_cluster(statistic, base + k0 + k);
+        l[k] = load_cluster(statistic + 1, base + k0 + k);
+        v[k] = load_cluster4(part, base + k0 + k);
       }
     }
     float top = r.top;

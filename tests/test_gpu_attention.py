@@ -373,3 +373,18 @@ def test_second_derivatives_are_refused(cuda_device):
     grad, = torch.autograd.grad(F.dropout(q, 0.5, seed=1).square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="only once"):
         torch.autograd.grad(grad.sum(), q)
+
+
+@pytest.mark.parametrize("lengths", [(3000, 40), (1, 2900, 700), (0, 0), (1500, 0, 1500, 3), (900, 3000, 0, 20, 2200)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1100, 5)])
+def test_step_of_sequences_of_very_different_lengths(cuda_device, lengths, window, sinks):
+    """Few sequences over a long cache: many blocks to each, dealt by the lengths."""
+    batch, heads, kv_heads, capacity, dim = len(lengths), 32 // len(lengths) * 2, 32 // len(lengths), 3001, 128
+    q, k, v = _make((batch, heads, dim), "bf16", 1), _make((batch, kv_heads, capacity, dim), "bf16", 2), _make(
+        (batch, kv_heads, capacity, dim), "bf16", 3)
+    got = F.sliding_window_attention_step(q.cuda(), k.cuda(), v.cuda(), torch.tensor(lengths, device="cuda"), window=window,
+                                          sinks=sinks)
+    for b, length in enumerate(lengths):
+        arrays = [_np(t) for t in (q[b:b + 1, :, None], k[b:b + 1, :, :length], v[b:b + 1, :, :length])]
+        o = dict(window=window or 0, sinks=sinks, offset=max(0, length - 1))
+        _within(got[b:b + 1, :, None], O.forward(*arrays, **o)[0], O.tolerances(*arrays, "bf16", **o)[0], f"sequence {b}")
