@@ -23,7 +23,10 @@ def _rows(tensor):
     """(tensor, address, strides of the first three dimensions): the tensor itself when the kernels
     take its layout, else a contiguous copy. They take a dense last dimension, no broadcast
     dimension, and 16-byte aligned rows where the width allows them (a tile copy needs them)."""
-    shape, strides, address, size = tensor.shape, tensor.stride(), tensor.data_ptr(), tensor.element_size()
+    strides, address = tensor.stride(), tensor.data_ptr()
+    if address % 16 == 0 and tensor.is_contiguous():
+        return tensor, address, strides[:3]
+    shape, size = tensor.shape, tensor.element_size()
     aligned = shape[3] * size % 16 == 0
     good = (shape[3] <= 1 or strides[3] == 1) and not (aligned and address % 16)
     for i in range(3):
