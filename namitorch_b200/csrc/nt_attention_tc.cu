@@ -491,6 +491,9 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
 // products hides the exponentials instead: dp(t) runs while P(t) is computed, out2(t) and s(t + 1)
 // while dS(t) is, out1(t) and dp(t + 1) while P(t + 1) is. Without it dp has two buffers and
 // dp(t + 1) does not wait for out1(t). Groups of four warps take 32 columns each.
+// Bound in long rows by the shared memory that the products of two tiles from there read (85 cycles
+// each instead of 64), then by the power cap: 16 heads of 128, 4096 causal tokens, 203 us, 1.18 PFLOP/s
+// of the seven products; in short windows by a block's start and end (2 x 2048 tokens, window 512: 103).
 // Heads of up to 64 leave room for two blocks on an SM, with half of TMEM and steps of 64 rows each: one
 // begins and ends, or waits for its products, while the other computes (8 x 1024 tokens of 12 heads of
 // 64, window 256: 97 us with one block and steps of 128, 70 with two; 2 x 4096 of 16, causal: 317, 267).
@@ -518,7 +521,8 @@ template <int DP> struct BwdShared {
 };
 static_assert(BwdShared<128>::kBytes <= 227 * 1024 && BwdShared<64>::kBytes <= 113 * 1024, "blocks on an SM");
 
-// delta of every query: as many lanes to a row as it has 16-byte vectors.
+// delta of every query: as many lanes to a row as it has 16-byte vectors. Bound by HBM (g, o and what
+// rounding took from o, once: 50 MB of 2 x 2048 tokens of 16 heads of 128 in 7.7 us, 6.5 TB/s).
 template <int DT, int DP>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_constant__ AttnParams P) {
   constexpr int LPR = DP / 8, ROWS = 256 / LPR;

@@ -6,7 +6,9 @@
 // Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011).
 //
 // Bound: HBM (x, residual in, y out; g in, dx out). One Philox call (7 rounds of two 32 x 32 ->
-// 64 products) gives four elements.
+// 64 products) gives four elements. 16384 x 2048 bfloat16: forward 33 us, 93 % of the measured copy rate;
+// backward with the bias gradient 31 and 4, 66 % in its first kernel, whose generator issues in 47 % of
+// all cycles (the rows left over after fours, loaded ahead too, cost an eighth of the blocks: 33).
 #include <cmath>
 
 #include "nt_rows.cuh"
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kDropoutThreads) dropout_backward_kernel(const
 }
 
 // Column sums of the partial rows: lane j of a column adds partial rows j, j + 32, ... in order,
-// then the lane sums are added in lane order.
+// then the lane sums are added in lane order. (592 partial rows of 2048: 4 us of loads one behind another.)
 constexpr int kReduceLanes = 32;
 template <int DT>
 __global__ void __launch_bounds__(32 * kReduceLanes)
