@@ -492,7 +492,8 @@ static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
 //   64 on one key head, 1000 tokens, window 100, 2 sequences, backward: 38 us uncut, 21 cut);
 // - a sink block sees every later query, an ordinary one those of its own width and one window: a
 //   sink block's piece is no longer than an ordinary block or piece (3000 tokens, window 200, 4 sinks, 8
-//   heads on 2: all cut alike 40 us, so 31).
+//   heads on 2: all cut alike 40 us, so 31), or half of an SM's share (it starts first: long rows
+//   take the same time with fewer parts to keep and join).
 // A join costs some 4 us and a step 1 on the tensor cores but 10 on the FP32 pipe, so whole blocks are
 // those of up to 16 steps there and 2 here (float32, 2 x 1024 tokens of 8 heads, window 256, backward: 294
 // us with 16, 174 with 2; 300 tokens of 2 heads: 148, 62; both with the passes in one launch).
@@ -511,6 +512,7 @@ static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_ro
   const int64_t share = tiles * ordinary * a.query_heads * a.batch * (window == 0 ? 1 : 2) / current_sm_count();
   const int64_t longest = ordinary * group;
   int64_t piece = longest > least ? longest : least, rest = 1;
+  if (piece < share / 2) piece = share / 2;
   if (longest >= least && longest > share) {
     piece = share > least ? share / 2 : least / 2;
     rest = up(longest, piece) < 32 ? up(longest, piece) : 32;
