@@ -345,11 +345,37 @@ attention_step_ring_kernel(const __grid_constant__ AttnParams P, const __grid_co
 // ---- float32, and 16-bit rows of any layout ------------------------------------------------
 // Lanes of 16 bytes share a row (LPR of them); every lane group keeps its own running maximum, sum
 // and output for HG query heads, joined over the warp by shuffles. (394 MB of float32, 32
-// sequences of 16 heads of 128 on 4, window 4096: 189 us, 32 % of the measured copy rate; what costs is a
-// row's sum over its lanes, five shuffles a head.)
+// sequences of 16 heads of 128 on 4, window 4096: 136 us, 44 % of the measured copy rate, 190 with a sum
+// over the lanes for each row and head; what costs is the instructions of a row beside its loads.)
 constexpr int kStepThreads = 256;
 constexpr int kStepWarps = kStepThreads / 32;
 constexpr int kStepRows = 4;   // rows in flight per lane group
+
+// Sums of N values (the rows and heads at hand) over a group of 2 O lanes: each step adds half of the values that are left to the
+// lanes on one side and the rest to the other, N - 1 shuffles in place of log2(2 O) a value. Lane by
+// lane the values then lie in their order, N / (2 O) to a lane or one to every 2 O / N lanes.
+template <int O, int N, int ALL>
+__device__ __forceinline__ void group_scatter(float (&v)[ALL], int lane) {
+  if constexpr (O >= 1) {
+    if constexpr (N > 1) {
+      const bool up = lane & O;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float give = up ? v[i] : v[i + N / 2], keep = up ? v[i + N / 2] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, O);
+      }
+      group_scatter<O / 2, N / 2>(v, lane);
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], O);
+      group_scatter<O / 2, 1>(v, lane);
+    }
+  }
+}
+template <int LPR, int N>
+__device__ __forceinline__ float group_value(const float (&v)[N], int lane, int i) {
+  constexpr int EACH = N > LPR ? N / LPR : 1, APART = LPR > N ? LPR / N : 1;
+  return __shfl_sync(0xffffffffu, v[i % EACH], (lane & ~(LPR - 1)) + i / EACH * APART);
+}
 
 template <int DT, int LPR, int HG>
 __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __grid_constant__ AttnParams P) {
@@ -402,7 +428,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
     for (int r = 0; r < kStepRows; ++r) load(kb, P.ks.t, n0 + r * STRIDE, kr[r]);
 #pragma unroll
     for (int r = 0; r < kStepRows; ++r) load(vb, P.vs.t, n0 + r * STRIDE, vr[r]);
-    float s[kStepRows][HG];
+    float part[kStepRows * HG], s[kStepRows][HG];
 #pragma unroll
     for (int r = 0; r < kStepRows; ++r) {
       float kf[EPV];
@@ -412,11 +438,17 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const __gr
         float d = 0.0f;
 #pragma unroll
         for (int e = 0; e < EPV; ++e) d = fmaf(q[g][e], kf[e], d);
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-        s[r][g] = n0 + r * STRIDE < to ? d : -INFINITY;
+        part[r * HG + g] = d;
       }
     }
+    group_scatter<LPR / 2, kStepRows * HG>(part, lane);
+#pragma unroll
+    for (int r = 0; r < kStepRows; ++r)
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        const float d = group_value<LPR, kStepRows * HG>(part, lane, r * HG + g);
+        s[r][g] = n0 + r * STRIDE < to ? d : -INFINITY;
+      }
 #pragma unroll
     for (int g = 0; g < HG; ++g) {
       float top = m[g];
