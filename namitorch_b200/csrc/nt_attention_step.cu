@@ -351,9 +351,10 @@ constexpr int kStepThreads = 256;
 constexpr int kStepWarps = kStepThreads / 32;
 constexpr int kStepRows = 4;   // rows in flight per lane group
 
-// Sums of N values (the rows and heads at hand) over a group of 2 O lanes: each step adds half of the values that are left to the
-// lanes on one side and the rest to the other, N - 1 shuffles in place of log2(2 O) a value. Lane by
-// lane the values then lie in their order, N / (2 O) to a lane or one to every 2 O / N lanes.
+// Sums of N values (the rows and heads at hand) over a group of 2 O lanes: each step adds half of the
+// values that are left to the lanes on one side and the rest to the other, N - 1 shuffles in place of
+// log2(2 O) a value. Lane by lane the values then lie in their order, N / (2 O) to a lane or one to
+// every 2 O / N lanes.
 template <int O, int N, int ALL>
 __device__ __forceinline__ void group_scatter(float (&v)[ALL], int lane) {
   if constexpr (O >= 1) {
