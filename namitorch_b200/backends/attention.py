@@ -43,6 +43,16 @@ def _heads_last(batch, heads, tokens, dim, like):
                                dtype=like.dtype, device=like.device)
 
 
+def _statistics_bytes(dtype, batch, heads, kv_heads, queries, keys, dim):
+    """What the backward keeps at the start of its scratch: delta, and for float16 the norms that the
+    scale of dS is taken from; the rest is for partial gradients, which one more kernel joins."""
+    rows = [batch * heads * queries]
+    if dtype == torch.float16:
+        each = 32 if dim <= 64 else 16
+        rows += [rows[0], batch * heads * -(-queries // each), batch * kv_heads * -(-keys // each)]
+    return sum((4 * n + 255) // 256 * 256 for n in rows)
+
+
 class AttentionCUDAKernels:
     def __init__(self, backend=None):
         self._backend = backend
@@ -105,7 +115,7 @@ class AttentionCUDAKernels:
         size = N.load().nt_attention_workspace_size(args + _NO_SCRATCH)
         workspace = torch.empty(size, dtype=torch.uint8, device=query.device)
         args += N.pack_attention_scratch(workspace.data_ptr(), size, self._error_word(query.device))
-        statistics = (batch * heads * queries * 4 + 255) // 256 * 256
+        statistics = _statistics_bytes(query.dtype, batch, heads, kv_heads, queries, keys, dim)
         N.on_device(query.device, "nt_attention_backward", args,
                     int(batch * queries > 0) + int(batch * keys > 0) + int(size > statistics))
         return dq, dk, dv

@@ -521,9 +521,19 @@ static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_ro
   return {parts > 1 ? (int)up(a.sinks, tile_rows) : 0, (int)parts, (int)rest};
 }
 
-static size_t delta_bytes(const nt_attention_args& a) {
-  return ((size_t)a.batch * a.query_heads * a.queries * 4 + 255) / 256 * 256;
-}
+// The statistics of the backward at the start of its workspace: delta, and for float16 the norms.
+struct StatisticsPlaces {
+  size_t g_norm, g_top, v_top, end;   // bytes from delta on
+  explicit StatisticsPlaces(const nt_attention_args& a) {
+    auto bytes = [](int64_t n) { return ((size_t)n * 4 + 255) / 256 * 256; };
+    auto tops = [&](int64_t rows) { return (int64_t)norm_tiles((int)rows, a.head_dim); };
+    const bool norms = a.dtype == NT_F16;
+    g_norm = bytes(a.batch * a.query_heads * a.queries);
+    g_top = g_norm + (norms ? bytes(a.batch * a.query_heads * a.queries) : 0);
+    v_top = g_top + (norms ? bytes(a.batch * a.query_heads * tops(a.queries)) : 0);
+    end = v_top + (norms ? bytes(a.batch * a.kv_heads * tops(a.keys)) : 0);
+  }
+};
 
 static void set_split(AttnParams& P, const KeySplit& split) {
   P.sink_tiles = split.sink_tiles;
@@ -618,7 +628,7 @@ size_t nt_attention_workspace_size(const nt_attention_args* args) {
   if (!args || check_attention(*args, "nt_attention_workspace_size")) return 0;
   const size_t a = partial_bytes(*args, kRows, kRows, kLeastPiece);
   const size_t b = partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim), kTcLeastPiece);
-  return delta_bytes(*args) + (a > b ? a : b);
+  return StatisticsPlaces(*args).end + (a > b ? a : b);
 }
 
 int nt_attention_forward(const nt_attention_args* args, void* stream) {
@@ -667,8 +677,13 @@ int nt_attention_backward(const nt_attention_args* args, void* stream) {
     return NT_EINVAL;
   }
   AttnParams P = attention_params(a, a.query_offset + a.queries);
-  P.delta = static_cast<float*>(a.workspace);
-  P.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + delta_bytes(a));
+  const StatisticsPlaces places(a);
+  auto at = [&](size_t bytes) { return reinterpret_cast<float*>(static_cast<char*>(a.workspace) + bytes); };
+  P.delta = at(0);
+  P.g_norm = at(places.g_norm);
+  P.g_top = at(places.g_top);
+  P.v_top = at(places.v_top);
+  P.partial = at(places.end);
   P.vec = vector_query(a, a.query, a.query_strides) && vector_key(a, a.key, a.key_strides) &&
           vector_key(a, a.value, a.value_strides) && vector_query(a, a.gradient, a.gradient_strides) &&
           vector_query(a, a.output, a.output_strides);

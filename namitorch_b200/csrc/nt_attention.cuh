@@ -23,6 +23,9 @@ struct AttnParams {
   AttnStrides qs, ks, vs, gs, os, dqs, dks, dvs;
   float* lse;        // [batch, heads, queries]
   float* delta;      // [batch, heads, queries]: sum over head_dim of g * o
+  // Tensor-core backward of float16: the row norms of g [batch, heads, queries], and the largest of
+  // each norm_rows rows of g [batch, heads, ..] and of v [batch, kv_heads, ..] (attention_delta_norms_kernel).
+  float *g_norm, *g_top, *v_top;
   float* partial;    // backward: partial gradients of the split key blocks
   const int32_t* lengths;
   int32_t* error;
@@ -108,6 +111,9 @@ int make_map(CUtensorMap* map, int dtype, const void* ptr, const AttnStrides& st
 int attention_step_launch(const AttnParams& P, int dtype, cudaStream_t s);
 // nt_attention_tc.cu: the tensor-core forms (16-bit types, 16-byte aligned rows).
 constexpr int kTcKeyRows = 128;    // keys of a block of the key / value gradients
+// Rows that share an entry of g_top and v_top, and the entries of `rows` rows.
+__host__ __device__ constexpr int norm_rows(int dim) { return dim <= 64 ? 32 : 16; }
+__host__ __device__ constexpr int norm_tiles(int rows, int dim) { return (rows + norm_rows(dim) - 1) / norm_rows(dim); }
 constexpr int tc_query_step(int dim) { return dim <= 64 ? 64 : 128; }   // queries it takes at a time
 int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s);
 int attention_tc_backward_launch(const AttnParams& P, int dtype, cudaStream_t s);

@@ -13,6 +13,14 @@
 // rounding would show: there it goes in as the sum of two 16-bit values, in two products (window 2:
 // dq has 1.15 times the error of rounding the exact gradient instead of 1.53; 2 x 4096 tokens of 16
 // heads of 128 take 137 us instead of 122; from 16 keys on the ratio is below 1.5 with one value).
+//
+// float16 holds 40 powers of two, and dS has the size of the upstream gradient times that of v times a
+// weight. Its backward therefore rounds dS times a power of two (one of each query for dq, one of each
+// block of keys for dk) and P times 2^14, and takes them out of the float32 sums at the end: the ratio
+// is below 1.5 for gradients and values of any size (without it 3.4 at gradients of 1e-3 over 2048 causal
+// tokens, and infinities where dS passes 65504). The norms and their maxima cost the backward 83 -> 93 us
+// (8 x 1024 tokens of 12 heads of 64, window 256) and 220 -> 232 (4096 causal of 16 of 128); bfloat16 has
+// float32's range and takes neither.
 #include <cmath>
 #include <utility>
 
@@ -25,6 +33,32 @@ constexpr int kTcRows = 128;
 constexpr uint32_t kTmemColumns = 512;
 constexpr float kRaiseSum = 8192.0f;
 constexpr int64_t kFineKeys = 16;
+// float16: weights are at most 1, so that 2^14 times them stays below 65504 and those from 2^-28 on are
+// normal numbers.
+constexpr int kWeightPower = 14;
+
+// The power of two e for dS = P (dP - delta) of rows whose norms of g and v are at most g and v: |dP| and
+// |delta| (delta is a mean of dP) are at most g v, so 2^e |dS| is below 2^14 and not far below it.
+// Norms of 0 have nothing to scale.
+__device__ __forceinline__ int gradient_power(float g, float v) {
+  const int exponent = (__float_as_int(2.0f * g * v) >> 23 & 255) - 127;
+  return min(max(13 - exponent, -100), 100);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
+// The largest of the entries that hold rows [lo, hi), 0 if there are none. A whole warp.
+__device__ __forceinline__ float largest_norm(const float* tops, int dim, int lo, int hi, int lane) {
+  float top = 0.0f;
+  const int end = norm_tiles(hi, dim);
+#pragma unroll 8
+  for (int i = lo / norm_rows(dim) + lane; i < end; i += 32) top = fmaxf(top, tops[i]);
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // (not negative)
+}
+// The largest norm of v among the keys that queries [q0, q1) see.
+__device__ __forceinline__ float largest_value_norm(const AttnParams& P, int length, int b, int hk, int q0, int q1, int lane) {
+  const AttnKeys range(P, length, q0, q1);
+  const float* tops = P.v_top + ((int64_t)b * P.kv_heads + hk) * norm_tiles(P.keys, P.dim);
+  return fmaxf(largest_norm(tops, P.dim, 0, range.sink_end, lane), largest_norm(tops, P.dim, range.lo, range.hi, lane));
+}
 
 // Which columns of a tile a row sees: c < end and (c >= begin or c < sink). word(c0) has bit e set
 // for column c0 + e, so that a masked tile costs one bit test and one select per element.
@@ -516,10 +550,36 @@ template <int DP> struct BwdShared {
         dp_full[2], ds_full[2],            // by the step's parity: dp(t + 1) may be there before dp(t) was waited for
         stat_full[2], stat_free[2], out_full;
     uint32_t tmem;
+    int power;                         // float16, gradients of keys: of the two that scales dS
   };
   static constexpr int kBytes = kControl + (int)sizeof(Control);
 };
 static_assert(BwdShared<128>::kBytes <= 227 * 1024 && BwdShared<64>::kBytes <= 113 * 1024, "blocks on an SM");
+
+// This lane's share of delta of a query, and of the square of its row of g (NORM).
+template <int DT, bool NORM>
+__device__ __forceinline__ void delta_share(const AttnParams& P, int b, int h, int64_t row, int c, float& d, float& squares) {
+  float x[8], y[8], z[8];
+  const int64_t o = P.os.at(b, h, row) + c;
+  unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.g) + P.gs.at(b, h, row) + c)), x);
+  unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o) + o)), y);
+  if (P.o_low != nullptr) {
+    unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o_low) + o)), z);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] += z[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    d = fmaf(x[e], y[e], d);
+    if constexpr (NORM) squares = fmaf(x[e], x[e], squares);
+  }
+}
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int w = LPR / 2; w > 0; w >>= 1) v += __shfl_xor_sync(0xffffffffu, v, w);
+  return v;
+}
 
 // delta of every query: as many lanes to a row as it has 16-byte vectors. Bound by HBM (g, o and what
 // rounding took from o, once: 50 MB of 2 x 2048 tokens of 16 heads of 128 in 7.7 us, 6.5 TB/s).
@@ -529,23 +589,60 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(const __grid_const
   grid_dependents_go();
   const int b = blockIdx.z, h = blockIdx.y, c = threadIdx.x % LPR * 8;
   const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LPR;
-  float d = 0.0f;
-  if (row < P.queries && c < P.dim) {
-    float x[8], y[8], z[8];
-    const int64_t o = P.os.at(b, h, row) + c;
-    unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.g) + P.gs.at(b, h, row) + c)), x);
-    unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o) + o)), y);
-    if (P.o_low != nullptr) {
-      unpack16<DT>(__ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.o_low) + o)), z);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] += z[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
-  }
-#pragma unroll
-  for (int w = LPR / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+  float d = 0.0f, unused = 0.0f;
+  if (row < P.queries && c < P.dim) delta_share<DT, false>(P, b, h, row, c, d, unused);
+  d = row_sum<LPR>(d);
   if (threadIdx.x % LPR == 0 && row < P.queries) P.delta[((int64_t)b * P.heads + h) * P.queries + row] = d;
+}
+
+// The same for float16, with what the scale of dS is taken from: the norm of every row of g, and the
+// largest norm of the block's rows of g, or of v among the keys that some query sees (what others hold
+// may be anything). A norm that is not finite counts as 0: the gradients of its row are lost, but not
+// those of its neighbours. Blocks of queries of a head come first, then those of keys. (67 MB of 2 x
+// 2048 tokens of 16 heads of 128: 15.4 us, 4.4 TB/s, for the block's join of its rows; entries of 128
+// rows took 17.6 to 25, an entry to a warp with its loads in flight together 19.)
+template <int DP>
+__global__ void __launch_bounds__(256) attention_delta_norms_kernel(const __grid_constant__ AttnParams P) {
+  constexpr int LPR = DP / 8, ROWS = 256 / LPR;
+  static_assert(ROWS == norm_rows(DP), "rows of an entry");
+  __shared__ float tops[8];
+  grid_dependents_go();
+  const int b = blockIdx.z, h = blockIdx.y, c = threadIdx.x % LPR * 8;
+  const int query_tiles = norm_tiles(P.queries, DP);
+  const bool queries = (int)blockIdx.x < query_tiles;
+  const int tile = queries ? blockIdx.x : blockIdx.x - query_tiles;
+  if (!queries && h >= P.kv_heads) return;
+  const int64_t row = (int64_t)tile * ROWS + threadIdx.x / LPR;
+  float d = 0.0f, squares = 0.0f;
+  if (queries) {
+    if (row < P.queries && c < P.dim) delta_share<NT_F16, true>(P, b, h, row, c, d, squares);
+  } else {
+    const AttnKeys seen(P, attn_length(P, b), 0, P.queries);
+    if (row < seen.hi && (row >= seen.lo || row < seen.sink_end) && c < P.dim) {
+      float x[8];
+      unpack16<NT_F16>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.v) + P.vs.at(b, h, row) + c)), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) squares = fmaf(x[e], x[e], squares);
+    }
+  }
+  squares = row_sum<LPR>(squares);
+  float top = squares < INFINITY ? sqrtf(squares) : 0.0f;
+  if (queries) {
+    d = row_sum<LPR>(d);
+    if (threadIdx.x % LPR == 0 && row < P.queries) {
+      const int64_t at = ((int64_t)b * P.heads + h) * P.queries + row;
+      P.delta[at] = d;
+      P.g_norm[at] = top;
+    }
+  }
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));   // (not negative)
+  if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) top = fmaxf(top, tops[w]);
+  if (queries) P.g_top[((int64_t)b * P.heads + h) * query_tiles + tile] = top;
+  else P.v_top[((int64_t)b * P.kv_heads + h) * norm_tiles(P.keys, DP) + tile] = top;
 }
 
 template <int DT, int DP, bool DKV, bool FINE>
@@ -675,6 +772,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       read = copied;
     }
     int n1 = min(steps, 1), n2 = n1;
+    float delta_scale = -1.0f;
     auto copies = [&](int t) {
       advance(copied);
       if (t >= RING1) ok = wait_warp(&ctl.y1_free[t % RING1], ring_phase(t - RING1, RING1));
@@ -693,8 +791,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       for (int i = 0; i < kStep / 32; ++i) {
         const int c = i * 32 + lane;
         const bool in = read.begin + c < read.end;
-        lse[i] = in ? -P.lse[stat + c] * kLog2eF : 0.0f;
-        delta[i] = in ? -P.delta[stat + c] : 0.0f;
+        lse[i] = in ? fmaf(-P.lse[stat + c], kLog2eF, DT == NT_F16 ? kWeightPower : 0) : 0.0f;
+        delta[i] = in ? delta_scale * P.delta[stat + c] : 0.0f;
       }
       advance(read);
       if (t >= 2) ok = wait_warp(&ctl.stat_free[t & 1], ring_phase(t - 2, 2));
@@ -712,6 +810,17 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     if (steps > 1) copies(1);
     if constexpr (DKV) {
       grid_dependency_wait();
+      if (DT == NT_F16 && steps > 0) {
+        // One power of two for the block: the sum over the queries is one accumulator.
+        float g = 0.0f;
+        for (int h = h0 * P.group; h < (h0 + 1) * P.group; ++h)
+          g = fmaxf(g, largest_norm(P.g_top + ((int64_t)b * P.heads + h) * norm_tiles(P.queries, P.dim), P.dim,
+                                    query_range.lo, query_range.hi, lane));
+        const int power = gradient_power(g, largest_value_norm(P, length, b, h0, query_range.lo, query_range.hi, lane));
+        delta_scale = -power_of_two(power - kWeightPower);
+        if (lane == 0) ctl.power = power;
+        __syncwarp();
+      }
       if (steps > 0) statistics(0);
     }
     for (int t = 0; t < steps && ok; ++t) {
@@ -810,12 +919,22 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t at_s = t_s + lanes + group * kColumns;
     float lse = 0.0f, delta = 0.0f;
+    // float16: the power of two that dS carries; for dq one of each row, which the weights bring in, with
+    // DKV one of the block, 2^kWeightPower of it from the weights and the rest from dP - delta.
+    float carried = 1.0f;
     if constexpr (!DKV) {
       grid_dependency_wait();
+      float g = 0.0f;
       if (r0 + row < r1) {
         const int64_t stat = ((int64_t)b * P.heads + h0) * P.queries + r0 + row;
         lse = -P.lse[stat] * kLog2eF;
         delta = -P.delta[stat];
+        if constexpr (DT == NT_F16) g = P.g_norm[stat];
+      }
+      if constexpr (DT == NT_F16) {
+        const int power = gradient_power(g, largest_value_norm(P, length, b, h0 / P.group, r0, r1, lane));
+        lse += power;
+        carried = power_of_two(power);
       }
     }
     // Steps without a masked pair: those whose rows are all there and lie within these bounds.
@@ -885,6 +1004,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       __syncwarp();
       tc_fence_after();
       const uint32_t at_dp = t_dp_of(t) + lanes + group * kColumns;
+      if constexpr (DT == NT_F16 && DKV) carried = power_of_two(ctl.power - kWeightPower);
       uint32_t d[kColumns];
       tmem_load32(at_dp, d);
       tmem_wait_load();
@@ -892,10 +1012,14 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       for (int c = 0; c < kColumns; c += 4) {
         float4 de = make_float4(delta, delta, delta, delta);   // negative
         if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * kColumns + c]);
+        auto difference = [&](Pair x, Pair y) {
+          if constexpr (DT == NT_F16 && DKV) return fma2(x, Pair(carried, carried), y);   // (delta comes scaled)
+          else return add2(x, y);
+        };
         float a, e;
-        mul2(Pair(p[c], p[c + 1]), add2(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
+        mul2(Pair(p[c], p[c + 1]), difference(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
         w[c / 2] = pack2<DT>(a, e);
-        mul2(Pair(p[c + 2], p[c + 3]), add2(Pair(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), Pair(de.z, de.w))).get(a, e);
+        mul2(Pair(p[c + 2], p[c + 3]), difference(Pair(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), Pair(de.z, de.w))).get(a, e);
         w[c / 2 + 1] = pack2<DT>(a, e);
       }
       if (!full) {
@@ -912,8 +1036,9 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
           if constexpr (DKV) de = *reinterpret_cast<const float2*>(&ctl.stats[t & 1][1][group * kColumns + c]);
           const float2 hi = unpack2<DT>(w[c / 2]);
           // (a masked element's low part is cleared with its high part)
-          const float a = seen >> c & 1 ? p[c] * (__uint_as_float(d[c]) + de.x) - hi.x : 0.0f;
-          const float e = seen >> (c + 1) & 1 ? p[c + 1] * (__uint_as_float(d[c + 1]) + de.y) - hi.y : 0.0f;
+          const float f = DT == NT_F16 && DKV ? carried : 1.0f;
+          const float a = seen >> c & 1 ? p[c] * fmaf(__uint_as_float(d[c]), f, de.x) - hi.x : 0.0f;
+          const float e = seen >> (c + 1) & 1 ? p[c + 1] * fmaf(__uint_as_float(d[c + 1]), f, de.y) - hi.y : 0.0f;
           w[c / 2] = pack2<DT>(a, e);
         }
         tmem_store16(at_dp + kColumns / 2, w);
@@ -934,7 +1059,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     constexpr int SHARERS = DKV ? Shape::kGroups / 2 : Shape::kGroups, WIDTH = DP / SHARERS, CHUNK = WIDTH < 32 ? WIDTH : 32;
     const int which = group / SHARERS, c_first = group % SHARERS * WIDTH;
     const uint32_t t_out = (which ? t_out2 : t_out1) + lanes + c_first;
-    const float f = which ? 1.0f : P.scale;
+    const float weights = DT == NT_F16 && DKV ? power_of_two(-kWeightPower) : 1.0f;
+    const float f = which ? weights : DT == NT_F16 ? P.scale / carried * weights : P.scale;
     const int row0 = r0 + (warp & 3) * 32;
     // The tiles of x1 and x2 are free now.
     uint8_t* stage = aligned + warp * 4096;
@@ -1069,8 +1195,13 @@ static int launch_tc_backward(const AttnParams& P, cudaStream_t s) {
   if (!rc) rc = make_map(&k, DT, P.k, P.ks, P.dim, P.keys, P.kv_heads, P.batch, BwdShared<DP>::kStep, who);
   if (!rc) rc = make_map(&v, DT, P.v, P.vs, P.dim, P.keys, P.kv_heads, P.batch, BwdShared<DP>::kStep, who);
   if (rc) return rc;
-  constexpr int ROWS = 256 / (DP / 8);
-  attention_delta_kernel<DT, DP><<<dim3((P.queries + ROWS - 1) / ROWS, P.heads, P.batch), 256, 0, s>>>(P);
+  if constexpr (DT == NT_F16) {
+    const int entries = norm_tiles(P.queries, DP) + norm_tiles(P.keys, DP);
+    attention_delta_norms_kernel<DP><<<dim3(entries, P.heads, P.batch), 256, 0, s>>>(P);
+  } else {
+    constexpr int ROWS = 256 / (DP / 8);
+    attention_delta_kernel<DT, DP><<<dim3((P.queries + ROWS - 1) / ROWS, P.heads, P.batch), 256, 0, s>>>(P);
+  }
   rc = launch_status("nt_attention_backward launch");
   if (rc) return rc;
   const uint32_t query_blocks = (uint32_t)((P.queries + kTcRows - 1) / kTcRows) * P.heads * P.batch;

@@ -18,8 +18,9 @@ the products, t = u for float32):
 * dq: scale max|k| (eps_ds + n u max|dP - delta|) + t |dq| (rows of P sum to 1); dk and dv: the same
   per unit of column sum of P over the queries and the heads of the group.
 
-* float16 weights and dS below its normal range lose up to 2^-25 each: n times that, times the
-  largest factor, per output.
+* float16 numbers below the normal range lose up to 2^-25 each. The forward's weights: n times that, times
+  the largest factor, per output. The backward's weights are held times 2^14, and dS times a power of two
+  that brings 2 max|g|_2 max|v|_2 to 2^13 at least: n 2^-39 and n 2^-37 of that product.
 
 Everything is doubled for the terms of second order.
 """
@@ -136,8 +137,9 @@ def tolerances(q, k, v, dtype, g=None, *, window=0, sinks=0, lengths=None, offse
             p, _ = _weights(q64[b, h], k64[b, h // group], seen, scale)
             columns[b, h // group, :, 0] += p.sum(axis=0)
     per = eps_ds + n * u * spread
-    lost = n * floor
+    norm = lambda x: top(np.linalg.norm(x, axis=-1))  # noqa: E731
+    lost = n * floor * 2.0 ** -12 * 2 * norm(g64) * norm(v64)
     t_dq = 2 * (scale * top(np.abs(k64)) * (per + lost) + t * np.abs(dq)) + floor
     t_dk = 2 * (scale * top(np.abs(q64)) * (per * columns + lost) + t * np.abs(dk)) + floor
-    t_dv = 2 * (((eps_p + t + n * u) * columns + lost) * top(np.abs(g64)) + t * np.abs(dv)) + floor
+    t_dv = 2 * (((eps_p + t + n * u) * columns + n * floor * 2.0 ** -14) * top(np.abs(g64)) + t * np.abs(dv)) + floor
     return t_out, t_lse, t_dq, t_dk, t_dv
