@@ -20,6 +20,7 @@ from numbers import Integral, Real
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as N
 from ..backends import get_backend
@@ -247,6 +248,20 @@ def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale)
     return window, sinks, lengths, scale
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether a derivative with respect to one of these (tensors or None) may be asked for: such a call
+    goes through its autograd function, which computes it or refuses."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # Outside of every level of forward-mode differentiation (where torch says so: asking each tensor
+    # costs a one-token step a tenth of its time) nothing has a tangent.
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Once(torch.autograd.Function):
     """Gradients tied to what they were computed from, so that a second derivative is an error
     rather than a term left out."""
@@ -297,9 +312,20 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
     options = {"window": window, "sinks": sinks, "query_offset": _count("query_position_offset", query_position_offset),
                "scale": scale}
-    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+    if _differentiated(query, key, value):
         return _SlidingWindowAttention.apply(query, key, value, lengths, options)
     return get_backend(query).attention.forward(query, key, value, lengths, save=False, **options)[0]
+
+
+class _SlidingWindowAttentionStep(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key_cache, value_cache, lengths, options):
+        return get_backend(query).attention.step(query, key_cache, value_cache, lengths, **options)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise RuntimeError("sliding_window_attention_step has no gradient; differentiate sliding_window_attention, or "
+                           "call the step under torch.no_grad().")
 
 
 def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -309,12 +335,15 @@ def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, 
 
     ``query`` is [batch, heads, head_dim], the caches [batch, kv_heads, capacity, head_dim].
     Sequence b holds ``lengths[b]`` keys, the new token's among them, and its query stands at
-    the last of them. Reads the keys and values it sees and nothing else of the cache."""
+    the last of them. Reads the keys and values it sees and nothing else of the cache. Has no
+    gradient: asking for one through the result is an error."""
     if lengths is None:
         raise TypeError("Attention lengths must be an int32 or int64 Tensor.")
     window, sinks, lengths, scale = _attention_arguments(query, key_cache, value_cache, 3, window, sinks, lengths, scale)
-    return get_backend(query).attention.step(query, key_cache, value_cache, lengths, window=window, sinks=sinks,
-                                             scale=scale)
+    options = {"window": window, "sinks": sinks, "scale": scale}
+    if _differentiated(query, key_cache, value_cache):
+        return _SlidingWindowAttentionStep.apply(query, key_cache, value_cache, lengths, options)
+    return get_backend(query).attention.step(query, key_cache, value_cache, lengths, **options)
 
 
 class _Dropout(torch.autograd.Function):
@@ -373,8 +402,7 @@ def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: 
     if input.device.type != "cuda":
         raise RuntimeError("namitorch_b200 dropout runs on a CUDA device; move the input there first.")
     p = float(p) if training else 0.0
-    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if _differentiated(input, bias, residual):
         return _Dropout.apply(input, bias, residual, p, int(seed), int(offset))
     return get_backend(input).dropout.forward(input, p, seed=int(seed), offset=int(offset), bias=bias, residual=residual)
 
