@@ -151,6 +151,7 @@ def train(steps=60, batch=16, tokens=64, device="cuda"):
         scaler.step(optimizer)
         scaler.update()
         losses.append(loss.item())
+        F.check_attention(device)
     return p, losses
 
 
@@ -173,6 +174,7 @@ def main(steps=60):
     p, losses = train(steps)
     prompt = batch_of(10_000, 4, 40, "cuda")[:, :-1]
     tokens, _ = generate(p, prompt, 24)
+    F.check_attention(tokens.device)
     right = float((tokens[:, 40:] == batch_of(10_000, 4, 64, "cuda")[:, 40:64]).float().mean())
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} in {len(losses)} steps; {100 * right:.0f}% of 96 generated tokens "
           "continue the pattern")

@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define NT_ABI_VERSION 9
+#define NT_ABI_VERSION 10
 #define NT_MAX_GROUPS 32      /* coefficient groups per nt_adamw_mt call */
 #define NT_MAX_FOUND_INF 16   /* optimizers combined by one nt_scaler_update call */
 
@@ -481,6 +481,11 @@ int nt_attention_backward(const nt_attention_args* args, void* stream);
 /* One new token per sequence over a cache: queries == 1, the query of sequence b stands at
    lengths[b] - 1 (lengths is required, query_offset is ignored). */
 int nt_attention_step(const nt_attention_args* args, void* stream);
+
+/* The address of a word of the current device that starts as 0 and that nothing here clears, for
+   `error`: no allocation and no launch, so a call that is captured into a graph can be the first to
+   use it. One word per device that loads the library. */
+int nt_attention_error_word(int32_t** word);
 
 /* ------------------------------------------------------------------------------------ */
 /* Dropout from a counter-based generator, with the bias before it and the residual after */

@@ -23,7 +23,7 @@ NT_DECAY_NONE, NT_DECAY_DECOUPLED, NT_DECAY_COUPLED = 0, 1, 2
 NT_MAX_GROUPS = 32
 NT_MAX_FOUND_INF = 16
 NT_MAX_RANKS = 8
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 
 class Segment(C.Structure):
@@ -229,6 +229,7 @@ SIGNATURES: dict[str, tuple] = {
     "nt_attention_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nt_attention_backward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nt_attention_step": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_attention_error_word": (C.c_int, [C.POINTER(C.c_void_p)]),
     "nt_dropout_workspace_size": (C.c_size_t, [C.c_int64, C.c_int64]),
     "nt_dropout_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "nt_dropout_backward": (C.c_int, [C.c_void_p, C.c_void_p]),

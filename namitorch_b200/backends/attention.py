@@ -53,6 +53,15 @@ def _statistics_bytes(dtype, batch, heads, kv_heads, queries, keys, dim):
     return sum((4 * n + 255) // 256 * 256 for n in rows)
 
 
+class _Word:
+    """The library's error word of the current device as an array that torch can view."""
+
+    def __init__(self):
+        address = N.C.c_void_p()
+        N.check(N.load().nt_attention_error_word(N.C.byref(address)), "nt_attention_error_word")
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address.value, False), "version": 3}
+
+
 class AttentionCUDAKernels:
     def __init__(self, backend=None):
         self._backend = backend
@@ -60,12 +69,13 @@ class AttentionCUDAKernels:
 
     def _error_word(self, device):
         if self._error is None:
-            self._error = torch.zeros(1, dtype=torch.int32, device=device)
+            with torch.cuda.device(device):
+                self._error = torch.as_tensor(_Word(), device=device)
         return self._error.data_ptr()
 
     def check(self) -> None:
         """Raises if a bounded wait inside an attention kernel of this device has ever run out
-        (reads one word from the device)."""
+        (waits for the current stream and reads one word)."""
         if self._error is not None and int(self._error.item()):
             raise RuntimeError("A wait inside an attention kernel ran out; the results of that call are incomplete.")
 

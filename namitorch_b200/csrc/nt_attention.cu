@@ -578,6 +578,10 @@ static int check_attention(const nt_attention_args& a, const char* who) {
   return NT_OK;
 }
 
+// Zero from the moment the library is there: a word that were allocated and cleared on a stream could be
+// cleared again by every replay of a graph, or after a kernel of another stream has set it.
+static __device__ int32_t attention_error_word;
+
 static AttnStrides strides(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
 // Rows are whole 16-byte vectors at 16-byte aligned addresses (the stride of a dimension of
@@ -720,6 +724,15 @@ int nt_attention_step(const nt_attention_args* args, void* stream) {
   AttnParams P = attention_params(a, a.keys);
   P.vec = vector_key(a, a.key, a.key_strides) && vector_key(a, a.value, a.value_strides);
   return attention_step_launch(P, a.dtype, as_stream(stream));
+}
+
+int nt_attention_error_word(int32_t** word) {
+  if (!word) { set_error("nt_attention_error_word: word is NULL"); return NT_EINVAL; }
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, attention_error_word);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(e, "nt_attention_error_word"); }
+  *word = static_cast<int32_t*>(p);
+  return NT_OK;
 }
 
 }  // extern "C"

@@ -308,7 +308,8 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     ``lengths[b]`` (an integer tensor [batch], clamped to the keys) has no effect; a NaN or an
     infinity that some query sees can reach other queries of its block of 256.
 
-    Differentiable once in query, key and value; sums run in float32 in a fixed order."""
+    Differentiable once in query, key and value; sums run in float32 in a fixed order.
+    ``check_attention`` tells whether every wait inside the kernels completed."""
     window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
     options = {"window": window, "sinks": sinks, "query_offset": _count("query_position_offset", query_position_offset),
                "scale": scale}
@@ -344,6 +345,16 @@ def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, 
     if _differentiated(query, key_cache, value_cache):
         return _SlidingWindowAttentionStep.apply(query, key_cache, value_cache, lengths, options)
     return get_backend(query).attention.step(query, key_cache, value_cache, lengths, **options)
+
+
+def check_attention(device: torch.device | str | None = None) -> None:
+    """Raises RuntimeError if a wait inside an attention kernel on ``device`` (the current one by
+    default) has ever run out, graph replays included.
+
+    The kernels bound every wait on their own copies and products at about two seconds. One that runs out
+    does not stop the program: the call's outputs are incomplete and a word on the device says so. This
+    reads it, which waits for the current stream: call it where the program reads a result anyway."""
+    get_backend(device).attention.check()
 
 
 class _Dropout(torch.autograd.Function):
@@ -407,5 +418,5 @@ def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: 
     return get_backend(input).dropout.forward(input, p, seed=int(seed), offset=int(offset), bias=bias, residual=residual)
 
 
-__all__ = ["cross_entropy", "dropout", "linear", "sliding_window_attention", "sliding_window_attention_step",
+__all__ = ["check_attention", "cross_entropy", "dropout", "linear", "sliding_window_attention", "sliding_window_attention_step",
            "softmax_cross_entropy"]
