@@ -494,6 +494,8 @@ static int64_t effective_window(const nt_attention_args& a, int64_t positions) {
 //   sink block's piece is no longer than an ordinary block or piece (3000 tokens, window 200, 4 sinks, 8
 //   heads on 2: all cut alike 40 us, so 31), or half of an SM's share (it starts first: long rows
 //   take the same time with fewer parts to keep and join).
+// The share counts the sink blocks' steps too: many sinks are most of the work, fill the SMs uncut and
+// would fill the workspace cut. So the pieces of all heads together stay below some 600.
 // A join costs some 4 us and a step 1 on the tensor cores but 10 on the FP32 pipe, so whole blocks are
 // those of up to 16 steps there and 2 here (float32, 2 x 1024 tokens of 8 heads, window 256, backward: 294
 // us with 16, 174 with 2; 300 tokens of 2 heads: 148, 62; both with the passes in one launch).
@@ -508,8 +510,10 @@ static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_ro
   if (tiles == 0 || steps == 0) return {0, 1, 1};
   int64_t ordinary = window == 0 ? steps : up(tile_rows + window - 1, step_rows) + 1;
   if (ordinary > steps) ordinary = steps;
+  const int64_t sinks = window > 0 ? up(a.sinks, tile_rows) : 0;   // (fewer than tiles)
   // Both passes; without a window about half of the blocks' pairs lie past the diagonal.
-  const int64_t share = tiles * ordinary * a.query_heads * a.batch * (window == 0 ? 1 : 2) / current_sm_count();
+  const int64_t share = (sinks * steps + (tiles - sinks) * ordinary) * a.query_heads * a.batch * (window == 0 ? 1 : 2) /
+                        current_sm_count();
   const int64_t longest = ordinary * group;
   int64_t piece = longest > least ? longest : least, rest = 1;
   if (piece < share / 2) piece = share / 2;
@@ -517,8 +521,8 @@ static KeySplit key_split(const nt_attention_args& a, int tile_rows, int step_ro
     piece = share > least ? share / 2 : least / 2;
     rest = up(longest, piece) < 32 ? up(longest, piece) : 32;
   }
-  const int64_t parts = window > 0 && a.sinks > 0 ? up(steps * group, piece) : 1;
-  return {parts > 1 ? (int)up(a.sinks, tile_rows) : 0, (int)parts, (int)rest};
+  const int64_t parts = sinks > 0 ? up(steps * group, piece) : 1;
+  return {parts > 1 ? (int)sinks : 0, (int)parts, (int)rest};
 }
 
 // The statistics of the backward at the start of its workspace: delta, and for float16 the norms.
@@ -631,7 +635,7 @@ extern "C" {
 size_t nt_attention_workspace_size(const nt_attention_args* args) {
   if (!args || check_attention(*args, "nt_attention_workspace_size")) return 0;
   const size_t a = partial_bytes(*args, kRows, kRows, kLeastPiece);
-  const size_t b = partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim), kTcLeastPiece);
+  const size_t b = args->dtype == NT_F32 ? 0 : partial_bytes(*args, kTcKeyRows, tc_query_step(args->head_dim), kTcLeastPiece);
   return StatisticsPlaces(*args).end + (a > b ? a : b);
 }
 
