@@ -226,8 +226,9 @@ def _attention_arguments(query, key, value, rank, window, sinks, lengths, scale)
                         f"{value.dtype}.")
     if device.type != "cuda" or key.device != device or value.device != device:
         raise RuntimeError("namitorch_b200 attention runs on one CUDA device; move query, key and value there first.")
-    window = 0 if window is None else _count("window", window, 1)
-    sinks = _count("sinks", sinks)
+    # (what lies beyond 2^62 is beyond every position)
+    window = 0 if window is None else min(_count("window", window, 1), 1 << 62)
+    sinks = min(_count("sinks", sinks), 1 << 62)
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError("Attention lengths must be an int32 or int64 Tensor or None.")
@@ -311,8 +312,8 @@ def sliding_window_attention(query: torch.Tensor, key: torch.Tensor, value: torc
     Differentiable once in query, key and value; sums run in float32 in a fixed order.
     ``check_attention`` tells whether every wait inside the kernels completed."""
     window, sinks, lengths, scale = _attention_arguments(query, key, value, 4, window, sinks, lengths, scale)
-    options = {"window": window, "sinks": sinks, "query_offset": _count("query_position_offset", query_position_offset),
-               "scale": scale}
+    offset = min(_count("query_position_offset", query_position_offset), 1 << 62)
+    options = {"window": window, "sinks": sinks, "query_offset": offset, "scale": scale}
     if _differentiated(query, key, value):
         return _SlidingWindowAttention.apply(query, key, value, lengths, options)
     return get_backend(query).attention.forward(query, key, value, lengths, save=False, **options)[0]
