@@ -96,6 +96,19 @@ def autocast_operands(operation, *operands):
     return tuple(None if value is None else value.to(dtype) for value in operands)
 
 
+def autocast_promoted(*operands):
+    """The operands of an elementwise operation that takes one dtype, as adding them would promote them:
+    inside an enabled autocast context non-None CUDA operands of several floating dtypes are converted to
+    float32 (a projection's low-precision result beside a float32 bias and residual), else as given."""
+    enabled, _ = _autocast_state.get()
+    values = tuple(v for v in operands if v is not None)
+    if not enabled or all(v.dtype == values[0].dtype for v in values):
+        return operands
+    if any(v.device.type != "cuda" or v.dtype not in (*_LOW, torch.float32) for v in values):
+        return operands
+    return tuple(None if v is None else v.to(torch.float32) for v in operands)
+
+
 def float32_function(function):
     """Promotes float16 / bfloat16 tensor arguments to float32 (namitorch/amp.py:64-75)."""
     if OPERATION_POLICIES.get(function.__name__) != "float32":
@@ -342,4 +355,4 @@ class GradScaler:
             self._tracker_dev.fill_(tracker)
 
 
-__all__ = ["autocast", "autocast_dtype", "autocast_operands", "float32_function", "GradScaler", "DeviceFlag", "OPERATION_POLICIES"]
+__all__ = ["autocast", "autocast_dtype", "autocast_operands", "autocast_promoted", "float32_function", "GradScaler", "DeviceFlag", "OPERATION_POLICIES"]

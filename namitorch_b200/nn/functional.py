@@ -383,10 +383,14 @@ def dropout(input: torch.Tensor, p: float, *, seed: int, offset: int = 0, bias: 
     counter (e // 4, ``offset``) under the key ``seed`` (both in [0, 2^64)) is below p * 2^32: the
     mask depends on (seed, offset, e) alone, is computed again by the backward and never stored.
     Use another offset for every call that needs a mask of its own. ``bias`` has the shape
-    [width] of the last dimension, ``residual`` that of ``input``. With ``training=False``
-    nothing is dropped."""
+    [width] of the last dimension, ``residual`` that of ``input``; all have one dtype, except inside
+    ``amp.autocast``, where several are promoted to float32 (a 16-bit projection beside a float32
+    bias and residual). With ``training=False`` nothing is dropped."""
+    from ..amp import autocast_promoted
     if not isinstance(input, torch.Tensor):
         raise TypeError("dropout input must be a NamiTorch Tensor.")
+    if all(t is None or isinstance(t, torch.Tensor) for t in (bias, residual)):
+        input, bias, residual = autocast_promoted(input, bias, residual)
     if input.dtype not in _DTYPES:
         raise TypeError(f"dropout supports float32, float16 and bfloat16 tensors, got {input.dtype}.")
     if input.dim() < 1:
