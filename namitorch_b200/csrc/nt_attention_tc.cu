@@ -295,9 +295,12 @@ attention_tc_forward(const __grid_constant__ AttnParams P, const __grid_constant
       begin = next_begin;
       end = next_end;
     }
-    if (!finished) commit(&ctl.o_full[0]);
-    if constexpr (GROUPS == 2) commit(&ctl.o_full[1]);
-    if (!ok) wait_bar(&ctl.o_full[GROUPS - 1], 0);   // no product is in flight when TMEM is given back
+    // (A block without tiles commits nothing: no one would wait for the arrival, and the block may end.)
+    if (blocks > 0) {
+      if (!finished) commit(&ctl.o_full[0]);
+      if constexpr (GROUPS == 2) commit(&ctl.o_full[1]);
+      if (!ok) wait_bar(&ctl.o_full[GROUPS - 1], 0);   // no product is in flight when TMEM is given back
+    }
   } else {
     const int g = GROUPS == 2 ? warp >> 3 : 0, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // lane 32 (w % 4) in the address's upper half
@@ -911,9 +914,11 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       tc_fence_after();
       sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * PIECE, now, t > 0, FINE, &ctl.y1_free[t % RING1]);
     }
-    if (elect_one()) tc_commit(&ctl.out_full);
-    __syncwarp();
-    if (!ok) wait_bar(&ctl.out_full, 0);
+    if (steps > 0) {   // (as in the forward)
+      if (elect_one()) tc_commit(&ctl.out_full);
+      __syncwarp();
+      if (!ok) wait_bar(&ctl.out_full, 0);
+    }
   } else {
     const int group = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;

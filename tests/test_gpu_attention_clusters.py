@@ -71,3 +71,24 @@ def test_a_cluster_repeats_bit_for_bit_and_leaves_other_rows(cuda_device):
     part = F.sliding_window_attention(q[:, :, 64:], k, v, query_position_offset=2064)
     assert torch.equal(whole, F.sliding_window_attention(q, k, v, query_position_offset=2000))
     np.testing.assert_allclose(part.float().cpu().numpy(), whole[:, :, 64:].float().cpu().numpy(), rtol=2.0 ** -6, atol=2e-3)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_blocks_without_work_beside_full_ones(cuda_device, dt, dim):
+    """Every second sequence is empty, so blocks that end at once share the SMs with blocks that compute: the
+    same bits, call after call, as of the sequences alone."""
+    from namitorch_b200.nn import functional as F
+    n = 12
+    arrays = [_make((n, h, 500, dim), dt, s).cuda() for h, s in ((4, 1), (2, 2), (2, 3), (4, 4))]
+    lengths = torch.tensor([500 * (b % 2) for b in range(n)], dtype=torch.int32, device="cuda")
+
+    def run(tensors, lengths):
+        leaves = [t.detach().requires_grad_() for t in tensors[:3]]
+        out = F.sliding_window_attention(*leaves, window=200, lengths=lengths)
+        return (out.detach(), *torch.autograd.grad(out, leaves, tensors[3]))
+
+    alone = run([t[1::2].contiguous() for t in arrays], None)
+    for _ in range(20):
+        for a, b in zip(run(arrays, lengths), alone):
+            assert torch.all(a[::2] == 0) and torch.equal(a[1::2], b)
