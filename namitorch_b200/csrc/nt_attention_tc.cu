@@ -8,11 +8,15 @@
 // afterwards.
 //
 // Roundings below 32 bits: the weights and dS are rounded to the inputs' type because the second
-// products take their operand in it; every sum, maximum and statistic is float32. Where no row sees
-// more than kFineKeys keys, dS is what is left of nearly equal numbers (P dP - P delta), and its
+// products take their operand in it; every sum, maximum and statistic is float32. Where a row sees
+// kFineKeys keys or fewer, dS is what is left of nearly equal numbers (P dP - P delta), and its
 // rounding would show: there it goes in as the sum of two 16-bit values, in two products (window 2:
 // dq has 1.15 times the error of rounding the exact gradient instead of 1.53; 2 x 4096 tokens of 16
 // heads of 128 take 137 us instead of 122; from 16 keys on the ratio is below 1.5 with one value).
+// Two calls have such rows in number: narrow windows, and batches with lengths, whose queries past a
+// sequence's end see what is left of it (8 sequences up to 777 tokens, window 100: 1.15 instead of 1.53,
+// 50 us the backward instead of 46). Without either only a sequence's first rows are, and they take one
+// value: the two alone cost other calls 4 to 12 % (4096 causal tokens of 16 heads of 64: 327 us for 292).
 //
 // float16 holds 40 powers of two, and dS has the size of the upstream gradient times that of v times a
 // weight. Its backward therefore rounds dS times a power of two (one of each query for dq, one of each
@@ -33,6 +37,17 @@ constexpr int kTcRows = 128;
 constexpr uint32_t kTmemColumns = 512;
 constexpr float kRaiseSum = 8192.0f;
 constexpr int64_t kFineKeys = 16;
+
+// Whether one of queries [i0, i1) sees at most kFineKeys keys. Along the queries the number of keys
+// first grows, then stays and then, past the sequence's length, falls: the least is at an end.
+__device__ __forceinline__ bool attn_few_keys(const AttnParams& P, int length, int i0, int i1) {
+  auto few = [&](int i) {
+    const int end = min(length, P.offset + i + 1);
+    const int start = P.window == 0 ? 0 : min(max(P.offset + i + 1 - P.window, 0), end);
+    return end - start + min(P.sinks, start) <= kFineKeys;
+  };
+  return few(i0) || few(i1 - 1);
+}
 // float16: weights are at most 1, so that 2^14 times them stays below 65504 and those from 2^-28 on are
 // normal numbers.
 constexpr int kWeightPower = 14;
@@ -718,6 +733,11 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       key_range.block(s.at, kStep, s.begin, s.end);
     }
   };
+  // FINE: whether a query of step s may see few keys, so that dS goes in as two values.
+  auto fine = [&](const Step& s) {
+    if constexpr (!FINE) return false;
+    return DKV ? attn_few_keys(P, length, s.begin, s.end) : attn_few_keys(P, length, r0, r1);
+  };
 
   // The copying warp sets up the barriers and issues the first copies while the rest is set up.
   auto load = [&](const CUtensorMap& map, int at, int token, int head, int rows, uint64_t* bar) {
@@ -900,6 +920,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       tc_fence_after();
       if constexpr (DKV) sum(t_out2, t_s, Shape::kY2 + t % RING2 * PIECE, rows, t > 0, false, &ctl.y2_free[t % RING2]);
       const int now = rows;
+      const bool low = fine(s);
       if (t + 1 < steps) {
         advance(s);
         rows = s.end - s.begin;
@@ -912,7 +933,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       ok = ok && wait_warp(&ctl.ds_full[t & 1], ring_phase(t, 2));
       if (!ok) break;
       tc_fence_after();
-      sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * PIECE, now, t > 0, FINE, &ctl.y1_free[t % RING1]);
+      sum(t_out1, t_dp_of(t), Shape::kY1 + t % RING1 * PIECE, now, t > 0, low, &ctl.y1_free[t % RING1]);
     }
     if (steps > 0) {   // (as in the forward)
       if (elect_one()) tc_commit(&ctl.out_full);
@@ -1013,40 +1034,46 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       uint32_t d[kColumns];
       tmem_load32(at_dp, d);
       tmem_wait_load();
-#pragma unroll
-      for (int c = 0; c < kColumns; c += 4) {
-        float4 de = make_float4(delta, delta, delta, delta);   // negative
-        if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * kColumns + c]);
-        auto difference = [&](Pair x, Pair y) {
-          if constexpr (DT == NT_F16 && DKV) return fma2(x, Pair(carried, carried), y);   // (delta comes scaled)
-          else return add2(x, y);
-        };
-        float a, e;
-        mul2(Pair(p[c], p[c + 1]), difference(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
-        w[c / 2] = pack2<DT>(a, e);
-        mul2(Pair(p[c + 2], p[c + 3]), difference(Pair(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), Pair(de.z, de.w))).get(a, e);
-        w[c / 2 + 1] = pack2<DT>(a, e);
-      }
-      if (!full) {
-        // dp of a key that is not there may be NaN: 0 * NaN is cleared here.
-#pragma unroll
-        for (int c = 0; c < kColumns; c += 2)
-          w[c / 2] &= (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u);
-      }
-      tmem_store16(at_dp, w);
-      if constexpr (FINE) {
+      auto difference = [&](Pair x, Pair y) {
+        if constexpr (DT == NT_F16 && DKV) return fma2(x, Pair(carried, carried), y);   // (delta comes scaled)
+        else return add2(x, y);
+      };
+      // dp of a key that is not there may be NaN: 0 * NaN is cleared.
+      auto there = [&](int c) { return (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u); };
+      if (FINE && fine(step)) {
+        uint32_t rest[kColumns / 2];   // what rounding takes away
 #pragma unroll
         for (int c = 0; c < kColumns; c += 2) {
-          float2 de = make_float2(delta, delta);
+          float2 de = make_float2(delta, delta);   // negative
           if constexpr (DKV) de = *reinterpret_cast<const float2*>(&ctl.stats[t & 1][1][group * kColumns + c]);
-          const float2 hi = unpack2<DT>(w[c / 2]);
-          // (a masked element's low part is cleared with its high part)
-          const float f = DT == NT_F16 && DKV ? carried : 1.0f;
-          const float a = seen >> c & 1 ? p[c] * fmaf(__uint_as_float(d[c]), f, de.x) - hi.x : 0.0f;
-          const float e = seen >> (c + 1) & 1 ? p[c + 1] * fmaf(__uint_as_float(d[c + 1]), f, de.y) - hi.y : 0.0f;
+          float a, e;
+          mul2(Pair(p[c], p[c + 1]), difference(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
           w[c / 2] = pack2<DT>(a, e);
+          const float2 hi = unpack2<DT>(w[c / 2]);
+          rest[c / 2] = pack2<DT>(a - hi.x, e - hi.y);
+          if (!full) {
+            w[c / 2] &= there(c);
+            rest[c / 2] &= there(c);
+          }
         }
-        tmem_store16(at_dp + kColumns / 2, w);
+        tmem_store16(at_dp, w);
+        tmem_store16(at_dp + kColumns / 2, rest);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 4) {
+          float4 de = make_float4(delta, delta, delta, delta);   // negative
+          if constexpr (DKV) de = *reinterpret_cast<const float4*>(&ctl.stats[t & 1][1][group * kColumns + c]);
+          float a, e;
+          mul2(Pair(p[c], p[c + 1]), difference(Pair(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), Pair(de.x, de.y))).get(a, e);
+          w[c / 2] = pack2<DT>(a, e);
+          mul2(Pair(p[c + 2], p[c + 3]), difference(Pair(__uint_as_float(d[c + 2]), __uint_as_float(d[c + 3])), Pair(de.z, de.w))).get(a, e);
+          w[c / 2 + 1] = pack2<DT>(a, e);
+        }
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < kColumns; c += 2) w[c / 2] &= there(c);
+        }
+        tmem_store16(at_dp, w);
       }
       tmem_wait_store();
       tc_fence_before();
@@ -1126,8 +1153,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
 
 // `key_blocks` blocks own keys, the others queries. The longer kind comes first: the key blocks, unless
 // all of them are cut (4 heads on one key head, 6508 tokens of 64: 138 us with the cut ones first, 103
-// with the query blocks). FINE is a variant of its own because the branch alone made every other call
-// spill registers.
+// with the query blocks). FINE is a variant of its own: see the top of this file.
 template <int DT, int DP, bool FINE>
 __global__ void __launch_bounds__(BwdShared<DP>::kThreads, BwdShared<DP>::kResident)
 attention_tc_backward(const __grid_constant__ AttnParams P, uint32_t key_blocks, const __grid_constant__ CUtensorMap map_q,
@@ -1235,7 +1261,7 @@ int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s) 
 
 template <int DT, int DP>
 static int dispatch_tc_backward(const AttnParams& P, cudaStream_t s) {
-  const bool fine = P.keys <= kFineKeys || (P.window > 0 && (int64_t)P.window + P.sinks <= kFineKeys);
+  const bool fine = P.lengths != nullptr || P.keys <= kFineKeys || (P.window > 0 && (int64_t)P.window + P.sinks <= kFineKeys);
   return fine ? launch_tc_backward<DT, DP, true>(P, s) : launch_tc_backward<DT, DP, false>(P, s);
 }
 
