@@ -13,10 +13,13 @@
 // rounding would show: there it goes in as the sum of two 16-bit values, in two products (window 2:
 // dq has 1.15 times the error of rounding the exact gradient instead of 1.53; 2 x 4096 tokens of 16
 // heads of 128 take 137 us instead of 122; from 16 keys on the ratio is below 1.5 with one value).
-// Two calls have such rows in number: narrow windows, and batches with lengths, whose queries past a
-// sequence's end see what is left of it (8 sequences up to 777 tokens, window 100: 1.15 instead of 1.53,
-// 50 us the backward instead of 46). Without either only a sequence's first rows are, and they take one
-// value: the two alone cost other calls 4 to 12 % (4096 causal tokens of 16 heads of 64: 327 us for 292).
+// Three kinds of calls have such rows in number: narrow windows; batches with lengths, whose queries past
+// a sequence's end see what is left of it (8 sequences up to 777 tokens, window 100: 1.15 instead of
+// 1.53, 50 us the backward instead of 46); and short sequences, whose first rows, with the largest
+// weights, have most of the gradients' norm (64 causal tokens of one head: 1.06 instead of 1.39 to 1.57,
+// as the sample falls; 4 x 256 tokens of 8 heads of 64 take 17.4 us instead of 15.4). Longer calls take
+// one value (1.41 to 1.46): the choice alone costs them 4 to 12 % (4096 causal tokens of 16 heads of
+// 64: 327 us for 292).
 //
 // float16 holds 40 powers of two, and dS has the size of the upstream gradient times that of v times a
 // weight. Its backward therefore rounds dS times a power of two (one of each query for dq, one of each
@@ -37,6 +40,7 @@ constexpr int kTcRows = 128;
 constexpr uint32_t kTmemColumns = 512;
 constexpr float kRaiseSum = 8192.0f;
 constexpr int64_t kFineKeys = 16;
+constexpr int kShortQueries = 512;
 
 // Whether one of queries [i0, i1) sees at most kFineKeys keys. Along the queries the number of keys
 // first grows, then stays and then, past the sequence's length, falls: the least is at an end.
@@ -1261,7 +1265,7 @@ int attention_tc_forward_launch(const AttnParams& P, int dtype, cudaStream_t s) 
 
 template <int DT, int DP>
 static int dispatch_tc_backward(const AttnParams& P, cudaStream_t s) {
-  const bool fine = P.lengths != nullptr || P.keys <= kFineKeys || (P.window > 0 && (int64_t)P.window + P.sinks <= kFineKeys);
+  const bool fine = P.lengths != nullptr || P.queries <= kShortQueries || P.keys <= kFineKeys || (P.window > 0 && (int64_t)P.window + P.sinks <= kFineKeys);
   return fine ? launch_tc_backward<DT, DP, true>(P, s) : launch_tc_backward<DT, DP, false>(P, s);
 }
 

@@ -1,4 +1,5 @@
-"""Gradients of ragged batches, where the queries past a sequence's end see its last few keys alone."""
+"""Gradients where rows that see few keys carry much of the norm: ragged batches, whose queries past a
+sequence's end see its last few keys alone, and short sequences."""
 import numpy as np
 import pytest
 import torch
@@ -26,3 +27,20 @@ def test_rows_with_few_keys_keep_their_precision(cuda_device, dt, dim, window, s
     for got, want, bound in zip(grads, wanted, (1.35, 1.35, 1.5)):
         rounded = _np(torch.from_numpy(want).to(TORCH[dt]))
         assert np.linalg.norm(_np(got) - want) <= bound * np.linalg.norm(rounded - want)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens", [17, 40, 64, 200, 400])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_short_sequences_keep_their_precision(cuda_device, dt, tokens, dim):
+    """Causal rows n see n keys and have about 1 / n of the squared norm: those with more than 16, which hold dS
+    in one value, have at most log(400 / 16) / log(400) = 0.54 of it, and delta's error is a few hundredths
+    beside it. sqrt(1.54) is 1.24, 1.35 with the spread of a single head's sample."""
+    for seed in range(6):
+        q, k, v, g = (_make((1, 1, tokens, dim), dt, 10 * seed + s) for s in (1, 2, 3, 4))
+        leaves = [t.cuda().requires_grad_() for t in (q, k, v)]
+        grads = torch.autograd.grad(F.sliding_window_attention(*leaves), leaves, g.cuda())
+        wanted = O.backward(*(_np(t) for t in (q, k, v, g)))
+        for got, want in list(zip(grads, wanted))[:2]:
+            rounded = _np(torch.from_numpy(want).to(TORCH[dt]))
+            assert np.linalg.norm(_np(got) - want) <= 1.35 * np.linalg.norm(rounded - want)
