@@ -479,7 +479,8 @@ int nt_attention_forward(const nt_attention_args* args, void* stream);
 int nt_attention_backward(const nt_attention_args* args, void* stream);
 
 /* One new token per sequence over a cache: queries == 1, the query of sequence b stands at
-   lengths[b] - 1 (lengths is required, query_offset is ignored). */
+   lengths[b] - 1 (lengths is required, query_offset is ignored). Up to 15 rows after the sinks and
+   after lengths[b] may be read beside those that are seen, whatever they hold. */
 int nt_attention_step(const nt_attention_args* args, void* stream);
 
 /* The address of a word of the current device that starts as 0 and that nothing here clears, for

@@ -1,7 +1,8 @@
 // Sliding-window attention of one new token per sequence over a cache of keys and values.
 //
 // Bound: HBM, one read of the visible keys and values (2 head_dim elements a key and key head
-// against 4 head_dim products per query head). The visible keys are the sinks [0, sink_end) and the
+// against 4 head_dim products per query head) for every 8 query heads of a key head, on the FP32 pipe
+// for every 4, 2 or 1 (what divides their number). The visible keys are the sinks [0, sink_end) and the
 // window [lo, length); number n of them is row n or n + skip. Blocks of a cluster share one
 // (sequence, key head, up to 8 query heads): each block takes a contiguous piece of the visible
 // keys, each warp pieces of that, with a running maximum, sum and output of its own; they are

@@ -337,7 +337,10 @@ def sliding_window_attention_step(query: torch.Tensor, key_cache: torch.Tensor, 
 
     ``query`` is [batch, heads, head_dim], the caches [batch, kv_heads, capacity, head_dim].
     Sequence b holds ``lengths[b]`` keys, the new token's among them, and its query stands at
-    the last of them. Reads the keys and values it sees and nothing else of the cache. Has no
+    the last of them. What the other rows of the cache hold has no effect, but up to 15 rows after
+    the sinks and after ``lengths[b]`` may be read with those that are seen. A cache is taken as it
+    lies when its last dimension is dense, no dimension is broadcast and, where rows are whole
+    16-byte vectors, they start on 16-byte boundaries; any other is copied first, all of it. Has no
     gradient: asking for one through the result is an error."""
     if lengths is None:
         raise TypeError("Attention lengths must be an int32 or int64 Tensor.")
