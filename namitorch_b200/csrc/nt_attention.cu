@@ -137,9 +137,11 @@ __device__ __forceinline__ float lanes16_sum(float v) {
 }
 
 // The maximum is kept of the scores before the scale: a difference of scores is formed before it
-// is scaled, so that scores near the ends of float32 do not overflow on the way. Bound by the FP32 pipe
-// and its operands' loads (4 x 1024 causal tokens of 4 heads of 128: 200 us, 23 TFLOP/s of the tiles'
-// products); 4 x 256 tokens of 4 heads of 64 are 64 blocks and 23 us of their latency.
+// is scaled, so that scores near the ends of float32 do not overflow on the way. 4 x 1024 causal tokens of
+// 4 heads of 128: 200 us, 23 TFLOP/s of the tiles' products, with shared memory busy for 42 % of the
+// cycles, instructions issued in 26 % and 18 % of the warps there: a block waits for its operands from
+// shared memory, then at its barriers for one tile after another, and 256 blocks on 148 SMs do not
+// cover that. 4 x 256 tokens of 4 heads of 64 are 64 blocks and 23 us of their latency.
 template <int DT, int DP>
 __global__ void __launch_bounds__(kSimtThreads) attention_forward_kernel(const __grid_constant__ AttnParams P) {
   extern __shared__ __align__(16) float smem[];
@@ -376,8 +378,9 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
 
 // Both kinds of blocks in one launch, so that one fills the SMs that the other leaves idle: `key_blocks`
 // own keys, the others queries; the longer kind comes first, the key blocks unless all of them are cut.
-// Bound by the FP32 pipe where there are blocks enough (4 x 1024 causal tokens of 4 heads of 128: 459 us,
-// 35 TFLOP/s of the tiles' products), else by the copies and products of one block after another.
+// Bound by the operands' reads of shared memory where there are blocks enough (4 x 1024 causal tokens of 4
+// heads of 128: 457 us, 35 TFLOP/s of the tiles' products, shared memory busy for 67 % of the cycles,
+// the FP32 pipe for about half), else by the copies and products of one block after another.
 template <int DT, int DP>
 __global__ void __launch_bounds__(kSimtThreads, DP <= 64 ? 2 : 1)
 attention_backward_kernel(const __grid_constant__ AttnParams P, uint32_t key_blocks) {

@@ -80,8 +80,8 @@ __device__ __forceinline__ void join_step(const AttnParams& P, float* acc, const
 // O^T += V^T P^T. (A tcgen05 product has 128 rows; a group of query heads has one to eight.) P^T is
 // the accumulator of the first as the second operand of the other, transposed between the lanes in
 // registers. The weights are rounded to the type of the values for the second product. (197 MB of 32
-// sequences of 16 heads of 128 on 4, window 4096: 39.5 us, 76 % of the measured copy rate; 8 full caches
-// of 32768: 84 us, 97 %.)
+// sequences of 16 heads of 128 on 4, window 4096: 40 us, 75 % of the measured copy rate; 8 full caches
+// of 32768, as pairs in clusters of 16: 88 us, 92 %.)
 constexpr int kRingWarps = 4;
 constexpr int kRingKeys = 16;
 

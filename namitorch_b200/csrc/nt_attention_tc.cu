@@ -11,8 +11,9 @@
 // products take their operand in it; every sum, maximum and statistic is float32. Where a row sees
 // kFineKeys keys or fewer, dS is what is left of nearly equal numbers (P dP - P delta), and its
 // rounding would show: there it goes in as the sum of two 16-bit values, in two products (window 2:
-// dq has 1.15 times the error of rounding the exact gradient instead of 1.53; 2 x 4096 tokens of 16
-// heads of 128 take 137 us instead of 122; from 16 keys on the ratio is below 1.5 with one value).
+// dq has 1.15 times the error of rounding the exact gradient instead of 1.53; the backward of 2 x 4096
+// tokens of 16 heads of 128 takes 160 us instead of 144; from 16 keys on the ratio is below 1.5 with
+// one value).
 // Three kinds of calls have such rows in number: narrow windows; batches with lengths, whose queries past
 // a sequence's end see what is left of it (8 sequences up to 777 tokens, window 100: 1.15 instead of
 // 1.53, 50 us the backward instead of 46); and short sequences, whose first rows, with the largest
@@ -124,9 +125,10 @@ __device__ __forceinline__ void clear_tail(uint8_t* tile, int rows, int lane) {
 // Eight warps do the softmax of a group: two threads share a row, 64 columns each. The products of one
 // group run under the exponentials of the other:
 //   s0(0) s1(0) | o0 += w0(0) v, s0(1) | o1 += w1(0) v, s1(1) | o0 += w0(1) v, ...
-// TMEM: s0, s1 (the weights over them), o0, o1. (16 heads of 128, 4096 causal tokens: 70 us, 0.98
-// PFLOP/s of the visible pairs; with a window of 512 of 2 x 2048 tokens 43 us, where a block's start and
-// end, some 5 us of 20, are bare.)
+// TMEM: s0, s1 (the weights over them), o0, o1. (16 heads of 128, 4096 causal tokens: 69 us, 1.0 PFLOP/s
+// of the visible pairs, the tensor pipe active for 47 % of the time, the exponentials' for 36, issue 44:
+// no pipe is full; what is left are the waits between a tile's scores, weights and product. With a
+// window of 512 of 2 x 2048 tokens 43 us, where a block's start and end, some 5 us of 20, are bare.)
 // Heads of up to 64: half of the bytes and of TMEM, so one group to a block and two blocks on an SM,
 // and the start and end of one lie under the other's work (8 x 1024 tokens of 12 heads, window 256: 40
 // us with two groups to a block, 34 so; 8192 tokens of 16 heads, window 128: 46, 34; 2 x 4096 causal of

@@ -37,6 +37,9 @@ CHILD = """
         out = F.sliding_window_attention(q, q, q, window=9)
     kernels = get_backend(q).attention
     word = kernels._error
+    from namitorch_b200 import _native as N
+    address = N.C.c_void_p()
+    assert N.load().nt_attention_error_word(N.C.byref(address)) == 0 and address.value == word.data_ptr()
     graph.replay()
     torch.cuda.synchronize()
     kernels.check()
