@@ -281,9 +281,11 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
     grid_dependency_wait();
     const int64_t stat = ((int64_t)b * P.heads + h) * P.queries;
     float lse[4], delta[4];
+    bool one_key[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i0 + 4 * ty + i;
+      one_key[i] = attn_key_count(P, length, r) == 1;
       lse[i] = r < i1 ? P.lse[stat + r] * kLog2eF : 0.0f;
       delta[i] = r < i1 ? P.delta[stat + r] : 0.0f;
     }
@@ -305,7 +307,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
           const int key = begin + tx + 16 * j;
           const bool seen = key < end && attn_visible(P, length, P.offset + i0 + 4 * ty + i, key);
           const float pr = exp2f(fmaf(s[i][j], P.scale_log2, -lse[i]));
-          wds[(4 * ty + i) * kWeightStride + tx + 16 * j] = seen ? pr * (dp[i][j] - delta[i]) : 0.0f;
+          wds[(4 * ty + i) * kWeightStride + tx + 16 * j] = seen && !one_key[i] ? pr * (dp[i][j] - delta[i]) : 0.0f;
         }
       __syncthreads();
       tile_accumulate<DP>(wds, y1, tx, ty, out1);
@@ -341,6 +343,9 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       float s[4][4], dp[4][4];
       tile_product<DP>(x1, y1, tx, ty, s);
       tile_product<DP>(x2, y2, tx, ty, dp);
+      bool one_key[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) one_key[j] = attn_key_count(P, length, begin + tx + 16 * j) == 1;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -349,7 +354,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
           const bool seen = begin + c < end && attn_visible(P, length, P.offset + begin + c, key);
           const float pr = seen ? exp2f(fmaf(s[i][j], P.scale_log2, -row_lse[c])) : 0.0f;
           wp[(4 * ty + i) * kWeightStride + c] = pr;
-          wds[(4 * ty + i) * kWeightStride + c] = seen ? pr * (dp[i][j] - row_delta[c]) : 0.0f;
+          wds[(4 * ty + i) * kWeightStride + c] = seen && !one_key[j] ? pr * (dp[i][j] - row_delta[c]) : 0.0f;
         }
       __syncthreads();
       tile_accumulate<DP>(wds, y1, tx, ty, out1);

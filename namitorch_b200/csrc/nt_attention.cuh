@@ -53,6 +53,14 @@ __device__ __forceinline__ bool attn_visible(const AttnParams& P, int length, in
   return j < length && j <= p && (P.window == 0 || p - j < P.window || j < P.sinks);
 }
 
+// How many keys query i sees. One key has the weight 1 whatever its score is, so dS of a query that sees
+// one is 0: what is left of P (dP - delta) in float32 is not the gradient of anything.
+__device__ __forceinline__ int attn_key_count(const AttnParams& P, int length, int i) {
+  const int end = min(length, P.offset + i + 1);
+  const int start = P.window == 0 ? 0 : min(max(P.offset + i + 1 - P.window, 0), end);
+  return end - start + min(P.sinks, start);
+}
+
 // Keys that queries [i0, i1) see: [0, sink_end) and [lo, hi), disjoint. The window's range
 // starts where the first query's window does, not at a multiple of the block.
 struct AttnKeys {

@@ -46,12 +46,7 @@ constexpr int kShortQueries = 512;
 // Whether one of queries [i0, i1) sees at most kFineKeys keys. Along the queries the number of keys
 // first grows, then stays and then, past the sequence's length, falls: the least is at an end.
 __device__ __forceinline__ bool attn_few_keys(const AttnParams& P, int length, int i0, int i1) {
-  auto few = [&](int i) {
-    const int end = min(length, P.offset + i + 1);
-    const int start = P.window == 0 ? 0 : min(max(P.offset + i + 1 - P.window, 0), end);
-    return end - start + min(P.sinks, start) <= kFineKeys;
-  };
-  return few(i0) || few(i1 - 1);
+  return attn_key_count(P, length, i0) <= kFineKeys || attn_key_count(P, length, i1 - 1) <= kFineKeys;
 }
 // float16: weights are at most 1, so that 2^14 times them stays below 65504 and those from 2^-28 on are
 // normal numbers.
@@ -980,6 +975,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
       full_lo = r0 + kTcRows - 1 - P.offset;                     // first query that sees the last key
       full_hi = r0 + kTcRows > length ? -1 : (int)(last < INT32_MAX ? last : INT32_MAX);
     }
+    const bool one_key = !DKV && attn_key_count(P, length, r0 + row) == 1;
     Step step;
     if (steps > 0) start(step);
     for (int t = 0; t < steps; ++t, advance(step)) {
@@ -1007,7 +1003,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
         fma2(Pair(p[c + 2], p[c + 3]), scale2, Pair(ls.z, ls.w)).get(p[c + 2], p[c + 3]);
       }
       exponentials(p, std::make_integer_sequence<int, kColumns / 2>{});
-      uint32_t seen = 0xffffffffu;
+      uint32_t seen = 0xffffffffu, moved = 0xffffffffu;   // moved: those with a dS (a full step has no other)
       if (!full) {
         ColumnMask mask;
         if constexpr (!DKV) {
@@ -1019,6 +1015,8 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
           mask = {key - first, key >= length ? 0 : (int)(last < end - begin ? last : end - begin), 0};
         }
         seen = mask.word(group * kColumns);
+        if constexpr (DKV) moved = seen & ~__ballot_sync(0xffffffffu, attn_key_count(P, length, begin + group * kColumns + lane) == 1);
+        else moved = one_key ? 0u : seen;
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) p[c] = seen >> c & 1 ? p[c] : 0.0f;
       }
@@ -1045,7 +1043,7 @@ __device__ __forceinline__ void backward_block(const AttnParams& P, uint32_t blo
         else return add2(x, y);
       };
       // dp of a key that is not there may be NaN: 0 * NaN is cleared.
-      auto there = [&](int c) { return (seen >> c & 1 ? 0xffffu : 0u) | (seen >> (c + 1) & 1 ? 0xffff0000u : 0u); };
+      auto there = [&](int c) { return (moved >> c & 1 ? 0xffffu : 0u) | (moved >> (c + 1) & 1 ? 0xffff0000u : 0u); };
       if (FINE && fine(step)) {
         uint32_t rest[kColumns / 2];   // what rounding takes away
 #pragma unroll

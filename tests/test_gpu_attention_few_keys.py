@@ -44,3 +44,29 @@ def test_short_sequences_keep_their_precision(cuda_device, dt, tokens, dim):
         for got, want in list(zip(grads, wanted))[:2]:
             rounded = _np(torch.from_numpy(want).to(TORCH[dt]))
             assert np.linalg.norm(_np(got) - want) <= 1.35 * np.linalg.norm(rounded - want)
+
+
+@pytest.mark.parametrize("dt", list(TORCH))
+@pytest.mark.parametrize("dim", [64, 128, 33])
+def test_rows_with_one_key_have_no_gradient(cuda_device, dt, dim):
+    """A single key has the weight 1 whatever its score: dq is 0, and dk gets nothing from the row, exactly."""
+    def grads(tokens, **options):
+        tensors = [_make((2, h, tokens, dim), dt, s).cuda().requires_grad_() for h, s in ((4, 1), (2, 2), (2, 3))]
+        g = _make((2, 4, tokens, dim), dt, 4).cuda()
+        out = F.sliding_window_attention(*tensors, **options)
+        return torch.autograd.grad(out, tensors, g), tensors, g
+
+    for tokens, options in ((1, {}), (300, {"window": 1}), (700, {"window": 1})):
+        (dq, dk, dv), tensors, g = grads(tokens, **options)
+        assert not dq.any() and not dk.any()
+        # dv is the sum of g over the group, to the bound that counts P's own rounding (P is exp(s - lse)).
+        arrays, o = [_np(t) for t in tensors], {"window": options.get("window", 0)}
+        want = _np(g).reshape(2, 2, 2, tokens, dim).sum(2)
+        assert np.all(np.abs(_np(dv) - want) <= O.tolerances(*arrays, dt, _np(g), **o)[4])
+    for tokens in (90, 1200):                                      # the first row of a causal sequence
+        (dq, dk, _), _, _ = grads(tokens)
+        assert not dq[:, :, 0].any() and dq[:, :, 1:].any() and dk[:, :, 0].any()
+    lengths = torch.tensor([1, 40], device="cuda")                 # every row of the first, some of the second
+    (dq, dk, _), _, _ = grads(100, lengths=lengths, window=30)
+    assert not dq[0].any() and not dk[0].any()
+    assert not dq[1, :, 68].any() and dq[1, :, 67].any()           # position 68 sees key 39 alone
